@@ -74,7 +74,7 @@ int mtc_sync_deadline(mtc_ctx *ctx, void *stream, int timeout_ms);
  * word was cleared; otherwise the code of the first report: 0x101-0x403, 0x501, 0x502 waits of the tensor-core kernel's roles (0x501 also
  * an expert id out of range in mtc_moe_sort), 0x601 + r rank r never arrived at a peer barrier, 0x701 / 0x702 phase counter /
  * partial-sum slot of a chained launch, 0x801-0x831 the tensor-memory decode kernel, 0x901 expert_offsets that run backwards or past the rows,
- * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 a row index that does not exist, 0xa01-0xa0b waits of the exact
+ * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 / 0x906 a row index that does not exist, 0x907 an expert that does not exist, 0xa01-0xa0b waits of the exact
  * grouped kernel's roles. */
 int mtc_status_word(mtc_ctx *ctx, uint32_t *word);
 int mtc_status_clear(mtc_ctx *ctx);
@@ -400,6 +400,46 @@ int mtc_swiglu(mtc_ctx *ctx, void *stream, const void *gate, const void *up, voi
  * layout is quantized.rs:4296-4314 and :4354-4379). */
 int mtc_unpack_codes(mtc_ctx *ctx, void *stream, const void *w, void *codes_u8, int N, int K,
                      int bits);
+
+/* ---- 8-bit floating point (e4m3 codes with an f32 scale for each block of 128 values) and the router's training side ----
+ * No counterpart in the reference, whose quantized formats are integers with affine scales and whose router is inference only; the products stand
+ * next to mt_qmm and mt_moe_gather_qmm, the loss next to mt_moe_router_topk.  Entries that need scratch memory take it from the caller: `workspace`,
+ * 256-byte aligned, at least what the *_workspace function says for the same arguments (0: NULL is fine), its contents nobody's business before and
+ * after the call.  Calls on different streams, or captured into different graphs, that have workspaces of their own do not disturb each other.
+ * Layouts, B(n) = ceil(n / 128):
+ *   activations  codes u8[M, K], scales f32[M, B(K)]       one scale for 128 values of a row
+ *   weights      codes u8[N, K], scales f32[B(N), B(K)]    one scale for 128 x 128 values; stacked experts [E, N, K], [E, B(N), B(K)] */
+/* codes = x / s rounded to the nearest e4m3 value (ties to even), where s = max(max |x| / 448, 2^-90) over the finite values of a block, or with pow2 != 0 the least
+ * power of two that is not below that; the quotient is rounded once, a tie or a border between two codes is told exactly.  Infinities and NaN become NaN.
+ * block_rows 1: x T[n_rows, K] -> the layout of activations (n_mats 1); 128: x T[n_mats, n_rows, K] -> that of weights.  rows (block_rows 1 only, else NULL): u32[n_rows],
+ * row r reads x[rows[r]] of n_src_rows rows (mtc_moe_permute folded in); an index outside reads row 0 and is reported through the status word (0x906). */
+int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows, void *codes, void *scales, int n_mats, int n_rows, int n_src_rows, int K,
+                     int block_rows, int pow2, int dtype);
+/* out[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k], sums in f32, rounded once to out_dtype (f32, f16, bf16).
+ * x_dtype MTC_E4M3: x holds codes, x_scales their scales.  x_dtype f32 / f16 / bf16: x T[M, K] is quantized in the call as mtc_fp8_quantize does with blocks
+ * of one row and pow2 0 (x_scales NULL): same results.  K a multiple of 16 with 16-byte aligned x and w runs on tensor cores, everything else on CUDA cores. */
+enum { MTC_E4M3 = 3 };
+int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int M, int N, int K, int x_dtype,
+               int out_dtype, void *workspace, size_t workspace_bytes);
+size_t mtc_fp8_mm_workspace(const mtc_ctx *ctx, int M, int N, int K, int x_dtype, int out_dtype);
+/* The same product of rows sorted by expert with stacked matrices: row t of expert_offsets[e] <= t < expert_offsets[e + 1] meets w[e] (u32[n_experts + 1], as
+ * mtc_moe_sort writes them; x is codes).  Rows in no range keep what `out` holds there.  Offsets that reach past m_total or run backwards are clamped and
+ * reported through the status word (0x901). */
+int mtc_fp8_gather_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, const void *expert_offsets, void *out,
+                      int m_total, int n_out, int k_in, int n_experts, int out_dtype, void *workspace, size_t workspace_bytes);
+size_t mtc_fp8_gather_mm_workspace(const mtc_ctx *ctx, int m_total, int n_out, int k_in, int n_experts, int out_dtype);
+/* The balance loss of a router.  Over the n rows t with mask[t] != 0 (u8[n_rows], NULL: all): p_t = softmax(logits_t), zeros for a row of minus infinities only;
+ *     counts[e] = how often topk_idx (u32[n_rows, k]) names e in them,   mean_probs[e] = (1 / n) sum_t p_t[e],
+ *     loss = coef * n_experts * sum_e counts[e] / (n k) * mean_probs[e]                    (n = 0: everything 0)
+ * loss f32, counts i32[n_experts], mean_probs f32[n_experts], n_counted i32 = n.  What masked rows hold does not matter.  An index outside the experts is not counted
+ * and is reported through the status word (0x907).  n_experts <= 1024, k <= 32 as in mtc_moe_router_topk.  Sums run in a fixed order.
+ * mtc_moe_balance_grad: grad T[n_rows, n_experts] = *grad_loss (f32, NULL: 1) * d loss / d logits
+ *     = *grad_loss * coef * n_experts / n * p_t[e] * (f[e] - sum_j f[j] p_t[j]),  f = counts / (n k) constants;  zeros for masked rows. */
+int mtc_moe_balance(mtc_ctx *ctx, void *stream, const void *logits, const void *topk_idx, const void *mask, float coef, void *loss, void *counts, void *mean_probs,
+                    void *n_counted, int n_rows, int n_experts, int k, int dtype, void *workspace, size_t workspace_bytes);
+size_t mtc_moe_balance_workspace(const mtc_ctx *ctx, int n_rows, int n_experts);
+int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const void *mask, const void *counts, const void *n_counted, const void *grad_loss, float coef,
+                         void *grad, int n_rows, int n_experts, int k, int dtype);
 
 /* ---- name-keyed dispatch with HOST buffers: Context::dispatch_with_grid
  *      (crates/metaltile-runtime/src/context.rs:269-284) ----

@@ -113,6 +113,14 @@ SIGNATURES = {
     "mtc_moe_permute": (_i, [_vp] * 5 + [_i] * 3),
     "mtc_moe_unpermute": (_i, [_vp] * 6 + [_i] * 4),
     "mtc_swiglu": (_i, [_vp] * 5 + [_sz, _i]),
+    "mtc_fp8_quantize": (_i, [_vp] * 6 + [_i] * 7),
+    "mtc_fp8_mm": (_i, [_vp] * 7 + [_i] * 5 + [_vp, _sz]),
+    "mtc_fp8_mm_workspace": (_sz, [_vp] + [_i] * 5),
+    "mtc_fp8_gather_mm": (_i, [_vp] * 8 + [_i] * 5 + [_vp, _sz]),
+    "mtc_fp8_gather_mm_workspace": (_sz, [_vp] + [_i] * 5),
+    "mtc_moe_balance": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_i] * 4 + [_vp, _sz]),
+    "mtc_moe_balance_workspace": (_sz, [_vp, _i, _i]),
+    "mtc_moe_balance_grad": (_i, [_vp] * 7 + [ctypes.c_float, _vp] + [_i] * 4),
     "mtc_set_option": (_i, [_vp, ctypes.c_char_p, _i]),
     "mtc_unpack_codes": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "mtc_measure": (_i, [_vp, ctypes.c_char_p, _i, ctypes.POINTER(NamedBuf), _i, _i, _i, _i, ctypes.POINTER(ctypes.c_double),

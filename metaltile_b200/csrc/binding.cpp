@@ -9,6 +9,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -631,6 +632,228 @@ PyObject *unpack_codes(Args a, Py_ssize_t n) {
     return wrap(std::move(codes));
 }
 
+// ---- 8-bit floating point, the router's training side --------------------------------------------------
+// Tensors may live on another device than the current one: the call runs on theirs, on its current stream, and leaves the caller's device as it was.
+void need_one_device(std::initializer_list<const at::Tensor *> ts) {
+    const at::Tensor *first = *ts.begin();
+    for (const at::Tensor *t : ts)
+        if (!t->is_cuda() || t->device() != first->device()) raise(PyExc_ValueError, "all operands must be tensors of one CUDA device");
+}
+void need_size(int64_t v, const char *what) {
+    if (v > 0x7FFFFFFF) raise(PyExc_ValueError, std::string(what) + " must be below 2^31");
+}
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+at::ScalarType out_type(long long dt) { return dt == MTC_F32 ? at::kFloat : dt == MTC_F16 ? at::kHalf : at::kBFloat16; }
+void *on_stream(const at::Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+PyObject *tuple_of(std::initializer_list<at::Tensor *> ts) {
+    PyObject *t = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+    if (!t) throw PyErr{};
+    Py_ssize_t i = 0;
+    for (at::Tensor *x : ts) {
+        PyObject *o = THPVariable_Wrap(std::move(*x));
+        if (!o) {
+            Py_DECREF(t);
+            throw PyErr{};
+        }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+// an index tensor: 32-bit integers, contiguous
+const at::Tensor &index_tensor(PyObject *o, const char *what) {
+    const at::Tensor &t = tensor(o, what);
+    if (t.scalar_type() != at::kInt && t.scalar_type() != at::kUInt32) raise(PyExc_TypeError, std::string(what) + " must be int32");
+    if (!t.is_contiguous()) raise(PyExc_ValueError, std::string(what) + " must be contiguous");
+    return t;
+}
+
+// fp8_quantize(x, block_rows, pow2, rows, ctx) -> (codes, scales)
+PyObject *fp8_quantize(Args a, Py_ssize_t n) {
+    nargs(n, 5);
+    const at::Tensor &x = tensor(a[0], "x");
+    const long long block_rows = integer(a[1]);
+    const int pow2 = PyObject_IsTrue(a[2]);
+    if (pow2 < 0) throw PyErr{};
+    const at::Tensor *rows = a[3] == Py_None ? nullptr : &index_tensor(a[3], "rows");
+    if (block_rows != 1 && block_rows != 128) raise(PyExc_ValueError, "block_rows must be 1 or 128");
+    if (x.dim() < (block_rows == 1 ? 1 : 2) || x.size(-1) == 0) raise(PyExc_ValueError, "x must be rows of at least one value (block_rows 128: [.., N, K])");
+    if (rows && (block_rows != 1 || x.dim() != 2)) raise(PyExc_ValueError, "rows needs x [tokens, K] and block_rows 1");
+    const int dt = need_dtype(x);
+    need_contiguous({&x});
+    if (rows) need_one_device({&x, rows}); else need_one_device({&x});
+    const int64_t K = x.size(-1), src = block_rows == 1 ? x.numel() / K : x.size(-2), M = rows ? rows->numel() : src;
+    const int64_t mats = block_rows == 1 ? 1 : M ? x.numel() / (M * K) : 0;
+    need_size(K, "K"), need_size(M, "rows"), need_size(src, "rows"), need_size(mats, "matrices");
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end()), s_shape = shape;
+    if (rows) shape = {M, K}, s_shape = shape;
+    s_shape.back() = blocks(K);
+    if (block_rows != 1) s_shape[s_shape.size() - 2] = blocks(M);
+    at::Tensor codes, scales;
+    const Call c(a[4], x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(x.device());
+        codes = empty(shape, at::kFloat8_e4m3fn, x);
+        scales = empty(s_shape, at::kFloat, x);
+        return mtc_fp8_quantize(c.h, on_stream(x), x.data_ptr(), rows ? rows->data_ptr() : nullptr, codes.data_ptr(), scales.data_ptr(), static_cast<int>(mats),
+                                static_cast<int>(M), static_cast<int>(src), static_cast<int>(K), static_cast<int>(block_rows), pow2, dt);
+    }));
+    return tuple_of({&codes, &scales});
+}
+
+// fp8_mm(x, w, w_scales, x_scales, out_dtype (-1: by x), out, ctx)
+PyObject *fp8_mm(Args a, Py_ssize_t n) {
+    nargs(n, 7);
+    const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &ws = tensor(a[2], "w_scales");
+    const at::Tensor *xs = a[3] == Py_None ? nullptr : &tensor(a[3], "x_scales");
+    const bool codes = x.scalar_type() == at::kFloat8_e4m3fn;
+    int xdt = MTC_E4M3;
+    if (!codes && (xdt = act_dtype(x)) < 0) raise(PyExc_TypeError, "x must be float8_e4m3fn codes, f32, f16 or bf16");
+    if (codes != (xs != nullptr)) raise(PyExc_ValueError, codes ? "codes need x_scales" : "x_scales go with codes: float activations are quantized in the call");
+    if (w.scalar_type() != at::kFloat8_e4m3fn || ws.scalar_type() != at::kFloat || (xs && xs->scalar_type() != at::kFloat))
+        raise(PyExc_TypeError, "w must be float8_e4m3fn codes, scales float32");
+    if (x.dim() == 0 || x.size(-1) == 0) raise(PyExc_ValueError, "x must be rows of at least one value");
+    const int64_t K = x.size(-1), M = x.numel() / K;
+    if (w.dim() != 2 || w.size(1) != K) raise(PyExc_ValueError, "w must be [N, K]");
+    const int64_t N = w.size(0);
+    if (ws.dim() != 2 || ws.size(0) != blocks(N) || ws.size(1) != blocks(K)) raise(PyExc_ValueError, "w_scales must be [ceil(N/128), ceil(K/128)]");
+    if (xs && (xs->dim() < 1 || xs->size(-1) != blocks(K) || xs->numel() != M * blocks(K))) raise(PyExc_ValueError, "x_scales must be [.., ceil(K/128)], as x is [.., K]");
+    need_contiguous({&x, &w, &ws});
+    if (xs) need_contiguous({xs}), need_one_device({&x, &w, &ws, xs});
+    else need_one_device({&x, &w, &ws});
+    need_size(M, "M"), need_size(N, "N"), need_size(K, "K");
+    const bool given = a[5] != Py_None;
+    at::Tensor out = given ? tensor(a[5], "out") : at::Tensor();
+    long long odt = integer(a[4]);
+    if (odt < 0) odt = given ? act_dtype(out) : codes ? MTC_BF16 : xdt;
+    if (odt != MTC_F32 && odt != MTC_F16 && odt != MTC_BF16) raise(PyExc_TypeError, "out must be f32, f16 or bf16");
+    if (given) {
+        if (out.device() != x.device() || out.scalar_type() != out_type(odt)) raise(PyExc_TypeError, "out must live on the device of x and have type out_dtype");
+        check_out(out, M, N, out);
+    }
+    const Call c(a[6], x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(x.device());
+        if (!given) out = empty({M, N}, out_type(odt), x);
+        const size_t need = mtc_fp8_mm_workspace(c.h, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), xdt, static_cast<int>(odt));
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, x);
+        return mtc_fp8_mm(c.h, on_stream(x), x.data_ptr(), xs ? xs->data_ptr() : nullptr, w.data_ptr(), ws.data_ptr(), out.data_ptr(), static_cast<int>(M),
+                          static_cast<int>(N), static_cast<int>(K), xdt, static_cast<int>(odt), need ? space.data_ptr() : nullptr, need);
+    }));
+    return given ? same(a[5]) : wrap(std::move(out));
+}
+
+// fp8_gather_mm(x, w, w_scales, expert_offsets, x_scales, out_dtype (-1: bf16), out, ctx)
+PyObject *fp8_gather_mm(Args a, Py_ssize_t n) {
+    nargs(n, 8);
+    const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &ws = tensor(a[2], "w_scales"), &off = index_tensor(a[3], "expert_offsets"),
+                     &xs = tensor(a[4], "x_scales");
+    if (x.scalar_type() != at::kFloat8_e4m3fn || w.scalar_type() != at::kFloat8_e4m3fn || xs.scalar_type() != at::kFloat || ws.scalar_type() != at::kFloat)
+        raise(PyExc_TypeError, "x and w must be float8_e4m3fn codes, scales float32");
+    if (x.dim() != 2 || x.size(1) == 0) raise(PyExc_ValueError, "x must be [rows, k_in]");
+    const int64_t M = x.size(0), K = x.size(1);
+    if (w.dim() != 3 || w.size(0) == 0 || w.size(2) != K) raise(PyExc_ValueError, "w must be [E, n_out, k_in]");
+    const int64_t E = w.size(0), N = w.size(1);
+    if (ws.dim() != 3 || ws.size(0) != E || ws.size(1) != blocks(N) || ws.size(2) != blocks(K))
+        raise(PyExc_ValueError, "w_scales must be [E, ceil(n_out/128), ceil(k_in/128)]");
+    if (xs.dim() != 2 || xs.size(0) != M || xs.size(1) != blocks(K)) raise(PyExc_ValueError, "x_scales must be [rows, ceil(k_in/128)]");
+    if (off.numel() != E + 1) raise(PyExc_ValueError, "expert_offsets must have E + 1 entries");
+    need_contiguous({&x, &w, &ws, &xs});
+    need_one_device({&x, &w, &ws, &xs, &off});
+    need_size(M, "rows"), need_size(N, "n_out"), need_size(K, "k_in"), need_size(E, "E");
+    const bool given = a[6] != Py_None;
+    at::Tensor out = given ? tensor(a[6], "out") : at::Tensor();
+    long long odt = integer(a[5]);
+    if (odt < 0) odt = given ? act_dtype(out) : MTC_BF16;
+    if (odt != MTC_F32 && odt != MTC_F16 && odt != MTC_BF16) raise(PyExc_TypeError, "out must be f32, f16 or bf16");
+    if (given) {
+        if (out.device() != x.device() || out.scalar_type() != out_type(odt)) raise(PyExc_TypeError, "out must live on the device of x and have type out_dtype");
+        check_out(out, M, N, out);
+    }
+    const Call c(a[7], x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(x.device());
+        if (!given) out = empty({M, N}, out_type(odt), x);
+        const size_t need = mtc_fp8_gather_mm_workspace(c.h, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), static_cast<int>(E), static_cast<int>(odt));
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, x);
+        return mtc_fp8_gather_mm(c.h, on_stream(x), x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), off.data_ptr(), out.data_ptr(), static_cast<int>(M),
+                                 static_cast<int>(N), static_cast<int>(K), static_cast<int>(E), static_cast<int>(odt), need ? space.data_ptr() : nullptr, need);
+    }));
+    return given ? same(a[6]) : wrap(std::move(out));
+}
+
+// one byte a row, not zero where the row counts
+const at::Tensor *row_mask(PyObject *o, int64_t rows) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor &m = tensor(o, "mask");
+    if (m.scalar_type() != at::kBool && m.scalar_type() != at::kByte) raise(PyExc_TypeError, "mask must be bool or uint8");
+    if (m.dim() != 1 || m.size(0) != rows || !m.is_contiguous()) raise(PyExc_ValueError, "mask must be [rows], contiguous");
+    return &m;
+}
+
+// moe_balance(logits, topk_idx, coef, mask, ctx) -> (loss, counts, mean_probs, n_counted)
+PyObject *moe_balance(Args a, Py_ssize_t n) {
+    nargs(n, 5);
+    const at::Tensor &l = tensor(a[0], "logits"), &idx = index_tensor(a[1], "topk_idx");
+    const double coef = PyFloat_AsDouble(a[2]);
+    if (coef == -1.0 && PyErr_Occurred()) throw PyErr{};
+    const int dt = need_dtype(l);
+    if (l.dim() != 2 || idx.dim() != 2 || idx.size(0) != l.size(0)) raise(PyExc_ValueError, "logits must be [rows, n_experts] and topk_idx [rows, k]");
+    const int64_t R = l.size(0), E = l.size(1), k = idx.size(1);
+    const at::Tensor *mask = row_mask(a[3], R);
+    need_contiguous({&l});
+    if (mask) need_one_device({&l, &idx, mask}); else need_one_device({&l, &idx});
+    need_size(R, "rows"), need_size(E, "n_experts");
+    at::Tensor loss, counts, mean, counted;
+    const Call c(a[4], l);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(l.device());
+        loss = empty({}, at::kFloat, l);
+        counts = empty({E}, at::kInt, l);
+        mean = empty({E}, at::kFloat, l);
+        counted = empty({}, at::kInt, l);
+        const size_t need = mtc_moe_balance_workspace(c.h, static_cast<int>(R), static_cast<int>(E));
+        const at::Tensor space = empty({static_cast<int64_t>(need)}, at::kByte, l);
+        return mtc_moe_balance(c.h, on_stream(l), l.data_ptr(), idx.data_ptr(), mask ? mask->data_ptr() : nullptr, static_cast<float>(coef), loss.data_ptr(),
+                               counts.data_ptr(), mean.data_ptr(), counted.data_ptr(), static_cast<int>(R), static_cast<int>(E), static_cast<int>(k), dt,
+                               space.data_ptr(), need);
+    }));
+    return tuple_of({&loss, &counts, &mean, &counted});
+}
+
+// moe_balance_grad(logits, counts, n_counted, k, grad_loss, coef, mask, out, ctx)
+PyObject *moe_balance_grad(Args a, Py_ssize_t n) {
+    nargs(n, 9);
+    const at::Tensor &l = tensor(a[0], "logits"), &counts = index_tensor(a[1], "counts"), &counted = index_tensor(a[2], "n_counted");
+    const long long k = integer(a[3]);
+    const at::Tensor *gl = a[4] == Py_None ? nullptr : &tensor(a[4], "grad_loss");
+    const double coef = PyFloat_AsDouble(a[5]);
+    if (coef == -1.0 && PyErr_Occurred()) throw PyErr{};
+    const int dt = need_dtype(l);
+    if (l.dim() != 2) raise(PyExc_ValueError, "logits must be [rows, n_experts]");
+    const int64_t R = l.size(0), E = l.size(1);
+    if (counts.numel() != E || counted.numel() != 1) raise(PyExc_ValueError, "counts must have n_experts entries and n_counted one");
+    if (gl && (gl->scalar_type() != at::kFloat || gl->numel() != 1)) raise(PyExc_TypeError, "grad_loss must be one float32");
+    const at::Tensor *mask = row_mask(a[6], R);
+    need_contiguous({&l});
+    need_one_device({&l, &counts, &counted, gl ? gl : &l, mask ? mask : &l});
+    need_size(R, "rows"), need_size(E, "n_experts"), need_size(k, "k");
+    const bool given = a[7] != Py_None;
+    at::Tensor out = given ? tensor(a[7], "out") : at::Tensor();
+    if (given) check_out(out, R, E, l);
+    const Call c(a[8], l);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(l.device());
+        if (!given) out = empty({R, E}, l.scalar_type(), l);
+        return mtc_moe_balance_grad(c.h, on_stream(l), l.data_ptr(), mask ? mask->data_ptr() : nullptr, counts.data_ptr(), counted.data_ptr(),
+                                    gl ? gl->data_ptr() : nullptr, static_cast<float>(coef), out.data_ptr(), static_cast<int>(R), static_cast<int>(E),
+                                    static_cast<int>(k), dt);
+    }));
+    return given ? same(a[7]) : wrap(std::move(out));
+}
+
 // ---- module ----------------------------------------------------------------------------------------
 PyObject *set_context(PyObject *, PyObject *fn) {
     Py_INCREF(fn);
@@ -654,6 +877,7 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     OP(dense), OP(qmv_batched), OP(qvm), OP(rms_norm_qmv), OP(swiglu), OP(moe_router_topk), OP(moe_sort), OP(moe_permute), OP(moe_unpermute),
     OP(gather_qmm), OP(moe_experts), OP(affine_quantize), OP(affine_dequantize), OP(dequant_gather), OP(unpack_codes),
+    OP(fp8_quantize), OP(fp8_mm), OP(fp8_gather_mm), OP(moe_balance), OP(moe_balance_grad),
     {"set_context", set_context, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1,0 +1,64 @@
+// e4m3 codes with an f32 scale for each block of 128 values: what the quantizer and the products share.
+//   activations  codes u8[M, K], scales f32[M, ceil(K/128)]                  (blocks of 1 x 128)
+//   weights      codes u8[N, K], scales f32[ceil(N/128), ceil(K/128)]        (blocks of 128 x 128)
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace mtc {
+namespace fp8 {
+
+constexpr int kBlock = 128;
+constexpr float kLeastScale = 8.077935669463161e-28f;      // 2^-90: below it the residual of a quotient could underflow (code_quotient)
+
+__host__ __device__ constexpr int blocks(int n) { return (n + kBlock - 1) / kBlock; }
+
+// two codes; lo in the low byte.  |v| above 448 becomes 448, NaN the code 0x7F.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(codes)));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+
+// The scale of a block with this largest magnitude
+__device__ __forceinline__ float scale_of(float amax, int pow2) {
+    float s = fmaxf(__fdiv_rn(amax, 448.0f), kLeastScale);
+    if (pow2) s = __uint_as_float((__float_as_uint(s) + 0x7FFFFFu) & 0xFF800000u);
+    return s;
+}
+
+// x / s such that rounding it to a code gives the code nearest to the true quotient.  A quotient rounded to f32 first may land on the border
+// between two codes that the true one lies beside (with s = amax / 448 rounded that is one value in a few hundred, since x and amax have few bits),
+// so the quotient is rounded to odd: corrected to within one unit, its exact remainder found, and an even result moved towards the truth.  Borders
+// are even numbers, so none is hit unless the quotient is exact.  Below 2^-11 every quotient becomes zero anyway.  inv = 1 / s.
+__device__ __forceinline__ float code_quotient(float x, float s, float inv) {
+    float r = x * inv;
+    r = fmaf(fmaf(-r, s, x), inv, r);
+    const float rest = fmaf(-r, s, x);
+    uint32_t b = __float_as_uint(r);
+    if (rest != 0.0f && !(b & 1u) && fabsf(r) >= 4.8828125e-4f) b += ((rest > 0.0f) == (r > 0.0f)) ? 1u : 0xFFFFFFFFu;
+    r = __uint_as_float(b);
+    return fabsf(x) < INFINITY ? r : __int_as_float(0x7FC00000);        // infinities have no code: NaN, as NaN is
+}
+
+}  // namespace fp8
+
+// Launchers
+cudaError_t launch_fp8_quantize(Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *rows, uint8_t *codes, float *scales, int n_mats,
+                                long long n_rows, long long n_src_rows, int K, int block_rows, int pow2, int dt);
+cudaError_t launch_fp8_mm_generic(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets,
+                                  void *out, int M, int N, int K, int n_experts, int out_dt);
+size_t moe_balance_workspace(int sms, int n_rows, int n_experts);
+cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float coef, float *loss,
+                               int *counts, float *mean_probs, int *n_counted, int n_rows, int n_experts, int k, int dt, void *workspace);
+cudaError_t launch_moe_balance_grad(Ctx *ctx, cudaStream_t st, const void *logits, const uint8_t *mask, const int *counts, const int *n_counted,
+                                    const float *grad_loss, float coef, void *grad, int n_rows, int n_experts, int k, int dt);
+
+}  // namespace mtc

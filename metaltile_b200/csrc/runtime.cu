@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "fp8.cuh"
 
 using mtc::Ctx;
 using mtc::fail;
@@ -1450,6 +1451,150 @@ int mtc_unpack_codes(mtc_ctx *ctx, void *stream, const void *w, void *codes_u8, 
         return fail(ctx, MTC_ERR_UNSUPPORTED, "unpack_codes: need 1 <= bits <= 8 and K*bits % 32 == 0");
     MTC_CUDA(ctx, mtc::launch_unpack_codes(static_cast<cudaStream_t>(stream), w, codes_u8, N, K, bits), MTC_ERR_DISPATCH);
     return MTC_OK;
+}
+
+// ---- 8-bit floating point, the router's training side ------------------------------------------------------
+// No C++ exception leaves an entry (a message that cannot be allocated, say).
+}  // extern "C"
+template <typename F>
+static int guarded(mtc_ctx *ctx, F &&f) {
+    if (!ctx) return MTC_ERR_INVALID;
+    try {
+        return f();
+    } catch (...) {
+        return MTC_ERR_DISPATCH;
+    }
+}
+extern "C" {
+static bool aligned_to(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+static int check_workspace(mtc_ctx *ctx, const char *who, const void *workspace, size_t have, size_t need) {
+    if (need == 0 || (workspace && have >= need && aligned_to(workspace, 256))) return MTC_OK;
+    return fail(ctx, MTC_ERR_BUFFER_SIZE, std::string(who) + ": needs a workspace of " + std::to_string(need) + " bytes, 256-byte aligned, got " +
+                                              (workspace ? std::to_string(have) : std::string("none")));
+}
+
+int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows, void *codes, void *scales, int n_mats, int n_rows, int n_src_rows, int K,
+                     int block_rows, int pow2, int dtype) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_quantize: dtype must be f32, f16 or bf16");
+        if (block_rows != 1 && block_rows != 128) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_quantize: blocks are of 1 or 128 rows");
+        if (n_mats < 0 || n_rows < 0 || K <= 0 || (block_rows == 1 && n_mats > 1) || (rows && (block_rows != 1 || n_src_rows < 0)))
+            return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: sizes must be positive; rows of an index and one matrix only with blocks of one row");
+        if (n_mats == 0 || n_rows == 0) return MTC_OK;
+        if (!x || !codes || !scales) return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: null pointer");
+        if (rows && n_src_rows == 0) return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: an index into no rows");
+        MTC_CUDA(ctx, mtc::launch_fp8_quantize(ctx, static_cast<cudaStream_t>(stream), x, static_cast<const uint32_t *>(rows), static_cast<uint8_t *>(codes),
+                                               static_cast<float *>(scales), n_mats, n_rows, n_src_rows, K, block_rows, pow2, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+size_t mtc_fp8_mm_workspace(const mtc_ctx *ctx, int M, int N, int K, int x_dtype, int out_dtype) {
+    (void)ctx;
+    (void)out_dtype;
+    if (M <= 0 || N <= 0 || K <= 0 || x_dtype == MTC_E4M3) return 0;
+    return align_up(static_cast<size_t>(M) * K, 256) + align_up(static_cast<size_t>(M) * mtc::fp8::blocks(K) * 4, 256);
+}
+
+int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int M, int N, int K, int x_dtype,
+               int out_dtype, void *workspace, size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        if (!dtype_ok(out_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_mm: out_dtype must be f32, f16 or bf16");
+        if (x_dtype != MTC_E4M3 && !dtype_ok(x_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_mm: x must be e4m3 codes, f32, f16 or bf16");
+        if (M < 0 || N < 0 || K <= 0) return fail(ctx, MTC_ERR_INVALID, "fp8_mm: sizes must be positive");
+        if (M == 0 || N == 0) return MTC_OK;
+        if (!x || !w || !w_scales || !out || (x_dtype == MTC_E4M3) != (x_scales != nullptr))
+            return fail(ctx, MTC_ERR_INVALID, "fp8_mm: null pointer, or scales that do not go with the type of x");
+        int rc = check_workspace(ctx, "fp8_mm", workspace, workspace_bytes, mtc_fp8_mm_workspace(ctx, M, N, K, x_dtype, out_dtype));
+        if (rc != MTC_OK) return rc;
+        const uint8_t *codes = static_cast<const uint8_t *>(x);
+        const float *scales = static_cast<const float *>(x_scales);
+        if (x_dtype != MTC_E4M3) {
+            uint8_t *c = static_cast<uint8_t *>(workspace);
+            float *s = reinterpret_cast<float *>(c + align_up(static_cast<size_t>(M) * K, 256));
+            rc = mtc_fp8_quantize(ctx, stream, x, nullptr, c, s, 1, M, M, K, 1, 0, x_dtype);
+            if (rc != MTC_OK) return rc;
+            codes = c;
+            scales = s;
+        }
+        MTC_CUDA(ctx, mtc::launch_fp8_mm_generic(ctx, static_cast<cudaStream_t>(stream), codes, scales, static_cast<const uint8_t *>(w),
+                                                 static_cast<const float *>(w_scales), nullptr, out, M, N, K, 1, out_dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+size_t mtc_fp8_gather_mm_workspace(const mtc_ctx *ctx, int m_total, int n_out, int k_in, int n_experts, int out_dtype) {
+    (void)ctx;
+    (void)m_total;
+    (void)n_out;
+    (void)k_in;
+    (void)n_experts;
+    (void)out_dtype;
+    return 0;
+}
+
+int mtc_fp8_gather_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, const void *expert_offsets, void *out,
+                      int m_total, int n_out, int k_in, int n_experts, int out_dtype, void *workspace, size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        if (!dtype_ok(out_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_gather_mm: out_dtype must be f32, f16 or bf16");
+        if (m_total < 0 || n_out < 0 || k_in <= 0 || n_experts <= 0) return fail(ctx, MTC_ERR_INVALID, "fp8_gather_mm: sizes must be positive");
+        if (m_total == 0 || n_out == 0) return MTC_OK;
+        if (!x || !x_scales || !w || !w_scales || !expert_offsets || !out) return fail(ctx, MTC_ERR_INVALID, "fp8_gather_mm: null pointer");
+        int rc = check_workspace(ctx, "fp8_gather_mm", workspace, workspace_bytes,
+                                 mtc_fp8_gather_mm_workspace(ctx, m_total, n_out, k_in, n_experts, out_dtype));
+        if (rc != MTC_OK) return rc;
+        MTC_CUDA(ctx, mtc::launch_fp8_mm_generic(ctx, static_cast<cudaStream_t>(stream), static_cast<const uint8_t *>(x), static_cast<const float *>(x_scales),
+                                                 static_cast<const uint8_t *>(w), static_cast<const float *>(w_scales),
+                                                 static_cast<const uint32_t *>(expert_offsets), out, m_total, n_out, k_in, n_experts, out_dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+size_t mtc_moe_balance_workspace(const mtc_ctx *ctx, int n_rows, int n_experts) {
+    return n_experts <= 0 ? 0 : mtc::moe_balance_workspace(ctx ? ctx->sm_count : mtc::kNumSMsB200, n_rows, n_experts);
+}
+
+static int balance_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int n_experts, int k, int dtype) {
+    if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": dtype must be f32, f16 or bf16");
+    if (n_rows < 0 || n_experts <= 0 || n_experts > 1024 || k <= 0 || k > 32 || k > n_experts)
+        return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": need 0 < k <= min(32, n_experts), n_experts <= 1024");
+    return MTC_OK;
+}
+
+int mtc_moe_balance(mtc_ctx *ctx, void *stream, const void *logits, const void *topk_idx, const void *mask, float coef, void *loss, void *counts, void *mean_probs,
+                    void *n_counted, int n_rows, int n_experts, int k, int dtype, void *workspace, size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        int rc = balance_args_ok(ctx, "moe_balance", n_rows, n_experts, k, dtype);
+        if (rc != MTC_OK) return rc;
+        if (!loss || !counts || !mean_probs || !n_counted || (n_rows > 0 && (!logits || !topk_idx)))
+            return fail(ctx, MTC_ERR_INVALID, "moe_balance: null pointer");
+        rc = check_workspace(ctx, "moe_balance", workspace, workspace_bytes, mtc_moe_balance_workspace(ctx, n_rows, n_experts));
+        if (rc != MTC_OK) return rc;
+        MTC_CUDA(ctx, mtc::launch_moe_balance(ctx, static_cast<cudaStream_t>(stream), logits, static_cast<const uint32_t *>(topk_idx),
+                                              static_cast<const uint8_t *>(mask), coef, static_cast<float *>(loss), static_cast<int *>(counts),
+                                              static_cast<float *>(mean_probs), static_cast<int *>(n_counted), n_rows, n_experts, k, dtype, workspace),
+                 MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const void *mask, const void *counts, const void *n_counted, const void *grad_loss, float coef,
+                         void *grad, int n_rows, int n_experts, int k, int dtype) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        int rc = balance_args_ok(ctx, "moe_balance_grad", n_rows, n_experts, k, dtype);
+        if (rc != MTC_OK) return rc;
+        if (n_rows == 0) return MTC_OK;
+        if (!logits || !counts || !n_counted || !grad) return fail(ctx, MTC_ERR_INVALID, "moe_balance_grad: null pointer");
+        MTC_CUDA(ctx, mtc::launch_moe_balance_grad(ctx, static_cast<cudaStream_t>(stream), logits, static_cast<const uint8_t *>(mask),
+                                                   static_cast<const int *>(counts), static_cast<const int *>(n_counted),
+                                                   static_cast<const float *>(grad_loss), coef, grad, n_rows, n_experts, k, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
 }
 
 int mtc_kernel_count(void) { return kNumKernels; }

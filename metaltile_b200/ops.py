@@ -169,3 +169,56 @@ def qvm(w, scales, biases, x, bits: int, group_size: int, out=None, ctx: Context
     x [M, K] -> out [M, N] (``mt_qvm_*``, crates/metaltile-std/src/mlx/quantized.rs:4397-4530).  Like the other dense products
     it requests its first weights while the previous kernel of the stream drains (option ``pdl_early_weights``)."""
     return _native.qvm(w, scales, biases, x, bits, group_size, out, ctx)
+
+
+# ---- 8-bit floating point: e4m3 codes with a float32 scale for each block of 128 values ---------------------------------------
+def _out_dtype(dtype):
+    if dtype is None:
+        return -1
+    if dtype not in _TORCH_DT:
+        raise TypeError("out_dtype must be float32, float16 or bfloat16")
+    return _TORCH_DT[dtype]
+
+
+def fp8_quantize(x, block_rows: int = 1, pow2: bool = False, rows=None, ctx: Context = None):
+    """Float tensor -> (codes ``float8_e4m3fn`` like ``x``, scales float32) in the layout the products below read.
+
+    ``block_rows=1``, activations: ``x [.., K]``, one scale for 128 values of a row, ``[.., ceil(K/128)]``; ``rows`` (int32) folds
+    ``moe_permute`` in: row r of the result is ``x[rows[r]]``.  ``block_rows=128``, weights: ``x [.., N, K]``, one scale for 128 x 128 values,
+    ``[.., ceil(N/128), ceil(K/128)]``.  A scale is ``max(max|x| / 448, 2**-90)`` over the finite values of its block, with ``pow2`` the least power
+    of two that is not below that; a code is the e4m3 value nearest to ``x / scale``, ties to even.  Infinities and NaN become NaN."""
+    return _native.fp8_quantize(x, block_rows, pow2, rows, ctx)
+
+
+def fp8_mm(x, w, w_scales, x_scales=None, out_dtype=None, out=None, ctx: Context = None):
+    """out[M, N] = x @ w^T with w ``[N, K]`` codes and ``w_scales [ceil(N/128), ceil(K/128)]``, block sums scaled and added in f32.
+
+    ``x [.., K]`` is codes with ``x_scales [.., ceil(K/128)]``, or f32 / f16 / bf16 activations, which are quantized in the call as
+    ``fp8_quantize(x)`` does (same result).  ``out_dtype`` (f32, f16, bf16) defaults to the type of float activations, bf16 for codes.
+    The gradient of x is the same product with the matrix the other way round: ``fp8_mm(dy, w.T.contiguous(), w_scales.T.contiguous())``
+    - blocks of 128 x 128 stay what they are."""
+    return _native.fp8_mm(x, w, w_scales, x_scales, _out_dtype(out_dtype), out, ctx)
+
+
+def fp8_gather_mm(x, w, w_scales, expert_offsets, x_scales, out_dtype=None, out=None, ctx: Context = None):
+    """The grouped form: ``x [rows, K]`` codes sorted by expert (``fp8_quantize(tokens, rows=sort_token_idx)``), w ``[E, N, K]``, w_scales
+    ``[E, ceil(N/128), ceil(K/128)]``, ``expert_offsets`` int32 ``[E + 1]`` from ``moe_sort``; out ``[rows, N]``, bf16 by default.  Rows that
+    no expert owns keep what ``out`` holds there."""
+    return _native.fp8_gather_mm(x, w, w_scales, expert_offsets, x_scales, _out_dtype(out_dtype), out, ctx)
+
+
+# ---- the training side of the router ---------------------------------------------------------------------------------------
+def moe_balance(logits, topk_idx, coef: float = 1.0, mask=None, ctx: Context = None):
+    """The balance loss of a router over the rows that ``mask`` (bool ``[rows]``) keeps: (loss float32 ``[]``, counts int32 ``[E]``, mean_probs
+    float32 ``[E]``, n_counted int32 ``[]``).
+
+    With p = softmax(logits), n rows kept and c_e slots of ``topk_idx [rows, k]`` that name expert e:
+    ``loss = coef * E * sum_e c_e / (n k) * mean_t p_te``.  Uniform routing gives ``coef``; no rows give 0."""
+    return _native.moe_balance(logits, topk_idx, coef, mask, ctx)
+
+
+def moe_balance_grad(logits, counts, n_counted, k: int, grad_loss=None, coef: float = 1.0, mask=None, out=None, ctx: Context = None):
+    """The gradient of the logits, ``[rows, E]`` in their type, from what ``moe_balance`` returned: ``grad_loss * coef * E / n * p_te *
+    (f_e - sum_j f_j p_tj)`` with ``f = counts / (n k)`` constant; zeros for masked rows.  ``grad_loss``: one float32 on the device (None: 1).
+    Where several ranks share a batch, add up their ``counts`` and ``n_counted`` first: the gradient is then that of the common loss."""
+    return _native.moe_balance_grad(logits, counts, n_counted, k, grad_loss, coef, mask, out, ctx)
