@@ -55,6 +55,9 @@ cudaError_t launch_fp8_quantize(Ctx *ctx, cudaStream_t st, const void *x, const 
                                 long long n_rows, long long n_src_rows, int K, int block_rows, int pow2, int dt);
 cudaError_t launch_fp8_mm_generic(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets,
                                   void *out, int M, int N, int K, int n_experts, int out_dt);
+bool fp8_tile_supported(int M, int N, int K, const void *x, const void *w);
+cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,
+                            int M, int N, int K, int n_experts, int out_dt, std::string *why);
 size_t moe_balance_workspace(int sms, int n_rows, int n_experts);
 cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float coef, float *loss,
                                int *counts, float *mean_probs, int *n_counted, int n_rows, int n_experts, int k, int dt, void *workspace);

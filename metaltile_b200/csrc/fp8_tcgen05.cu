@@ -1,0 +1,422 @@
+// Products of e4m3 codes with block scales on tcgen05, for few tokens a tile (dense: fp8_mm; grouped by expert: fp8_gather_mm):
+//
+//   out[t, n] = sum_b xs[t, b] * ws[n / 128, b] * D_b[n, t],      D_b[n, t] = sum_{k in block b} w[n, k] * x[t, k]
+//
+// An item is 128 weight rows x up to TN tokens x a slice of K.  Its weight rows share ws, so a block of 128 codes is one MMA chain (four steps of K = 32,
+// kind::f8f6f4) into an accumulator of its own in tensor memory, which the epilogue takes out, multiplies by xs * ws and adds up in registers: lane = weight
+// row, register = token.  The products and block sums are the tensor core's (codes have 4 bits, their products are exact), the sums over blocks f32.
+//
+// Bound by reading the weights once: a block of an item is 16 KB of them, 700 cycles of an SM's share of the memory's rate, against 128 to 256 cycles of MMAs and
+// about as many of epilogue.  So the ring is what matters: two CTAs an SM with some 100 KB of stages each, one CTA an item; few tokens and few rows of
+// weights: K is cut into up to 8 slices, the CTAs of a cluster, which add up through shared memory in the order of K.
+//
+//   warps 0-3  epilogue   factors of a few dozen blocks at a time into shared memory, accumulators out, sums, stores
+//   warp 4     producer   TMA: 128 x 128 codes of the weights, TN x 128 of the tokens, a stage
+//   warp 5     MMA        and the tensor memory's allocation
+// Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited (bounded too).
+#include <cstddef>
+
+#include "fp8.cuh"
+#include "tcgen05.cuh"
+
+namespace mtc {
+namespace {
+
+using namespace fp8;
+
+constexpr int kRows = 128;                       // weight rows of an item: TMEM lanes, MMA M; they share their scales
+constexpr int kWBytes = kRows * kBlock;          // of a stage
+constexpr int kMaxStages = 8;
+constexpr int kMaxSlices = 8;
+
+template <int TN>
+struct Form {
+    static constexpr int kGroups = TN == 128 ? 2 : 1;                // of four epilogue warps; each takes its part of the columns
+    static constexpr int kPart = TN / kGroups;
+    static constexpr int kEpi = 128 * kGroups, kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kThreads = kEpi + 64;
+    static constexpr int kPerSM = TN == 128 ? 1 : 2;                 // CTAs an SM, by shared memory and registers
+    static constexpr int kSmemBytes = kPerSM == 1 ? 226 * 1024 : 113 * 1024;
+    static constexpr int kAcc = 4;                                   // accumulators in tensor memory
+    static constexpr int kCols = kAcc * TN;
+    static constexpr int kHeld = 32;                                 // blocks whose factors are in shared memory
+    static constexpr int kPitch = TN + 4;
+    static constexpr int kStage = kWBytes + TN * kBlock;
+    static constexpr int kRing = 1024 + (kHeld * kPitch * 4 + 1023) / 1024 * 1024;       // where the stages start
+    static constexpr int kStages = (kSmemBytes - 1024 - kRing) / kStage;
+    static_assert(kStages >= 2 && kStages <= kMaxStages, "stages");
+    static_assert(kStages * kStage >= TN * kRows * 4, "the sums of a slice go where the ring was");
+};
+
+struct TArgs {
+    const float *xs, *ws;
+    const uint32_t *expert_offsets;              // nullptr: dense
+    void *out;
+    uint32_t *status;
+    int M, N, nkb, n_experts;
+    int tiles;                                   // of 128 weight rows
+    int chunks;                                  // dense: of TN tokens
+    int slices;
+    int out_dt;
+    int early;                                   // weights may be requested before the previous kernel is complete
+};
+struct TMaps {
+    CUtensorMap w, x;
+};
+
+struct __align__(16) TCtrl {
+    uint64_t full[kMaxStages], empty[kMaxStages], d_full[4], d_empty[4], drained;
+    uint32_t tmem_base, issued;
+    volatile uint32_t abort;
+    int expert, tok0, ntok;
+};
+static_assert(sizeof(TCtrl) <= 1024, "control block");
+
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// acc += d * f, both halves of a pair
+__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t d0, uint32_t d1, float f0, float f1) {
+    uint64_t d, f;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(f) : "f"(f0), "f"(f1));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(f));
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+
+// The chunk with this index among the chunks of all experts, by one warp: expert e with r rows has ceil(r / TN).  Offsets that run backwards or past the rows are
+// clamped and reported.
+__device__ __forceinline__ void find_chunk(const uint32_t *offsets, int n_experts, int m_total, int TN, int want, uint32_t *status, bool report, int &expert, int &tok0,
+                                           int &ntok) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    expert = tok0 = ntok = 0;
+    for (int e0 = 0; e0 < n_experts; e0 += 32) {
+        const int e = e0 + lane;
+        int lo = 0, hi = 0;
+        if (e < n_experts) {
+            const uint32_t a = offsets[e], b = offsets[e + 1], m = static_cast<uint32_t>(m_total);
+            lo = static_cast<int>(min(a, m));
+            hi = max(lo, static_cast<int>(min(b, m)));
+            if (report && (a > m || b > m || b < a)) atomicCAS(status, 0u, 0x901u);
+        }
+        const int np = (hi - lo + TN - 1) / TN;
+        int upto = np;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        const int mine = want - before - (upto - np);                // index of the wanted chunk among this expert's
+        const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0 && mine < np);
+        if (has) {
+            const int src = __ffs(has) - 1;
+            expert = e0 + src;
+            tok0 = __shfl_sync(0xffffffffu, lo + mine * TN, src);
+            ntok = min(TN, __shfl_sync(0xffffffffu, hi, src) - tok0);
+            if (!report) return;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
+// Giving up, once every role has ended: lets what is on its way arrive before the CTA tears down.
+__device__ __noinline__ void rest(TCtrl *ctl, int stages, int load_warp) {
+    const int warp = threadIdx.x >> 5;
+    if (warp == load_warp + 1 && elect_one()) {
+        umma_commit(&ctl->drained);
+        drain_ring(&ctl->drained, 1, 1);
+    } else if (warp == load_warp && (threadIdx.x & 31) == 0) {
+        drain_ring(ctl->full, ctl->issued, stages);
+    }
+    __syncthreads();
+}
+
+template <int TN>
+__global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
+    using F = Form<TN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    TCtrl *const ctl = reinterpret_cast<TCtrl *>(smem);
+    float *const factors = reinterpret_cast<float *>(smem + 1024);   // [kHeld][kPitch]
+    const uint32_t ring = smem_u32(smem) + F::kRing;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(blockIdx.x % a.slices), unit = static_cast<int>(blockIdx.x / a.slices);
+    const int kb0 = static_cast<int>(static_cast<long long>(a.nkb) * rank / a.slices), kb1 = static_cast<int>(static_cast<long long>(a.nkb) * (rank + 1) / a.slices);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < F::kStages; ++s) {
+            mbar_init(&ctl->full[s], 1);
+            mbar_init(&ctl->empty[s], 1);
+        }
+        for (int s = 0; s < F::kAcc; ++s) {
+            mbar_init(&ctl->d_full[s], 1);
+            mbar_init(&ctl->d_empty[s], F::kEpi / 32);
+        }
+        mbar_init(&ctl->drained, 1);
+        ctl->abort = 0;
+        ctl->issued = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == F::kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "n"(F::kCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    int tile, expert = 0, tok0, ntok;
+    bool waited = false;
+    if (a.expert_offsets) {
+        pdl_enter();
+        waited = true;
+        tile = unit % a.tiles;
+        if (warp == F::kLoadWarp) {
+            find_chunk(a.expert_offsets, a.n_experts, a.M, TN, unit / a.tiles, a.status, blockIdx.x == 0, expert, tok0, ntok);
+            if (lane == 0) {
+                ctl->expert = expert;
+                ctl->tok0 = tok0;
+                ctl->ntok = ntok;
+            }
+        }
+    } else {
+        tile = unit / a.chunks;
+        tok0 = unit % a.chunks * TN;
+        ntok = min(TN, a.M - tok0);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (a.expert_offsets) {
+        expert = ctl->expert;
+        tok0 = ctl->tok0;
+        ntok = ctl->ntok;
+    }
+    const uint32_t tmem = ctl->tmem_base;
+    const int n0 = tile * kRows;
+    uint64_t acc[F::kPart / 2] = {};
+    const int part0 = F::kGroups == 1 ? 0 : warp / 4 * F::kPart;     // first column (token) of this warp's part
+
+    if (ntok > 0) {
+        if (warp == F::kLoadWarp) {
+            if (lane == 0) {
+                const int row = static_cast<int>(static_cast<long long>(expert) * a.N) + n0;
+                int ahead = 0;
+                if (!waited) {
+                    if (a.early) {
+                        asm volatile("griddepcontrol.launch_dependents;");
+                        for (int kb = kb0; kb < kb1 && ahead < F::kStages; ++kb, ++ahead) {
+                            mbar_expect_tx(&ctl->full[ahead], F::kStage);
+                            tma_load_2d(ring + ahead * F::kStage, &maps.w, kb * kBlock, row, &ctl->full[ahead]);
+                        }
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                    } else {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                        asm volatile("griddepcontrol.launch_dependents;");
+                    }
+                }
+                int s = 0;
+                uint32_t phase = 1;              // of `empty`: the first round passes
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const bool requested = kb - kb0 < ahead;
+                    if (!requested && kb - kb0 >= F::kStages && !mbar_wait(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u)) break;
+                    const uint32_t at = ring + s * F::kStage;
+                    if (!requested) {
+                        mbar_expect_tx(&ctl->full[s], F::kStage);
+                        tma_load_2d(at, &maps.w, kb * kBlock, row, &ctl->full[s]);
+                    }
+                    tma_load_2d(at + kWBytes, &maps.x, kb * kBlock, tok0, &ctl->full[s]);
+                    ++ctl->issued;
+                    if (++s == F::kStages) s = 0, phase ^= 1;
+                }
+            }
+        } else if (warp == F::kMmaWarp) {
+            constexpr uint32_t idesc = 1u << 4 | static_cast<uint32_t>(TN >> 3) << 17 | static_cast<uint32_t>(kRows >> 4) << 24;
+            int s = 0, d = 0;
+            uint32_t phase = 0, d_phase = 1;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_vote(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u)) break;
+                if (!mbar_wait_vote(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_f8(tmem + d * TN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
+                    umma_commit(&ctl->empty[s]);
+                    umma_commit(&ctl->d_full[d]);
+                }
+                __syncwarp();
+                if (++s == F::kStages) s = 0, phase ^= 1;
+                if (++d == F::kAcc) d = 0, d_phase ^= 1;
+            }
+        } else {
+            if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+            const float *const xs = a.xs + static_cast<size_t>(tok0) * a.nkb;
+            const float *const ws = a.ws + (static_cast<size_t>(expert) * a.tiles + tile) * a.nkb;
+            const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + part0;      // lane 32 * warp in bits 16 and up
+            int d = 0, held = 0;
+            uint32_t phase = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (kb == kb0 + held) {                  // the next blocks' factors
+                    if (held) asm volatile("bar.sync 1, %0;" ::"n"(F::kEpi) : "memory");
+                    const int here = min(F::kHeld, kb1 - kb);
+                    for (int i = threadIdx.x; i < F::kHeld * TN; i += F::kEpi) {
+                        const int t = i / F::kHeld, b = i % F::kHeld;
+                        factors[b * F::kPitch + t] = t < ntok && b < here ? xs[static_cast<size_t>(t) * a.nkb + kb + b] * __ldg(ws + kb + b) : 0.0f;
+                    }
+                    held += F::kHeld;
+                    asm volatile("bar.sync 1, %0;" ::"n"(F::kEpi) : "memory");
+                }
+                mbar_wait(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);      // (giving up, the warps go on to the end: they meet at barriers)
+                __syncwarp();
+                tc_fence_after();
+                const float *const f = factors + (kb - kb0) % F::kHeld * F::kPitch + part0;
+                constexpr int STEP = TN < 32 ? TN : 32;
+#pragma unroll
+                for (int c = 0; c < F::kPart; c += STEP) {
+                    uint32_t v[STEP];
+                    tmem_ld<STEP>(lanes + d * TN + c, v);
+                    tmem_wait_ld();
+                    if (c + STEP == F::kPart) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&ctl->d_empty[d]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < STEP; i += 4) {
+                        const float4 q = *reinterpret_cast<const float4 *>(f + c + i);
+                        fma2(acc[(c + i) / 2], v[i], v[i + 1], q.x, q.y);
+                        fma2(acc[(c + i) / 2 + 1], v[i + 2], v[i + 3], q.z, q.w);
+                    }
+                }
+                if (++d == F::kAcc) d = 0, phase ^= 1;
+            }
+        }
+    }
+    __syncthreads();
+    if (ctl->abort) rest(ctl, F::kStages, F::kLoadWarp);
+
+    const bool store = ntok > 0 && warp < F::kLoadWarp && !ctl->abort;
+    const int r = threadIdx.x & (kRows - 1), n = n0 + r;
+    if (a.slices == 1) {
+        if (store && n < a.N) {
+#pragma unroll
+            for (int i = 0; i < F::kPart; i += 2) {
+                const float2 v = halves(acc[i / 2]);
+                const int t = part0 + i;
+                if (t < ntok) st_from_f32(a.out, static_cast<size_t>(tok0 + t) * a.N + n, v.x, a.out_dt);
+                if (t + 1 < ntok) st_from_f32(a.out, static_cast<size_t>(tok0 + t + 1) * a.N + n, v.y, a.out_dt);
+            }
+        }
+    } else {
+        // every slice's sums into its shared memory [token][weight row]; slice r adds up tokens r, r + slices, ...
+        if (warp < F::kLoadWarp) {
+#pragma unroll
+            for (int i = 0; i < F::kPart; i += 2) {
+                const float2 v = halves(acc[i / 2]);
+                const int t = part0 + i;
+                if (t < ntok) st_shared(ring + (t * kRows + r) * 4, v.x);
+                if (t + 1 < ntok) st_shared(ring + ((t + 1) * kRows + r) * 4, v.y);
+            }
+        }
+        cluster_sync();
+        if (store && n < a.N) {
+            for (int t = rank + (warp / 4) * a.slices; t < ntok; t += F::kGroups * a.slices) {
+                float part[kMaxSlices], sum = 0.0f;
+#pragma unroll
+                for (int q = 0; q < kMaxSlices; ++q) part[q] = q < a.slices ? ld_cluster(ring + (t * kRows + r) * 4, q) : 0.0f;
+#pragma unroll
+                for (int q = 0; q < kMaxSlices; ++q)
+                    if (q < a.slices) sum += part[q];
+                st_from_f32(a.out, static_cast<size_t>(tok0 + t) * a.N + n, sum, a.out_dt);
+            }
+        }
+        cluster_sync();                          // no CTA leaves while its sums are read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == F::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kCols));
+}
+
+template <int TN>
+cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w, TArgs a, int K, std::string *why) {
+    TMaps maps;
+    cudaError_t e = make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, static_cast<long long>(a.n_experts) * a.N, K, kRows, kBlock, why);
+    if (e == cudaSuccess) e = make_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, a.M, K, TN, kBlock, why);
+    if (e != cudaSuccess) return e;
+    static PerDeviceAttr attr;
+    if ((e = attr.set(fp8_tile_kernel<TN>, Form<TN>::kSmemBytes)) != cudaSuccess) return e;
+    const long long units = a.expert_offsets ? (static_cast<long long>(std::min(a.M, a.n_experts)) + a.M / TN) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
+    if (units * a.slices > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(units * a.slices));
+    cfg.blockDim = dim3(Form<TN>::kThreads);
+    cfg.dynamicSmemBytes = Form<TN>::kSmemBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = static_cast<unsigned>(a.slices);
+    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, fp8_tile_kernel<TN>, maps, a);
+}
+
+}  // namespace
+
+// K slices: as many as fill the SMs' places once, at least four blocks each
+static int slices_for(int sms, long long units, int nkb) {
+    int s = 1;
+    while (s < kMaxSlices && units * (s + 1) <= 2ll * sms && nkb / (s + 1) >= 4) ++s;
+    return s;
+}
+
+bool fp8_tile_supported(int M, int N, int K, const void *x, const void *w) {
+    return M > 0 && N > 0 && K % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+}
+
+cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,
+                            int M, int N, int K, int n_experts, int out_dt, std::string *why) {
+    TArgs a{};
+    a.xs = xs;
+    a.ws = ws;
+    a.expert_offsets = expert_offsets;
+    a.out = out;
+    a.status = ctx->d_status;
+    a.M = M;
+    a.N = N;
+    a.nkb = blocks(K);
+    a.n_experts = n_experts;
+    a.tiles = blocks(N);
+    a.out_dt = out_dt;
+    const int rows = expert_offsets ? (M + n_experts - 1) / n_experts * 2 : M;       // that a tile may have to hold
+    const int TN = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    a.chunks = (M + TN - 1) / TN;
+    const long long units = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
+    a.slices = slices_for(ctx->sm_count, units, a.nkb);
+    a.early = expert_offsets ? 0 : early_weights(ctx, st);
+    switch (TN) {
+        case 16: return launch<16>(ctx, st, x, w, a, K, why);
+        case 32: return launch<32>(ctx, st, x, w, a, K, why);
+        case 64: return launch<64>(ctx, st, x, w, a, K, why);
+        default: return launch<128>(ctx, st, x, w, a, K, why);
+    }
+}
+
+}  // namespace mtc

@@ -1486,8 +1486,22 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
         if (rows && n_src_rows == 0) return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: an index into no rows");
         MTC_CUDA(ctx, mtc::launch_fp8_quantize(ctx, static_cast<cudaStream_t>(stream), x, static_cast<const uint32_t *>(rows), static_cast<uint8_t *>(codes),
                                                static_cast<float *>(scales), n_mats, n_rows, n_src_rows, K, block_rows, pow2, dtype), MTC_ERR_DISPATCH);
+        if (block_rows != 1) mtc::weights_written(ctx, static_cast<cudaStream_t>(stream));
         return MTC_OK;
     });
+}
+
+static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_t *x, const float *xs, const void *w, const void *ws, const void *expert_offsets, void *out,
+                       int M, int N, int K, int n_experts, int out_dtype) {
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const uint8_t *const codes = static_cast<const uint8_t *>(w);
+    const float *const scales = static_cast<const float *>(ws);
+    const uint32_t *const offsets = static_cast<const uint32_t *>(expert_offsets);
+    std::string why;
+    const cudaError_t e = mtc::fp8_tile_supported(M, N, K, x, w) ? mtc::launch_fp8_tile(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype, &why)
+                                                                 : mtc::launch_fp8_mm_generic(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype);
+    if (e != cudaSuccess) return fail(ctx, MTC_ERR_DISPATCH, std::string(who) + " launch: " + (why.empty() ? std::string(cudaGetErrorString(e)) : why));
+    return MTC_OK;
 }
 
 size_t mtc_fp8_mm_workspace(const mtc_ctx *ctx, int M, int N, int K, int x_dtype, int out_dtype) {
@@ -1519,9 +1533,7 @@ int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, 
             codes = c;
             scales = s;
         }
-        MTC_CUDA(ctx, mtc::launch_fp8_mm_generic(ctx, static_cast<cudaStream_t>(stream), codes, scales, static_cast<const uint8_t *>(w),
-                                                 static_cast<const float *>(w_scales), nullptr, out, M, N, K, 1, out_dtype), MTC_ERR_DISPATCH);
-        return MTC_OK;
+        return fp8_product(ctx, "fp8_mm", stream, codes, scales, w, w_scales, nullptr, out, M, N, K, 1, out_dtype);
     });
 }
 
@@ -1546,10 +1558,8 @@ int mtc_fp8_gather_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_s
         int rc = check_workspace(ctx, "fp8_gather_mm", workspace, workspace_bytes,
                                  mtc_fp8_gather_mm_workspace(ctx, m_total, n_out, k_in, n_experts, out_dtype));
         if (rc != MTC_OK) return rc;
-        MTC_CUDA(ctx, mtc::launch_fp8_mm_generic(ctx, static_cast<cudaStream_t>(stream), static_cast<const uint8_t *>(x), static_cast<const float *>(x_scales),
-                                                 static_cast<const uint8_t *>(w), static_cast<const float *>(w_scales),
-                                                 static_cast<const uint32_t *>(expert_offsets), out, m_total, n_out, k_in, n_experts, out_dtype), MTC_ERR_DISPATCH);
-        return MTC_OK;
+        return fp8_product(ctx, "fp8_gather_mm", stream, static_cast<const uint8_t *>(x), static_cast<const float *>(x_scales), w, w_scales, expert_offsets, out,
+                           m_total, n_out, k_in, n_experts, out_dtype);
     });
 }
 
