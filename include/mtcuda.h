@@ -310,6 +310,8 @@ int mtc_peer_barrier(mtc_ctx *ctx, void *stream, void *const *peer_flags, int n_
  *                      safe; a caller whose own previous kernel on the stream WRITES weights (an on-stream repack or copy of
  *                      the shard) must set this to 0 or synchronise first.  x and every store always wait.  The grouped
  *                      products, the codec and the M = 1 MoE tail wait for everything.
+ *   "fp8_kernel"       0 (default): the products of e4m3 codes pick their kernel by shape; 1 CUDA cores, 2 tiles of 128 weight rows
+ *                      (csrc/fp8_tcgen05.cu), 3 pairs of CTAs (csrc/fp8_pair.cu) wherever that kernel takes the arguments
  *   "peer_poll_limit"  polls of a wait on another GPU (mtc_peer_barrier, mtc_qmv_batched_sync) before it gives up
  *                      and records 0x601 + rank in the status word (default 4194304)
  * Scratch blocks.  mtc_qmm and mtc_qmm_multi (bf16: staged activations; both types: the partial sums of a launch that cuts K into

@@ -70,6 +70,7 @@ struct Ctx {
     void *d_ksplit = nullptr;      // tcgen05 qmm with K slices: the f32 partial sums of a launch (grow-only)
     size_t ksplit_bytes = 0;
     int qmm_ksplit = 1;            // option "qmm_ksplit": 0 = a dense launch with few weight-row tiles never cuts K into slices
+    int fp8_kernel = 0;            // option "fp8_kernel": 0 = by shape, 1 CUDA cores, 2 tiles, 3 pairs where they take the shape
     int qmv_small_m_tc = 1;        // option "qmv_small_m_tc": 0 = M <= 16 never takes the tcgen05 kernel; 2 = whenever it supports the shape (M >= 2)
     void *d_flush = nullptr;       // mtc_measure with cold_l2: a block larger than L2 that a memset rewrites between timed launches
     size_t flush_bytes = 0;

@@ -48,6 +48,22 @@ __device__ __forceinline__ float code_quotient(float x, float s, float inv) {
     return fabsf(x) < INFINITY ? r : __int_as_float(0x7FC00000);        // infinities have no code: NaN, as NaN is
 }
 
+// acc += d * f, both halves of a pair
+__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t d0, uint32_t d1, float f0, float f1) {
+    uint64_t d, f;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(f) : "f"(f0), "f"(f1));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(f));
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 }  // namespace fp8
 
 // Launchers
@@ -57,6 +73,9 @@ cudaError_t launch_fp8_mm_generic(Ctx *ctx, cudaStream_t st, const uint8_t *x, c
                                   void *out, int M, int N, int K, int n_experts, int out_dt);
 bool fp8_tile_supported(int M, int N, int K, const void *x, const void *w);
 cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,
+                            int M, int N, int K, int n_experts, int out_dt, std::string *why);
+bool fp8_pair_supported(int M, int N, int K, int n_experts, const void *x, const void *w);
+cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,
                             int M, int N, int K, int n_experts, int out_dt, std::string *why);
 size_t moe_balance_workspace(int sms, int n_rows, int n_experts);
 cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float coef, float *loss,

@@ -1183,6 +1183,11 @@ int mtc_set_option(mtc_ctx *ctx, const char *name, int value) {
         ctx->qmm_ksplit = value ? 1 : 0;
         return MTC_OK;
     }
+    if (std::strcmp(name, "fp8_kernel") == 0) {
+        if (value < 0 || value > 3) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_kernel must be 0 to 3");
+        ctx->fp8_kernel = value;
+        return MTC_OK;
+    }
     if (std::strcmp(name, "qmv_small_m_tc") == 0) {
         ctx->qmv_small_m_tc = value < 0 ? 0 : (value > 2 ? 2 : value);
         return MTC_OK;
@@ -1491,6 +1496,15 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
     });
 }
 
+enum Fp8Kernel { FP8_CUDA_CORE, FP8_TILE, FP8_PAIR };
+static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_experts, bool grouped, const void *x, const void *w) {
+    const int forced = ctx ? ctx->fp8_kernel : 0;
+    if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, x, w)) return FP8_CUDA_CORE;
+    const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
+    if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
+    return pair && (grouped ? M / n_experts >= 96 : M >= 256) ? FP8_PAIR : FP8_TILE;
+}
+
 static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_t *x, const float *xs, const void *w, const void *ws, const void *expert_offsets, void *out,
                        int M, int N, int K, int n_experts, int out_dtype) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1498,8 +1512,12 @@ static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_
     const float *const scales = static_cast<const float *>(ws);
     const uint32_t *const offsets = static_cast<const uint32_t *>(expert_offsets);
     std::string why;
-    const cudaError_t e = mtc::fp8_tile_supported(M, N, K, x, w) ? mtc::launch_fp8_tile(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype, &why)
-                                                                 : mtc::launch_fp8_mm_generic(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype);
+    cudaError_t e;
+    switch (fp8_kernel_for(ctx, M, N, K, n_experts, expert_offsets != nullptr, x, w)) {
+        case FP8_PAIR: e = mtc::launch_fp8_pair(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype, &why); break;
+        case FP8_TILE: e = mtc::launch_fp8_tile(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype, &why); break;
+        default: e = mtc::launch_fp8_mm_generic(ctx, st, x, xs, codes, scales, offsets, out, M, N, K, n_experts, out_dtype);
+    }
     if (e != cudaSuccess) return fail(ctx, MTC_ERR_DISPATCH, std::string(who) + " launch: " + (why.empty() ? std::string(cudaGetErrorString(e)) : why));
     return MTC_OK;
 }

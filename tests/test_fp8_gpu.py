@@ -41,6 +41,15 @@ def _same_codes(codes, want):
     assert not bad.any(), (int(bad.sum()), got[bad][:4], want[bad][:4])
 
 
+@pytest.fixture(params=[0, 2, 3], ids=["by shape", "tiles", "pairs"])
+def kernel(request):
+    """The products by each of their kernels, wherever it takes the shape."""
+    from metaltile_b200 import ops
+    ops.context(0).set_option("fp8_kernel", request.param)
+    yield request.param
+    ops.context(0).set_option("fp8_kernel", 0)
+
+
 # ---- the quantizer ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("pow2", [False, True])
@@ -142,7 +151,7 @@ SHAPES = [(1, 1, 1), (1, 5, 16), (2, 128, 128), (3, 129, 130), (1, 300, 4096), (
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_mm(m, n, k, dt):
+def test_mm(m, n, k, dt, kernel):
     from metaltile_b200 import ops
     x, xs, w, ws = _operands(m, n, k, m + n + k)
     out = ops.fp8_mm(x, w, ws, x_scales=xs, out_dtype=TYPES[dt])
@@ -203,7 +212,7 @@ def test_mm_operands_that_start_anywhere(m, by):
 
 
 @pytest.mark.parametrize("m", [1, 9, 40, 300])
-def test_mm_special_values(m):
+def test_mm_special_values(m, kernel):
     """NaN codes and scales reach their rows and columns and no others; zeros and scales far apart are as the definition has them."""
     from metaltile_b200 import ops
     x, xs, w, ws = _operands(m, 300, 400, 11)
@@ -240,7 +249,7 @@ def _check_groups(out, x, xs, w, ws, off, untouched):
     ([16, 17, 15, 1, 33], 384, 1024, 1, 0), ([0, 0, 0], 64, 64, 0, 4), ([300, 20], 1000, 130, 0, 0), ([64, 65, 63, 128, 129, 127, 32, 31, 33], 257, 512, 0, 1),
     ([1000, 1, 0, 600], 512, 640, 3, 2),
 ])
-def test_gather(counts, n, k, lead, tail, dt):
+def test_gather(counts, n, k, lead, tail, dt, kernel):
     from metaltile_b200 import ops
     m = sum(counts) + lead + tail
     x, xs, w, ws = _operands(m, n, k, m + n, experts=len(counts))
@@ -264,7 +273,7 @@ def test_gather_nothing_and_defaults():
 
 
 @pytest.mark.parametrize("off", [[0, 3, 2, 6], [0, 2, 4, 9], [0, -1, 3, 6]])
-def test_gather_offsets_that_make_no_sense_are_reported(off):
+def test_gather_offsets_that_make_no_sense_are_reported(off, kernel):
     """Nothing outside the rows is read or written; the rows of ranges that hold are right."""
     from metaltile_b200 import ops
     ctx = ops.context(0)
@@ -280,7 +289,7 @@ def test_gather_offsets_that_make_no_sense_are_reported(off):
 
 # ---- streams, graphs, threads --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (40, 512, 2880), (300, 384, 1024)])
-def test_mm_on_another_stream_and_in_graphs(m, n, k):
+def test_mm_on_another_stream_and_in_graphs(m, n, k, kernel):
     """Two captured graphs replay in turn and at once with new inputs, each with its own workspace."""
     from metaltile_b200 import ops
     x = [_x(m, k, "bf16", i) for i in range(4)]
