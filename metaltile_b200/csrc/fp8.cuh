@@ -48,22 +48,6 @@ __device__ __forceinline__ float code_quotient(float x, float s, float inv) {
     return fabsf(x) < INFINITY ? r : __int_as_float(0x7FC00000);        // infinities have no code: NaN, as NaN is
 }
 
-// acc += d * f, both halves of a pair
-__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t d0, uint32_t d1, float f0, float f1) {
-    uint64_t d, f;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
-    asm("mov.b64 %0, {%1, %2};" : "=l"(f) : "f"(f0), "f"(f1));
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(f));
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 }  // namespace fp8
 
 // Launchers

@@ -3,25 +3,28 @@
 //   out[t, n] = sum_b xs[t, b] * ws[n / 128, b] * D_b[t, n],      D_b[t, n] = sum_{k in block b} x[t, k] * w[n, k]
 //
 // A pair of CTAs (a cluster of two SMs) owns a tile of 256 tokens x 256 weight rows: each SM holds 128 tokens of A and half of the weight rows of B, and the MMAs
-// (cta_group::2, 256 x 128, kind::f8f6f4) read both.  A block of 128 codes is a chain of four of them for each half of the weight rows, into an accumulator of its own in
-// tensor memory; a half is one block of scales.  The epilogue takes the accumulators out, multiplies by xs * ws, one number a thread (lane = token), and adds up in
-// registers: 128 sums a thread, eight warps.
+// (cta_group::2, 256 x 256, kind::f8f6f4) read both.  A block of 128 codes is a chain of four of them into an accumulator of its own in tensor memory.  The epilogue takes
+// it out, multiplies by xs * ws, one number a thread (lane = token, and a warp's 128 columns share their ws), and adds up in registers: 128 sums a thread, eight warps.
 //
-// Bound by what an SM can take in.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM of a
-// pair: 64 bytes a cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Out of tensor memory and into the sums is 256 cycles
-// of the FMA pipes.  The four accumulators are all of the tensor memory, two blocks deep, so the MMAs of a block run while the one before is read.
+// What bounds it.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM of a pair: 64 bytes a
+// cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Without the epilogue the ring and the MMAs run at 585 cycles a block.  With it a
+// block takes 860: 64 packed FMAs, as many moves and four loads of tensor memory in a row in each of eight warps.  Two accumulators are all of the tensor memory, so the
+// MMAs of one block run while the one before is read, no further.  2048 x 28672 x 4096: 226 us, 2.1 PFLOP/s.
+//
+// Steps on the way (us for that case): hand-offs that release at cluster scope 587, relaxed ones 348; one try in front of the polling loop, whose entry costs 200 cycles,
+// and results out by TMA instead of a row a lane 303; the registers of the other roles for the epilogue, so that nothing spills, and the next columns loaded while the
+// last are added 235; MMAs of 256 columns instead of two chains of 128, which read A twice, 226.  16 epilogue warps of 64 columns: 297 (104 registers each spill).
 //
 //   warps 0-7    epilogue   warps 0-3 the first half of the weight rows, 4-7 the second
-//   warps 8-9    scales     xs of 128 tokens, 16 blocks at a time, turned round into shared memory (a load of each lane's own row would cost
-//                           the load pipe ten cycles a lane), and ws
+//   warps 8-9    scales     xs of 128 tokens, 16 blocks at a time, and ws, by cp.async into shared memory (a load of each lane's own row would cost the load pipe ten
+//                           cycles a lane)
 //   warp 10      producer   TMA, both CTAs of a pair into their own memory, one barrier in the first
 //   warp 11      MMA        issued by the first CTA
 // A persistent pair walks the tiles, tokens fastest.  Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave and what is in
 // flight is awaited (bounded too).
 #include <cstddef>
 
-#include "fp8.cuh"
-#include "tcgen05.cuh"
+#include "fp8_tc.cuh"
 
 namespace mtc {
 namespace {
@@ -29,11 +32,12 @@ namespace {
 using namespace fp8;
 
 constexpr int kTokens = 256, kCols = 256;        // of a tile; a CTA of a pair has 128 of the tokens
-constexpr int kABytes = 128 * kBlock, kBBytes = 64 * kBlock, kStage = kABytes + 2 * kBBytes;
-constexpr int kStages = 6;
+constexpr int kABytes = 128 * kBlock, kBBytes = 128 * kBlock, kStage = kABytes + kBBytes;
+constexpr int kStages = 4;                       // (five: the same)
+constexpr int kOutBytes = 4096;                  // of an epilogue warp: 32 rows x 128 bytes of results on their way out
 constexpr int kEpiWarps = 8, kScaleWarp0 = 8, kScaleWarps = 2, kLoadWarp = 10, kMmaWarp = 11, kThreads = 384;
-constexpr int kHeld = 16, kPitch = 132;          // blocks whose scales are in shared memory, floats of a block's xs
-constexpr int kScaleFloats = kHeld * kPitch + 2 * kHeld;
+constexpr int kHeld = 16, kPitch = 20;           // blocks whose scales are in shared memory, floats of a row of xs (four-float loads of 8 neighbouring rows meet no bank twice)
+constexpr int kScaleFloats = 128 * kPitch + 2 * kHeld;
 constexpr int kMaxExperts = 1024;
 
 struct PArgs {
@@ -44,13 +48,13 @@ struct PArgs {
     int M, N, nkb, n_experts;
     int col_tiles, row_blocks;                   // ceil(N / 256), ceil(N / 128)
     int out_dt;
-    int wide;                                    // rows of the output can be stored 16 bytes at a time
+    int wide;                                    // rows of the output are whole 16-byte pieces at 16-byte boundaries: `out` of the maps holds
 };
 struct PMaps {
-    CUtensorMap x, w;
+    CUtensorMap x, w, out;
 };
 struct __align__(16) PCtrl {
-    uint64_t full[kStages], empty[kStages], d_full[2][2], d_empty[2][2], s_full[2], s_empty[2], drained;
+    uint64_t full[kStages], empty[kStages], d_full[2], d_empty[2], s_full[2], s_empty[2], drained;
     uint32_t tmem_base, issued;
     volatile uint32_t abort;
     uint32_t n_chunks;
@@ -59,7 +63,7 @@ struct __align__(16) PCtrl {
 };
 constexpr int kCtlBytes = (sizeof(PCtrl) + 1023) / 1024 * 1024;
 constexpr int kScaleBytes = (2 * kScaleFloats * 4 + 1023) / 1024 * 1024;
-constexpr int kSmemBytes = 1024 + kCtlBytes + kScaleBytes + kStages * kStage;
+constexpr int kSmemBytes = 1024 + kCtlBytes + kScaleBytes + 8 * kOutBytes + kStages * kStage;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ uint32_t on_cta(uint32_t addr, uint32_t rank) {
@@ -84,8 +88,10 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
 }
+// Relaxed: what it hands over is tensor memory, ordered by the tcgen05 fence in front.  (A release at cluster scope waits for everything the thread has in flight: 1150
+// cycles a block, 2048 x 28672 x 4096 in 587 us instead of 348.)
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // The chunks of the experts, by one warp: ceil(rows / 256) each.  Offsets that run backwards or past the rows are clamped and reported.
@@ -147,30 +153,69 @@ __device__ __forceinline__ Tile tile_of(const PCtrl *ctl, const PArgs &a, int in
     return t;
 }
 
+// Sixteen bytes of neighbouring results from the sums acc[i] on: eight of 16 bits, four of 32
 template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if constexpr (DT == MTC_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&h);
+__device__ __forceinline__ uint4 piece(const uint64_t (&acc)[64], int i) {
+    uint32_t w[4];
+    if constexpr (DT == MTC_F32) {
+        const float2 lo = halves(acc[i]), hi = halves(acc[i + 1]);
+        return make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y));
     } else {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 v = halves(acc[i + j]);
+            if constexpr (DT == MTC_BF16) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(v.x, v.y);
+                w[j] = *reinterpret_cast<const uint32_t *>(&p);
+            } else {
+                const __half2 p = __floats2half2_rn(v.x, v.y);
+                w[j] = *reinterpret_cast<const uint32_t *>(&p);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
-__device__ __forceinline__ void store16(void *p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) { *static_cast<uint4 *>(p) = make_uint4(a, b, c, d); }
 
-// Eight neighbouring results of a row
+// A warp's 32 rows x 128 columns.  All rows there: through shared memory, 128 bytes a row at a time, and out by TMA, which goes on while the next tile's blocks are added
+// (a lane storing its own row costs the load pipe a cycle a row and 16 bytes: 67 us of 330 for 2048 x 28672 x 4096).  Else every lane its own row.
 template <int DT>
-__device__ __forceinline__ void store8(void *out, size_t at, const uint64_t (&acc)[64], int i) {
-    float2 v[4];
+__device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[64], uint32_t staged, int row, int rows, int n) {
+    constexpr int PER = DT == MTC_F32 ? 4 : 8;                       // results of a piece
+    const int lane = threadIdx.x & 31;
+    if (a.wide && rows >= 32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = halves(acc[i + j]);
-    if constexpr (DT == MTC_F32) {
-        float *const p = static_cast<float *>(out) + at;
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
-    } else {
-        store16(static_cast<uint16_t *>(out) + at, pack2<DT>(v[0].x, v[0].y), pack2<DT>(v[1].x, v[1].y), pack2<DT>(v[2].x, v[2].y), pack2<DT>(v[3].x, v[3].y));
+        for (int c = 0; c < 128; c += 8 * PER) {
+            if (n + c >= a.N) break;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const uint4 v = piece<DT>(acc, (c + q * PER) / 2);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                             ::"l"(reinterpret_cast<uint64_t>(&maps.out)), "r"(n + c), "r"(row), "r"(staged) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        }
+    } else if (lane < rows) {
+        const size_t at = static_cast<size_t>(row + lane) * a.N + n;
+#pragma unroll
+        for (int c = 0; c < 128; c += PER) {
+            if (n + c >= a.N) break;
+            if (a.wide) {
+                *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (at + c) * (16 / PER)) = piece<DT>(acc, c / 2);
+            } else {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const float2 v = halves(acc[(c + j) / 2]);
+                    if (n + c + j < a.N) st_from_f32(a.out, at + c + j, j & 1 ? v.y : v.x, DT);
+                }
+            }
+        }
     }
 }
 
@@ -178,8 +223,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     PCtrl *const ctl = reinterpret_cast<PCtrl *>(smem);
-    float *const scales = reinterpret_cast<float *>(smem + kCtlBytes);       // two of [kHeld][kPitch] of xs, [2][kHeld] of ws
-    const uint32_t ring = smem_u32(smem) + kCtlBytes + kScaleBytes;
+    float *const scales = reinterpret_cast<float *>(smem + kCtlBytes);       // two of [128][kPitch] of xs, [2][kHeld] of ws
+    const uint32_t staged = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + kCtlBytes + kScaleBytes, ring = staged + kEpiWarps * kOutBytes;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = static_cast<int>(blockIdx.x & 1), pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
     if (threadIdx.x == 0) {
@@ -188,11 +233,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
             mbar_init(&ctl->empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int h = 0; h < 2; ++h) {
-                mbar_init(&ctl->d_full[h][i], 1);
-                mbar_init(&ctl->d_empty[h][i], kEpiWarps);       // four warps of each CTA, in the first one's memory
-            }
-            mbar_init(&ctl->s_full[i], kScaleWarps);
+            mbar_init(&ctl->d_full[i], 1);
+            mbar_init(&ctl->d_empty[i], 2 * kEpiWarps);              // those of both CTAs, in the first one's memory
+            mbar_init(&ctl->s_full[i], 32 * kScaleWarps);
             mbar_init(&ctl->s_empty[i], kEpiWarps);
         }
         mbar_init(&ctl->drained, 1);
@@ -213,19 +256,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     tc_fence_before();
     cluster_sync();                              // both CTAs' barriers exist
     tc_fence_after();
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
     const int n_tiles = static_cast<int>(ctl->n_chunks) * a.col_tiles;
 
     if (warp == kLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (lane == 0) {
             int s = 0;
             uint32_t phase = 1;
             bool go = true;
             for (int i = pair; go && i < n_tiles; i += pairs) {
                 const Tile t = tile_of(ctl, a, i);
-                const int row = static_cast<int>(static_cast<long long>(t.expert) * a.N) + t.n0 + rank * 64;
+                const int row = static_cast<int>(static_cast<long long>(t.expert) * a.N) + t.n0 + rank * 128;
                 for (int kb = 0; kb < a.nkb; ++kb) {
-                    if (!mbar_wait(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb11u)) {
+                    if (!wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb11u)) {
                         go = false;
                         break;
                     }
@@ -233,47 +277,45 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     if (rank == 0) mbar_expect_tx(&ctl->full[s], 2 * kStage);
                     tma_load_pair(at, &maps.x, kb * kBlock, t.tok0 + rank * 128, bar);
                     tma_load_pair(at + kABytes, &maps.w, kb * kBlock, row, bar);
-                    tma_load_pair(at + kABytes + kBBytes, &maps.w, kb * kBlock, row + 128, bar);
                     ++ctl->issued;
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
             }
         }
     } else if (warp == kMmaWarp) {
-        if (rank == 0) {
-            constexpr uint32_t idesc = 1u << 4 | (128u >> 3) << 17 | (256u >> 4) << 24;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (rank == 0) {                         // the whole warp walks the loop, so that the operands of the MMAs are uniform; one thread issues
+            constexpr uint32_t idesc = 1u << 4 | (256u >> 3) << 17 | (256u >> 4) << 24;
             int s = 0, d = 0;
             uint32_t phase = 0, d_phase = 1;
             bool go = true;
             for (int i = pair; go && i < n_tiles; i += pairs)
-                for (int kb = 0; go && kb < a.nkb; ++kb) {
-                    if (!mbar_wait_vote(&ctl->full[s], phase, &ctl->abort, a.status, 0xb12u)) {
+                for (int kb = 0; kb < a.nkb; ++kb) {
+                    if (!wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb12u)) {
                         go = false;
                         break;
                     }
-                    const uint64_t xd = make_desc_sw128(ring + s * kStage);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (!mbar_wait_vote(&ctl->d_empty[h][d], d_phase, &ctl->abort, a.status, 0xb13u)) {
-                            go = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint64_t wd = make_desc_sw128(ring + s * kStage + kABytes + h * kBBytes);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mma_pair(tmem + (2 * h + d) * 128, xd + 2 * k, wd + 2 * k, idesc, k > 0);
-                            if (h == 1) commit_pair(&ctl->empty[s]);
-                            commit_pair(&ctl->d_full[h][d]);
-                        }
-                        __syncwarp();
+                    const uint64_t xd = make_desc_sw128(ring + s * kStage), wd = make_desc_sw128(ring + s * kStage + kABytes);
+                    if (!wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb13u)) {
+                        go = false;
+                        break;
                     }
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_pair(tmem + d * 256, xd + 2 * k, wd + 2 * k, idesc, k > 0);
+                        commit_pair(&ctl->d_full[d]);
+                        commit_pair(&ctl->empty[s]);
+                    }
+                    __syncwarp();
                     if (++s == kStages) s = 0, phase ^= 1;
                     if (d ^= 1; d == 0) d_phase ^= 1;
                 }
         }
     } else if (warp >= kScaleWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         const int half = warp - kScaleWarp0;     // of the CTA's 128 tokens
+        const int k = lane & (kHeld - 1), r0 = lane / kHeld;
         int b = 0;
         uint32_t phase = 1;
         bool go = true;
@@ -286,86 +328,85 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     go = false;
                     break;
                 }
-                float *const to = scales + b * kScaleFloats;
-                const int k = lane & (kHeld - 1), r0 = lane / kHeld;         // two tokens at a time, 16 blocks of each
-                const bool have = kb + k < a.nkb;
-#pragma unroll
-                for (int r = 0; r < 64; r += 32) {
-                    float v[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int tok = first + r + 2 * j + r0;
-                        v[j] = have && tok < t.ntok ? a.xs[static_cast<size_t>(t.tok0 + tok) * a.nkb + kb + k] : 0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) to[k * kPitch + half * 64 + r + 2 * j + r0] = v[j];
-                }
+                // two tokens at a time, 16 blocks of each; what does not exist is filled with zeros
+                const uint32_t to = smem_u32(scales) + (b * kScaleFloats + (half * 64 + r0) * kPitch + k) * 4;
+                const float *const from = a.xs + static_cast<size_t>(t.tok0 + first + r0) * a.nkb + kb + k;
+                const int last = kb + k < a.nkb ? t.ntok - first - r0 : 0;
+#pragma unroll 8
+                for (int r = 0; r < 64; r += 2)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * kPitch * 4), "l"(r < last ? from + static_cast<size_t>(r) * a.nkb : a.xs), "r"(r < last ? 4 : 0) : "memory");
                 if (half == 0) {
-                    const bool there = have && t.n0 / kBlock + r0 < a.row_blocks;
-                    to[kHeld * kPitch + lane] = there ? __ldg(ws + static_cast<size_t>(r0) * a.nkb + kb + k) : 0.0f;
+                    const bool there = kb + k < a.nkb && t.n0 / kBlock + r0 < a.row_blocks;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(scales) + (b * kScaleFloats + 128 * kPitch + lane) * 4),
+                                 "l"(there ? ws + static_cast<size_t>(r0) * a.nkb + kb + k : a.ws), "r"(there ? 4 : 0) : "memory");
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->s_full[b]);
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->s_full[b])) : "memory");
                 if (b ^= 1; b == 0) phase ^= 1;
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");         // 256 threads x 224 + 128 x 56 = 384 x 168 that the block starts with
         const int h = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + h * 256;
-        const uint32_t freed = on_cta(smem_u32(&ctl->d_empty[h][0]), 0);
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + h * 128;
+        const uint32_t freed = on_cta(smem_u32(&ctl->d_empty[0]), 0);
         int d = 0, b = 0;
         uint32_t phase = 0, s_phase = 0;
         for (int i = pair; i < n_tiles; i += pairs) {
             const Tile t = tile_of(ctl, a, i);
             uint64_t acc[64] = {};
-            for (int kb = 0; kb < a.nkb; ++kb) {
-                const int at = kb % kHeld;
+            uint32_t v[2][32];                   // the next columns are on their way while these are added
+            bool early = false;
+            for (int kb = 0; kb < a.nkb; kb += 4) {
+                const int at = kb % kHeld, here = min(4, a.nkb - kb);
                 const float *const held = scales + b * kScaleFloats;
-                if (at == 0) mbar_wait(&ctl->s_full[b], s_phase, &ctl->abort, a.status, 0xb15u);
-                const float f = held[at * kPitch + r] * held[kHeld * kPitch + h * kHeld + at];
-                mbar_wait(&ctl->d_full[h][d], phase, &ctl->abort, a.status, 0xb16u);
-                __syncwarp();
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t v[32];
-                    tmem_ld<32>(lanes + d * 128 + c, v);
-                    tmem_wait_ld();
-                    if (c == 96) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) arrive_at(freed + d * 8);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) fma2(acc[(c + j) / 2], v[j], v[j + 1], f, f);
-                }
-                if (d ^= 1; d == 0) phase ^= 1;
-                if (at == kHeld - 1 || kb == a.nkb - 1) {
+                if (at == 0) wait_soon(&ctl->s_full[b], s_phase, &ctl->abort, a.status, 0xb15u);
+                const float4 fx = *reinterpret_cast<const float4 *>(held + r * kPitch + at), fw = *reinterpret_cast<const float4 *>(held + 128 * kPitch + h * kHeld + at);
+                float f = fx.x * fw.x, f1 = fx.y * fw.y, f2 = fx.z * fw.z, f3 = fx.w * fw.w;
+                if (at + 4 == kHeld || kb + 4 >= a.nkb) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl->s_empty[b]);
                     if (b ^= 1; b == 0) s_phase ^= 1;
                 }
-            }
-            const int tok = rank * 128 + r, n = t.n0 + h * 128;
-            if (tok >= t.ntok || ctl->abort) continue;
-            const size_t out = static_cast<size_t>(t.tok0 + tok) * a.N + n;
-            if (a.wide) {
-#pragma unroll
-                for (int c = 0; c < 128; c += 8)
-                    if (n + c < a.N) {           // (N is a multiple of eight)
-                        if (a.out_dt == MTC_BF16) store8<MTC_BF16>(a.out, out + c, acc, c / 2);
-                        else if (a.out_dt == MTC_F16) store8<MTC_F16>(a.out, out + c, acc, c / 2);
-                        else store8<MTC_F32>(a.out, out + c, acc, c / 2);
+#pragma unroll 1
+                for (int u = 0; u < here; ++u) {
+                    if (!early) {
+                        wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb16u);
+                        __syncwarp();
+                        tc_fence_after();
+                        tmem_ld<32>(lanes + d * 256, v[0]);
                     }
-            } else {
 #pragma unroll
-                for (int c = 0; c < 128; c += 2) {
-                    const float2 v = halves(acc[c / 2]);
-                    if (n + c < a.N) st_from_f32(a.out, out + c, v.x, a.out_dt);
-                    if (n + c + 1 < a.N) st_from_f32(a.out, out + c + 1, v.y, a.out_dt);
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_wait_ld(v[c & 1]);
+                        if (c < 3) {
+                            tmem_ld<32>(lanes + d * 256 + (c + 1) * 32, v[~c & 1]);
+                        } else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) arrive_at(freed + d * 8);
+                            if (d ^= 1; d == 0) phase ^= 1;
+                            // the next block's first columns, if they are there, come while the last of this one are added
+                            early = kb + u + 1 < a.nkb && __all_sync(0xffffffffu, mbar_try(&ctl->d_full[d], phase));
+                            if (early) {
+                                tc_fence_after();
+                                tmem_ld<32>(lanes + d * 256, v[0]);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) fma2(acc[c * 16 + j / 2], v[c & 1][j], v[c & 1][j + 1], f, f);
+                    }
+                    f = f1, f1 = f2, f2 = f3;
                 }
             }
+            if (ctl->abort) continue;
+            const int first = rank * 128 + (warp & 3) * 32, rows = t.ntok - first, n = t.n0 + h * 128;
+            if (rows <= 0 || n >= a.N) continue;
+            if (a.out_dt == MTC_BF16) store_rows<MTC_BF16>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
+            else if (a.out_dt == MTC_F16) store_rows<MTC_F16>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
+            else store_rows<MTC_F32>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncthreads();
     if (ctl->abort) {                            // gave up: let what is on its way arrive (the first CTA's barriers count both CTAs' copies)
@@ -404,10 +445,13 @@ cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     a.col_tiles = (N + kCols - 1) / kCols;
     a.row_blocks = blocks(N);
     a.out_dt = out_dt;
-    a.wide = N % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    PMaps maps;
-    cudaError_t e = make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, static_cast<long long>(n_experts) * N, K, 64, kBlock, why);
+    const int size = static_cast<int>(dtype_size(out_dt));
+    a.wide = static_cast<long long>(N) * size % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    PMaps maps{};
+    cudaError_t e = make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, static_cast<long long>(n_experts) * N, K, 128, kBlock, why);
     if (e == cudaSuccess) e = make_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, M, K, 128, kBlock, why);
+    if (e == cudaSuccess && a.wide)
+        e = make_map_2d(&maps.out, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, size, out, M, N, 32, 128 / size, why);
     if (e != cudaSuccess) return e;
     static PerDeviceAttr attr;
     if ((e = attr.set(fp8_pair_kernel, kSmemBytes)) != cudaSuccess) return e;

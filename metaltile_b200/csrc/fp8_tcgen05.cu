@@ -16,8 +16,7 @@
 // Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited (bounded too).
 #include <cstddef>
 
-#include "fp8.cuh"
-#include "tcgen05.cuh"
+#include "fp8_tc.cuh"
 
 namespace mtc {
 namespace {
@@ -142,7 +141,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     TCtrl *const ctl = reinterpret_cast<TCtrl *>(smem);
     float *const factors = reinterpret_cast<float *>(smem + 1024);   // [kHeld][kPitch]
-    const uint32_t ring = smem_u32(smem) + F::kRing;
+    const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + F::kRing;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = static_cast<int>(blockIdx.x % a.slices), unit = static_cast<int>(blockIdx.x / a.slices);
     const int kb0 = static_cast<int>(static_cast<long long>(a.nkb) * rank / a.slices), kb1 = static_cast<int>(static_cast<long long>(a.nkb) * (rank + 1) / a.slices);
@@ -191,7 +190,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
         tok0 = ctl->tok0;
         ntok = ctl->ntok;
     }
-    const uint32_t tmem = ctl->tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
     const int n0 = tile * kRows;
     uint64_t acc[F::kPart / 2] = {};
     const int part0 = F::kGroups == 1 ? 0 : warp / 4 * F::kPart;     // first column (token) of this warp's part
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
                 uint32_t phase = 1;              // of `empty`: the first round passes
                 for (int kb = kb0; kb < kb1; ++kb) {
                     const bool requested = kb - kb0 < ahead;
-                    if (!requested && kb - kb0 >= F::kStages && !mbar_wait(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u)) break;
+                    if (!requested && kb - kb0 >= F::kStages && !wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u)) break;
                     const uint32_t at = ring + s * F::kStage;
                     if (!requested) {
                         mbar_expect_tx(&ctl->full[s], F::kStage);
@@ -234,15 +233,15 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
             int s = 0, d = 0;
             uint32_t phase = 0, d_phase = 1;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait_vote(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u)) break;
-                if (!mbar_wait_vote(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) break;
+                if (!wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u)) break;
+                if (!wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) break;
                 tc_fence_after();
+                const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
                 if (elect_one()) {
-                    const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) mma_f8(tmem + d * TN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
-                    umma_commit(&ctl->empty[s]);
                     umma_commit(&ctl->d_full[d]);
+                    umma_commit(&ctl->empty[s]);
                 }
                 __syncwarp();
                 if (++s == F::kStages) s = 0, phase ^= 1;
@@ -266,7 +265,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
                     held += F::kHeld;
                     asm volatile("bar.sync 1, %0;" ::"n"(F::kEpi) : "memory");
                 }
-                mbar_wait(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);      // (giving up, the warps go on to the end: they meet at barriers)
+                wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);      // (giving up, the warps go on to the end: they meet at barriers)
                 __syncwarp();
                 tc_fence_after();
                 const float *const f = factors + (kb - kb0) % F::kHeld * F::kPitch + part0;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
                 for (int c = 0; c < F::kPart; c += STEP) {
                     uint32_t v[STEP];
                     tmem_ld<STEP>(lanes + d * TN + c, v);
-                    tmem_wait_ld();
+                    tmem_wait_ld<STEP>(v);
                     if (c + STEP == F::kPart) {
                         tc_fence_before();
                         __syncwarp();
