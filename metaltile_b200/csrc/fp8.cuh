@@ -27,25 +27,37 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// The scale of a block with this largest magnitude
+// The scale of a block with this largest magnitude.  amax / 448 correctly rounded: the quotient by the rounded reciprocal, its exact remainder, and a step (all 2^23
+// mantissas agree with the division, which costs 120 instructions).
 __device__ __forceinline__ float scale_of(float amax, int pow2) {
-    float s = fmaxf(__fdiv_rn(amax, 448.0f), kLeastScale);
+    constexpr float r = 1.0f / 448.0f;
+    const float q = amax * r;
+    float s = fmaxf(fmaf(fmaf(-q, 448.0f, amax), r, q), kLeastScale);
     if (pow2) s = __uint_as_float((__float_as_uint(s) + 0x7FFFFFu) & 0xFF800000u);
     return s;
 }
+// 1 / s, within a unit or two; exact where s is a power of two (s is never subnormal, nor is this)
+__device__ __forceinline__ float inverse_of(float s) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    return r;
+}
 
-// x / s such that rounding it to a code gives the code nearest to the true quotient.  A quotient rounded to f32 first may land on the border
-// between two codes that the true one lies beside (with s = amax / 448 rounded that is one value in a few hundred, since x and amax have few bits),
-// so the quotient is rounded to odd: corrected to within one unit, its exact remainder found, and an even result moved towards the truth.  Borders
-// are even numbers, so none is hit unless the quotient is exact.  Below 2^-11 every quotient becomes zero anyway.  inv = 1 / s.
-__device__ __forceinline__ float code_quotient(float x, float s, float inv) {
-    float r = x * inv;
-    r = fmaf(fmaf(-r, s, x), inv, r);
+// x / s within a unit: one step from x * inv
+__device__ __forceinline__ float quotient(float x, float s, float inv) {
+    const float r = x * inv;
+    return fmaf(fmaf(-r, s, x), inv, r);
+}
+// ... such that rounding it to a code gives the code nearest to the true quotient.  A quotient rounded to f32 may land on the border between two codes that the true one lies
+// beside (with s = amax / 448 rounded that is one value in a few hundred, since x and amax have few bits), so it is rounded to odd: its exact remainder tells the
+// side, and an even result is moved there.  Borders are even numbers, so none is hit unless the quotient is exact.  Below 2^-11 every quotient becomes zero anyway.
+__device__ __forceinline__ float odd_quotient(float x, float s, float r) {       // r: quotient()
     const float rest = fmaf(-r, s, x);
-    uint32_t b = __float_as_uint(r);
-    if (rest != 0.0f && !(b & 1u) && fabsf(r) >= 4.8828125e-4f) b += ((rest > 0.0f) == (r > 0.0f)) ? 1u : 0xFFFFFFFFu;
-    r = __uint_as_float(b);
-    return fabsf(x) < INFINITY ? r : __int_as_float(0x7FC00000);        // infinities have no code: NaN, as NaN is
+    const uint32_t b = __float_as_uint(r), away = (__float_as_uint(rest) ^ b) >> 31;       // 1: the true one is smaller in magnitude
+    return rest != 0.0f && !(b & 1u) && fabsf(r) >= 4.8828125e-4f ? __uint_as_float(b + 1u - 2u * away) : r;
+}
+__device__ __forceinline__ float code_quotient(float x, float s, float inv) {
+    return fabsf(x) < INFINITY ? odd_quotient(x, s, quotient(x, s, inv)) : __int_as_float(0x7FC00000);        // infinities have no code: NaN, as NaN is
 }
 
 }  // namespace fp8

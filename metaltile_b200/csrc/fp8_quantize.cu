@@ -4,7 +4,9 @@
 //   s = max(max |x| / 448, 2^-90) over the finite values of the block (pow2: the least power of two that is not below)
 //   code = x / s rounded to the nearest e4m3 value, ties to even; infinities and NaN become NaN
 //
-// Bound by memory: every value is read once and stays in registers between the maximum and the codes.
+// Bound by memory: every value is read once and stays in registers, as it was read, between the maximum and the codes; sixteen lanes share a row of a
+// block, eight values a lane.  What matters beside the loads in flight is the number of instructions a value: the maximum is that of the bit patterns (two 16-bit values at
+// a time, monotone for all but NaN), and a quotient is three instructions and three that look whether it may be on a border, or one with powers of two.
 #include "fp8.cuh"
 
 namespace mtc {
@@ -12,155 +14,262 @@ namespace {
 
 using namespace fp8;
 
-// eight consecutive values of a row; `n` of them exist
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void *base, size_t at, int n, float (&v)[8]) {
-    if constexpr (VEC) {
-        if (n <= 0) {
+// Eight neighbouring values of a row as they were read
+template <int DT>
+struct Eight {
+    uint32_t w[DT == MTC_F32 ? 8 : 4];
+
+    // `n` of them exist; VEC: all or none do, and they start at a 16-byte boundary
+    template <bool VEC>
+    __device__ __forceinline__ void load(const void *base, size_t at, int n) {
+        constexpr int W = DT == MTC_F32 ? 8 : 4;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            return;
-        }
-        if constexpr (DT == MTC_F32) {
-            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-            const float4 a = p[0], b = p[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        for (int i = 0; i < W; ++i) w[i] = 0;
+        if constexpr (VEC) {
+            if (n <= 0) return;
+            const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(base) + at * (DT == MTC_F32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) {
+                const uint4 q = p[i];
+                w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+            }
         } else {
-            const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
-            const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DT == MTC_BF16) {
-                    v[2 * i] = __uint_as_float(u[i] << 16);
-                    v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-                } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                }
+            for (int i = 0; i < 8; ++i) {
+                if (i >= n) break;
+                if constexpr (DT == MTC_F32) w[i] = static_cast<const uint32_t *>(base)[at + i];
+                else w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(base)[at + i]) << (i & 1) * 16;
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? ld_written_as_f32(base, at + i, DT) : 0.0f;
     }
+    // The largest magnitude as a bit pattern (16-bit types: of either half); infinities and NaN are above all others.
+    __device__ __forceinline__ uint32_t most() const {
+        uint32_t m = 0;
+        if constexpr (DT == MTC_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        }
+        return m;
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (DT == MTC_F32) return __uint_as_float(w[i]);
+        const uint32_t u = w[i / 2];
+        if constexpr (DT == MTC_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? u >> 16 : u)));
+    }
+    // ... over the finite values only, as an f32
+    __device__ __forceinline__ float most_finite() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(value(i));
+            if (a < INFINITY) m = fmaxf(m, a);
+        }
+        return m;
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    if constexpr (DT == MTC_F32) return max(a, b);
+    else return __vmaxu2(a, b);
+}
+// of a pattern that `larger` left: is there an infinity or a NaN, and the magnitude otherwise
+template <int DT>
+__device__ __forceinline__ bool has_special(uint32_t m) {
+    if constexpr (DT == MTC_F32) return m >= 0x7F800000u;
+    else return max(m & 0xFFFFu, m >> 16) >= (DT == MTC_BF16 ? 0x7F80u : 0x7C00u);
+}
+template <int DT>
+__device__ __forceinline__ float magnitude(uint32_t m) {
+    if constexpr (DT == MTC_F32) return __uint_as_float(m);
+    const uint32_t h = max(m & 0xFFFFu, m >> 16);
+    if constexpr (DT == MTC_BF16) return __uint_as_float(h << 16);
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
 }
 
-__device__ __forceinline__ float largest(const float (&v)[8]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i]);
-        m = fmaxf(m, a < INFINITY ? a : 0.0f);      // (a NaN compares false)
-    }
-    return m;
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t *codes, size_t at, int n, const float (&v)[8], float s, float inv) {
+// Eight codes.  special: infinities or NaN may be among the values.
+template <int DT, bool POW2>
+__device__ __forceinline__ uint2 codes_of(const Eight<DT> &v, float s, float inv, bool special) {
     uint32_t c[4];
+    if (!special) {
+        // Borders between codes are the numbers of exactly five bits, and below the least normal code the odd multiples of 2^-10: only there can it matter on
+        // which side of its f32 the quotient is (code_quotient).
+        float q[8], least = INFINITY;
+        int border = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = to_e4m3x2(code_quotient(v[2 * i], s, inv), code_quotient(v[2 * i + 1], s, inv));
+        for (int i = 0; i < 8; ++i) {
+            const float x = v.value(i);
+            if constexpr (POW2) {
+                q[i] = x * inv;                  // exact (or far below the least code)
+            } else {
+                q[i] = quotient(x, s, inv);
+                border = min(border, static_cast<int>(__float_as_uint(q[i]) << 12));
+                least = fminf(least, fabsf(q[i]));
+            }
+        }
+        if (!POW2 && (border == static_cast<int>(0x80000000u) || least < 0.015625f)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = odd_quotient(v.value(i), s, q[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = to_e4m3x2(q[2 * i], q[2 * i + 1]);
+        return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = to_e4m3x2(code_quotient(v.value(2 * i), s, inv), code_quotient(v.value(2 * i + 1), s, inv));
+    return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(uint8_t *codes, size_t at, int n, uint2 c) {
     if constexpr (VEC) {
-        if (n > 0) *reinterpret_cast<uint2 *>(codes + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        if (n > 0) *reinterpret_cast<uint2 *>(codes + at) = c;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) codes[at + i] = static_cast<uint8_t>(c[i / 2] >> (i & 1) * 8);
+            if (i < n) codes[at + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (i & 3) * 8);
     }
 }
 
-// Blocks of 1 x 128: sixteen lanes a block, eight values a lane.
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void *x, const uint32_t *rows, uint8_t *codes, float *scales, long long n_rows,
-                                                            long long n_src_rows, int K, int pow2, uint32_t *status) {
+constexpr int kThreads = 256, kGroups = kThreads / 16;
+
+// Blocks of 1 x 128.  A CTA has 16 groups of 16 lanes: 2^shift of them side by side in a row, TURNS times, the others in the next rows.
+template <int DT, bool VEC, bool POW2, int TURNS>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void *x, const uint32_t *rows, uint8_t *codes, float *scales, long long n_rows,
+                                                                 long long n_src_rows, int K, int shift, uint32_t *status) {
     pdl_enter();
-    const int kb = blocks(K), lane = threadIdx.x & 15;
-    const long long total = n_rows * kb, step = static_cast<long long>(gridDim.x) * (blockDim.x / 16);
-    // (both halves of a warp go round equally often: the shuffles below take all lanes)
-    const long long first = static_cast<long long>(blockIdx.x) * (blockDim.x / 16) + threadIdx.x / 16, trips = (total - (first & ~1ll) + step - 1) / step;
-    for (long long t = 0; t < trips; ++t) {
-        const long long i = first + t * step;
-        const bool have = i < total;
-        const long long r = have ? i / kb : 0;
-        const int b = static_cast<int>(have ? i - r * kb : 0), k0 = b * kBlock + lane * 8;
-        long long src = r;
-        if (rows && have) {
-            const uint32_t id = rows[r];
-            src = id;
-            if (id >= n_src_rows) {
-                if (lane == 0 && b == 0) atomicCAS(status, 0u, 0x906u);      // an index outside the tensor reads row 0
-                src = 0;
-            }
+    const int kb = blocks(K), lane = threadIdx.x & 15, g = threadIdx.x >> 4, wide = 1 << shift;
+    const long long r = static_cast<long long>(blockIdx.x) * (kGroups >> shift) + (g >> shift);
+    const int b0 = blockIdx.y * (wide * TURNS) + (g & (wide - 1));
+    const bool row = r < n_rows;
+    long long src = row ? r : 0;
+    if (rows && row) {
+        const uint32_t id = rows[r];
+        src = id;
+        if (id >= n_src_rows) {
+            if (lane == 0 && b0 == 0) atomicCAS(status, 0u, 0x906u);         // an index outside the tensor reads row 0
+            src = 0;
         }
-        const int n = have ? K - k0 : 0;
-        float v[8];
-        load8<DT, VEC>(x, static_cast<size_t>(src) * K + k0, n, v);
-        float m = largest(v);
+    }
+    Eight<DT> v[TURNS];
+    int n[TURNS];
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const float s = scale_of(m, pow2), inv = __frcp_rn(s);
-        if (have && lane == 0) scales[i] = s;
-        store8<VEC>(codes, static_cast<size_t>(r) * K + k0, n, v, s, inv);
+    for (int u = 0; u < TURNS; ++u) {
+        const int b = b0 + u * wide;
+        n[u] = row && b < kb ? K - b * kBlock - lane * 8 : 0;
+        v[u].template load<VEC>(x, static_cast<size_t>(src) * K + b * kBlock + lane * 8, n[u]);
+    }
+    uint32_t m[TURNS];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) m[u] = v[u].most();
+    if constexpr (DT != MTC_F32 && TURNS == 2) {                     // both blocks' maxima in one word
+        uint32_t both = __vmaxu2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+        m[0] = both & 0xFFFFu;
+        m[1] = both >> 16;
+    } else {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m[u] = larger<DT>(m[u], __shfl_xor_sync(0xffffffffu, m[u], o));
+    }
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+        const int b = b0 + u * wide;
+        const bool special = has_special<DT>(m[u]);
+        float amax = magnitude<DT>(m[u]);
+        if (__any_sync(0xffffffffu, special)) {
+            float f = v[u].most_finite();
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, o));
+            amax = f;
+        }
+        const float s = scale_of(amax, POW2), inv = inverse_of(s);
+        if (lane == 0 && row && b < kb) scales[static_cast<size_t>(r) * kb + b] = s;
+        store8<VEC>(codes, static_cast<size_t>(r) * K + b * kBlock + lane * 8, n[u], codes_of<DT, POW2>(v[u], s, inv, special));
     }
 }
 
-// Blocks of 128 x 128: a CTA a block; a warp two rows of 128 at a time, eight times.
-template <int DT, bool VEC>
-__global__ void __launch_bounds__(256) quantize_blocks_kernel(const void *x, uint8_t *codes, float *scales, long long n_rows, int K, int pow2) {
+// Blocks of 128 x 128: a CTA a block, 16 rows at a time.
+template <int DT, bool VEC, bool POW2>
+__global__ void __launch_bounds__(kThreads) quantize_blocks_kernel(const void *x, uint8_t *codes, float *scales, long long n_rows, int K, int row_blocks) {
     pdl_enter();
     const int kb = blocks(K);
-    const long long nb = (n_rows + kBlock - 1) / kBlock;
-    const long long id = blockIdx.x;                          // (matrix, block of rows, block of columns)
-    const int b = static_cast<int>(id % kb);
-    const long long rb = id / kb % nb, mat = id / kb / nb;
-    const int lane = threadIdx.x & 15, row = threadIdx.x / 16, k0 = b * kBlock + lane * 8;
-    float v[8][8];
-    float m = 0.0f;
+    const uint32_t id = blockIdx.x, b = id % kb, rest = id / kb, rb = rest % row_blocks, mat = rest / row_blocks;      // (matrix, block of rows, block of columns)
+    const int lane = threadIdx.x & 15, k0 = b * kBlock + lane * 8;
+    const long long r0 = static_cast<long long>(rb) * kBlock + (threadIdx.x >> 4);
+    const size_t at = (static_cast<size_t>(mat) * n_rows + r0) * K + k0;
+    Eight<DT> v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long r = rb * kBlock + i * 16 + row;
-        load8<DT, VEC>(x, static_cast<size_t>(mat * n_rows + r) * K + k0, r < n_rows ? K - k0 : 0, v[i]);
-        m = fmaxf(m, largest(v[i]));
-    }
+    for (int i = 0; i < 8; ++i) v[i].template load<VEC>(x, at + static_cast<size_t>(i) * 16 * K, r0 + i * 16 < n_rows ? K - k0 : 0);
+    uint32_t m = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __shared__ float most[8];
+    for (int i = 0; i < 8; ++i) m = larger<DT>(m, v[i].most());
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = larger<DT>(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __shared__ uint32_t most[8];
+    __shared__ float most_f[8];
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, most[i]);
-    const float s = scale_of(m, pow2), inv = __frcp_rn(s);
+    for (int i = 0; i < 8; ++i) m = larger<DT>(m, most[i]);
+    const bool special = has_special<DT>(m);                         // the same in all threads
+    float amax = magnitude<DT>(m);
+    if (special) {
+        amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, v[i].most_finite());
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((threadIdx.x & 31) == 0) most_f[threadIdx.x >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, most_f[i]);
+    }
+    const float s = scale_of(amax, POW2), inv = inverse_of(s);
     if (threadIdx.x == 0) scales[id] = s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long r = rb * kBlock + i * 16 + row;
-        store8<VEC>(codes, static_cast<size_t>(mat * n_rows + r) * K + k0, r < n_rows ? K - k0 : 0, v[i], s, inv);
-    }
+    for (int i = 0; i < 8; ++i)
+        store8<VEC>(codes, at + static_cast<size_t>(i) * 16 * K, r0 + i * 16 < n_rows ? K - k0 : 0, codes_of<DT, POW2>(v[i], s, inv, special));
 }
 
-template <int DT, bool VEC>
+template <int DT, bool VEC, bool POW2>
 cudaError_t launch(Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *rows, uint8_t *codes, float *scales, int n_mats, long long n_rows,
-                   long long n_src_rows, int K, int block_rows, int pow2) {
+                   long long n_src_rows, int K, int block_rows) {
+    const int kb = blocks(K);
     if (block_rows == 1) {
-        const long long ctas = (n_rows * blocks(K) + 15) / 16;
-        return launch_pdl(quantize_rows_kernel<DT, VEC>, static_cast<unsigned>(ctas < 1ll << 30 ? ctas : 1ll << 30), 256, 0, st, x, rows, codes, scales,
-                          n_rows, n_src_rows, K, pow2, ctx->d_status);
+        int shift = 0;
+        while (shift < 4 && 1 << shift < kb) ++shift;
+        const long long ctas = (n_rows + (kGroups >> shift) - 1) / (kGroups >> shift);
+        // two blocks a group, all loads in flight at once, where that leaves every SM its eight CTAs
+        const bool two = kb > 16 && ctas * ((kb + 31) / 32) >= 8ll * ctx->sm_count;
+        const int turns = two ? 2 : 1;
+        return launch_pdl(two ? quantize_rows_kernel<DT, VEC, POW2, 2> : quantize_rows_kernel<DT, VEC, POW2, 1>,
+                          dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((kb + (turns << shift) - 1) / (turns << shift))), kThreads, 0, st, x, rows, codes, scales,
+                          n_rows, n_src_rows, K, shift, ctx->d_status);
     }
-    const long long ctas = n_mats * ((n_rows + kBlock - 1) / kBlock) * blocks(K);
+    const long long row_blocks = (n_rows + kBlock - 1) / kBlock, ctas = n_mats * row_blocks * kb;
     if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    return launch_pdl(quantize_blocks_kernel<DT, VEC>, static_cast<unsigned>(ctas), 256, 0, st, x, codes, scales, n_rows, K, pow2);
+    return launch_pdl(quantize_blocks_kernel<DT, VEC, POW2>, static_cast<unsigned>(ctas), kThreads, 0, st, x, codes, scales, n_rows, K, static_cast<int>(row_blocks));
+}
+template <int DT>
+cudaError_t launch(bool vec, bool pow2, Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *rows, uint8_t *codes, float *scales, int n_mats, long long n_rows,
+                   long long n_src_rows, int K, int block_rows) {
+    auto *f = vec ? (pow2 ? launch<DT, true, true> : launch<DT, true, false>) : (pow2 ? launch<DT, false, true> : launch<DT, false, false>);
+    return f(ctx, st, x, rows, codes, scales, n_mats, n_rows, n_src_rows, K, block_rows);
 }
 
 }  // namespace
 
-cudaError_t launch_fp8_quantize(Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *rows, uint8_t *codes, float *scales, int n_mats,
-                                long long n_rows, long long n_src_rows, int K, int block_rows, int pow2, int dt) {
+cudaError_t launch_fp8_quantize(Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *rows, uint8_t *codes, float *scales, int n_mats, long long n_rows,
+                                long long n_src_rows, int K, int block_rows, int pow2, int dt) {
     const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 8 == 0;
-    auto *f = dt == MTC_F32    ? (vec ? launch<MTC_F32, true> : launch<MTC_F32, false>)
-              : dt == MTC_BF16 ? (vec ? launch<MTC_BF16, true> : launch<MTC_BF16, false>)
-                               : (vec ? launch<MTC_F16, true> : launch<MTC_F16, false>);
-    return f(ctx, st, x, rows, codes, scales, n_mats, n_rows, n_src_rows, K, block_rows, pow2);
+    return (dt == MTC_F32 ? launch<MTC_F32> : dt == MTC_BF16 ? launch<MTC_BF16> : launch<MTC_F16>)(vec, pow2 != 0, ctx, st, x, rows, codes, scales, n_mats, n_rows,
+                                                                                                n_src_rows, K, block_rows);
 }
 
 }  // namespace mtc

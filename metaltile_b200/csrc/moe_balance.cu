@@ -6,8 +6,10 @@
 //   loss = coef * E * sum_e f_e P_e;  n = 0: f, P and loss are 0
 //   d loss / d logit_te = coef * E / n * p_te * (f_e - sum_j f_j p_tj)       (counts are constants)
 //
-// Bound by reading the logits: a warp has a row in registers, every lane adds up its own experts over the rows of the warp.  Sums over rows are f32 in a warp
-// (a few dozen rows) and f64 from there on, always in the same order; counts are integers, whose order does not matter.
+// Bound by reading the logits: a warp has a row in registers (two at a time while there are many), every lane adds up its own experts over the rows of the warp; rows are
+// dealt out to the warps of the grid in turn, so that masked ones, which lie together, are spread.  Sums over rows are f32 in a warp and in its CTA (at most a few dozen
+// rows a warp) and f64 from there on, always in the same order; counts are integers, whose order does not matter.  A second launch, a cluster of eight CTAs with an
+// eighth of the experts each, adds up the CTAs' parts and meets over distributed shared memory for the loss.
 #include <algorithm>
 
 #include "common.cuh"
@@ -15,7 +17,7 @@
 namespace mtc {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;      // of the gradient
 
 // Expert of slot (chunk c, i) of a lane: (c * 32 + lane) * V + i; V neighbours are one load.
 template <int DT, int V>
@@ -85,13 +87,14 @@ __device__ __forceinline__ void softmax_row(float (&z)[CH][V]) {
         for (int i = 0; i < V; ++i) most = fmaxf(most, z[c][i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    // exp(z - most) as a power of two; below 2^-126 it is zero
     if (most == -INFINITY) most = 0.0f;
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            z[c][i] = expf(z[c][i] - most);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z[c][i]) : "f"((z[c][i] - most) * 1.4426950408889634f));
             sum += z[c][i];
         }
 #pragma unroll
@@ -103,38 +106,56 @@ __device__ __forceinline__ void softmax_row(float (&z)[CH][V]) {
         for (int i = 0; i < V; ++i) z[c][i] *= inv;
 }
 
+// Warps of a CTA that adds up rows: a lane holds two sets of CH x V values, so few warps where that is many registers
+__host__ __device__ constexpr int row_warps(int ch, int v) { return ch * v <= 8 ? 32 : 16; }
+
 // Sums of each CTA: part_p f32[grid][E], part_c i32[grid][E], part_n i32[grid]
 template <int DT, int V, int CH>
-__global__ void __launch_bounds__(kThreads) balance_rows_kernel(const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float *part_p, int *part_c,
-                                                                int *part_n, int n_rows, int n_experts, int k, uint32_t *status) {
+__global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float *part_p, int *part_c,
+                                                                           int *part_n, int n_rows, int n_experts, int k, uint32_t *status) {
     pdl_enter();
+    constexpr int W = row_warps(CH, V), T = 32 * W;
     extern __shared__ float sm[];
-    float *const warp_p = sm;                                    // [kWarps][E]
-    int *const hist = reinterpret_cast<int *>(sm + kWarps * n_experts);
+    float *const warp_p = sm;                                    // [W][E]
+    int *const hist = reinterpret_cast<int *>(sm + W * n_experts);
     __shared__ int counted;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int r0 = static_cast<int>(static_cast<long long>(n_rows) * blockIdx.x / gridDim.x);
-    const int r1 = static_cast<int>(static_cast<long long>(n_rows) * (blockIdx.x + 1) / gridDim.x);
-    for (int e = threadIdx.x; e < n_experts; e += kThreads) hist[e] = 0;
+    for (int e = threadIdx.x; e < n_experts; e += T) hist[e] = 0;
     if (threadIdx.x == 0) counted = 0;
     __syncthreads();
     float acc[CH][V] = {};
     int n = 0;
-    for (int r = r0 + warp; r < r1; r += kWarps) {
-        if (mask && mask[r] == 0) continue;
+    auto kept = [&](long long r) { return r < n_rows && (!mask || mask[r] != 0); };
+    auto count = [&](long long r) {
         ++n;
         for (int j = lane; j < k; j += 32) {
             const uint32_t e = topk_idx[static_cast<size_t>(r) * k + j];
             if (e < static_cast<uint32_t>(n_experts)) atomicAdd(&hist[e], 1);
             else atomicCAS(status, 0u, 0x907u);                  // an expert that does not exist: recorded, not counted
         }
-        float z[CH][V];
-        load_row<DT, V, CH>(logits, r, n_experts, z);
-        softmax_row<V, CH>(z);
+    };
+    auto add = [&](const float (&z)[CH][V]) {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
             for (int i = 0; i < V; ++i) acc[c][i] += z[c][i];
+    };
+    const long long step = static_cast<long long>(gridDim.x) * W;
+    for (long long r = static_cast<long long>(warp) * gridDim.x + blockIdx.x; r < n_rows; r += 2 * step) {
+        const bool one = kept(r), two = kept(r + step);
+        float a[CH][V], b[CH][V];
+        if (one) load_row<DT, V, CH>(logits, r, n_experts, a);
+        if (two) load_row<DT, V, CH>(logits, r + step, n_experts, b);
+        if (one) {
+            count(r);
+            softmax_row<V, CH>(a);
+            add(a);
+        }
+        if (two) {
+            count(r + step);
+            softmax_row<V, CH>(b);
+            add(b);
+        }
     }
     if (lane == 0 && n) atomicAdd(&counted, n);
 #pragma unroll
@@ -145,51 +166,81 @@ __global__ void __launch_bounds__(kThreads) balance_rows_kernel(const void *logi
             if (e < n_experts) warp_p[warp * n_experts + e] = acc[c][i];
         }
     __syncthreads();
-    for (int e = threadIdx.x; e < n_experts; e += kThreads) {
+    for (int e = threadIdx.x; e < n_experts; e += T) {
         float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += warp_p[w * n_experts + e];
+#pragma unroll 8
+        for (int w = 0; w < W; ++w) s += warp_p[w * n_experts + e];
         part_p[static_cast<size_t>(blockIdx.x) * n_experts + e] = s;
         part_c[static_cast<size_t>(blockIdx.x) * n_experts + e] = hist[e];
     }
     if (threadIdx.x == 0) part_n[blockIdx.x] = counted;
 }
 
-constexpr int kJoinThreads = 1024;
-__global__ void __launch_bounds__(kJoinThreads) balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, int parts, float coef, float *loss,
-                                                                    int *counts, float *mean_probs, int *n_counted, int n_experts, int k) {
+constexpr int kJoinCtas = 8, kJoinThreads = 512;
+// A CTA has the experts of its eighth side by side (2^shift of its threads) and as many groups of parts as threads are left.
+__global__ void __cluster_dims__(kJoinCtas, 1, 1) __launch_bounds__(kJoinThreads)
+balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, int parts, float coef, float *loss, int *counts, float *mean_probs, int *n_counted,
+                    int n_experts, int k, int shift) {
     pdl_enter();
     __shared__ double sums[kJoinThreads];
+    __shared__ int cnts[kJoinThreads];
     __shared__ int total;
+    __shared__ double share;
+    const int rank = blockIdx.x, e0 = n_experts * rank / kJoinCtas, e1 = n_experts * (rank + 1) / kJoinCtas;
+    const int wide = 1 << shift, groups = kJoinThreads >> shift, g = threadIdx.x >> shift, e = e0 + (threadIdx.x & (wide - 1));
     if (threadIdx.x == 0) total = 0;
     __syncthreads();
     int mine = 0;
     for (int i = threadIdx.x; i < parts; i += kJoinThreads) mine += part_n[i];
     if (mine) atomicAdd(&total, mine);
-    __syncthreads();
-    const int n = total;
-    double term = 0.0;
-    for (int e = threadIdx.x; e < n_experts; e += kJoinThreads) {
-        double p = 0.0;
-        int c = 0;
-        for (int i = 0; i < parts; ++i) {
+    double p = 0.0;
+    int c = 0;
+    if (e < e1) {
+#pragma unroll 4
+        for (int i = g; i < parts; i += groups) {
             p += part_p[static_cast<size_t>(i) * n_experts + e];
             c += part_c[static_cast<size_t>(i) * n_experts + e];
         }
-        const double mean = n ? p / n : 0.0;
-        counts[e] = c;
-        mean_probs[e] = static_cast<float>(mean);
-        term += n ? mean * c / (static_cast<double>(n) * k) : 0.0;
     }
-    sums[threadIdx.x] = term;
-    for (int o = kJoinThreads / 2; o > 0; o >>= 1) {
+    sums[threadIdx.x] = p;
+    cnts[threadIdx.x] = c;
+    for (int o = groups >> 1; o > 0; o >>= 1) {
+        __syncthreads();
+        if (g < o) {
+            sums[threadIdx.x] += sums[threadIdx.x + (o << shift)];
+            cnts[threadIdx.x] += cnts[threadIdx.x + (o << shift)];
+        }
+    }
+    __syncthreads();
+    const int n = total;
+    double term = 0.0;
+    if (g == 0 && e < e1) {
+        const double mean = n ? sums[threadIdx.x] / n : 0.0;
+        counts[e] = cnts[threadIdx.x];
+        mean_probs[e] = static_cast<float>(mean);
+        term = n ? mean * cnts[threadIdx.x] / (static_cast<double>(n) * k) : 0.0;
+    }
+    __syncthreads();
+    if (g == 0) sums[threadIdx.x] = term;
+    for (int o = wide >> 1; o > 0; o >>= 1) {
         __syncthreads();
         if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
     }
-    if (threadIdx.x == 0) {
-        *loss = static_cast<float>(static_cast<double>(coef) * n_experts * sums[0]);
+    if (threadIdx.x == 0) share = sums[0];
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0 && threadIdx.x == 0) {
+        double all = 0.0;
+        for (int q = 0; q < kJoinCtas; ++q) {
+            uint32_t there;
+            double v;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&share))), "r"(q));
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(there) : "memory");
+            all += v;
+        }
+        *loss = static_cast<float>(static_cast<double>(coef) * n_experts * all);
         *n_counted = n;
     }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves while its share is read
 }
 
 template <int DT, int V, int CH>
@@ -208,10 +259,8 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const void *logi
             const int e = (c * 32 + lane) * V + i;
             f[c][i] = e < n_experts ? static_cast<float>(counts[e]) * each : 0.0f;
         }
-    for (long long r = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < n_rows; r += warps) {
-        float z[CH][V] = {};
-        if (!mask || mask[r] != 0) {
-            load_row<DT, V, CH>(logits, r, n_experts, z);
+    auto finish = [&](long long r, bool kept, float (&z)[CH][V]) {
+        if (kept) {
             softmax_row<V, CH>(z);
             float dot = 0.0f;
 #pragma unroll
@@ -224,16 +273,31 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const void *logi
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < V; ++i) z[c][i] = g * z[c][i] * (f[c][i] - dot);
+        } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[c][i] = 0.0f;
         }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int e = (c * 32 + lane) * V;
             if (e < n_experts) store_v<DT, V>(grad, static_cast<size_t>(r) * n_experts + e, z[c]);
         }
+    };
+    for (long long r = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < n_rows; r += 2 * warps) {
+        const long long r2 = r + warps;
+        const bool one = !mask || mask[r] != 0, two = r2 < n_rows && (!mask || mask[r2] != 0);
+        float a[CH][V], b[CH][V];
+        if (one) load_row<DT, V, CH>(logits, r, n_experts, a);
+        if (two) load_row<DT, V, CH>(logits, r2, n_experts, b);
+        finish(r, one, a);
+        if (r2 < n_rows) finish(r2, two, b);
     }
 }
 
-int balance_ctas(int sms, int n_rows) { return std::max(1, std::min(sms, (n_rows + kWarps - 1) / kWarps)); }
+// CTAs that add up rows: eight rows each at least, so that few rows make few parts
+int balance_ctas(int sms, int n_rows) { return std::max(1, std::min(sms, (n_rows + 7) / 8)); }
 
 // The instance that holds a row: four neighbouring experts a load where rows of them are aligned
 template <template <int, int, int> class F, int DT, typename... A>
@@ -255,9 +319,16 @@ cudaError_t with_form(int dt, bool vec, int n_experts, A... args) {
 }
 template <int DT, int V, int CH>
 struct RowsForm {
-    static cudaError_t run(Ctx *ctx, cudaStream_t st, int ctas, size_t smem, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc,
-                           int *pn, int n_rows, int n_experts, int k) {
-        return launch_pdl(balance_rows_kernel<DT, V, CH>, ctas, kThreads, smem, st, logits, idx, mask, pp, pc, pn, n_rows, n_experts, k, ctx->d_status);
+    static cudaError_t run(Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn, int n_rows,
+                           int n_experts, int k) {
+        constexpr int W = row_warps(CH, V);
+        const size_t smem = static_cast<size_t>(W + 1) * n_experts * 4;
+        static PerDeviceAttr attr;
+        if (smem > 48 * 1024) {
+            const cudaError_t e = attr.set(balance_rows_kernel<DT, V, CH>, static_cast<size_t>(W + 1) * 1024 * 4);
+            if (e != cudaSuccess) return e;
+        }
+        return launch_pdl(balance_rows_kernel<DT, V, CH>, ctas, 32 * W, smem, st, logits, idx, mask, pp, pc, pn, n_rows, n_experts, k, ctx->d_status);
     }
 };
 template <int DT, int V, int CH>
@@ -283,17 +354,17 @@ cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, co
     const int ctas = balance_ctas(ctx->sm_count, n_rows);
     float *pp = static_cast<float *>(workspace);
     int *pc = reinterpret_cast<int *>(pp + static_cast<size_t>(ctas) * n_experts), *pn = pc + static_cast<size_t>(ctas) * n_experts;
-    const size_t smem = static_cast<size_t>(kWarps + 1) * n_experts * 4;
-    cudaError_t e = with_form<RowsForm>(dt, in_fours(n_experts, dt, logits, logits), n_experts, ctx, st, ctas, smem, logits, topk_idx, mask, pp, pc, pn, n_rows,
-                                        n_experts, k);
+    cudaError_t e = with_form<RowsForm>(dt, in_fours(n_experts, dt, logits, logits), n_experts, ctx, st, ctas, logits, topk_idx, mask, pp, pc, pn, n_rows, n_experts, k);
     if (e != cudaSuccess) return e;
-    return launch_pdl(balance_join_kernel, 1, kJoinThreads, 0, st, pp, pc, pn, ctas, coef, loss, counts, mean_probs, n_counted, n_experts, k);
+    int shift = 0;
+    while (1 << shift < (n_experts + kJoinCtas - 1) / kJoinCtas) ++shift;
+    return launch_pdl(balance_join_kernel, kJoinCtas, kJoinThreads, 0, st, pp, pc, pn, ctas, coef, loss, counts, mean_probs, n_counted, n_experts, k, shift);
 }
 
 cudaError_t launch_moe_balance_grad(Ctx *ctx, cudaStream_t st, const void *logits, const uint8_t *mask, const int *counts, const int *n_counted,
                                     const float *grad_loss, float coef, void *grad, int n_rows, int n_experts, int k, int dt) {
     if (n_rows <= 0) return cudaSuccess;
-    const int ctas = std::min(ctx->sm_count * 4, (n_rows + kWarps - 1) / kWarps);
+    const int ctas = std::min(ctx->sm_count * 8, (n_rows + kWarps - 1) / kWarps);
     return with_form<GradForm>(dt, in_fours(n_experts, dt, logits, grad), n_experts, st, ctas, logits, mask, counts, n_counted, grad_loss, coef, grad, n_rows,
                                n_experts, k);
 }
