@@ -10,8 +10,8 @@
 // about as many of epilogue.  So the ring is what matters: two CTAs an SM with some 100 KB of stages each, one CTA an item; few tokens and few rows of
 // weights: K is cut into up to 8 slices, the CTAs of a cluster, which add up through shared memory in the order of K.
 //
-//   warps 0-3  epilogue   factors of a few dozen blocks at a time into shared memory, accumulators out, sums, stores
-//   warp 4     producer   TMA: 128 x 128 codes of the weights, TN x 128 of the tokens, a stage
+//   warps 0-3  epilogue   accumulators out, scaled, added up, stored (TN = 128: eight warps)
+//   warp 4     producer   TMA: 128 x 128 codes of the weights, TN x 128 of the tokens, a stage; by cp.async the scales of 16 blocks
 //   warp 5     MMA        and the tensor memory's allocation
 // Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited (bounded too).
 #include <cstddef>
@@ -37,10 +37,11 @@ struct Form {
     static constexpr int kSmemBytes = kPerSM == 1 ? 226 * 1024 : 113 * 1024;
     static constexpr int kAcc = 4;                                   // accumulators in tensor memory
     static constexpr int kCols = kAcc * TN;
-    static constexpr int kHeld = 32;                                 // blocks whose factors are in shared memory
+    static constexpr int kHeld = 16;                                 // blocks whose scales are in shared memory, [block][token], twice
     static constexpr int kPitch = TN + 4;
     static constexpr int kStage = kWBytes + TN * kBlock;
-    static constexpr int kRing = 1024 + (kHeld * kPitch * 4 + 1023) / 1024 * 1024;       // where the stages start
+    static constexpr int kScales = kHeld * (kPitch + 1);             // floats: xs, then ws of the blocks
+    static constexpr int kRing = 1024 + (2 * kScales * 4 + 1023) / 1024 * 1024;          // where the stages start
     static constexpr int kStages = (kSmemBytes - 1024 - kRing) / kStage;
     static_assert(kStages >= 2 && kStages <= kMaxStages, "stages");
     static_assert(kStages * kStage >= TN * kRows * 4, "the sums of a slice go where the ring was");
@@ -63,10 +64,10 @@ struct TMaps {
 };
 
 struct __align__(16) TCtrl {
-    uint64_t full[kMaxStages], empty[kMaxStages], d_full[4], d_empty[4], drained;
+    uint64_t full[kMaxStages], empty[kMaxStages], d_full[4], d_empty[4], s_full[2], s_empty[2], drained;
     uint32_t tmem_base, issued;
     volatile uint32_t abort;
-    int expert, tok0, ntok;
+    int n_chunks;                                // of all experts, or of the dense rows
 };
 static_assert(sizeof(TCtrl) <= 1024, "control block");
 
@@ -86,13 +87,14 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
-// The chunk with this index among the chunks of all experts, by one warp: expert e with r rows has ceil(r / TN).  Offsets that run backwards or past the rows are
-// clamped and reported.
-__device__ __forceinline__ void find_chunk(const uint32_t *offsets, int n_experts, int m_total, int TN, int want, uint32_t *status, bool report, int &expert, int &tok0,
-                                           int &ntok) {
+// Chunks of TN rows: expert e with r rows has ceil(r / TN).  By one warp: how many there are in all (want < 0), or the one with index `want`.  Offsets that run
+// backwards or past the rows are clamped, and reported by the block that is told to.
+struct Chunk {
+    int expert, tok0, ntok;
+};
+__device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts, int m_total, int TN, int want, uint32_t *status, Chunk &found) {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    expert = tok0 = ntok = 0;
     for (int e0 = 0; e0 < n_experts; e0 += 32) {
         const int e = e0 + lane;
         int lo = 0, hi = 0;
@@ -100,7 +102,7 @@ __device__ __forceinline__ void find_chunk(const uint32_t *offsets, int n_expert
             const uint32_t a = offsets[e], b = offsets[e + 1], m = static_cast<uint32_t>(m_total);
             lo = static_cast<int>(min(a, m));
             hi = max(lo, static_cast<int>(min(b, m)));
-            if (report && (a > m || b > m || b < a)) atomicCAS(status, 0u, 0x901u);
+            if (status && (a > m || b > m || b < a)) atomicCAS(status, 0u, 0x901u);
         }
         const int np = (hi - lo + TN - 1) / TN;
         int upto = np;
@@ -110,16 +112,17 @@ __device__ __forceinline__ void find_chunk(const uint32_t *offsets, int n_expert
             if (lane >= d) upto += v;
         }
         const int mine = want - before - (upto - np);                // index of the wanted chunk among this expert's
-        const uint32_t has = __ballot_sync(0xffffffffu, mine >= 0 && mine < np);
+        const uint32_t has = __ballot_sync(0xffffffffu, want >= 0 && mine >= 0 && mine < np);
         if (has) {
             const int src = __ffs(has) - 1;
-            expert = e0 + src;
-            tok0 = __shfl_sync(0xffffffffu, lo + mine * TN, src);
-            ntok = min(TN, __shfl_sync(0xffffffffu, hi, src) - tok0);
-            if (!report) return;
+            found.expert = e0 + src;
+            found.tok0 = __shfl_sync(0xffffffffu, lo + mine * TN, src);
+            found.ntok = min(TN, __shfl_sync(0xffffffffu, hi, src) - found.tok0);
+            return want;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
+    return before;
 }
 
 // Giving up, once every role has ended: lets what is on its way arrive before the CTA tears down.
@@ -135,15 +138,15 @@ __device__ __noinline__ void rest(TCtrl *ctl, int stages, int load_warp) {
 }
 
 template <int TN>
-__global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
+__global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
     using F = Form<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     TCtrl *const ctl = reinterpret_cast<TCtrl *>(smem);
-    float *const factors = reinterpret_cast<float *>(smem + 1024);   // [kHeld][kPitch]
+    float *const scales = reinterpret_cast<float *>(smem + 1024);    // two of kScales
     const uint32_t ring = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + F::kRing;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int rank = static_cast<int>(blockIdx.x % a.slices), unit = static_cast<int>(blockIdx.x / a.slices);
+    const int rank = static_cast<int>(blockIdx.x % a.slices), first = static_cast<int>(blockIdx.x / a.slices), step = static_cast<int>(gridDim.x / a.slices);
     const int kb0 = static_cast<int>(static_cast<long long>(a.nkb) * rank / a.slices), kb1 = static_cast<int>(static_cast<long long>(a.nkb) * (rank + 1) / a.slices);
     if (threadIdx.x == 0) {
         for (int s = 0; s < F::kStages; ++s) {
@@ -154,87 +157,119 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
             mbar_init(&ctl->d_full[s], 1);
             mbar_init(&ctl->d_empty[s], F::kEpi / 32);
         }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&ctl->s_full[s], 32);
+            mbar_init(&ctl->s_empty[s], F::kEpi / 32);
+        }
         mbar_init(&ctl->drained, 1);
         ctl->abort = 0;
         ctl->issued = 0;
+        ctl->n_chunks = a.chunks;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == F::kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "n"(F::kCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    int tile, expert = 0, tok0, ntok;
-    bool waited = false;
     if (a.expert_offsets) {
         pdl_enter();
-        waited = true;
-        tile = unit % a.tiles;
         if (warp == F::kLoadWarp) {
-            find_chunk(a.expert_offsets, a.n_experts, a.M, TN, unit / a.tiles, a.status, blockIdx.x == 0, expert, tok0, ntok);
-            if (lane == 0) {
-                ctl->expert = expert;
-                ctl->tok0 = tok0;
-                ctl->ntok = ntok;
-            }
+            Chunk none;
+            const int n = find_chunk(a.expert_offsets, a.n_experts, a.M, TN, -1, blockIdx.x == 0 ? a.status : nullptr, none);
+            __syncwarp();
+            if (lane == 0) ctl->n_chunks = n;
         }
-    } else {
-        tile = unit / a.chunks;
-        tok0 = unit % a.chunks * TN;
-        ntok = min(TN, a.M - tok0);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (a.expert_offsets) {
-        expert = ctl->expert;
-        tok0 = ctl->tok0;
-        ntok = ctl->ntok;
-    }
     const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-    const int n0 = tile * kRows;
-    uint64_t acc[F::kPart / 2] = {};
-    const int part0 = F::kGroups == 1 ? 0 : warp / 4 * F::kPart;     // first column (token) of this warp's part
+    const int units = ctl->n_chunks * a.tiles;
+    // grouped: the tiles of a chunk behind each other; dense: the chunks of a tile, which read the same weights
+    auto tile_of = [&](int unit) { return a.expert_offsets ? unit % a.tiles : unit / a.chunks; };
+    auto chunk_of = [&](int unit) {
+        Chunk c;
+        if (a.expert_offsets) {
+            find_chunk(a.expert_offsets, a.n_experts, a.M, TN, unit / a.tiles, nullptr, c);
+        } else {
+            c.expert = 0;
+            c.tok0 = unit % a.chunks * TN;
+            c.ntok = min(TN, a.M - c.tok0);
+        }
+        return c;
+    };
 
-    if (ntok > 0) {
-        if (warp == F::kLoadWarp) {
-            if (lane == 0) {
-                const int row = static_cast<int>(static_cast<long long>(expert) * a.N) + n0;
-                int ahead = 0;
-                if (!waited) {
-                    if (a.early) {
-                        asm volatile("griddepcontrol.launch_dependents;");
-                        for (int kb = kb0; kb < kb1 && ahead < F::kStages; ++kb, ++ahead) {
-                            mbar_expect_tx(&ctl->full[ahead], F::kStage);
-                            tma_load_2d(ring + ahead * F::kStage, &maps.w, kb * kBlock, row, &ctl->full[ahead]);
-                        }
-                        asm volatile("griddepcontrol.wait;" ::: "memory");
-                    } else {
-                        asm volatile("griddepcontrol.wait;" ::: "memory");
-                        asm volatile("griddepcontrol.launch_dependents;");
+    if (warp == F::kLoadWarp) {
+        int s = 0;
+        uint32_t phase = 1, s_phase = 1;         // of `empty`: the first round passes
+        int b = 0;
+        bool go = true;
+        if (!a.expert_offsets && !a.early) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            asm volatile("griddepcontrol.launch_dependents;");
+        }
+        for (int unit = first; go && unit < units; unit += step) {
+            const Chunk c = chunk_of(unit);
+            const int tile = tile_of(unit), row = static_cast<int>(static_cast<long long>(c.expert) * a.N) + tile * kRows;
+            int ahead = 0;
+            if (a.early && unit == first) {      // weights are constants: as many as the ring holds while the previous kernel ends
+                if (lane == 0) {
+                    asm volatile("griddepcontrol.launch_dependents;");
+                    for (int i = 0; kb0 + i < kb1 && i < F::kStages; ++i) {
+                        mbar_expect_tx(&ctl->full[i], F::kStage);
+                        tma_load_2d(ring + i * F::kStage, &maps.w, (kb0 + i) * kBlock, row, &ctl->full[i]);
                     }
                 }
-                int s = 0;
-                uint32_t phase = 1;              // of `empty`: the first round passes
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    const bool requested = kb - kb0 < ahead;
-                    if (!requested && kb - kb0 >= F::kStages && !wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u)) break;
-                    const uint32_t at = ring + s * F::kStage;
-                    if (!requested) {
-                        mbar_expect_tx(&ctl->full[s], F::kStage);
-                        tma_load_2d(at, &maps.w, kb * kBlock, row, &ctl->full[s]);
-                    }
-                    tma_load_2d(at + kWBytes, &maps.x, kb * kBlock, tok0, &ctl->full[s]);
-                    ++ctl->issued;
-                    if (++s == F::kStages) s = 0, phase ^= 1;
-                }
+                ahead = min(kb1 - kb0, F::kStages);
+                asm volatile("griddepcontrol.wait;" ::: "memory");
             }
-        } else if (warp == F::kMmaWarp) {
-            constexpr uint32_t idesc = 1u << 4 | static_cast<uint32_t>(TN >> 3) << 17 | static_cast<uint32_t>(kRows >> 4) << 24;
-            int s = 0, d = 0;
-            uint32_t phase = 0, d_phase = 1;
+            const float *const xs = a.xs + static_cast<size_t>(c.tok0) * a.nkb;
+            const float *const ws = a.ws + (static_cast<size_t>(c.expert) * a.tiles + tile) * a.nkb;
+            for (int kb = kb0; go && kb < kb1; ++kb) {
+                if ((kb - kb0) % F::kHeld == 0) {        // scales of the next blocks, on their way as the codes are: a lane a block, two tokens at a time
+                    if (!wait_all(&ctl->s_empty[b], s_phase, &ctl->abort, a.status, 0xb05u)) {
+                        go = false;
+                        break;
+                    }
+                    const int k = lane % F::kHeld, t0 = lane / F::kHeld;
+                    const uint32_t to = smem_u32(scales) + b * F::kScales * 4;
+                    if (kb + k < kb1) {
+                        for (int t = t0; t < c.ntok; t += 32 / F::kHeld)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + (k * F::kPitch + t) * 4), "l"(xs + static_cast<size_t>(t) * a.nkb + kb + k) : "memory");
+                        if (t0 == 0) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + (F::kHeld * F::kPitch + k) * 4), "l"(ws + kb + k) : "memory");
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl->s_full[b])) : "memory");
+                    if (b ^= 1; b == 0) s_phase ^= 1;
+                }
+                const bool requested = kb - kb0 < ahead;
+                if (lane == 0) {
+                    go = requested || wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u);
+                    if (go) {
+                        const uint32_t at = ring + s * F::kStage;
+                        if (!requested) {
+                            mbar_expect_tx(&ctl->full[s], F::kStage);
+                            tma_load_2d(at, &maps.w, kb * kBlock, row, &ctl->full[s]);
+                        }
+                        tma_load_2d(at + kWBytes, &maps.x, kb * kBlock, c.tok0, &ctl->full[s]);
+                        ++ctl->issued;
+                    }
+                }
+                if (++s == F::kStages) s = 0, phase ^= 1;
+                if ((kb + 1 - kb0) % F::kHeld == 0 || kb + 1 == kb1) go = __shfl_sync(0xffffffffu, go, 0);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == F::kMmaWarp) {
+        constexpr uint32_t idesc = 1u << 4 | static_cast<uint32_t>(TN >> 3) << 17 | static_cast<uint32_t>(kRows >> 4) << 24;
+        int s = 0, d = 0;
+        uint32_t phase = 0, d_phase = 1;
+        bool go = true;
+        for (int unit = first; go && unit < units; unit += step)
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u)) break;
-                if (!wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) break;
+                if (!wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u) || !wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) {
+                    go = false;
+                    break;
+                }
                 tc_fence_after();
                 const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
                 if (elect_one()) {
@@ -247,86 +282,97 @@ __global__ void __launch_bounds__(Form<TN>::kThreads) fp8_tile_kernel(const __gr
                 if (++s == F::kStages) s = 0, phase ^= 1;
                 if (++d == F::kAcc) d = 0, d_phase ^= 1;
             }
-        } else {
-            if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-            const float *const xs = a.xs + static_cast<size_t>(tok0) * a.nkb;
-            const float *const ws = a.ws + (static_cast<size_t>(expert) * a.tiles + tile) * a.nkb;
-            const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + part0;      // lane 32 * warp in bits 16 and up
-            int d = 0, held = 0;
-            uint32_t phase = 0;
+    } else {
+        if (!a.expert_offsets) asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int part0 = F::kGroups == 1 ? 0 : warp / 4 * F::kPart;                    // first column (token) of this warp's part
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + part0;      // lane 32 * warp in bits 16 and up
+        const int r = threadIdx.x & (kRows - 1);
+        int d = 0, b = 0;
+        uint32_t phase = 0, s_phase = 0;
+        for (int unit = first; unit < units; unit += step) {
+            const Chunk c = chunk_of(unit);
+            const int tile = tile_of(unit);
+            uint64_t acc[F::kPart / 2] = {};
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (kb == kb0 + held) {                  // the next blocks' factors
-                    if (held) asm volatile("bar.sync 1, %0;" ::"n"(F::kEpi) : "memory");
-                    const int here = min(F::kHeld, kb1 - kb);
-                    for (int i = threadIdx.x; i < F::kHeld * TN; i += F::kEpi) {
-                        const int t = i / F::kHeld, b = i % F::kHeld;
-                        factors[b * F::kPitch + t] = t < ntok && b < here ? xs[static_cast<size_t>(t) * a.nkb + kb + b] * __ldg(ws + kb + b) : 0.0f;
-                    }
-                    held += F::kHeld;
-                    asm volatile("bar.sync 1, %0;" ::"n"(F::kEpi) : "memory");
-                }
-                wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);      // (giving up, the warps go on to the end: they meet at barriers)
+                const int at = (kb - kb0) % F::kHeld;
+                const float *const f = scales + b * F::kScales + at * F::kPitch + part0;
+                if (at == 0) wait_soon(&ctl->s_full[b], s_phase, &ctl->abort, a.status, 0xb06u);
+                const float ws = scales[b * F::kScales + F::kHeld * F::kPitch + at];
+                wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);
                 __syncwarp();
                 tc_fence_after();
-                const float *const f = factors + (kb - kb0) % F::kHeld * F::kPitch + part0;
-                constexpr int STEP = TN < 32 ? TN : 32;
+                constexpr int STEP = TN < 32 ? TN : 32, LOADS = F::kPart / STEP;
+                uint32_t v[LOADS > 1 ? 2 : 1][STEP];
+                tmem_ld<STEP>(lanes + d * TN, v[0]);
 #pragma unroll
-                for (int c = 0; c < F::kPart; c += STEP) {
-                    uint32_t v[STEP];
-                    tmem_ld<STEP>(lanes + d * TN + c, v);
-                    tmem_wait_ld<STEP>(v);
-                    if (c + STEP == F::kPart) {
+                for (int q = 0; q < LOADS; ++q) {
+                    tmem_wait_ld(v[q & 1]);
+                    if (q + 1 < LOADS) {
+                        tmem_ld<STEP>(lanes + d * TN + (q + 1) * STEP, v[~q & 1]);
+                    } else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&ctl->d_empty[d]);
                     }
 #pragma unroll
                     for (int i = 0; i < STEP; i += 4) {
-                        const float4 q = *reinterpret_cast<const float4 *>(f + c + i);
-                        fma2(acc[(c + i) / 2], v[i], v[i + 1], q.x, q.y);
-                        fma2(acc[(c + i) / 2 + 1], v[i + 2], v[i + 3], q.z, q.w);
+                        const float4 w = *reinterpret_cast<const float4 *>(f + q * STEP + i);
+                        fma2(acc[(q * STEP + i) / 2], v[q & 1][i], v[q & 1][i + 1], w.x * ws, w.y * ws);
+                        fma2(acc[(q * STEP + i) / 2 + 1], v[q & 1][i + 2], v[q & 1][i + 3], w.z * ws, w.w * ws);
                     }
                 }
                 if (++d == F::kAcc) d = 0, phase ^= 1;
+                if (at == F::kHeld - 1 || kb == kb1 - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->s_empty[b]);
+                    if (b ^= 1; b == 0) s_phase ^= 1;
+                }
+            }
+            const int n = tile * kRows + r;
+            if (a.slices == 1) {
+                if (n < a.N && !ctl->abort) {
+#pragma unroll
+                    for (int i = 0; i < F::kPart; i += 2) {
+                        const float2 v = halves(acc[i / 2]);
+                        const int t = part0 + i;
+                        if (t < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t) * a.N + n, v.x, a.out_dt);
+                        if (t + 1 < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t + 1) * a.N + n, v.y, a.out_dt);
+                    }
+                }
+            } else {                             // one unit a cluster: the sums of a slice go where the ring was, [token][weight row]
+#pragma unroll
+                for (int i = 0; i < F::kPart; i += 2) {
+                    const float2 v = halves(acc[i / 2]);
+                    const int t = part0 + i;
+                    if (t < c.ntok) st_shared(ring + (t * kRows + r) * 4, v.x);
+                    if (t + 1 < c.ntok) st_shared(ring + ((t + 1) * kRows + r) * 4, v.y);
+                }
             }
         }
     }
     __syncthreads();
     if (ctl->abort) rest(ctl, F::kStages, F::kLoadWarp);
-
-    const bool store = ntok > 0 && warp < F::kLoadWarp && !ctl->abort;
-    const int r = threadIdx.x & (kRows - 1), n = n0 + r;
-    if (a.slices == 1) {
-        if (store && n < a.N) {
-#pragma unroll
-            for (int i = 0; i < F::kPart; i += 2) {
-                const float2 v = halves(acc[i / 2]);
-                const int t = part0 + i;
-                if (t < ntok) st_from_f32(a.out, static_cast<size_t>(tok0 + t) * a.N + n, v.x, a.out_dt);
-                if (t + 1 < ntok) st_from_f32(a.out, static_cast<size_t>(tok0 + t + 1) * a.N + n, v.y, a.out_dt);
-            }
-        }
-    } else {
-        // every slice's sums into its shared memory [token][weight row]; slice r adds up tokens r, r + slices, ...
-        if (warp < F::kLoadWarp) {
-#pragma unroll
-            for (int i = 0; i < F::kPart; i += 2) {
-                const float2 v = halves(acc[i / 2]);
-                const int t = part0 + i;
-                if (t < ntok) st_shared(ring + (t * kRows + r) * 4, v.x);
-                if (t + 1 < ntok) st_shared(ring + ((t + 1) * kRows + r) * 4, v.y);
-            }
-        }
+    if (a.slices > 1) {                          // slice r adds up tokens r, r + slices, ... of all slices
         cluster_sync();
-        if (store && n < a.N) {
-            for (int t = rank + (warp / 4) * a.slices; t < ntok; t += F::kGroups * a.slices) {
-                float part[kMaxSlices], sum = 0.0f;
+        if (first < units && warp < F::kLoadWarp && !ctl->abort) {
+            const Chunk c = chunk_of(first);
+            const int r = threadIdx.x & (kRows - 1), n = tile_of(first) * kRows + r;
+            const int every = F::kGroups * a.slices;
+            for (int t0 = rank + (warp / 4) * a.slices; t0 < c.ntok && n < a.N; t0 += 4 * every) {
+                float part[4][kMaxSlices];
 #pragma unroll
-                for (int q = 0; q < kMaxSlices; ++q) part[q] = q < a.slices ? ld_cluster(ring + (t * kRows + r) * 4, q) : 0.0f;
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int q = 0; q < kMaxSlices; ++q)
-                    if (q < a.slices) sum += part[q];
-                st_from_f32(a.out, static_cast<size_t>(tok0 + t) * a.N + n, sum, a.out_dt);
+                    for (int q = 0; q < kMaxSlices; ++q)
+                        part[i][q] = q < a.slices && t0 + i * every < c.ntok ? ld_cluster(ring + ((t0 + i * every) * kRows + r) * 4, q) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float sum = part[i][0];
+#pragma unroll
+                    for (int q = 1; q < kMaxSlices; ++q)
+                        if (q < a.slices) sum += part[i][q];
+                    if (t0 + i * every < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t0 + i * every) * a.N + n, sum, a.out_dt);
+                }
             }
         }
         cluster_sync();                          // no CTA leaves while its sums are read
@@ -345,9 +391,11 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w
     static PerDeviceAttr attr;
     if ((e = attr.set(fp8_tile_kernel<TN>, Form<TN>::kSmemBytes)) != cudaSuccess) return e;
     const long long units = a.expert_offsets ? (static_cast<long long>(std::min(a.M, a.n_experts)) + a.M / TN) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
-    if (units * a.slices > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    if (units > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    // slices: a cluster a unit; else no more CTAs than run at once, each with units in turn
+    const long long ctas = a.slices > 1 ? units * a.slices : std::min<long long>(units, static_cast<long long>(Form<TN>::kPerSM) * ctx->sm_count);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(units * a.slices));
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
     cfg.blockDim = dim3(Form<TN>::kThreads);
     cfg.dynamicSmemBytes = Form<TN>::kSmemBytes;
     cfg.stream = st;
