@@ -6,11 +6,13 @@
 // kind::f8f6f4) into an accumulator of its own in tensor memory, which the epilogue takes out, multiplies by xs * ws and adds up in registers: lane = weight
 // row, register = token.  The products and block sums are the tensor core's (codes have 4 bits, their products are exact), the sums over blocks f32.
 //
-// Bound by reading the weights once: a block of an item is 16 KB of them, 700 cycles of an SM's share of the memory's rate, against 128 to 256 cycles of MMAs and
-// about as many of epilogue.  So the ring is what matters: two CTAs an SM with some 100 KB of stages each, one CTA an item; few tokens and few rows of
-// weights: K is cut into up to 8 slices, the CTAs of a cluster, which add up through shared memory in the order of K.
+// Bound by reading the weights once: a block of an item is 16 KB of them, 700 cycles of an SM's share of the memory's rate, against 128 cycles of MMAs.  Two CTAs an SM with
+// some 100 KB of stages each walk the items, the copies running ahead from one to the next; with few items and no experts K is cut into up to 8
+// slices, the CTAs of a cluster, which add up through shared memory in the order of K.  What an item takes beside its bytes is the way through the hand-offs: a wait, a load of
+// tensor memory and the sums were 470 cycles a block, whatever its columns, so two or four blocks make one hand-off.
+// Measured (graph, us): 1 x 4096 x 4096 7.3, 1 x 14336 x 4096 14 (58.7 MB; each further matrix of that size 9.4, the memory's rate).
 //
-//   warps 0-3  epilogue   accumulators out, scaled, added up, stored (TN = 128: eight warps)
+//   warps 0-3  epilogue   accumulators out, scaled, added up, stored
 //   warp 4     producer   TMA: 128 x 128 codes of the weights, TN x 128 of the tokens, a stage; by cp.async the scales of 16 blocks
 //   warp 5     MMA        and the tensor memory's allocation
 // Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited (bounded too).
@@ -26,17 +28,15 @@ using namespace fp8;
 constexpr int kRows = 128;                       // weight rows of an item: TMEM lanes, MMA M; they share their scales
 constexpr int kWBytes = kRows * kBlock;          // of a stage
 constexpr int kMaxStages = 8;
+constexpr int kEpi = 128, kLoadWarp = 4, kMmaWarp = 5, kThreads = 192, kPerSM = 2;
+constexpr int kSmemBytes = 113 * 1024;           // of one of the two CTAs of an SM
 constexpr int kMaxSlices = 8;
 
 template <int TN>
 struct Form {
-    static constexpr int kGroups = TN == 128 ? 2 : 1;                // of four epilogue warps; each takes its part of the columns
-    static constexpr int kPart = TN / kGroups;
-    static constexpr int kEpi = 128 * kGroups, kLoadWarp = 4 * kGroups, kMmaWarp = kLoadWarp + 1, kThreads = kEpi + 64;
-    static constexpr int kPerSM = TN == 128 ? 1 : 2;                 // CTAs an SM, by shared memory and registers
-    static constexpr int kSmemBytes = kPerSM == 1 ? 226 * 1024 : 113 * 1024;
-    static constexpr int kAcc = 4;                                   // accumulators in tensor memory
-    static constexpr int kCols = kAcc * TN;
+    static constexpr int kTogether = TN == 64 ? 2 : 4;               // blocks of a hand-off to the epilogue
+    static constexpr int kCols = 2 * kTogether * TN;                 // two hand-offs in tensor memory
+    static constexpr int kStep = TN < 32 ? TN : 32, kLoads = 64 / kStep;      // columns of a load of tensor memory, loads at a time
     static constexpr int kHeld = 16;                                 // blocks whose scales are in shared memory, [block][token], twice
     static constexpr int kPitch = TN + 4;
     static constexpr int kStage = kWBytes + TN * kBlock;
@@ -64,7 +64,7 @@ struct TMaps {
 };
 
 struct __align__(16) TCtrl {
-    uint64_t full[kMaxStages], empty[kMaxStages], d_full[4], d_empty[4], s_full[2], s_empty[2], drained;
+    uint64_t full[kMaxStages], empty[kMaxStages], d_full[2], d_empty[2], s_full[2], s_empty[2], drained;
     uint32_t tmem_base, issued;
     volatile uint32_t abort;
     int n_chunks;                                // of all experts, or of the dense rows
@@ -126,19 +126,19 @@ __device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts
 }
 
 // Giving up, once every role has ended: lets what is on its way arrive before the CTA tears down.
-__device__ __noinline__ void rest(TCtrl *ctl, int stages, int load_warp) {
+__device__ __noinline__ void rest(TCtrl *ctl, int stages) {
     const int warp = threadIdx.x >> 5;
-    if (warp == load_warp + 1 && elect_one()) {
+    if (warp == kMmaWarp && elect_one()) {
         umma_commit(&ctl->drained);
         drain_ring(&ctl->drained, 1, 1);
-    } else if (warp == load_warp && (threadIdx.x & 31) == 0) {
+    } else if (warp == kLoadWarp && (threadIdx.x & 31) == 0) {
         drain_ring(ctl->full, ctl->issued, stages);
     }
     __syncthreads();
 }
 
 template <int TN>
-__global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
     using F = Form<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -153,13 +153,11 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
             mbar_init(&ctl->full[s], 1);
             mbar_init(&ctl->empty[s], 1);
         }
-        for (int s = 0; s < F::kAcc; ++s) {
-            mbar_init(&ctl->d_full[s], 1);
-            mbar_init(&ctl->d_empty[s], F::kEpi / 32);
-        }
         for (int s = 0; s < 2; ++s) {
+            mbar_init(&ctl->d_full[s], 1);
+            mbar_init(&ctl->d_empty[s], kEpi / 32);
             mbar_init(&ctl->s_full[s], 32);
-            mbar_init(&ctl->s_empty[s], F::kEpi / 32);
+            mbar_init(&ctl->s_empty[s], kEpi / 32);
         }
         mbar_init(&ctl->drained, 1);
         ctl->abort = 0;
@@ -167,13 +165,13 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
         ctl->n_chunks = a.chunks;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == F::kMmaWarp) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)), "n"(F::kCols));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (a.expert_offsets) {
         pdl_enter();
-        if (warp == F::kLoadWarp) {
+        if (warp == kLoadWarp) {
             Chunk none;
             const int n = find_chunk(a.expert_offsets, a.n_experts, a.M, TN, -1, blockIdx.x == 0 ? a.status : nullptr, none);
             __syncwarp();
@@ -199,7 +197,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
         return c;
     };
 
-    if (warp == F::kLoadWarp) {
+    if (warp == kLoadWarp) {
         int s = 0;
         uint32_t phase = 1, s_phase = 1;         // of `empty`: the first round passes
         int b = 0;
@@ -259,70 +257,78 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == F::kMmaWarp) {
+    } else if (warp == kMmaWarp) {
         constexpr uint32_t idesc = 1u << 4 | static_cast<uint32_t>(TN >> 3) << 17 | static_cast<uint32_t>(kRows >> 4) << 24;
         int s = 0, d = 0;
         uint32_t phase = 0, d_phase = 1;
         bool go = true;
         for (int unit = first; go && unit < units; unit += step)
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u) || !wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) {
-                    go = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
-                if (elect_one()) {
+            for (int kb = kb0; go && kb < kb1; kb += F::kTogether) {
+                const int here = min(F::kTogether, kb1 - kb);
+                go = wait_all(&ctl->d_empty[d], d_phase, &ctl->abort, a.status, 0xb02u);
+                for (int g = 0; go && g < here; ++g) {
+                    if (!wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb03u)) {
+                        go = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t wd = make_desc_sw128(ring + s * F::kStage), xd = make_desc_sw128(ring + s * F::kStage + kWBytes);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_f8(tmem + d * TN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
-                    umma_commit(&ctl->d_full[d]);
-                    umma_commit(&ctl->empty[s]);
+                        for (int k = 0; k < 4; ++k) mma_f8(tmem + (d * F::kTogether + g) * TN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
+                        umma_commit(&ctl->empty[s]);
+                        if (g == here - 1) umma_commit(&ctl->d_full[d]);
+                    }
+                    __syncwarp();
+                    if (++s == F::kStages) s = 0, phase ^= 1;
                 }
-                __syncwarp();
-                if (++s == F::kStages) s = 0, phase ^= 1;
-                if (++d == F::kAcc) d = 0, d_phase ^= 1;
+                if (d ^= 1; d == 0) d_phase ^= 1;
             }
     } else {
         if (!a.expert_offsets) asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int part0 = F::kGroups == 1 ? 0 : warp / 4 * F::kPart;                    // first column (token) of this warp's part
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + part0;      // lane 32 * warp in bits 16 and up
-        const int r = threadIdx.x & (kRows - 1);
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);              // lane 32 * warp in bits 16 and up
+        const int r = threadIdx.x;
         int d = 0, b = 0;
         uint32_t phase = 0, s_phase = 0;
         for (int unit = first; unit < units; unit += step) {
             const Chunk c = chunk_of(unit);
             const int tile = tile_of(unit);
-            uint64_t acc[F::kPart / 2] = {};
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int at = (kb - kb0) % F::kHeld;
-                const float *const f = scales + b * F::kScales + at * F::kPitch + part0;
+            uint64_t acc[TN / 2] = {};
+            for (int kb = kb0; kb < kb1; kb += F::kTogether) {
+                const int at = (kb - kb0) % F::kHeld, here = min(F::kTogether, kb1 - kb);
+                const float *const held = scales + b * F::kScales;
                 if (at == 0) wait_soon(&ctl->s_full[b], s_phase, &ctl->abort, a.status, 0xb06u);
-                const float ws = scales[b * F::kScales + F::kHeld * F::kPitch + at];
                 wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb04u);
                 __syncwarp();
                 tc_fence_after();
-                constexpr int STEP = TN < 32 ? TN : 32, LOADS = F::kPart / STEP;
-                uint32_t v[LOADS > 1 ? 2 : 1][STEP];
-                tmem_ld<STEP>(lanes + d * TN, v[0]);
 #pragma unroll
-                for (int q = 0; q < LOADS; ++q) {
-                    tmem_wait_ld(v[q & 1]);
-                    if (q + 1 < LOADS) {
-                        tmem_ld<STEP>(lanes + d * TN + (q + 1) * STEP, v[~q & 1]);
-                    } else {
+                for (int q = 0; q < F::kTogether * TN; q += F::kLoads * F::kStep) {     // 64 columns at a time: of four blocks, of two, or of one
+                    uint32_t v[F::kLoads][F::kStep];
+#pragma unroll
+                    for (int l = 0; l < F::kLoads; ++l) tmem_ld<F::kStep>(lanes + d * F::kTogether * TN + q + l * F::kStep, v[l]);
+#pragma unroll
+                    for (int l = 0; l < F::kLoads; ++l) tmem_wait_ld(v[l]);
+                    if (q + F::kLoads * F::kStep == F::kTogether * TN) {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&ctl->d_empty[d]);
                     }
 #pragma unroll
-                    for (int i = 0; i < STEP; i += 4) {
-                        const float4 w = *reinterpret_cast<const float4 *>(f + q * STEP + i);
-                        fma2(acc[(q * STEP + i) / 2], v[q & 1][i], v[q & 1][i + 1], w.x * ws, w.y * ws);
-                        fma2(acc[(q * STEP + i) / 2 + 1], v[q & 1][i + 2], v[q & 1][i + 3], w.z * ws, w.w * ws);
+                    for (int l = 0; l < F::kLoads; ++l) {
+                        const int g = (q + l * F::kStep) / TN, col = (q + l * F::kStep) % TN;
+                        if (g >= here) break;
+                        const float *const f = held + (at + g) * F::kPitch + col;
+                        const float ws = held[F::kHeld * F::kPitch + at + g];
+#pragma unroll
+                        for (int i = 0; i < F::kStep; i += 4) {
+                            const float4 w = *reinterpret_cast<const float4 *>(f + i);
+                            fma2(acc[(col + i) / 2], v[l][i], v[l][i + 1], w.x * ws, w.y * ws);
+                            fma2(acc[(col + i) / 2 + 1], v[l][i + 2], v[l][i + 3], w.z * ws, w.w * ws);
+                        }
                     }
                 }
-                if (++d == F::kAcc) d = 0, phase ^= 1;
-                if (at == F::kHeld - 1 || kb == kb1 - 1) {
+                if (d ^= 1; d == 0) phase ^= 1;
+                if (at + F::kTogether == F::kHeld || kb + F::kTogether >= kb1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl->s_empty[b]);
                     if (b ^= 1; b == 0) s_phase ^= 1;
@@ -332,18 +338,16 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
             if (a.slices == 1) {
                 if (n < a.N && !ctl->abort) {
 #pragma unroll
-                    for (int i = 0; i < F::kPart; i += 2) {
-                        const float2 v = halves(acc[i / 2]);
-                        const int t = part0 + i;
+                    for (int t = 0; t < TN; t += 2) {
+                        const float2 v = halves(acc[t / 2]);
                         if (t < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t) * a.N + n, v.x, a.out_dt);
                         if (t + 1 < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t + 1) * a.N + n, v.y, a.out_dt);
                     }
                 }
             } else {                             // one unit a cluster: the sums of a slice go where the ring was, [token][weight row]
 #pragma unroll
-                for (int i = 0; i < F::kPart; i += 2) {
-                    const float2 v = halves(acc[i / 2]);
-                    const int t = part0 + i;
+                for (int t = 0; t < TN; t += 2) {
+                    const float2 v = halves(acc[t / 2]);
                     if (t < c.ntok) st_shared(ring + (t * kRows + r) * 4, v.x);
                     if (t + 1 < c.ntok) st_shared(ring + ((t + 1) * kRows + r) * 4, v.y);
                 }
@@ -351,14 +355,13 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
         }
     }
     __syncthreads();
-    if (ctl->abort) rest(ctl, F::kStages, F::kLoadWarp);
+    if (ctl->abort) rest(ctl, F::kStages);
     if (a.slices > 1) {                          // slice r adds up tokens r, r + slices, ... of all slices
         cluster_sync();
-        if (first < units && warp < F::kLoadWarp && !ctl->abort) {
+        if (first < units && warp < kLoadWarp && !ctl->abort) {
             const Chunk c = chunk_of(first);
-            const int r = threadIdx.x & (kRows - 1), n = tile_of(first) * kRows + r;
-            const int every = F::kGroups * a.slices;
-            for (int t0 = rank + (warp / 4) * a.slices; t0 < c.ntok && n < a.N; t0 += 4 * every) {
+            const int r = threadIdx.x, n = tile_of(first) * kRows + r, every = a.slices;
+            for (int t0 = rank; t0 < c.ntok && n < a.N; t0 += 4 * every) {
                 float part[4][kMaxSlices];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(Form<TN>::kThreads, Form<TN>::kPerSM) fp8_tile
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == F::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kCols));
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kCols));
 }
 
 template <int TN>
@@ -389,15 +392,15 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w
     if (e == cudaSuccess) e = make_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, a.M, K, TN, kBlock, why);
     if (e != cudaSuccess) return e;
     static PerDeviceAttr attr;
-    if ((e = attr.set(fp8_tile_kernel<TN>, Form<TN>::kSmemBytes)) != cudaSuccess) return e;
+    if ((e = attr.set(fp8_tile_kernel<TN>, kSmemBytes)) != cudaSuccess) return e;
     const long long units = a.expert_offsets ? (static_cast<long long>(std::min(a.M, a.n_experts)) + a.M / TN) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
     if (units > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     // slices: a cluster a unit; else no more CTAs than run at once, each with units in turn
-    const long long ctas = a.slices > 1 ? units * a.slices : std::min<long long>(units, static_cast<long long>(Form<TN>::kPerSM) * ctx->sm_count);
+    const long long ctas = a.slices > 1 ? units * a.slices : std::min<long long>(units, static_cast<long long>(kPerSM) * ctx->sm_count);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-    cfg.blockDim = dim3(Form<TN>::kThreads);
-    cfg.dynamicSmemBytes = Form<TN>::kSmemBytes;
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
     cfg.stream = st;
     cudaLaunchAttribute la[2];
     la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -415,7 +418,7 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w
 // K slices: as many as fill the SMs' places once, at least four blocks each
 static int slices_for(int sms, long long units, int nkb) {
     int s = 1;
-    while (s < kMaxSlices && units * (s + 1) <= 2ll * sms && nkb / (s + 1) >= 4) ++s;
+    while (s < kMaxSlices && units * (s + 1) <= static_cast<long long>(kPerSM) * sms && nkb / (s + 1) >= 4) ++s;
     return s;
 }
 
@@ -437,17 +440,18 @@ cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     a.n_experts = n_experts;
     a.tiles = blocks(N);
     a.out_dt = out_dt;
-    const int rows = expert_offsets ? (M + n_experts - 1) / n_experts * 2 : M;       // that a tile may have to hold
-    const int TN = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    // Tokens of a tile.  Dense: what holds them, but 64 as two of 32, whose epilogues share the work (64 x 4096 x 4096 10.0 us, in one of 64 11.1).  Grouped: 16 below eight rows
+    // an expert on average (128 experts of 768 x 2048: 4 rows 26.0 us, with 32 29.6; 8 rows 32.9 and 31.6; 32 rows 47.0, with 64 50.4).  128 were slower than both this and pairs.
+    const int rows = expert_offsets ? (M >= 8 * n_experts ? 32 : 16) : M;
+    const int TN = rows <= 16 ? 16 : rows <= 64 ? 32 : 64;
     a.chunks = (M + TN - 1) / TN;
-    const long long units = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
-    a.slices = slices_for(ctx->sm_count, units, a.nkb);
+    // An expert's tiles never make slices: what a cluster costs is more than it gives (32 experts of 1536 x 2048, 8 rows: 9.5 us, in slices 16.0)
+    a.slices = expert_offsets ? 1 : slices_for(ctx->sm_count, static_cast<long long>(a.chunks) * a.tiles, a.nkb);
     a.early = expert_offsets ? 0 : early_weights(ctx, st);
     switch (TN) {
         case 16: return launch<16>(ctx, st, x, w, a, K, why);
         case 32: return launch<32>(ctx, st, x, w, a, K, why);
-        case 64: return launch<64>(ctx, st, x, w, a, K, why);
-        default: return launch<128>(ctx, st, x, w, a, K, why);
+        default: return launch<64>(ctx, st, x, w, a, K, why);
     }
 }
 

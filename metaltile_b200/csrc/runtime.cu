@@ -1502,7 +1502,7 @@ static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_exper
     if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, x, w)) return FP8_CUDA_CORE;
     const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
     if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
-    return pair && (grouped ? M / n_experts >= 96 : M >= 256) ? FP8_PAIR : FP8_TILE;
+    return pair && (grouped ? M / n_experts >= 48 : M > 128) ? FP8_PAIR : FP8_TILE;
 }
 
 static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_t *x, const float *xs, const void *w, const void *ws, const void *expert_offsets, void *out,
