@@ -176,23 +176,25 @@ __device__ __forceinline__ uint4 piece(const uint64_t (&acc)[64], int i) {
     }
 }
 
-// A warp's 32 rows x 128 columns.  All rows there: through shared memory, 128 bytes a row at a time, and out by TMA, which goes on while the next tile's blocks are added
-// (a lane storing its own row costs the load pipe a cycle a row and 16 bytes: 67 us of 330 for 2048 x 28672 x 4096).  Else every lane its own row.
+// A warp's rows (32 at most) x 128 columns, through shared memory, 128 bytes a row at a time: all 32 rows out by TMA, which goes on while the next tile's blocks are
+// added; fewer, or rows that 16-byte pieces do not fit, by stores that run along the rows.  (A lane storing its own row costs the load pipe a cycle a row and store:
+// 67 us of 330 for 2048 x 28672 x 4096 in 16-byte pieces, and 30 us for one tile of odd rows, element by element.)
 template <int DT>
 __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[64], uint32_t staged, int row, int rows, int n) {
-    constexpr int PER = DT == MTC_F32 ? 4 : 8;                       // results of a piece
+    constexpr int PER = DT == MTC_F32 ? 4 : 8;                       // results of a 16-byte piece
     const int lane = threadIdx.x & 31;
-    if (a.wide && rows >= 32) {
+    const bool whole = a.wide && rows >= 32;
 #pragma unroll
-        for (int c = 0; c < 128; c += 8 * PER) {
-            if (n + c >= a.N) break;
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
+    for (int c = 0; c < 128; c += 8 * PER) {
+        if (n + c >= a.N) break;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const uint4 v = piece<DT>(acc, (c + q * PER) / 2);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            }
+        for (int q = 0; q < 8; ++q) {
+            const uint4 v = piece<DT>(acc, (c + q * PER) / 2);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        }
+        if (whole) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
@@ -200,22 +202,37 @@ __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, co
                              ::"l"(reinterpret_cast<uint64_t>(&maps.out)), "r"(n + c), "r"(row), "r"(staged) : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+            continue;
         }
-    } else if (lane < rows) {
-        const size_t at = static_cast<size_t>(row + lane) * a.N + n;
-#pragma unroll
-        for (int c = 0; c < 128; c += PER) {
-            if (n + c >= a.N) break;
-            if (a.wide) {
-                *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (at + c) * (16 / PER)) = piece<DT>(acc, c / 2);
-            } else {
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const float2 v = halves(acc[(c + j) / 2]);
-                    if (n + c + j < a.N) st_from_f32(a.out, at + c + j, j & 1 ? v.y : v.x, DT);
+        __syncwarp();
+        if (a.wide) {                            // eight lanes a row
+            const int q = lane & 7;
+            if (n + c + q * PER < a.N) {
+                for (int i = lane >> 3; i < min(rows, 32); i += 4) {
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged + i * 128 + ((q ^ (i & 7)) << 4)));
+                    *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (static_cast<size_t>(row + i) * a.N + n + c + q * PER) * (16 / PER)) = v;
                 }
             }
+        } else {
+            for (int i = 0; i < min(rows, 32); ++i)
+#pragma unroll
+                for (int e = lane; e < 8 * PER; e += 32) {
+                    if (n + c + e >= a.N) break;
+                    const uint32_t from = staged + i * 128 + (((e / PER) ^ (i & 7)) << 4) + e % PER * (16 / PER);
+                    const size_t to = static_cast<size_t>(row + i) * a.N + n + c + e;
+                    if constexpr (DT == MTC_F32) {
+                        uint32_t v;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(from));
+                        static_cast<uint32_t *>(a.out)[to] = v;
+                    } else {
+                        uint16_t v;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from));
+                        static_cast<uint16_t *>(a.out)[to] = v;
+                    }
+                }
         }
+        __syncwarp();                            // read before the next piece is written
     }
 }
 
