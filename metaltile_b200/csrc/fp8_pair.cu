@@ -8,12 +8,13 @@
 //
 // What bounds it.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM of a pair: 64 bytes a
 // cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Without the epilogue the ring and the MMAs run at 585 cycles a block.  With it a
-// block takes 860: 64 packed FMAs, as many moves and four loads of tensor memory in a row in each of eight warps.  Two accumulators are all of the tensor memory, so the
-// MMAs of one block run while the one before is read, no further.  2048 x 28672 x 4096: 226 us, 2.1 PFLOP/s.
+// block takes 780: two accumulators are all of the tensor memory, so a block's MMAs (512), the way to the epilogue, its four loads of tensor memory in a row, the way
+// back and the issue of the next are one chain for two blocks.  2048 x 28672 x 4096: 214 us, 2.25 PFLOP/s.
 //
 // Steps on the way (us for that case): hand-offs that release at cluster scope 587, relaxed ones 348; one try in front of the polling loop, whose entry costs 200 cycles,
 // and results out by TMA instead of a row a lane 303; the registers of the other roles for the epilogue, so that nothing spills, and the next columns loaded while the
-// last are added 235; MMAs of 256 columns instead of two chains of 128, which read A twice, 226.  16 epilogue warps of 64 columns: 297 (104 registers each spill).
+// last are added 235; MMAs of 256 columns instead of two chains of 128, which read A twice, 226; 32-bit
+// addresses and one plain loop over the blocks in the epilogue 214.  16 epilogue warps of 64 columns: 264 (96 registers each spill).
 //
 //   warps 0-7    epilogue   warps 0-3 the first half of the weight rows, 4-7 the second
 //   warps 8-9    scales     xs of 128 tokens, 16 blocks at a time, and ws, by cp.async into shared memory (a load of each lane's own row would cost the load pipe ten
@@ -36,7 +37,7 @@ constexpr int kABytes = 128 * kBlock, kBBytes = 128 * kBlock, kStage = kABytes +
 constexpr int kStages = 4;                       // (five: the same)
 constexpr int kOutBytes = 4096;                  // of an epilogue warp: 32 rows x 128 bytes of results on their way out
 constexpr int kEpiWarps = 8, kScaleWarp0 = 8, kScaleWarps = 2, kLoadWarp = 10, kMmaWarp = 11, kThreads = 384;
-constexpr int kHeld = 16, kPitch = 20;           // blocks whose scales are in shared memory, floats of a row of xs (four-float loads of 8 neighbouring rows meet no bank twice)
+constexpr int kHeld = 16, kPitch = 20;           // blocks whose scales are in shared memory, floats of a row of xs
 constexpr int kScaleFloats = 128 * kPitch + 2 * kHeld;
 constexpr int kMaxExperts = 1024;
 
@@ -124,6 +125,22 @@ __device__ void count_chunks(PCtrl *ctl, const PArgs &a) {
         ctl->first_chunk[a.n_experts] = before;
         ctl->n_chunks = before;
     }
+}
+
+// Waits of the epilogue by addresses: its registers are sums and values on their way, and a 64-bit pointer more makes them spill.  Not inlined: the way that rarely runs.
+__device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, uint32_t abort, uint32_t *status, uint32_t code) {
+    const uint32_t r = mbar_poll(bar, parity, abort);
+    if (r != 1) mbar_gave_up(r, abort, status, code);
+}
+__device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, uint32_t abort, uint32_t *status, uint32_t code) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (!ok) wait_long(bar, parity, abort, status, code);
+}
+__device__ __forceinline__ float ld_shared(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 struct Tile {
@@ -364,58 +381,45 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");         // 256 threads x 224 + 128 x 56 = 384 x 168 that the block starts with
-        const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int h = warp >> 2;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + h * 128;
-        const uint32_t freed = on_cta(smem_u32(&ctl->d_empty[0]), 0);
+        const uint32_t bars = staged - kCtlBytes - kScaleBytes;                          // the control block
+        const uint32_t freed = on_cta(bars + offsetof(PCtrl, d_empty), 0);
+        const uint32_t xs_at = bars + kCtlBytes + ((warp & 3) * 32 + lane) * kPitch * 4, ws_at = bars + kCtlBytes + (128 * kPitch + h * kHeld) * 4;
         int d = 0, b = 0;
         uint32_t phase = 0, s_phase = 0;
         for (int i = pair; i < n_tiles; i += pairs) {
-            const Tile t = tile_of(ctl, a, i);
             uint64_t acc[64] = {};
             uint32_t v[2][32];                   // the next columns are on their way while these are added
-            bool early = false;
-            for (int kb = 0; kb < a.nkb; kb += 4) {
-                const int at = kb % kHeld, here = min(4, a.nkb - kb);
-                const float *const held = scales + b * kScaleFloats;
-                if (at == 0) wait_soon(&ctl->s_full[b], s_phase, &ctl->abort, a.status, 0xb15u);
-                const float4 fx = *reinterpret_cast<const float4 *>(held + r * kPitch + at), fw = *reinterpret_cast<const float4 *>(held + 128 * kPitch + h * kHeld + at);
-                float f = fx.x * fw.x, f1 = fx.y * fw.y, f2 = fx.z * fw.z, f3 = fx.w * fw.w;
-                if (at + 4 == kHeld || kb + 4 >= a.nkb) {
+            for (int kb = 0; kb < a.nkb; ++kb) {
+                const int at = kb % kHeld;
+                if (at == 0) wait_at(bars + offsetof(PCtrl, s_full) + b * 8, s_phase, bars + offsetof(PCtrl, abort), a.status, 0xb15u);
+                const float f = ld_shared(xs_at + (b * kScaleFloats + at) * 4) * ld_shared(ws_at + (b * kScaleFloats + at) * 4);
+                wait_at(bars + offsetof(PCtrl, d_full) + d * 8, phase, bars + offsetof(PCtrl, abort), a.status, 0xb16u);
+                __syncwarp();
+                tc_fence_after();
+                tmem_ld<32>(lanes + d * 256, v[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_wait_ld(v[c & 1]);
+                    if (c < 3) {
+                        tmem_ld<32>(lanes + d * 256 + (c + 1) * 32, v[~c & 1]);
+                    } else {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_at(freed + d * 8);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) fma2(acc[c * 16 + j / 2], v[c & 1][j], v[c & 1][j + 1], f, f);
+                }
+                if (d ^= 1; d == 0) phase ^= 1;
+                if (at == kHeld - 1 || kb == a.nkb - 1) {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->s_empty[b]);
+                    if (lane == 0) mbar_arrive(bars + offsetof(PCtrl, s_empty) + b * 8);
                     if (b ^= 1; b == 0) s_phase ^= 1;
                 }
-#pragma unroll 1
-                for (int u = 0; u < here; ++u) {
-                    if (!early) {
-                        wait_soon(&ctl->d_full[d], phase, &ctl->abort, a.status, 0xb16u);
-                        __syncwarp();
-                        tc_fence_after();
-                        tmem_ld<32>(lanes + d * 256, v[0]);
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_wait_ld(v[c & 1]);
-                        if (c < 3) {
-                            tmem_ld<32>(lanes + d * 256 + (c + 1) * 32, v[~c & 1]);
-                        } else {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) arrive_at(freed + d * 8);
-                            if (d ^= 1; d == 0) phase ^= 1;
-                            // the next block's first columns, if they are there, come while the last of this one are added
-                            early = kb + u + 1 < a.nkb && __all_sync(0xffffffffu, mbar_try(&ctl->d_full[d], phase));
-                            if (early) {
-                                tc_fence_after();
-                                tmem_ld<32>(lanes + d * 256, v[0]);
-                            }
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) fma2(acc[c * 16 + j / 2], v[c & 1][j], v[c & 1][j + 1], f, f);
-                    }
-                    f = f1, f1 = f2, f2 = f3;
-                }
             }
+            const Tile t = tile_of(ctl, a, i);
             if (ctl->abort) continue;
             const int first = rank * 128 + (warp & 3) * 32, rows = t.ntok - first, n = t.n0 + h * 128;
             if (rows <= 0 || n >= a.N) continue;
