@@ -66,6 +66,7 @@ constexpr int kCtlBytes = (sizeof(PCtrl) + 1023) / 1024 * 1024;
 constexpr int kScaleBytes = (2 * kScaleFloats * 4 + 1023) / 1024 * 1024;
 constexpr int kSmemBytes = 1024 + kCtlBytes + kScaleBytes + 8 * kOutBytes + kStages * kStage;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+static_assert(kStages * kStage >= 128 * kCols * 4, "the sums of a slice go where the ring was");
 
 __device__ __forceinline__ uint32_t on_cta(uint32_t addr, uint32_t rank) {
     uint32_t r;
@@ -84,10 +85,10 @@ __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uin
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-// arrives at the barrier of this offset in both CTAs when the MMAs so far are complete
-__device__ __forceinline__ void commit_pair(uint64_t *bar) {
+// arrives at the barrier of this offset in both CTAs (a bit each of their rank in the cluster) when the MMAs so far are complete
+__device__ __forceinline__ void commit_pair(uint64_t *bar, uint32_t both) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(3)) : "memory");
+                 ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(both)) : "memory");
 }
 // Relaxed: what it hands over is tensor memory, ordered by the tcgen05 fence in front.  (A release at cluster scope waits for everything the thread has in flight: 1150
 // cycles a block, 2048 x 28672 x 4096 in 587 us instead of 348.)
@@ -171,8 +172,8 @@ __device__ __forceinline__ Tile tile_of(const PCtrl *ctl, const PArgs &a, int in
 }
 
 // Sixteen bytes of neighbouring results from the sums acc[i] on: eight of 16 bits, four of 32
-template <int DT>
-__device__ __forceinline__ uint4 piece(const uint64_t (&acc)[64], int i) {
+template <int DT, int N>
+__device__ __forceinline__ uint4 piece(const uint64_t (&acc)[N], int i) {
     uint32_t w[4];
     if constexpr (DT == MTC_F32) {
         const float2 lo = halves(acc[i]), hi = halves(acc[i + 1]);
@@ -193,21 +194,22 @@ __device__ __forceinline__ uint4 piece(const uint64_t (&acc)[64], int i) {
     }
 }
 
-// A warp's rows (32 at most) x 128 columns, through shared memory, 128 bytes a row at a time: all 32 rows out by TMA, which goes on while the next tile's blocks are
+// A warp's rows (32 at most) x NC columns, through shared memory, 128 bytes a row at a time: all 32 rows out by TMA, which goes on while the next tile's blocks are
 // added; fewer, or rows that 16-byte pieces do not fit, by stores that run along the rows.  (A lane storing its own row costs the load pipe a cycle a row and store:
 // 67 us of 330 for 2048 x 28672 x 4096 in 16-byte pieces, and 30 us for one tile of odd rows, element by element.)
-template <int DT>
-__device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[64], uint32_t staged, int row, int rows, int n) {
+template <int DT, int NC>
+__device__ __forceinline__ void store_rows_as(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[NC / 2], uint32_t staged, int row, int rows, int n) {
     constexpr int PER = DT == MTC_F32 ? 4 : 8;                       // results of a 16-byte piece
+    constexpr int NP = NC < 8 * PER ? NC / PER : 8;                  // pieces of a row at a time
     const int lane = threadIdx.x & 31;
-    const bool whole = a.wide && rows >= 32;
+    const bool whole = NP == 8 && a.wide && rows >= 32;
 #pragma unroll
-    for (int c = 0; c < 128; c += 8 * PER) {
+    for (int c = 0; c < NC; c += NP * PER) {
         if (n + c >= a.N) break;
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < NP; ++q) {
             const uint4 v = piece<DT>(acc, (c + q * PER) / 2);
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
         }
@@ -222,10 +224,10 @@ __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, co
             continue;
         }
         __syncwarp();
-        if (a.wide) {                            // eight lanes a row
-            const int q = lane & 7;
+        if (a.wide) {                            // NP lanes a row
+            const int q = lane % NP;
             if (n + c + q * PER < a.N) {
-                for (int i = lane >> 3; i < min(rows, 32); i += 4) {
+                for (int i = lane / NP; i < min(rows, 32); i += 32 / NP) {
                     uint4 v;
                     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staged + i * 128 + ((q ^ (i & 7)) << 4)));
                     *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + (static_cast<size_t>(row + i) * a.N + n + c + q * PER) * (16 / PER)) = v;
@@ -234,7 +236,7 @@ __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, co
         } else {
             for (int i = 0; i < min(rows, 32); ++i)
 #pragma unroll
-                for (int e = lane; e < 8 * PER; e += 32) {
+                for (int e = lane; e < NP * PER; e += 32) {
                     if (n + c + e >= a.N) break;
                     const uint32_t from = staged + i * 128 + (((e / PER) ^ (i & 7)) << 4) + e % PER * (16 / PER);
                     const size_t to = static_cast<size_t>(row + i) * a.N + n + c + e;
@@ -253,6 +255,52 @@ __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, co
     }
 }
 
+template <int NC>
+__device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[NC / 2], uint32_t staged, int row, int rows, int n) {
+    if (rows <= 0 || n >= a.N) return;
+    if (a.out_dt == MTC_BF16) store_rows_as<MTC_BF16, NC>(maps, a, acc, staged, row, rows, n);
+    else if (a.out_dt == MTC_F16) store_rows_as<MTC_F16, NC>(maps, a, acc, staged, row, rows, n);
+    else store_rows_as<MTC_F32, NC>(maps, a, acc, staged, row, rows, n);
+}
+
+// The sums of all S slices of this CTA's tokens, and out: a warp its 32 tokens x 128 / S columns, 32 at a time.  Sums lie as [column][token] where the ring was, in the
+// CTAs of the same rank of each pair; they are added in the order of K.
+template <int S>
+__device__ __forceinline__ void join_slices(const PMaps &maps, const PArgs &a, uint32_t sums, uint32_t staged, int slice, int rank, int first, int rows, const Tile &t) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int p = 0; p < 4 / S; ++p) {
+        const int c0 = (warp >> 2) * 128 + (slice * (4 / S) + p) * 32;
+        uint64_t acc[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 16) {       // sixteen columns in flight
+            float v[S][16];
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                const uint32_t from = on_cta(sums + ((c0 + c) * 128 + (warp & 3) * 32 + lane) * 4, 2 * q + rank);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q][i]) : "r"(from + i * 512) : "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                float lo = v[0][i], hi = v[0][i + 1];
+#pragma unroll
+                for (int q = 1; q < S; ++q) lo += v[q][i], hi += v[q][i + 1];
+                asm("mov.b64 %0, {%1, %2};" : "=l"(acc[(c + i) / 2]) : "f"(lo), "f"(hi));
+            }
+        }
+        store_rows<32>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, t.n0 + c0);
+    }
+}
+
+// Registers: 384 threads start with 168, 256 of them go on with more and 128 with fewer.  What leaves the epilogue's loop without spills, or with the fewest.
+template <int SLICES>
+constexpr int kEpiRegs = SLICES == 4 ? 216 : 224;
+template <int SLICES>
+constexpr int kOtherRegs = 3 * 168 - 2 * kEpiRegs<SLICES>;
+
+// SLICES of K: pairs of a cluster that own a tile together; 1: a pair walks tiles.
+template <int SLICES>
 __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_constant__ PMaps maps, const __grid_constant__ PArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -260,7 +308,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     float *const scales = reinterpret_cast<float *>(smem + kCtlBytes);       // two of [128][kPitch] of xs, [2][kHeld] of ws
     const uint32_t staged = __shfl_sync(0xffffffffu, smem_u32(smem), 0) + kCtlBytes + kScaleBytes, ring = staged + kEpiWarps * kOutBytes;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int rank = static_cast<int>(blockIdx.x & 1), pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+    const int in_cluster = static_cast<int>(blockIdx.x) % (2 * SLICES), rank = in_cluster & 1, slice = in_cluster >> 1, leader = SLICES == 1 ? 0 : in_cluster & ~1;
+    const int pair = static_cast<int>(blockIdx.x) / (2 * SLICES), pairs = static_cast<int>(gridDim.x) / (2 * SLICES);
+    const int kb0 = SLICES == 1 ? 0 : static_cast<int>(static_cast<long long>(a.nkb) * slice / SLICES);
+    const int kb1 = SLICES == 1 ? a.nkb : static_cast<int>(static_cast<long long>(a.nkb) * (slice + 1) / SLICES);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&ctl->full[s], 1);
@@ -294,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     const int n_tiles = static_cast<int>(ctl->n_chunks) * a.col_tiles;
 
     if (warp == kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs<SLICES>));
         if (lane == 0) {
             int s = 0;
             uint32_t phase = 1;
@@ -302,12 +353,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
             for (int i = pair; go && i < n_tiles; i += pairs) {
                 const Tile t = tile_of(ctl, a, i);
                 const int row = static_cast<int>(static_cast<long long>(t.expert) * a.N) + t.n0 + rank * 128;
-                for (int kb = 0; kb < a.nkb; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb11u)) {
                         go = false;
                         break;
                     }
-                    const uint32_t at = ring + s * kStage, bar = on_cta(smem_u32(&ctl->full[s]), 0);
+                    const uint32_t at = ring + s * kStage, bar = on_cta(smem_u32(&ctl->full[s]), leader);
                     if (rank == 0) mbar_expect_tx(&ctl->full[s], 2 * kStage);
                     tma_load_pair(at, &maps.x, kb * kBlock, t.tok0 + rank * 128, bar);
                     tma_load_pair(at + kABytes, &maps.w, kb * kBlock, row, bar);
@@ -317,14 +368,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
             }
         }
     } else if (warp == kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs<SLICES>));
         if (rank == 0) {                         // the whole warp walks the loop, so that the operands of the MMAs are uniform; one thread issues
             constexpr uint32_t idesc = 1u << 4 | (256u >> 3) << 17 | (256u >> 4) << 24;
             int s = 0, d = 0;
             uint32_t phase = 0, d_phase = 1;
             bool go = true;
             for (int i = pair; go && i < n_tiles; i += pairs)
-                for (int kb = 0; kb < a.nkb; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!wait_all(&ctl->full[s], phase, &ctl->abort, a.status, 0xb12u)) {
                         go = false;
                         break;
@@ -338,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) mma_pair(tmem + d * 256, xd + 2 * k, wd + 2 * k, idesc, k > 0);
-                        commit_pair(&ctl->d_full[d]);
-                        commit_pair(&ctl->empty[s]);
+                        commit_pair(&ctl->d_full[d], 3u << leader);
+                        commit_pair(&ctl->empty[s], 3u << leader);
                     }
                     __syncwarp();
                     if (++s == kStages) s = 0, phase ^= 1;
@@ -347,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                 }
         }
     } else if (warp >= kScaleWarp0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs<SLICES>));
         const int half = warp - kScaleWarp0;     // of the CTA's 128 tokens
         const int k = lane & (kHeld - 1), r0 = lane / kHeld;
         int b = 0;
@@ -357,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
             const Tile t = tile_of(ctl, a, i);
             const int first = rank * 128 + half * 64;
             const float *const ws = a.ws + (static_cast<size_t>(t.expert) * a.row_blocks + t.n0 / kBlock) * a.nkb;
-            for (int kb = 0; kb < a.nkb; kb += kHeld) {
+            for (int kb = kb0; kb < kb1; kb += kHeld) {
                 if (!mbar_wait_vote(&ctl->s_empty[b], phase, &ctl->abort, a.status, 0xb14u)) {
                     go = false;
                     break;
@@ -365,12 +416,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                 // two tokens at a time, 16 blocks of each; what does not exist is filled with zeros
                 const uint32_t to = smem_u32(scales) + (b * kScaleFloats + (half * 64 + r0) * kPitch + k) * 4;
                 const float *const from = a.xs + static_cast<size_t>(t.tok0 + first + r0) * a.nkb + kb + k;
-                const int last = kb + k < a.nkb ? t.ntok - first - r0 : 0;
+                const int last = kb + k < kb1 ? t.ntok - first - r0 : 0;
 #pragma unroll 8
                 for (int r = 0; r < 64; r += 2)
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + r * kPitch * 4), "l"(r < last ? from + static_cast<size_t>(r) * a.nkb : a.xs), "r"(r < last ? 4 : 0) : "memory");
                 if (half == 0) {
-                    const bool there = kb + k < a.nkb && t.n0 / kBlock + r0 < a.row_blocks;
+                    const bool there = kb + k < kb1 && t.n0 / kBlock + r0 < a.row_blocks;
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(scales) + (b * kScaleFloats + 128 * kPitch + lane) * 4),
                                  "l"(there ? ws + static_cast<size_t>(r0) * a.nkb + kb + k : a.ws), "r"(there ? 4 : 0) : "memory");
                 }
@@ -380,19 +431,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");         // 256 threads x 224 + 128 x 56 = 384 x 168 that the block starts with
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs<SLICES>));
         const int h = warp >> 2;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + h * 128;
         const uint32_t bars = staged - kCtlBytes - kScaleBytes;                          // the control block
-        const uint32_t freed = on_cta(bars + offsetof(PCtrl, d_empty), 0);
+        const uint32_t freed = on_cta(bars + offsetof(PCtrl, d_empty), leader);
         const uint32_t xs_at = bars + kCtlBytes + ((warp & 3) * 32 + lane) * kPitch * 4, ws_at = bars + kCtlBytes + (128 * kPitch + h * kHeld) * 4;
         int d = 0, b = 0;
         uint32_t phase = 0, s_phase = 0;
         for (int i = pair; i < n_tiles; i += pairs) {
             uint64_t acc[64] = {};
             uint32_t v[2][32];                   // the next columns are on their way while these are added
-            for (int kb = 0; kb < a.nkb; ++kb) {
-                const int at = kb % kHeld;
+#pragma unroll 1
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int at = (kb - kb0) % kHeld;
                 if (at == 0) wait_at(bars + offsetof(PCtrl, s_full) + b * 8, s_phase, bars + offsetof(PCtrl, abort), a.status, 0xb15u);
                 const float f = ld_shared(xs_at + (b * kScaleFloats + at) * 4) * ld_shared(ws_at + (b * kScaleFloats + at) * 4);
                 wait_at(bars + offsetof(PCtrl, d_full) + d * 8, phase, bars + offsetof(PCtrl, abort), a.status, 0xb16u);
@@ -413,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     for (int j = 0; j < 32; j += 2) fma2(acc[c * 16 + j / 2], v[c & 1][j], v[c & 1][j + 1], f, f);
                 }
                 if (d ^= 1; d == 0) phase ^= 1;
-                if (at == kHeld - 1 || kb == a.nkb - 1) {
+                if (at == kHeld - 1 || kb == kb1 - 1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bars + offsetof(PCtrl, s_empty) + b * 8);
                     if (b ^= 1; b == 0) s_phase ^= 1;
@@ -421,18 +473,37 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
             }
             const Tile t = tile_of(ctl, a, i);
             if (ctl->abort) continue;
-            const int first = rank * 128 + (warp & 3) * 32, rows = t.ntok - first, n = t.n0 + h * 128;
-            if (rows <= 0 || n >= a.N) continue;
-            if (a.out_dt == MTC_BF16) store_rows<MTC_BF16>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
-            else if (a.out_dt == MTC_F16) store_rows<MTC_F16>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
-            else store_rows<MTC_F32>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, rows, n);
+            if constexpr (SLICES == 1) {
+                const int first = rank * 128 + (warp & 3) * 32;
+                store_rows<128>(maps, a, acc, staged + warp * kOutBytes, t.tok0 + first, t.ntok - first, t.n0 + h * 128);
+            } else {                             // the only tile of this cluster: its copies have all arrived, and its MMAs have read them
+#pragma unroll
+                for (int c = 0; c < 128; c += 2) {
+                    const float2 v2 = halves(acc[c / 2]);
+                    const uint32_t to = ring + ((h * 128 + c) * 128 + (warp & 3) * 32 + lane) * 4;
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(to), "f"(v2.x) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 512), "f"(v2.y) : "memory");
+                }
+            }
+        }
+        if constexpr (SLICES > 1) {
+            cluster_sync();                      // the sums of all slices are there
+            if (pair < n_tiles && !ctl->abort) {
+                const Tile t = tile_of(ctl, a, pair);
+                const int first = rank * 128 + (warp & 3) * 32;
+                join_slices<SLICES>(maps, a, ring, staged, slice, rank, first, t.ntok - first, t);
+            }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    if (SLICES > 1 && warp >= kEpiWarps) {     // (the epilogue met this barrier above)
+        __syncwarp();
+        cluster_sync();
     }
     __syncthreads();
     if (ctl->abort) {                            // gave up: let what is on its way arrive (the first CTA's barriers count both CTAs' copies)
         if (warp == kMmaWarp && rank == 0 && elect_one()) {
-            commit_pair(&ctl->drained);
+            commit_pair(&ctl->drained, 3u << leader);
             drain_ring(&ctl->drained, 1, 1);
         } else if (warp == kLoadWarp && rank == 0 && lane == 0) {
             drain_ring(ctl->full, ctl->issued, kStages);
@@ -443,6 +514,50 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     cluster_sync();                              // nobody leaves while the other may still arrive at its barriers or read its memory
     tc_fence_after();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+}
+
+template <int S>
+cudaError_t config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&la)[2], cudaStream_t st, long long clusters) {
+    static PerDeviceAttr attr;
+    const cudaError_t e = attr.set(fp8_pair_kernel<S>, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * 2 * S));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cfg.stream = st;
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = 2 * S;
+    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    return cudaSuccess;
+}
+template <int S>
+cudaError_t launch(cudaStream_t st, const PMaps &maps, const PArgs &a, long long clusters) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute la[2];
+    const cudaError_t e = config<S>(cfg, la, st, clusters);
+    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, fp8_pair_kernel<S>, maps, a);
+}
+// Clusters that the device runs at once: asked for once a device (clusters have to fit into groups of SMs of different sizes).  0 where it cannot be told.
+template <int S>
+int clusters_at_once() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute la[2];
+        if (config<S>(cfg, la, nullptr, 1) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, fp8_pair_kernel<S>, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = -1;
+        }
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 }  // namespace
@@ -474,24 +589,12 @@ cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     if (e == cudaSuccess && a.wide)
         e = make_map_2d(&maps.out, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, size, out, M, N, 32, 128 / size, why);
     if (e != cudaSuccess) return e;
-    static PerDeviceAttr attr;
-    if ((e = attr.set(fp8_pair_kernel, kSmemBytes)) != cudaSuccess) return e;
     const long long chunks = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) + M / kTokens : (M + kTokens - 1) / kTokens, tiles = chunks * a.col_tiles;
-    const int pairs = static_cast<int>(std::min<long long>(ctx->sm_count / 2, tiles));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmemBytes;
-    cfg.stream = st;
-    cudaLaunchAttribute la[2];
-    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    la[0].val.programmaticStreamSerializationAllowed = 1;
-    la[1].id = cudaLaunchAttributeClusterDimension;
-    la[1].val.clusterDim.x = 2;
-    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
-    cfg.attrs = la;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp8_pair_kernel, maps, a);
+    // K slices where tiles would leave SMs without work, all clusters at once (15 of four pairs, 33 of two).  Joining them takes 3 us: 256 x 4096 x 4096 18.3 us, in two slices
+    // 16.2; x 14336 50.1 and 34.3; 256 x 1024 x 4096 17.7, in four 13.0; but x 2048 11.6 to 11.8 and 12.1 to 12.4.
+    if (!expert_offsets && a.nkb >= 24 && tiles <= clusters_at_once<4>()) return launch<4>(st, maps, a, tiles);
+    if (!expert_offsets && a.nkb >= 24 && tiles <= clusters_at_once<2>()) return launch<2>(st, maps, a, tiles);
+    return launch<1>(st, maps, a, std::min<long long>(ctx->sm_count / 2, tiles));
 }
 
 }  // namespace mtc

@@ -1502,7 +1502,11 @@ static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_exper
     if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, x, w)) return FP8_CUDA_CORE;
     const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
     if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
-    return pair && (grouped ? M / n_experts >= 48 : M > 128) ? FP8_PAIR : FP8_TILE;
+    // Pairs of CTAs have tiles of 256 tokens.  Grouped (128 experts of 768 x 2048, us of tiles and pairs): 32 rows an expert 47 and 52, 64 69 and 59.  Dense: from more than 64
+    // tokens on, unless that is so few tiles of 64 x 128 that cutting K into four slices and more fills the GPU (256 x 1024 x 4096 10.8 and 13.0, 256 x 4096 x 4096 20 and 16,
+    // 128 x 4096 x 14336 26 and 34, 64 x 14336 x 4096 19 and 20, 128 x 14336 x 4096 26 and 21).
+    if (grouped) return pair && M / n_experts >= 48 ? FP8_PAIR : FP8_TILE;
+    return pair && M > 64 && static_cast<long long>((M + 63) / 64) * mtc::fp8::blocks(N) > 64 ? FP8_PAIR : FP8_TILE;
 }
 
 static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_t *x, const float *xs, const void *w, const void *ws, const void *expert_offsets, void *out,
