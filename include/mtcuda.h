@@ -75,7 +75,7 @@ int mtc_sync_deadline(mtc_ctx *ctx, void *stream, int timeout_ms);
  * an expert id out of range in mtc_moe_sort), 0x601 + r rank r never arrived at a peer barrier, 0x701 / 0x702 phase counter /
  * partial-sum slot of a chained launch, 0x801-0x831 the tensor-memory decode kernel, 0x901 expert_offsets that run backwards or past the rows,
  * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 / 0x906 a row index that does not exist, 0x907 an expert that does not exist, 0xa01-0xa0b waits of the exact
- * grouped kernel's roles. */
+ * grouped kernel's roles, 0xb01-0xb06 and 0xb11-0xb16 of the roles of the two tensor-core kernels of e4m3 codes. */
 int mtc_status_word(mtc_ctx *ctx, uint32_t *word);
 int mtc_status_clear(mtc_ctx *ctx);
 
@@ -419,11 +419,15 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
                      int block_rows, int pow2, int dtype);
 /* out[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k], sums in f32, rounded once to out_dtype (f32, f16, bf16).
  * x_dtype MTC_E4M3: x holds codes, x_scales their scales.  x_dtype f32 / f16 / bf16: x T[M, K] is quantized in the call as mtc_fp8_quantize does with blocks
- * of one row and pow2 0 (x_scales NULL): same results.  K a multiple of 16 with 16-byte aligned x and w runs on tensor cores, everything else on CUDA cores. */
+ * of one row and pow2 0 (x_scales NULL): same results.  K a multiple of 16 with 16-byte aligned x and w runs on tensor cores, everything else on CUDA cores.  w and w_scales
+ * are constants, as for the other dense products (option "pdl_early_weights"; mtc_fp8_quantize in front is known to the context). */
 enum { MTC_E4M3 = 3 };
 int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int M, int N, int K, int x_dtype,
                int out_dtype, void *workspace, size_t workspace_bytes);
 size_t mtc_fp8_mm_workspace(const mtc_ctx *ctx, int M, int N, int K, int x_dtype, int out_dtype);
+/* The kernel that a product takes with aligned pointers under the options of `ctx` (NULL: the default ones), n_experts 0 for mtc_fp8_mm: "fp8_mm_" or "fp8_gather_mm_" and
+ * "cuda_core", "tile" (csrc/fp8_tcgen05.cu) or "pair" (csrc/fp8_pair.cu); "" for sizes that no kernel takes.  The entries decide by the same function. */
+const char *mtc_fp8_kernel(const mtc_ctx *ctx, int M, int N, int K, int n_experts);
 /* The same product of rows sorted by expert with stacked matrices: row t of expert_offsets[e] <= t < expert_offsets[e + 1] meets w[e] (u32[n_experts + 1], as
  * mtc_moe_sort writes them; x is codes).  Rows in no range keep what `out` holds there.  Offsets that reach past m_total or run backwards are clamped and
  * reported through the status word (0x901). */

@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmtcuda.so")
 
 F32, F16, BF16 = 0, 1, 2
+E4M3 = 3                       # the type of x in fp8_mm when it holds codes
 
 STATUS_NAMES = {
     0: "Ok", -1: "NoDevice", -2: "Buffer", -3: "BufferSize", -4: "Dispatch",
@@ -116,6 +117,7 @@ SIGNATURES = {
     "mtc_fp8_quantize": (_i, [_vp] * 6 + [_i] * 7),
     "mtc_fp8_mm": (_i, [_vp] * 7 + [_i] * 5 + [_vp, _sz]),
     "mtc_fp8_mm_workspace": (_sz, [_vp] + [_i] * 5),
+    "mtc_fp8_kernel": (ctypes.c_char_p, [_vp] + [_i] * 4),
     "mtc_fp8_gather_mm": (_i, [_vp] * 8 + [_i] * 5 + [_vp, _sz]),
     "mtc_fp8_gather_mm_workspace": (_sz, [_vp] + [_i] * 5),
     "mtc_moe_balance": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_i] * 4 + [_vp, _sz]),

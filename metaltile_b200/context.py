@@ -365,6 +365,32 @@ class Context:
         self._check(self._lib.mtc_gather_qmm_static(self._h, stream, x, w, scales, biases, expert_offsets, indices,
                                                     out, m_total, n_out, k_in, n_experts, bits, group_size, _dt(dtype)))
 
+    # ---- 8-bit floating point, the router's training side (device pointers; workspaces of at least what the *_workspace functions say) ----
+    def fp8_kernel(self, M, N, K, n_experts: int = 0) -> str:
+        """The kernel that ``fp8_mm`` (``n_experts`` 0) or ``fp8_gather_mm`` takes under this context's options (``mtc_fp8_kernel``)."""
+        return self._lib.mtc_fp8_kernel(self._h, M, N, K, n_experts).decode()
+
+    def fp8_quantize(self, x, codes, scales, n_rows, K, dtype, block_rows=1, pow2=False, n_mats=1, rows=None, n_src_rows=0, stream: int = 0):
+        self._check(self._lib.mtc_fp8_quantize(self._h, stream, x, rows, codes, scales, n_mats, n_rows, n_src_rows, K, block_rows, int(pow2), _dt(dtype)))
+
+    def fp8_mm(self, x, x_scales, w, w_scales, out, M, N, K, out_dtype, x_dtype=None, workspace=None, workspace_bytes: int = 0, stream: int = 0):
+        """``x_dtype`` None: x holds codes."""
+        self._check(self._lib.mtc_fp8_mm(self._h, stream, x, x_scales, w, w_scales, out, M, N, K, _lib.E4M3 if x_dtype is None else _dt(x_dtype),
+                                         _dt(out_dtype), workspace, workspace_bytes))
+
+    def fp8_gather_mm(self, x, x_scales, w, w_scales, expert_offsets, out, m_total, n_out, k_in, n_experts, out_dtype, workspace=None,
+                      workspace_bytes: int = 0, stream: int = 0):
+        self._check(self._lib.mtc_fp8_gather_mm(self._h, stream, x, x_scales, w, w_scales, expert_offsets, out, m_total, n_out, k_in, n_experts,
+                                                _dt(out_dtype), workspace, workspace_bytes))
+
+    def moe_balance(self, logits, topk_idx, mask, coef, loss, counts, mean_probs, n_counted, n_rows, n_experts, k, dtype, workspace=None,
+                    workspace_bytes: int = 0, stream: int = 0):
+        self._check(self._lib.mtc_moe_balance(self._h, stream, logits, topk_idx, mask, coef, loss, counts, mean_probs, n_counted, n_rows, n_experts, k,
+                                              _dt(dtype), workspace, workspace_bytes))
+
+    def moe_balance_grad(self, logits, mask, counts, n_counted, grad_loss, coef, grad, n_rows, n_experts, k, dtype, stream: int = 0):
+        self._check(self._lib.mtc_moe_balance_grad(self._h, stream, logits, mask, counts, n_counted, grad_loss, coef, grad, n_rows, n_experts, k, _dt(dtype)))
+
     def moe_experts(self, x, sort_token_idx, n_tokens, gate, up, down, expert_offsets, y, m_total, hidden, inter, n_experts,
                     bits, group_size, dtype, stream: int = 0):
         """``mtc_moe_experts``; gate / up / down are (w, scales, biases) device pointers."""

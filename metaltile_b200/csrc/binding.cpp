@@ -815,10 +815,11 @@ PyObject *moe_balance(Args a, Py_ssize_t n) {
         mean = empty({E}, at::kFloat, l);
         counted = empty({}, at::kInt, l);
         const size_t need = mtc_moe_balance_workspace(c.h, static_cast<int>(R), static_cast<int>(E));
-        const at::Tensor space = empty({static_cast<int64_t>(need)}, at::kByte, l);
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, l);
         return mtc_moe_balance(c.h, on_stream(l), l.data_ptr(), idx.data_ptr(), mask ? mask->data_ptr() : nullptr, static_cast<float>(coef), loss.data_ptr(),
                                counts.data_ptr(), mean.data_ptr(), counted.data_ptr(), static_cast<int>(R), static_cast<int>(E), static_cast<int>(k), dt,
-                               space.data_ptr(), need);
+                               need ? space.data_ptr() : nullptr, need);
     }));
     return tuple_of({&loss, &counts, &mean, &counted});
 }

@@ -13,6 +13,8 @@ namespace fp8 {
 constexpr int kBlock = 128;
 constexpr float kLeastScale = 8.077935669463161e-28f;      // 2^-90: below it the residual of a quotient could underflow (code_quotient)
 
+constexpr int kMostSize = 0x7FFFFFFF - 1024;    // of rows and columns: what is rounded up to a tile stays an int
+
 __host__ __device__ constexpr int blocks(int n) { return (n + kBlock - 1) / kBlock; }
 
 // two codes; lo in the low byte.  |v| above 448 becomes 448, NaN the code 0x7F.
@@ -67,7 +69,7 @@ cudaError_t launch_fp8_quantize(Ctx *ctx, cudaStream_t st, const void *x, const 
                                 long long n_rows, long long n_src_rows, int K, int block_rows, int pow2, int dt);
 cudaError_t launch_fp8_mm_generic(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets,
                                   void *out, int M, int N, int K, int n_experts, int out_dt);
-bool fp8_tile_supported(int M, int N, int K, const void *x, const void *w);
+bool fp8_tile_supported(int M, int N, int K, int n_experts, const void *x, const void *w);
 cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,
                             int M, int N, int K, int n_experts, int out_dt, std::string *why);
 bool fp8_pair_supported(int M, int N, int K, int n_experts, const void *x, const void *w);

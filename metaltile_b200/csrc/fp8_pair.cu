@@ -563,7 +563,7 @@ int clusters_at_once() {
 }  // namespace
 
 bool fp8_pair_supported(int M, int N, int K, int n_experts, const void *x, const void *w) {
-    return fp8_tile_supported(M, N, K, x, w) && n_experts <= kMaxExperts && static_cast<long long>(blocks(M) + n_experts) * blocks(N) < 0x7FFFFFFF;
+    return fp8_tile_supported(M, N, K, n_experts, x, w) && n_experts <= kMaxExperts && static_cast<long long>(blocks(M) + n_experts) * blocks(N) < 0x7FFFFFFF;
 }
 
 cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,

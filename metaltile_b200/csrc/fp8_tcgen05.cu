@@ -422,8 +422,10 @@ static int slices_for(int sms, long long units, int nkb) {
     return s;
 }
 
-bool fp8_tile_supported(int M, int N, int K, const void *x, const void *w) {
-    return M > 0 && N > 0 && K % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+// (a copy of codes starts at rows of 16-byte pieces; rows of all experts are one coordinate)
+bool fp8_tile_supported(int M, int N, int K, int n_experts, const void *x, const void *w) {
+    return M > 0 && N > 0 && K % 16 == 0 && static_cast<long long>(n_experts) * N <= kMostSize && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+           reinterpret_cast<uintptr_t>(w) % 16 == 0;
 }
 
 cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const float *xs, const uint8_t *w, const float *ws, const uint32_t *expert_offsets, void *out,

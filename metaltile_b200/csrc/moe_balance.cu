@@ -6,10 +6,10 @@
 //   loss = coef * E * sum_e f_e P_e;  n = 0: f, P and loss are 0
 //   d loss / d logit_te = coef * E / n * p_te * (f_e - sum_j f_j p_tj)       (counts are constants)
 //
-// Bound by reading the logits: a warp has a row in registers (two at a time while there are many), every lane adds up its own experts over the rows of the warp; rows are
-// dealt out to the warps of the grid in turn, so that masked ones, which lie together, are spread.  Sums over rows are f32 in a warp and in its CTA (at most a few dozen
-// rows a warp) and f64 from there on, always in the same order; counts are integers, whose order does not matter.  A second launch, a cluster of eight CTAs with an
-// eighth of the experts each, adds up the CTAs' parts and meets over distributed shared memory for the loss.
+// Bound by reading the logits where there are many rows, by launches and latencies where there are few.  A warp has two or four rows in registers at a time, every lane adds up
+// its own experts over the rows of the warp; rows are dealt out to the warps of the grid in turn, so that masked ones, which lie together, are spread.  Sums over rows are
+// f32 for 32 rows of a warp at most and f64 from there on, always in the same order; counts are integers, whose order does not matter.  Few rows are one launch, a
+// cluster of eight CTAs that meet over distributed shared memory; many are a launch of a CTA an SM and one of such a cluster that adds up their parts.
 #include <algorithm>
 
 #include "common.cuh"
@@ -65,128 +65,222 @@ __device__ __forceinline__ void store_v(void *base, size_t at, const float (&v)[
     }
 }
 
-// The logits of a row (minus infinity where there is no expert)
+// The logits of a row, minus infinity where there is no expert or (there: false) no row
 template <int DT, int V, int CH>
-__device__ __forceinline__ void load_row(const void *logits, size_t row, int n_experts, float (&z)[CH][V]) {
+__device__ __forceinline__ void load_row(const void *logits, size_t row, bool there, int n_experts, float (&z)[CH][V]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
         for (int i = 0; i < V; ++i) z[c][i] = -INFINITY;
         const int e = (c * 32 + lane) * V;
-        if (e < n_experts) load_v<DT, V>(logits, row * n_experts + e, z[c]);
+        if (there && e < n_experts) load_v<DT, V>(logits, row * n_experts + e, z[c]);
     }
 }
-// ... become its probabilities
-template <int V, int CH>
-__device__ __forceinline__ void softmax_row(float (&z)[CH][V]) {
-    float most = -INFINITY;
+// ... of R rows become their probabilities, the steps of the rows side by side
+template <int V, int CH, int R>
+__device__ __forceinline__ void softmax_rows(float (&z)[R][CH][V]) {
+    float most[R], sum[R];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int u = 0; u < R; ++u) {
+        float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < V; ++i) most = fmaxf(most, z[c][i]);
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            for (int i = 0; i < V; ++i) m = fmaxf(m, z[u][c][i]);
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(most[u]) : "f"(m));
+    }
     // exp(z - most) as a power of two; below 2^-126 it is zero
-    if (most == -INFINITY) most = 0.0f;
-    float sum = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int u = 0; u < R; ++u) {
+        if (most[u] == -INFINITY) most[u] = 0.0f;
+        sum[u] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z[c][i]) : "f"((z[c][i] - most) * 1.4426950408889634f));
-            sum += z[c][i];
-        }
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            for (int i = 0; i < V; ++i) {
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z[u][c][i]) : "f"((z[u][c][i] - most[u]) * 1.4426950408889634f));
+                sum[u] += z[u][c][i];
+            }
+    }
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[c][i] *= inv;
+        for (int u = 0; u < R; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+        const float inv = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int i = 0; i < V; ++i) z[u][c][i] *= inv;
+    }
 }
 
-// Warps of a CTA that adds up rows: a lane holds two sets of CH x V values, so few warps where that is many registers
+constexpr int kCluster = 8;
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t on_cta(const void *p, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ double ld_double(uint32_t at) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_int(uint32_t at) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+struct Results {
+    float coef;
+    float *loss;
+    int *counts;
+    float *mean_probs;
+    int *n_counted;
+};
+// What comes of the sums of an expert (thread e - e0 of a CTA of the cluster has that of expert e, `mine`: it has one), and of all: the loss.  scratch: a double a warp and one more.
+__device__ __forceinline__ void conclude(const Results &out, int rank, bool mine, int e, double p, int c, int n, int n_experts, int k, double *scratch) {
+    double term = 0.0;
+    if (mine) {
+        const double mean = n ? p / n : 0.0;
+        out.counts[e] = c;
+        out.mean_probs[e] = static_cast<float>(mean);
+        term = n ? mean * c / (static_cast<double>(n) * k) : 0.0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = term;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = 0.0;
+        for (int w = 0; w < warps; ++w) all += scratch[w];
+        scratch[warps] = all;
+    }
+    cluster_sync();
+    if (rank == 0 && threadIdx.x == 0) {
+        double all = 0.0;
+        for (int q = 0; q < kCluster; ++q) all += ld_double(on_cta(scratch + warps, q));
+        *out.loss = static_cast<float>(static_cast<double>(out.coef) * n_experts * all);
+        *out.n_counted = n;
+    }
+    cluster_sync();                              // nobody leaves while its share is read
+}
+
+// Warps of a CTA that adds up rows: a lane holds so many rows' values and their sums, so few warps where that is many registers
 __host__ __device__ constexpr int row_warps(int ch, int v) { return ch * v <= 8 ? 32 : 16; }
 
-// Sums of each CTA: part_p f32[grid][E], part_c i32[grid][E], part_n i32[grid]
-template <int DT, int V, int CH>
+// Sums of each CTA: part_p f32[grid][E], part_c i32[grid][E], part_n i32[grid]; ONE: the grid is a cluster that goes on to the results
+template <int DT, int V, int CH, bool ONE>
 __global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float *part_p, int *part_c,
-                                                                           int *part_n, int n_rows, int n_experts, int k, uint32_t *status) {
+                                                                           int *part_n, Results out, int n_rows, int n_experts, int k, uint32_t *status) {
     pdl_enter();
-    constexpr int W = row_warps(CH, V), T = 32 * W;
-    extern __shared__ float sm[];
-    float *const warp_p = sm;                                    // [W][E]
-    int *const hist = reinterpret_cast<int *>(sm + W * n_experts);
+    constexpr int W = row_warps(CH, V), T = 32 * W, R = CH * V <= 4 ? 4 : 2;
+    extern __shared__ double sm[];
+    constexpr int ROW = 32 * CH * V;             // a warp's sums: those of a lane under each other, so that no bank is met twice
+    auto place = [](int e) { return (e / (32 * V) * V + e % V) * 32 + e / V % 32; };
+    double *const warp_p = sm;                                   // [W][ROW]
+    int *const hist = reinterpret_cast<int *>(sm + W * ROW);
     __shared__ int counted;
+    __shared__ double scratch[W + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e < n_experts; e += T) hist[e] = 0;
     if (threadIdx.x == 0) counted = 0;
     __syncthreads();
     float acc[CH][V] = {};
-    int n = 0;
-    auto kept = [&](long long r) { return r < n_rows && (!mask || mask[r] != 0); };
-    auto count = [&](long long r) {
-        ++n;
-        for (int j = lane; j < k; j += 32) {
-            const uint32_t e = topk_idx[static_cast<size_t>(r) * k + j];
-            if (e < static_cast<uint32_t>(n_experts)) atomicAdd(&hist[e], 1);
-            else atomicCAS(status, 0u, 0x907u);                  // an expert that does not exist: recorded, not counted
-        }
-    };
-    auto add = [&](const float (&z)[CH][V]) {
+    int n = 0, held = 0;
+    bool first = true;
+    auto flush = [&] {                           // a lane has its own places
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[c][i] += z[c][i];
+            for (int i = 0; i < V; ++i) {
+                double &at = warp_p[warp * ROW + (c * V + i) * 32 + lane];
+                at = first ? static_cast<double>(acc[c][i]) : at + acc[c][i];
+                acc[c][i] = 0.0f;
+            }
+        first = false;
+        held = 0;
     };
     const long long step = static_cast<long long>(gridDim.x) * W;
-    for (long long r = static_cast<long long>(warp) * gridDim.x + blockIdx.x; r < n_rows; r += 2 * step) {
-        const bool one = kept(r), two = kept(r + step);
-        float a[CH][V], b[CH][V];
-        if (one) load_row<DT, V, CH>(logits, r, n_experts, a);
-        if (two) load_row<DT, V, CH>(logits, r + step, n_experts, b);
-        if (one) {
-            count(r);
-            softmax_row<V, CH>(a);
-            add(a);
+    for (long long r0 = static_cast<long long>(warp) * gridDim.x + blockIdx.x; r0 < n_rows; r0 += R * step) {
+        bool kept[R];
+        float z[R][CH][V];
+        uint32_t id[R];                          // a lane a slot (k <= 32)
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const long long r = r0 + u * step;
+            kept[u] = r < n_rows && (!mask || mask[r] != 0);
+            load_row<DT, V, CH>(logits, r, kept[u], n_experts, z[u]);
+            id[u] = kept[u] && lane < k ? topk_idx[static_cast<size_t>(r) * k + lane] : 0;
         }
-        if (two) {
-            count(r + step);
-            softmax_row<V, CH>(b);
-            add(b);
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            if (!kept[u]) continue;
+            ++n;
+            if (lane < k) {
+                if (id[u] < static_cast<uint32_t>(n_experts)) atomicAdd(&hist[id[u]], 1);
+                else atomicCAS(status, 0u, 0x907u);              // an expert that does not exist: recorded, not counted
+            }
         }
+        softmax_rows<V, CH, R>(z);
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[c][i] += z[u][c][i];
+        if ((held += R) >= 32) flush();
     }
+    flush();
     if (lane == 0 && n) atomicAdd(&counted, n);
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = (c * 32 + lane) * V + i;
-            if (e < n_experts) warp_p[warp * n_experts + e] = acc[c][i];
-        }
     __syncthreads();
     for (int e = threadIdx.x; e < n_experts; e += T) {
-        float s = 0.0f;
+        double s = 0.0;
 #pragma unroll 8
-        for (int w = 0; w < W; ++w) s += warp_p[w * n_experts + e];
-        part_p[static_cast<size_t>(blockIdx.x) * n_experts + e] = s;
-        part_c[static_cast<size_t>(blockIdx.x) * n_experts + e] = hist[e];
+        for (int w = 0; w < W; ++w) s += warp_p[w * ROW + place(e)];
+        if constexpr (ONE) {
+            warp_p[place(e)] = s;
+        } else {
+            part_p[static_cast<size_t>(blockIdx.x) * n_experts + e] = static_cast<float>(s);
+            part_c[static_cast<size_t>(blockIdx.x) * n_experts + e] = hist[e];
+        }
     }
-    if (threadIdx.x == 0) part_n[blockIdx.x] = counted;
+    if constexpr (ONE) {
+        cluster_sync();
+        const int rank = blockIdx.x, e = n_experts * rank / kCluster + threadIdx.x;
+        const bool mine = e < n_experts * (rank + 1) / kCluster;
+        double p = 0.0;
+        int c = 0, all = 0;
+#pragma unroll
+        for (int q = 0; q < kCluster; ++q) {
+            all += ld_int(on_cta(&counted, q));
+            if (mine) {
+                p += ld_double(on_cta(warp_p + place(e), q));
+                c += ld_int(on_cta(hist + e, q));
+            }
+        }
+        conclude(out, rank, mine, e, p, c, all, n_experts, k, scratch);
+    } else if (threadIdx.x == 0) {
+        part_n[blockIdx.x] = counted;
+    }
 }
 
-constexpr int kJoinCtas = 8, kJoinThreads = 512;
+constexpr int kJoinThreads = 512;
 // A CTA has the experts of its eighth side by side (2^shift of its threads) and as many groups of parts as threads are left.
-__global__ void __cluster_dims__(kJoinCtas, 1, 1) __launch_bounds__(kJoinThreads)
-balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, int parts, float coef, float *loss, int *counts, float *mean_probs, int *n_counted,
-                    int n_experts, int k, int shift) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kJoinThreads)
+balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, int parts, Results out, int n_experts, int k, int shift) {
     pdl_enter();
-    __shared__ double sums[kJoinThreads];
+    __shared__ double sums[kJoinThreads], scratch[kJoinThreads / 32 + 1];
     __shared__ int cnts[kJoinThreads];
     __shared__ int total;
-    __shared__ double share;
-    const int rank = blockIdx.x, e0 = n_experts * rank / kJoinCtas, e1 = n_experts * (rank + 1) / kJoinCtas;
+    const int rank = blockIdx.x, e0 = n_experts * rank / kCluster, e1 = n_experts * (rank + 1) / kCluster;
     const int wide = 1 << shift, groups = kJoinThreads >> shift, g = threadIdx.x >> shift, e = e0 + (threadIdx.x & (wide - 1));
     if (threadIdx.x == 0) total = 0;
     __syncthreads();
@@ -212,35 +306,7 @@ balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, i
         }
     }
     __syncthreads();
-    const int n = total;
-    double term = 0.0;
-    if (g == 0 && e < e1) {
-        const double mean = n ? sums[threadIdx.x] / n : 0.0;
-        counts[e] = cnts[threadIdx.x];
-        mean_probs[e] = static_cast<float>(mean);
-        term = n ? mean * cnts[threadIdx.x] / (static_cast<double>(n) * k) : 0.0;
-    }
-    __syncthreads();
-    if (g == 0) sums[threadIdx.x] = term;
-    for (int o = wide >> 1; o > 0; o >>= 1) {
-        __syncthreads();
-        if (threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    }
-    if (threadIdx.x == 0) share = sums[0];
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0 && threadIdx.x == 0) {
-        double all = 0.0;
-        for (int q = 0; q < kJoinCtas; ++q) {
-            uint32_t there;
-            double v;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&share))), "r"(q));
-            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(there) : "memory");
-            all += v;
-        }
-        *loss = static_cast<float>(static_cast<double>(coef) * n_experts * all);
-        *n_counted = n;
-    }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");      // nobody leaves while its share is read
+    conclude(out, rank, g == 0 && e < e1, e, sums[threadIdx.x], cnts[threadIdx.x], total, n_experts, k, scratch);
 }
 
 template <int DT, int V, int CH>
@@ -259,40 +325,39 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const void *logi
             const int e = (c * 32 + lane) * V + i;
             f[c][i] = e < n_experts ? static_cast<float>(counts[e]) * each : 0.0f;
         }
-    auto finish = [&](long long r, bool kept, float (&z)[CH][V]) {
-        if (kept) {
-            softmax_row<V, CH>(z);
-            float dot = 0.0f;
+    constexpr int R = 2;
+    for (long long r0 = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r0 < n_rows; r0 += R * warps) {
+        float z[R][CH][V], dot[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const long long r = r0 + u * warps;
+            load_row<DT, V, CH>(logits, r, r < n_rows && (!mask || mask[r] != 0), n_experts, z[u]);
+        }
+        softmax_rows<V, CH, R>(z);               // (a masked row: zeros)
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            dot[u] = 0.0f;
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < V; ++i) dot = fmaf(z[c][i], f[c][i], dot);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[c][i] = g * z[c][i] * (f[c][i] - dot);
-        } else {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[c][i] = 0.0f;
+                for (int i = 0; i < V; ++i) dot[u] = fmaf(z[u][c][i], f[c][i], dot[u]);
         }
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int e = (c * 32 + lane) * V;
-            if (e < n_experts) store_v<DT, V>(grad, static_cast<size_t>(r) * n_experts + e, z[c]);
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < R; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const long long r = r0 + u * warps;
+            if (r >= n_rows) break;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[u][c][i] = g * z[u][c][i] * (f[c][i] - dot[u]);
+                const int e = (c * 32 + lane) * V;
+                if (e < n_experts) store_v<DT, V>(grad, static_cast<size_t>(r) * n_experts + e, z[u][c]);
+            }
         }
-    };
-    for (long long r = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); r < n_rows; r += 2 * warps) {
-        const long long r2 = r + warps;
-        const bool one = !mask || mask[r] != 0, two = r2 < n_rows && (!mask || mask[r2] != 0);
-        float a[CH][V], b[CH][V];
-        if (one) load_row<DT, V, CH>(logits, r, n_experts, a);
-        if (two) load_row<DT, V, CH>(logits, r2, n_experts, b);
-        finish(r, one, a);
-        if (r2 < n_rows) finish(r2, two, b);
     }
 }
 
@@ -319,16 +384,33 @@ cudaError_t with_form(int dt, bool vec, int n_experts, A... args) {
 }
 template <int DT, int V, int CH>
 struct RowsForm {
-    static cudaError_t run(Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn, int n_rows,
-                           int n_experts, int k) {
+    template <bool ONE>
+    static cudaError_t go(Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn, const Results &out,
+                          int n_rows, int n_experts, int k) {
         constexpr int W = row_warps(CH, V);
-        const size_t smem = static_cast<size_t>(W + 1) * n_experts * 4;
+        const size_t smem = static_cast<size_t>(W) * 32 * CH * V * 8 + static_cast<size_t>(n_experts) * 4;
         static PerDeviceAttr attr;
-        if (smem > 48 * 1024) {
-            const cudaError_t e = attr.set(balance_rows_kernel<DT, V, CH>, static_cast<size_t>(W + 1) * 1024 * 4);
-            if (e != cudaSuccess) return e;
-        }
-        return launch_pdl(balance_rows_kernel<DT, V, CH>, ctas, 32 * W, smem, st, logits, idx, mask, pp, pc, pn, n_rows, n_experts, k, ctx->d_status);
+        const cudaError_t e = attr.set(balance_rows_kernel<DT, V, CH, ONE>, static_cast<size_t>(2 * W + 1) * 32 * CH * V * 4);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(ctas);
+        cfg.blockDim = dim3(32 * W);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute la[2];
+        la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        la[0].val.programmaticStreamSerializationAllowed = 1;
+        la[1].id = cudaLaunchAttributeClusterDimension;
+        la[1].val.clusterDim.x = kCluster;
+        la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+        cfg.attrs = la;
+        cfg.numAttrs = ONE ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, balance_rows_kernel<DT, V, CH, ONE>, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k, ctx->d_status);
+    }
+    static cudaError_t run(bool one, Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn,
+                           const Results &out, int n_rows, int n_experts, int k) {
+        return one ? go<true>(ctx, st, kCluster, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k)
+                   : go<false>(ctx, st, ctas, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k);
     }
 };
 template <int DT, int V, int CH>
@@ -345,8 +427,11 @@ bool in_fours(int n_experts, int dt, const void *a, const void *b) {
 
 }  // namespace
 
+// One launch up to here (128 experts, us: 64 rows 6.3 in one and 6.8 in two, 256 6.6 and 6.8, 512 7.5 and 7.2, 1024 9.3 and 7.5)
+static bool in_one(int n_rows) { return n_rows <= 256; }
+
 size_t moe_balance_workspace(int sms, int n_rows, int n_experts) {
-    return static_cast<size_t>(balance_ctas(sms, n_rows)) * (2 * static_cast<size_t>(n_experts) + 1) * 4;
+    return in_one(n_rows) ? 0 : static_cast<size_t>(balance_ctas(sms, n_rows)) * (2 * static_cast<size_t>(n_experts) + 1) * 4;
 }
 
 cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float coef, float *loss,
@@ -354,11 +439,13 @@ cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, co
     const int ctas = balance_ctas(ctx->sm_count, n_rows);
     float *pp = static_cast<float *>(workspace);
     int *pc = reinterpret_cast<int *>(pp + static_cast<size_t>(ctas) * n_experts), *pn = pc + static_cast<size_t>(ctas) * n_experts;
-    cudaError_t e = with_form<RowsForm>(dt, in_fours(n_experts, dt, logits, logits), n_experts, ctx, st, ctas, logits, topk_idx, mask, pp, pc, pn, n_rows, n_experts, k);
-    if (e != cudaSuccess) return e;
+    const Results out{coef, loss, counts, mean_probs, n_counted};
+    const bool one = in_one(n_rows);
+    cudaError_t e = with_form<RowsForm>(dt, in_fours(n_experts, dt, logits, logits), n_experts, one, ctx, st, ctas, logits, topk_idx, mask, pp, pc, pn, out, n_rows, n_experts, k);
+    if (e != cudaSuccess || one) return e;
     int shift = 0;
-    while (1 << shift < (n_experts + kJoinCtas - 1) / kJoinCtas) ++shift;
-    return launch_pdl(balance_join_kernel, kJoinCtas, kJoinThreads, 0, st, pp, pc, pn, ctas, coef, loss, counts, mean_probs, n_counted, n_experts, k, shift);
+    while (1 << shift < (n_experts + kCluster - 1) / kCluster) ++shift;
+    return launch_pdl(balance_join_kernel, kCluster, kJoinThreads, 0, st, pp, pc, pn, ctas, out, n_experts, k, shift);
 }
 
 cudaError_t launch_moe_balance_grad(Ctx *ctx, cudaStream_t st, const void *logits, const uint8_t *mask, const int *counts, const int *n_counted,

@@ -1471,6 +1471,7 @@ static int guarded(mtc_ctx *ctx, F &&f) {
     }
 }
 extern "C" {
+static bool fp8_sizes_ok(int a, int b, int K) { return a >= 0 && a <= mtc::fp8::kMostSize && b >= 0 && b <= mtc::fp8::kMostSize && K > 0 && K <= mtc::fp8::kMostSize; }
 static bool aligned_to(const void *p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 static int check_workspace(mtc_ctx *ctx, const char *who, const void *workspace, size_t have, size_t need) {
     if (need == 0 || (workspace && have >= need && aligned_to(workspace, 256))) return MTC_OK;
@@ -1484,8 +1485,8 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
         MTC_ENTER(ctx);
         if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_quantize: dtype must be f32, f16 or bf16");
         if (block_rows != 1 && block_rows != 128) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_quantize: blocks are of 1 or 128 rows");
-        if (n_mats < 0 || n_rows < 0 || K <= 0 || (block_rows == 1 && n_mats > 1) || (rows && (block_rows != 1 || n_src_rows < 0)))
-            return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: sizes must be positive; rows of an index and one matrix only with blocks of one row");
+        if (n_mats < 0 || !fp8_sizes_ok(n_rows, n_src_rows, K) || (block_rows == 1 && n_mats > 1) || (rows && block_rows != 1))
+            return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: sizes must be positive and below 2^31 - 1024; rows of an index and one matrix only with blocks of one row");
         if (n_mats == 0 || n_rows == 0) return MTC_OK;
         if (!x || !codes || !scales) return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: null pointer");
         if (rows && n_src_rows == 0) return fail(ctx, MTC_ERR_INVALID, "fp8_quantize: an index into no rows");
@@ -1499,7 +1500,7 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
 enum Fp8Kernel { FP8_CUDA_CORE, FP8_TILE, FP8_PAIR };
 static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_experts, bool grouped, const void *x, const void *w) {
     const int forced = ctx ? ctx->fp8_kernel : 0;
-    if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, x, w)) return FP8_CUDA_CORE;
+    if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, n_experts, x, w)) return FP8_CUDA_CORE;
     const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
     if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
     // Pairs of CTAs have tiles of 256 tokens.  Grouped (128 experts of 768 x 2048, us of tiles and pairs): 32 rows an expert 47 and 52, 64 69 and 59.  Dense: from more than 64
@@ -1507,6 +1508,12 @@ static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_exper
     // 128 x 4096 x 14336 26 and 34, 64 x 14336 x 4096 19 and 20, 128 x 14336 x 4096 26 and 21).
     if (grouped) return pair && M / n_experts >= 48 ? FP8_PAIR : FP8_TILE;
     return pair && M > 64 && static_cast<long long>((M + 63) / 64) * mtc::fp8::blocks(N) > 64 ? FP8_PAIR : FP8_TILE;
+}
+
+const char *mtc_fp8_kernel(const mtc_ctx *ctx, int M, int N, int K, int n_experts) {
+    if (!fp8_sizes_ok(M, N, K) || M == 0 || N == 0 || n_experts < 0) return "";
+    static const char *const names[2][3] = {{"fp8_mm_cuda_core", "fp8_mm_tile", "fp8_mm_pair"}, {"fp8_gather_mm_cuda_core", "fp8_gather_mm_tile", "fp8_gather_mm_pair"}};
+    return names[n_experts > 0][fp8_kernel_for(ctx, M, N, K, std::max(n_experts, 1), n_experts > 0, nullptr, nullptr)];
 }
 
 static int fp8_product(mtc_ctx *ctx, const char *who, void *stream, const uint8_t *x, const float *xs, const void *w, const void *ws, const void *expert_offsets, void *out,
@@ -1539,7 +1546,7 @@ int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, 
         MTC_ENTER(ctx);
         if (!dtype_ok(out_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_mm: out_dtype must be f32, f16 or bf16");
         if (x_dtype != MTC_E4M3 && !dtype_ok(x_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_mm: x must be e4m3 codes, f32, f16 or bf16");
-        if (M < 0 || N < 0 || K <= 0) return fail(ctx, MTC_ERR_INVALID, "fp8_mm: sizes must be positive");
+        if (!fp8_sizes_ok(M, N, K)) return fail(ctx, MTC_ERR_INVALID, "fp8_mm: sizes must be positive and below 2^31 - 1024");
         if (M == 0 || N == 0) return MTC_OK;
         if (!x || !w || !w_scales || !out || (x_dtype == MTC_E4M3) != (x_scales != nullptr))
             return fail(ctx, MTC_ERR_INVALID, "fp8_mm: null pointer, or scales that do not go with the type of x");
@@ -1574,7 +1581,8 @@ int mtc_fp8_gather_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_s
     return guarded(ctx, [&]() -> int {
         MTC_ENTER(ctx);
         if (!dtype_ok(out_dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, "fp8_gather_mm: out_dtype must be f32, f16 or bf16");
-        if (m_total < 0 || n_out < 0 || k_in <= 0 || n_experts <= 0) return fail(ctx, MTC_ERR_INVALID, "fp8_gather_mm: sizes must be positive");
+        if (!fp8_sizes_ok(m_total, n_out, k_in) || n_experts <= 0 || n_experts > mtc::fp8::kMostSize)
+            return fail(ctx, MTC_ERR_INVALID, "fp8_gather_mm: sizes must be positive and below 2^31 - 1024");
         if (m_total == 0 || n_out == 0) return MTC_OK;
         if (!x || !x_scales || !w || !w_scales || !expert_offsets || !out) return fail(ctx, MTC_ERR_INVALID, "fp8_gather_mm: null pointer");
         int rc = check_workspace(ctx, "fp8_gather_mm", workspace, workspace_bytes,

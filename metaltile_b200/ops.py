@@ -195,8 +195,9 @@ def fp8_mm(x, w, w_scales, x_scales=None, out_dtype=None, out=None, ctx: Context
 
     ``x [.., K]`` is codes with ``x_scales [.., ceil(K/128)]``, or f32 / f16 / bf16 activations, which are quantized in the call as
     ``fp8_quantize(x)`` does (same result).  ``out_dtype`` (f32, f16, bf16) defaults to the type of float activations, bf16 for codes.
-    The gradient of x is the same product with the matrix the other way round: ``fp8_mm(dy, w.T.contiguous(), w_scales.T.contiguous())``
-    - blocks of 128 x 128 stay what they are."""
+    The gradient of x is the same product with the matrix the other way round, ``fp8_mm(dy, wt, wt_scales)`` with ``wt = w.T.contiguous()`` and
+    ``wt_scales = w_scales.T.contiguous()`` - blocks of 128 x 128 stay what they are.  Like the other dense products it requests its first weights
+    while the previous kernel of the stream drains (option ``pdl_early_weights``): keep such matrices, or synchronise after making them."""
     return _native.fp8_mm(x, w, w_scales, x_scales, _out_dtype(out_dtype), out, ctx)
 
 

@@ -84,8 +84,18 @@ def test_workspaces_cover_what_the_call_stages():
     lib = _lib.load()
     for m, k in ((1, 16), (3, 130), (2048, 4096), (70000, 40000)):
         assert lib.mtc_fp8_mm_workspace(None, m, 64, k, 2, 2) >= m * k + 4 * m * -(-k // 128)
-    for rows, e in ((0, 8), (1, 1), (65536, 1024)):
-        assert lib.mtc_moe_balance_workspace(None, rows, e) > 0
+    assert lib.mtc_moe_balance_workspace(None, 0, 8) == 0 and lib.mtc_moe_balance_workspace(None, 65536, 1024) > 65536 * 8
+
+
+@pytest.mark.parametrize("args,want", [
+    ((1, 4096, 4096, 0), "tile"), ((64, 14336, 4096, 0), "tile"), ((65, 4096, 4096, 0), "tile"), ((65, 4097, 4096, 0), "pair"), ((256, 2048, 4096, 0), "tile"),
+    ((257, 2048, 4096, 0), "pair"), ((2048, 28672, 4096, 0), "pair"), ((1, 64, 130, 0), "cuda_core"), ((2048, 4096, 4088, 0), "cuda_core"),
+    ((32, 768, 2048, 128), "tile"), ((6143, 768, 2048, 128), "tile"), ((6144, 768, 2048, 128), "pair"), ((60000, 768, 2048, 1025), "tile"), ((64, 64, 100, 8), "cuda_core"),
+    ((8, 2 ** 20, 16, 2 ** 12), "cuda_core"), ((0, 64, 64, 0), None), ((2 ** 31 - 1, 64, 64, 0), None), ((1, 64, 2 ** 31 - 8, 0), None),
+])
+def test_kernels_on_both_sides_of_the_rules(args, want):
+    name = _lib.load().mtc_fp8_kernel(None, *args).decode()
+    assert name == ("" if want is None else ("fp8_gather_mm_" if args[3] else "fp8_mm_") + want)
 
 
 def test_the_table_of_codes_is_the_types():
