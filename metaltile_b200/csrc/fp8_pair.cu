@@ -138,11 +138,6 @@ __device__ __forceinline__ void wait_at(uint32_t bar, uint32_t parity, uint32_t 
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     if (!ok) wait_long(bar, parity, abort, status, code);
 }
-__device__ __forceinline__ float ld_shared(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 
 struct Tile {
     int expert, tok0, ntok, n0;

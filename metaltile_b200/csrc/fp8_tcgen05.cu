@@ -32,7 +32,9 @@ constexpr int kEpi = 128, kLoadWarp = 4, kMmaWarp = 5, kThreads = 192, kPerSM = 
 constexpr int kSmemBytes = 113 * 1024;           // of one of the two CTAs of an SM
 constexpr int kMaxSlices = 8;
 
-template <int TN>
+// SLICED: slices of K meet in shared memory.  A token's sums go to the CTA of rank token % slices, one place a slice, by stores that nobody waits for before the barrier of
+// the cluster: (a + i * slices) has i-th place.  Tiles of 64 tokens have no room beside the ring and are fetched from where it was, after the barrier.
+template <int TN, bool SLICED>
 struct Form {
     static constexpr int kTogether = TN == 64 ? 2 : 4;               // blocks of a hand-off to the epilogue
     static constexpr int kCols = 2 * kTogether * TN;                 // two hand-offs in tensor memory
@@ -41,7 +43,9 @@ struct Form {
     static constexpr int kPitch = TN + 4;
     static constexpr int kStage = kWBytes + TN * kBlock;
     static constexpr int kScales = kHeld * (kPitch + 1);             // floats: xs, then ws of the blocks
-    static constexpr int kRing = 1024 + (2 * kScales * 4 + 1023) / 1024 * 1024;          // where the stages start
+    static constexpr bool kPush = SLICED && TN < 64;
+    static constexpr int kJoin = 1024 + (2 * kScales * 4 + 1023) / 1024 * 1024;          // where the slices' sums come in
+    static constexpr int kRing = kJoin + (kPush ? (TN + kMaxSlices) * kRows * 4 : 0);    // where the stages start
     static constexpr int kStages = (kSmemBytes - 1024 - kRing) / kStage;
     static_assert(kStages >= 2 && kStages <= kMaxStages, "stages");
     static_assert(kStages * kStage >= TN * kRows * 4, "the sums of a slice go where the ring was");
@@ -84,6 +88,11 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
     return v;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
 }
 __device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
@@ -137,9 +146,9 @@ __device__ __noinline__ void rest(TCtrl *ctl, int stages) {
     __syncthreads();
 }
 
-template <int TN>
+template <int TN, bool SLICED>
 __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid_constant__ TMaps maps, const __grid_constant__ TArgs a) {
-    using F = Form<TN>;
+    using F = Form<TN, SLICED>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *const smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     TCtrl *const ctl = reinterpret_cast<TCtrl *>(smem);
@@ -183,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
     const int units = ctl->n_chunks * a.tiles;
+    if constexpr (SLICED) asm volatile("barrier.cluster.arrive.relaxed.aligned;");        // this CTA runs: awaited before anything is stored into another
     // grouped: the tiles of a chunk behind each other; dense: the chunks of a tile, which read the same weights
     auto tile_of = [&](int unit) { return a.expert_offsets ? unit % a.tiles : unit / a.chunks; };
     auto chunk_of = [&](int unit) {
@@ -286,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
             }
     } else {
         if (!a.expert_offsets) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if constexpr (SLICED) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);              // lane 32 * warp in bits 16 and up
         const int r = threadIdx.x;
         int d = 0, b = 0;
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
                 }
             }
             const int n = tile * kRows + r;
-            if (a.slices == 1) {
+            if constexpr (!SLICED) {
                 if (n < a.N && !ctl->abort) {
 #pragma unroll
                     for (int t = 0; t < TN; t += 2) {
@@ -344,55 +355,74 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
                         if (t + 1 < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t + 1) * a.N + n, v.y, a.out_dt);
                     }
                 }
-            } else {                             // one unit a cluster: the sums of a slice go where the ring was, [token][weight row]
+            } else {                             // one unit a cluster
+                const uint32_t join = ring - F::kRing + F::kJoin;
+                int owner = 0, at = rank;        // of token t: t % slices, t / slices * slices + rank
 #pragma unroll
-                for (int t = 0; t < TN; t += 2) {
+                for (int t = 0; t < TN; ++t) {
                     const float2 v = halves(acc[t / 2]);
-                    if (t < c.ntok) st_shared(ring + (t * kRows + r) * 4, v.x);
-                    if (t + 1 < c.ntok) st_shared(ring + ((t + 1) * kRows + r) * 4, v.y);
+                    if (t < c.ntok) {
+                        if constexpr (F::kPush) st_cluster(join + (at * kRows + r) * 4, owner, t & 1 ? v.y : v.x);
+                        else st_shared(ring + (t * kRows + r) * 4, t & 1 ? v.y : v.x);
+                    }
+                    if (++owner == a.slices) owner = 0, at += a.slices;
                 }
             }
         }
     }
-    __syncthreads();
-    if (ctl->abort) rest(ctl, F::kStages);
-    if (a.slices > 1) {                          // slice r adds up tokens r, r + slices, ... of all slices
+    if constexpr (SLICED) {
+        __syncwarp();
+        if (warp >= kLoadWarp) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         cluster_sync();
-        if (first < units && warp < kLoadWarp && !ctl->abort) {
+    } else {
+        __syncthreads();
+    }
+    if (ctl->abort) rest(ctl, F::kStages);
+    if constexpr (SLICED) {
+        if (first < units && warp < kLoadWarp && !ctl->abort) {      // the tokens of this rank
             const Chunk c = chunk_of(first);
-            const int r = threadIdx.x, n = tile_of(first) * kRows + r, every = a.slices;
-            for (int t0 = rank; t0 < c.ntok && n < a.N; t0 += 4 * every) {
+            const int r = threadIdx.x, n = tile_of(first) * kRows + r;
+            const uint32_t join = ring - F::kRing + F::kJoin;
+            for (int t0 = rank, at = 0; t0 < c.ntok && n < a.N; t0 += 4 * a.slices, at += 4 * a.slices) {
                 float part[4][kMaxSlices];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int q = 0; q < kMaxSlices; ++q)
-                        part[i][q] = q < a.slices && t0 + i * every < c.ntok ? ld_cluster(ring + ((t0 + i * every) * kRows + r) * 4, q) : 0.0f;
+                    for (int q = 0; q < kMaxSlices; ++q) {
+                        const int t = t0 + i * a.slices;
+                        if (q >= a.slices || t >= c.ntok) part[i][q] = 0.0f;
+                        else if constexpr (F::kPush) part[i][q] = ld_shared(join + ((at + i * a.slices + q) * kRows + r) * 4);
+                        else part[i][q] = ld_cluster(ring + (t * kRows + r) * 4, q);
+                    }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + i * a.slices;
                     float sum = part[i][0];
 #pragma unroll
                     for (int q = 1; q < kMaxSlices; ++q)
                         if (q < a.slices) sum += part[i][q];
-                    if (t0 + i * every < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t0 + i * every) * a.N + n, sum, a.out_dt);
+                    if (t < c.ntok) st_from_f32(a.out, static_cast<size_t>(c.tok0 + t) * a.N + n, sum, a.out_dt);
                 }
             }
         }
-        cluster_sync();                          // no CTA leaves while its sums are read
+        if constexpr (!F::kPush) {
+            __syncwarp();
+            cluster_sync();                      // no CTA leaves while its sums are read
+        }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kCols));
 }
 
-template <int TN>
-cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w, TArgs a, int K, std::string *why) {
+template <int TN, bool SLICED>
+cudaError_t launch_as(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w, TArgs a, int K, std::string *why) {
     TMaps maps;
     cudaError_t e = make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, static_cast<long long>(a.n_experts) * a.N, K, kRows, kBlock, why);
     if (e == cudaSuccess) e = make_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x, a.M, K, TN, kBlock, why);
     if (e != cudaSuccess) return e;
     static PerDeviceAttr attr;
-    if ((e = attr.set(fp8_tile_kernel<TN>, kSmemBytes)) != cudaSuccess) return e;
+    if ((e = attr.set(fp8_tile_kernel<TN, SLICED>, kSmemBytes)) != cudaSuccess) return e;
     const long long units = a.expert_offsets ? (static_cast<long long>(std::min(a.M, a.n_experts)) + a.M / TN) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
     if (units > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     // slices: a cluster a unit; else no more CTAs than run at once, each with units in turn
@@ -410,7 +440,11 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w
     la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
     cfg.attrs = la;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp8_tile_kernel<TN>, maps, a);
+    return cudaLaunchKernelEx(&cfg, fp8_tile_kernel<TN, SLICED>, maps, a);
+}
+template <int TN>
+cudaError_t launch(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t *w, const TArgs &a, int K, std::string *why) {
+    return a.slices > 1 ? launch_as<TN, true>(ctx, st, x, w, a, K, why) : launch_as<TN, false>(ctx, st, x, w, a, K, why);
 }
 
 }  // namespace
