@@ -11,6 +11,7 @@
 // f32 for 32 rows of a warp at most and f64 from there on, always in the same order; counts are integers, whose order does not matter.  Few rows are one launch, a
 // cluster of eight CTAs that meet over distributed shared memory; many are a launch of a CTA an SM and one of such a cluster that adds up their parts.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -77,12 +78,12 @@ __device__ __forceinline__ void load_row(const void *logits, size_t row, bool th
         if (there && e < n_experts) load_v<DT, V>(logits, row * n_experts + e, z[c]);
     }
 }
-// ... of R rows become their probabilities, the steps of the rows side by side
-template <int V, int CH, int R>
+// ... of the first N of R rows become their probabilities, the steps of the rows side by side
+template <int N, int V, int CH, int R>
 __device__ __forceinline__ void softmax_rows(float (&z)[R][CH][V]) {
-    float most[R], sum[R];
+    float most[N], sum[N];
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
+    for (int u = 0; u < N; ++u) {
         float m = -INFINITY;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -92,7 +93,7 @@ __device__ __forceinline__ void softmax_rows(float (&z)[R][CH][V]) {
     }
     // exp(z - most) as a power of two; below 2^-126 it is zero
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
+    for (int u = 0; u < N; ++u) {
         if (most[u] == -INFINITY) most[u] = 0.0f;
         sum[u] = 0.0f;
 #pragma unroll
@@ -106,9 +107,9 @@ __device__ __forceinline__ void softmax_rows(float (&z)[R][CH][V]) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for (int u = 0; u < R; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
+        for (int u = 0; u < N; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], o);
 #pragma unroll
-    for (int u = 0; u < R; ++u) {
+    for (int u = 0; u < N; ++u) {
         const float inv = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -229,13 +230,18 @@ __global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(con
                 else atomicCAS(status, 0u, 0x907u);              // an expert that does not exist: recorded, not counted
             }
         }
-        softmax_rows<V, CH, R>(z);
+        auto add = [&](auto rows) {
+            constexpr int N = decltype(rows)::value;
+            softmax_rows<N>(z);
 #pragma unroll
-        for (int u = 0; u < R; ++u)
+            for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[c][i] += z[u][c][i];
+                    for (int i = 0; i < V; ++i) acc[c][i] += z[u][c][i];
+        };
+        if (r0 + step < n_rows) add(std::integral_constant<int, R>{});       // (a masked row adds zeros)
+        else add(std::integral_constant<int, 1>{});
         if ((held += R) >= 32) flush();
     }
     flush();
@@ -290,8 +296,8 @@ balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, i
     double p = 0.0;
     int c = 0;
     if (e < e1) {
-#pragma unroll 4
-        for (int i = g; i < parts; i += groups) {
+#pragma unroll 8
+        for (int i = g; i < parts; i += groups) {            // (eight parts in flight)
             p += part_p[static_cast<size_t>(i) * n_experts + e];
             c += part_c[static_cast<size_t>(i) * n_experts + e];
         }
@@ -333,31 +339,33 @@ __global__ void __launch_bounds__(kThreads) balance_grad_kernel(const void *logi
             const long long r = r0 + u * warps;
             load_row<DT, V, CH>(logits, r, r < n_rows && (!mask || mask[r] != 0), n_experts, z[u]);
         }
-        softmax_rows<V, CH, R>(z);               // (a masked row: zeros)
+        auto finish = [&](auto rows) {
+            constexpr int N = decltype(rows)::value;
+            softmax_rows<N>(z);                  // (a masked row: zeros)
 #pragma unroll
-        for (int u = 0; u < R; ++u) {
-            dot[u] = 0.0f;
+            for (int u = 0; u < N; ++u) {
+                dot[u] = 0.0f;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+                for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int i = 0; i < V; ++i) dot[u] = fmaf(z[u][c][i], f[c][i], dot[u]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-            for (int u = 0; u < R; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
-#pragma unroll
-        for (int u = 0; u < R; ++u) {
-            const long long r = r0 + u * warps;
-            if (r >= n_rows) break;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[u][c][i] = g * z[u][c][i] * (f[c][i] - dot[u]);
-                const int e = (c * 32 + lane) * V;
-                if (e < n_experts) store_v<DT, V>(grad, static_cast<size_t>(r) * n_experts + e, z[u][c]);
+                    for (int i = 0; i < V; ++i) dot[u] = fmaf(z[u][c][i], f[c][i], dot[u]);
             }
-        }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int u = 0; u < N; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) z[u][c][i] = g * z[u][c][i] * (f[c][i] - dot[u]);
+                    const int e = (c * 32 + lane) * V;
+                    if (e < n_experts) store_v<DT, V>(grad, static_cast<size_t>(r0 + u * warps) * n_experts + e, z[u][c]);
+                }
+        };
+        if (r0 + warps < n_rows) finish(std::integral_constant<int, R>{});
+        else finish(std::integral_constant<int, 1>{});
     }
 }
 
