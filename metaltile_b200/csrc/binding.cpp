@@ -793,6 +793,14 @@ const at::Tensor *row_mask(PyObject *o, int64_t rows) {
     return &m;
 }
 
+// A contiguous tensor of 4-byte values in the storage of `block`, from this byte on
+at::Tensor part_of(const at::Tensor &block, at::ScalarType type, int64_t byte, at::IntArrayRef size) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()), block.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    t.unsafeGetTensorImpl()->set_storage_offset(byte / 4);
+    return t;
+}
+
 // moe_balance(logits, topk_idx, coef, mask, ctx) -> (loss, counts, mean_probs, n_counted)
 PyObject *moe_balance(Args a, Py_ssize_t n) {
     nargs(n, 5);
@@ -810,10 +818,12 @@ PyObject *moe_balance(Args a, Py_ssize_t n) {
     const Call c(a[4], l);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(l.device());
-        loss = empty({}, at::kFloat, l);
-        counts = empty({E}, at::kInt, l);
-        mean = empty({E}, at::kFloat, l);
-        counted = empty({}, at::kInt, l);
+        // the four results in one block (an allocation is a microsecond of the host's time): loss, n_counted, counts, mean_probs
+        const at::Tensor block = empty({8 + 8 * E}, at::kByte, l);
+        loss = part_of(block, at::kFloat, 0, {});
+        counted = part_of(block, at::kInt, 4, {});
+        counts = part_of(block, at::kInt, 8, {E});
+        mean = part_of(block, at::kFloat, 8 + 4 * E, {E});
         const size_t need = mtc_moe_balance_workspace(c.h, static_cast<int>(R), static_cast<int>(E));
         at::Tensor space;
         if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, l);
