@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
         int s = 0;
         uint32_t phase = 1, s_phase = 1;         // of `empty`: the first round passes
         int b = 0;
-        bool go = true;
+        bool go = true, ok = true;               // of the warp; of the lane that requests the codes, which the others hear of once per kHeld blocks
         if (!a.expert_offsets && !a.early) {
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;");
@@ -250,9 +250,9 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
                     if (b ^= 1; b == 0) s_phase ^= 1;
                 }
                 const bool requested = kb - kb0 < ahead;
-                if (lane == 0) {
-                    go = requested || wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u);
-                    if (go) {
+                if (lane == 0 && ok) {
+                    ok = requested || wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u);
+                    if (ok) {
                         const uint32_t at = ring + s * F::kStage;
                         if (!requested) {
                             mbar_expect_tx(&ctl->full[s], F::kStage);
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
                     }
                 }
                 if (++s == F::kStages) s = 0, phase ^= 1;
-                if ((kb + 1 - kb0) % F::kHeld == 0 || kb + 1 == kb1) go = __shfl_sync(0xffffffffu, go, 0);
+                if ((kb + 1 - kb0) % F::kHeld == 0 || kb + 1 == kb1) go = __shfl_sync(0xffffffffu, ok, 0);
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");

@@ -247,7 +247,7 @@ def _check_groups(out, x, xs, w, ws, off, untouched):
 @pytest.mark.parametrize("counts,n,k,lead,tail", [
     ([1], 130, 256, 0, 0), ([0, 0, 5], 129, 144, 0, 0), ([3, 0, 1, 0, 0, 7], 256, 400, 2, 3), ([1] * 32, 96, 128, 0, 0), ([130, 0, 257, 64], 200, 272, 0, 5),
     ([16, 17, 15, 1, 33], 384, 1024, 1, 0), ([0, 0, 0], 64, 64, 0, 4), ([300, 20], 1000, 130, 0, 0), ([64, 65, 63, 128, 129, 127, 32, 31, 33], 257, 512, 0, 1),
-    ([1000, 1, 0, 600], 512, 640, 3, 2),
+    ([1000, 1, 0, 600], 512, 640, 3, 2), ([1, 0, 2] * 70, 130, 160, 1, 1), ([2] * 1030, 64, 128, 0, 0),
 ])
 def test_gather(counts, n, k, lead, tail, dt, kernel):
     from metaltile_b200 import ops
@@ -319,6 +319,56 @@ def test_mm_on_another_stream_and_in_graphs(m, n, k, kernel):
         assert torch.equal(outs[0], want[a]) and torch.equal(outs[1], want[b])
 
 
+def test_a_captured_layer_replays_with_other_routing(kernel):
+    """Offsets are read on the device: the same graph serves other rows, other experts, and none."""
+    from metaltile_b200 import ops
+    e, k = 6, 2
+    _, _, w, ws = _operands(1, 256, 384, 4, experts=e)
+    cases = []
+    for i in range(3):
+        x = _x(150, 384, "bf16", i)
+        logits = torch.randn(150, e, device="cuda", generator=_gen(i)) + torch.tensor([0.0, 9.0, 0.0, -9.0, 0.0, 3.0], device="cuda") * i
+        idx, _ = ops.moe_router_topk(logits, k)
+        cases.append((x, idx))
+
+    def layer(x, idx):
+        order, _, off, _ = ops.moe_sort(idx, e)
+        codes, scales = ops.fp8_quantize(x, rows=order)
+        return codes, scales, off, ops.fp8_gather_mm(codes, w, ws, off, scales)
+
+    x, idx = (t.clone() for t in cases[0])
+    layer(x, idx)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        codes, scales, off, out = layer(x, idx)
+    for xx, ii in cases:
+        x.copy_(xx), idx.copy_(ii)
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_groups(out, codes, scales, w, ws, off.tolist(), out)
+
+
+def test_a_product_right_behind_the_quantizer_of_its_weights():
+    """The context keeps a product from requesting weights that are still being written."""
+    from metaltile_b200 import ops
+    mats = [(torch.randn(1024, 2048, device="cuda", generator=_gen(i)) * 0.02).bfloat16() for i in range(4)]
+    x = _x(3, 2048, "bf16")
+    want = []
+    for m in mats:
+        w, ws = ops.fp8_quantize(m, block_rows=128)
+        torch.cuda.synchronize()
+        want.append(ops.fp8_mm(x, w, ws))
+        torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for m in mats:
+            w, ws = ops.fp8_quantize(m, block_rows=128)
+            got.append(ops.fp8_mm(x, w, ws))
+            got.append(ops.fp8_mm(x, w, ws))
+        assert all(torch.equal(g, want[i // 2]) for i, g in enumerate(got))
+
+
 def test_calls_of_two_threads_at_once():
     from metaltile_b200 import ops
     jobs = []
@@ -347,7 +397,9 @@ def test_gradient_of_x_is_the_product_with_the_matrix_the_other_way_round():
     _, _, w, ws = _operands(1, 384, 640, 5)
     dy = _x(50, 384, "bf16", 3)
     dyq, dys = ops.fp8_quantize(dy)
-    dx = ops.fp8_mm(dy, w.T.contiguous(), ws.T.contiguous(), out_dtype=torch.float32)
+    wt, wst = w.T.contiguous(), ws.T.contiguous()
+    torch.cuda.synchronize()                                         # weights are there before a product that may request them early
+    dx = ops.fp8_mm(dy, wt, wst, out_dtype=torch.float32)
     want = (dyq.double() * ref.spread(dys, 50, 384, 1)) @ (w.double() * ref.spread(ws, 384, 640, 128))
     size = (dyq.double() * ref.spread(dys, 50, 384, 1)).abs() @ (w.double() * ref.spread(ws, 384, 640, 128)).abs()
     assert ((dx.double() - want).abs() <= 140 * 2.0 ** -23 * size).all()
