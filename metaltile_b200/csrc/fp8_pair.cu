@@ -47,6 +47,7 @@ struct PArgs {
     void *out;
     uint32_t *status;
     int M, N, nkb, n_experts;
+    int chunks;                                  // of 256 tokens; grouped: the most that offsets in order make
     int col_tiles, row_blocks;                   // ceil(N / 256), ceil(N / 128)
     int out_dt;
     int wide;                                    // rows of the output are whole 16-byte pieces at 16-byte boundaries: `out` of the maps holds
@@ -99,6 +100,7 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
 // The chunks of the experts, by one warp: ceil(rows / 256) each.  Offsets that run backwards or past the rows are clamped and reported.
 __device__ void count_chunks(PCtrl *ctl, const PArgs &a) {
     const int lane = threadIdx.x & 31;
+    constexpr uint32_t kMany = 0x7FFFFFFFu;      // sums end there: offsets that run backwards may hold any number of rows
     uint32_t before = 0;
     for (int e0 = 0; e0 < a.n_experts; e0 += 32) {
         const int e = e0 + lane;
@@ -114,17 +116,17 @@ __device__ void count_chunks(PCtrl *ctl, const PArgs &a) {
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += v;
+            if (lane >= d) upto = min(upto + v, kMany);
         }
         if (e < a.n_experts) {
-            ctl->first_chunk[e] = before + upto - np;
+            ctl->first_chunk[e] = min(before + (upto - np), kMany);
             ctl->offset[e] = lo;
         }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        before = min(before + __shfl_sync(0xffffffffu, upto, 31), kMany);
     }
     if (lane == 0) {
         ctl->first_chunk[a.n_experts] = before;
-        ctl->n_chunks = before;
+        ctl->n_chunks = min(before, static_cast<uint32_t>(a.chunks));
     }
 }
 
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     }
     pdl_enter();
     if (!a.expert_offsets) {
-        if (threadIdx.x == 0) ctl->n_chunks = (a.M + kTokens - 1) / kTokens;
+        if (threadIdx.x == 0) ctl->n_chunks = a.chunks;
     } else if (warp == 0) {
         count_chunks(ctl, a);
     }
@@ -585,6 +587,8 @@ cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
         e = make_map_2d(&maps.out, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, size, out, M, N, 32, 128 / size, why);
     if (e != cudaSuccess) return e;
     const long long chunks = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) + M / kTokens : (M + kTokens - 1) / kTokens, tiles = chunks * a.col_tiles;
+    if (tiles > kMostSize) return cudaErrorInvalidConfiguration;
+    a.chunks = static_cast<int>(chunks);
     // K slices where tiles would leave SMs without work, all clusters at once (15 of four pairs, 33 of two).  Joining them takes 3 us: 256 x 4096 x 4096 18.3 us, in two slices
     // 16.2; x 14336 50.1 and 34.3; 256 x 1024 x 4096 17.7, in four 13.0; but x 2048 11.6 to 11.8 and 12.1 to 12.4.
     if (!expert_offsets && a.nkb >= 24 && tiles <= clusters_at_once<4>()) return launch<4>(st, maps, a, tiles);

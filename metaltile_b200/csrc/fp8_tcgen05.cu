@@ -58,7 +58,7 @@ struct TArgs {
     uint32_t *status;
     int M, N, nkb, n_experts;
     int tiles;                                   // of 128 weight rows
-    int chunks;                                  // dense: of TN tokens
+    int chunks;                                  // dense: of TN tokens; grouped: the most that offsets in order make
     int slices;
     int out_dt;
     int early;                                   // weights may be requested before the previous kernel is complete
@@ -103,7 +103,8 @@ struct Chunk {
 };
 __device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts, int m_total, int TN, int want, uint32_t *status, Chunk &found) {
     const int lane = threadIdx.x & 31;
-    int before = 0;
+    constexpr uint32_t kMany = 0x7FFFFFFFu;      // sums end there: offsets that run backwards may hold any number of rows
+    uint32_t before = 0;
     for (int e0 = 0; e0 < n_experts; e0 += 32) {
         const int e = e0 + lane;
         int lo = 0, hi = 0;
@@ -114,13 +115,13 @@ __device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts
             if (status && (a > m || b > m || b < a)) atomicCAS(status, 0u, 0x901u);
         }
         const int np = (hi - lo + TN - 1) / TN;
-        int upto = np;
+        uint32_t upto = np;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += v;
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto = min(upto + v, kMany);
         }
-        const int mine = want - before - (upto - np);                // index of the wanted chunk among this expert's
+        const int mine = want - static_cast<int>(before) - (static_cast<int>(upto) - np);      // index of the wanted chunk among this expert's
         const uint32_t has = __ballot_sync(0xffffffffu, want >= 0 && mine >= 0 && mine < np);
         if (has) {
             const int src = __ffs(has) - 1;
@@ -129,9 +130,9 @@ __device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts
             found.ntok = min(TN, __shfl_sync(0xffffffffu, hi, src) - found.tok0);
             return want;
         }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        before = min(before + __shfl_sync(0xffffffffu, upto, 31), kMany);
     }
-    return before;
+    return static_cast<int>(before);
 }
 
 // Giving up, once every role has ended: lets what is on its way arrive before the CTA tears down.
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
             Chunk none;
             const int n = find_chunk(a.expert_offsets, a.n_experts, a.M, TN, -1, blockIdx.x == 0 ? a.status : nullptr, none);
             __syncwarp();
-            if (lane == 0) ctl->n_chunks = n;
+            if (lane == 0) ctl->n_chunks = min(n, a.chunks);         // offsets that run backwards may hold rows many times over
         }
     }
     tc_fence_before();
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
     // grouped: the tiles of a chunk behind each other; dense: the chunks of a tile, which read the same weights
     auto tile_of = [&](int unit) { return a.expert_offsets ? unit % a.tiles : unit / a.chunks; };
     auto chunk_of = [&](int unit) {
-        Chunk c;
+        Chunk c{0, 0, 0};
         if (a.expert_offsets) {
             find_chunk(a.expert_offsets, a.n_experts, a.M, TN, unit / a.tiles, nullptr, c);
         } else {
@@ -423,8 +424,8 @@ cudaError_t launch_as(Ctx *ctx, cudaStream_t st, const uint8_t *x, const uint8_t
     if (e != cudaSuccess) return e;
     static PerDeviceAttr attr;
     if ((e = attr.set(fp8_tile_kernel<TN, SLICED>, kSmemBytes)) != cudaSuccess) return e;
-    const long long units = a.expert_offsets ? (static_cast<long long>(std::min(a.M, a.n_experts)) + a.M / TN) * a.tiles : static_cast<long long>(a.chunks) * a.tiles;
-    if (units > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    const long long units = static_cast<long long>(a.chunks) * a.tiles;
+    if (units > kMostSize) return cudaErrorInvalidConfiguration;
     // slices: a cluster a unit; else no more CTAs than run at once, each with units in turn
     const long long ctas = a.slices > 1 ? units * a.slices : std::min<long long>(units, static_cast<long long>(kPerSM) * ctx->sm_count);
     cudaLaunchConfig_t cfg{};
@@ -480,7 +481,9 @@ cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     // an expert on average (128 experts of 768 x 2048: 4 rows 26.0 us, with 32 29.6; 8 rows 32.9 and 31.6; 32 rows 47.0, with 64 50.4).  128 were slower than both this and pairs.
     const int rows = expert_offsets ? (M >= 8 * n_experts ? 32 : 16) : M;
     const int TN = rows <= 16 ? 16 : rows <= 64 ? 32 : 64;
-    a.chunks = (M + TN - 1) / TN;
+    const long long chunks = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) + M / TN : (M + TN - 1) / TN;
+    if (chunks > kMostSize) return cudaErrorInvalidConfiguration;
+    a.chunks = static_cast<int>(chunks);
     // An expert's tiles never make slices: what a cluster costs is more than it gives (32 experts of 1536 x 2048, 8 rows: 9.5 us, in slices 16.0)
     a.slices = expert_offsets ? 1 : slices_for(ctx->sm_count, static_cast<long long>(a.chunks) * a.tiles, a.nkb);
     a.early = expert_offsets ? 0 : early_weights(ctx, st);

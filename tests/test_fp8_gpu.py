@@ -287,6 +287,23 @@ def test_gather_offsets_that_make_no_sense_are_reported(off, kernel):
         ctx.status_clear()
 
 
+@pytest.mark.parametrize("m,e", [(64, 9), (700, 33), (1500, 200)])
+def test_gather_offsets_that_hold_the_rows_many_times_over(m, e, kernel):
+    """Ranges that overlap make more chunks than the launch was sized for: they end, are reported, and write no row of another tensor."""
+    from metaltile_b200 import ops
+    ctx = ops.context(0)
+    x, xs, w, ws = _operands(m, 160, 256, experts=e)
+    off = torch.tensor([m * (i % 2) for i in range(e + 1)], device="cuda", dtype=torch.int32)
+    held = torch.full((m + 8, 160), 5.0, device="cuda")
+    try:
+        ops.fp8_gather_mm(x, w, ws, off, xs, out=held[4:-4])
+        torch.cuda.synchronize()
+        assert ctx.status_word() == 0x901
+        assert (held[:4] == 5).all() and (held[-4:] == 5).all() and held.isfinite().all()
+    finally:
+        ctx.status_clear()
+
+
 # ---- streams, graphs, threads --------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (40, 512, 2880), (300, 384, 1024)])
 def test_mm_on_another_stream_and_in_graphs(m, n, k, kernel):
