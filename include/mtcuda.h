@@ -438,7 +438,7 @@ size_t mtc_fp8_gather_mm_workspace(const mtc_ctx *ctx, int m_total, int n_out, i
  *     counts[e] = how often topk_idx (u32[n_rows, k]) names e in them,   mean_probs[e] = (1 / n) sum_t p_t[e],
  *     loss = coef * n_experts * sum_e counts[e] / (n k) * mean_probs[e]                    (n = 0: everything 0)
  * loss f32, counts i32[n_experts], mean_probs f32[n_experts], n_counted i32 = n.  What masked rows hold does not matter.  An index outside the experts is not counted
- * and is reported through the status word (0x907).  n_experts <= 1024, k <= 32 as in mtc_moe_router_topk.  Sums run in a fixed order.
+ * and is reported through the status word (0x907).  n_experts <= 1024, k <= 32 as in mtc_moe_router_topk, n_rows * k < 2^31.  Sums run in a fixed order.
  * mtc_moe_balance_grad: grad T[n_rows, n_experts] = *grad_loss (f32, NULL: 1) * d loss / d logits
  *     = *grad_loss * coef * n_experts / n * p_t[e] * (f[e] - sum_j f[j] p_t[j]),  f = counts / (n k) constants;  zeros for masked rows. */
 int mtc_moe_balance(mtc_ctx *ctx, void *stream, const void *logits, const void *topk_idx, const void *mask, float coef, void *loss, void *counts, void *mean_probs,

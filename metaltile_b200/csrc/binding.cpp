@@ -642,6 +642,16 @@ void need_one_device(std::initializer_list<const at::Tensor *> ts) {
 void need_size(int64_t v, const char *what) {
     if (v > 0x7FFFFFFF) raise(PyExc_ValueError, std::string(what) + " must be below 2^31");
 }
+// A context launches on its own device: one that the caller names has to be of that of the tensors.
+void need_context_of(PyObject *given, const at::Tensor &x) {
+    if (given == Py_None) return;
+    PyObject *d = PyObject_GetAttrString(given, "device");
+    if (!d) throw PyErr{};
+    const long long device = PyLong_AsLongLong(d);
+    Py_DECREF(d);
+    if (device == -1 && PyErr_Occurred()) throw PyErr{};
+    if (device != x.device().index()) raise(PyExc_ValueError, "ctx is of another device than the tensors");
+}
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 at::ScalarType out_type(long long dt) { return dt == MTC_F32 ? at::kFloat : dt == MTC_F16 ? at::kHalf : at::kBFloat16; }
 void *on_stream(const at::Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -690,6 +700,7 @@ PyObject *fp8_quantize(Args a, Py_ssize_t n) {
     s_shape.back() = blocks(K);
     if (block_rows != 1) s_shape[s_shape.size() - 2] = blocks(M);
     at::Tensor codes, scales;
+    need_context_of(a[4], x);
     const Call c(a[4], x);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(x.device());
@@ -731,6 +742,7 @@ PyObject *fp8_mm(Args a, Py_ssize_t n) {
         if (out.device() != x.device() || out.scalar_type() != out_type(odt)) raise(PyExc_TypeError, "out must live on the device of x and have type out_dtype");
         check_out(out, M, N, out);
     }
+    need_context_of(a[6], x);
     const Call c(a[6], x);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(x.device());
@@ -771,6 +783,7 @@ PyObject *fp8_gather_mm(Args a, Py_ssize_t n) {
         if (out.device() != x.device() || out.scalar_type() != out_type(odt)) raise(PyExc_TypeError, "out must live on the device of x and have type out_dtype");
         check_out(out, M, N, out);
     }
+    need_context_of(a[7], x);
     const Call c(a[7], x);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(x.device());
@@ -815,6 +828,7 @@ PyObject *moe_balance(Args a, Py_ssize_t n) {
     if (mask) need_one_device({&l, &idx, mask}); else need_one_device({&l, &idx});
     need_size(R, "rows"), need_size(E, "n_experts");
     at::Tensor loss, counts, mean, counted;
+    need_context_of(a[4], l);
     const Call c(a[4], l);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(l.device());
@@ -854,6 +868,7 @@ PyObject *moe_balance_grad(Args a, Py_ssize_t n) {
     const bool given = a[7] != Py_None;
     at::Tensor out = given ? tensor(a[7], "out") : at::Tensor();
     if (given) check_out(out, R, E, l);
+    need_context_of(a[8], l);
     const Call c(a[8], l);
     c.check(unlocked([&] {
         const c10::cuda::CUDAGuard guard(l.device());

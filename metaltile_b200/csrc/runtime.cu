@@ -1601,6 +1601,7 @@ static int balance_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int n_expe
     if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": dtype must be f32, f16 or bf16");
     if (n_rows < 0 || n_experts <= 0 || n_experts > 1024 || k <= 0 || k > 32 || k > n_experts)
         return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": need 0 < k <= min(32, n_experts), n_experts <= 1024");
+    if (static_cast<long long>(n_rows) * k > 0x7FFFFFFF) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": n_rows * k must be below 2^31 (counts are 32 bits)");
     return MTC_OK;
 }
 

@@ -145,3 +145,21 @@ def test_refusals_of_sizes():
     for e, k in ((1025, 8), (64, 33), (4, 5), (4, 0)):
         with pytest.raises(MetalTileError):
             ops.moe_balance(torch.zeros(3, e, device="cuda"), torch.zeros(3, k, device="cuda", dtype=torch.int32))
+    with pytest.raises(MetalTileError, match="2\\^31"):               # counts are 32 bits
+        ops.context(0).moe_balance(0, 0, None, 1.0, 0, 0, 0, 0, 2 ** 26, 64, 32, torch.float32)
+
+
+def test_a_context_of_another_device_is_refused():
+    from types import SimpleNamespace
+    from metaltile_b200 import ops
+    other = SimpleNamespace(device=1, _h=None)
+    logits, idx = torch.zeros(3, 8, device="cuda"), torch.zeros(3, 2, device="cuda", dtype=torch.int32)
+    _, counts, _, counted = ops.moe_balance(logits, idx)
+    x = torch.zeros(4, 128, device="cuda")
+    w, ws = ops.fp8_quantize(x, block_rows=128)
+    xq, xs = ops.fp8_quantize(x)
+    off = torch.tensor([0, 4], device="cuda", dtype=torch.int32)
+    for call in (lambda: ops.moe_balance(logits, idx, ctx=other), lambda: ops.moe_balance_grad(logits, counts, counted, 2, ctx=other),
+                 lambda: ops.fp8_quantize(x, ctx=other), lambda: ops.fp8_mm(x, w, ws, ctx=other), lambda: ops.fp8_gather_mm(xq, w[None], ws[None], off, xs, ctx=other)):
+        with pytest.raises(ValueError, match="another device"):
+            call()
