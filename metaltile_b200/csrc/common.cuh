@@ -24,6 +24,7 @@ struct FreshWeights {
     std::atomic<int> n{0};
     std::atomic<bool> anywhere{false};     // more streams than the list holds: no product starts on its weights early any more
     cudaStream_t streams[kMost] = {};
+    bool captured[kMost] = {};             // written by a graph under capture: what runs now has its own entry
 };
 
 struct Ctx {
@@ -104,15 +105,21 @@ inline cudaError_t grow_block(Ctx *ctx, cudaStream_t st, void **block, size_t *h
 // time that product lets the next one start, its own wait has made the quantizer's stores visible.  (That next one, and
 // everything on other streams that is ordered by an event, needs nothing more.)  A product that does not start early waits
 // before it signals its dependents.
+inline bool under_capture(cudaStream_t st) {
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(st, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
+}
 inline void weights_written(Ctx *ctx, cudaStream_t st) {
     if (st == cudaStreamLegacy) st = nullptr;
     FreshWeights &f = ctx->fresh;
+    const bool captured = under_capture(st);
     const std::lock_guard<std::mutex> hold(f.lock);
     const int n = f.n.load(std::memory_order_relaxed);
     for (int i = 0; i < n; ++i)
-        if (f.streams[i] == st) return;
+        if (f.streams[i] == st && f.captured[i] == captured) return;
     if (n < FreshWeights::kMost) {
         f.streams[n] = st;
+        f.captured[n] = captured;
         f.n.store(n + 1, std::memory_order_release);
     } else {
         f.anywhere.store(true);
@@ -123,11 +130,13 @@ inline int early_weights(Ctx *ctx, cudaStream_t st) {
     FreshWeights &f = ctx->fresh;
     if (f.n.load(std::memory_order_acquire) != 0) {
         if (st == cudaStreamLegacy) st = nullptr;
+        const bool captured = under_capture(st);
         const std::lock_guard<std::mutex> hold(f.lock);
         const int n = f.n.load(std::memory_order_relaxed);
         for (int i = 0; i < n; ++i)
-            if (f.streams[i] == st) {
+            if (f.streams[i] == st && f.captured[i] == captured) {
                 f.streams[i] = f.streams[n - 1];
+                f.captured[i] = f.captured[n - 1];
                 f.n.store(n - 1, std::memory_order_release);
                 return 0;
             }

@@ -386,6 +386,30 @@ def test_a_product_right_behind_the_quantizer_of_its_weights():
         assert all(torch.equal(g, want[i // 2]) for i, g in enumerate(got))
 
 
+def test_a_product_captured_behind_a_quantizer_leaves_the_next_one_waiting():
+    """The captured product does not run: the first that does is the one to wait for the weights."""
+    from metaltile_b200 import ops
+    m = (torch.randn(2048, 2048, device="cuda", generator=_gen(9)) * 0.02).bfloat16()
+    xq, xs = ops.fp8_quantize(_x(2, 2048, "bf16"))
+    w, ws = ops.fp8_quantize(m, block_rows=128)
+    torch.cuda.synchronize()
+    want = ops.fp8_mm(xq, w, ws, xs)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            torch.cuda._sleep(20_000_000)                            # the quantizer is still to come when the products are launched
+            w, ws = ops.fp8_quantize(m, block_rows=128)
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            captured = ops.fp8_mm(xq, w, ws, xs)
+            graph.capture_end()
+            got = ops.fp8_mm(xq, w, ws, xs)
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(got, want) and torch.equal(captured, want)
+
+
 def test_calls_of_two_threads_at_once():
     from metaltile_b200 import ops
     jobs = []
