@@ -93,6 +93,25 @@ def test_quotients_on_a_border_between_codes(dt):
         _same_codes(codes, want)
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dt,bits", [("bf16", 8), ("f16", 11)])
+def test_every_mantissa_in_a_block_of_every_maximum(dt, bits, block_rows):
+    """16-bit types decide codes by a factor that depends on which side of amax / 448 its scale is rounded to: every pair of mantissas, over as many binary
+    orders as a code has, and subnormal ones."""
+    from metaltile_b200 import ops
+    half = 1 << (bits - 1)
+    top = torch.arange(half, 2 * half, device="cuda", dtype=torch.float64)
+    x = top[None, :, None] * torch.exp2(-torch.arange(16384 // half, device="cuda", dtype=torch.float64) % 17)         # [1, mantissa, order]
+    x = torch.where(x > top[:, None, None], x / 2, x).reshape(half, -1, 128)
+    x[:, :, 0] = top[:, None]
+    for scale in (2.0 ** -5, 2.0 ** -20 if dt == "f16" else 2.0 ** -130):
+        v = (x * scale).to(TYPES[dt]).reshape(-1, 128)
+        codes, scales = ops.fp8_quantize(v, block_rows=block_rows)
+        want, s = ref.quantize(v, block_rows)
+        assert torch.equal(scales.double(), s)
+        _same_codes(codes, want)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_quantize_special_values(dt):
     from metaltile_b200 import ops
