@@ -8,8 +8,10 @@
 //
 // What bounds it.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM of a pair: 64 bytes a
 // cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Without the epilogue the ring and the MMAs run at 585 cycles a block.  With it a
-// block takes 780: two accumulators are all of the tensor memory, so a block's MMAs (512), the way to the epilogue, its four loads of tensor memory in a row, the way
-// back and the issue of the next are one chain for two blocks.  2048 x 28672 x 4096: 214 us, 2.25 PFLOP/s.
+// block takes 780 to 840, the MMA warp waiting for an accumulator: two are all of the tensor memory, so a block's MMAs (512), the way to the epilogue, its four loads of tensor
+// memory in a row, the way back and the issue of the next are one chain for two blocks.  But no single link is the bound (1184 x 4096 x 28672, 838 cycles a block): handed back
+// before it is read 822, one load of four 800, no additions 755, all three together 746.  Waits that spin instead of sleeping slow the others' shared memory (2 to 8 % more).
+// A tile ends with 2300 cycles of stores (f32 4000) and 300 to 900 to find the next; MMAs of two blocks run beside that.  2048 x 28672 x 4096: 214 us, 2.25 PFLOP/s.
 //
 // Steps on the way (us for that case): hand-offs that release at cluster scope 587, relaxed ones 348; one try in front of the polling loop, whose entry costs 200 cycles,
 // and results out by TMA instead of a row a lane 303; the registers of the other roles for the epilogue, so that nothing spills, and the next columns loaded while the
