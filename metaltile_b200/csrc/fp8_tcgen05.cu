@@ -96,38 +96,56 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v
 }
 __device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
-// Chunks of TN rows: expert e with r rows has ceil(r / TN).  By one warp: how many there are in all (want < 0), or the one with index `want`.  Offsets that run
-// backwards or past the rows are clamped, and reported by the block that is told to.
+// Chunks of TN rows: expert e with r rows has ceil(r / TN).  By one warp, four experts a lane: how many there are in all (want < 0), or the one with index `want`.  Offsets that
+// run backwards or past the rows are clamped, and reported by the block that is told to.  (A load and a scan for 128 experts; with one for 32 128 experts of 768 x 2048 and 32
+// rows in all 14.7 us for 13.1, 4096 rows 46.0 for 43.4, 512 experts of 512 x 1024 and 512 rows 43.4 for 34.9.)
 struct Chunk {
     int expert, tok0, ntok;
 };
 __device__ __forceinline__ int find_chunk(const uint32_t *offsets, int n_experts, int m_total, int TN, int want, uint32_t *status, Chunk &found) {
-    const int lane = threadIdx.x & 31;
     constexpr uint32_t kMany = 0x7FFFFFFFu;      // sums end there: offsets that run backwards may hold any number of rows
+    const int lane = threadIdx.x & 31;
+    const uint32_t m = static_cast<uint32_t>(m_total);
     uint32_t before = 0;
-    for (int e0 = 0; e0 < n_experts; e0 += 32) {
-        const int e = e0 + lane;
-        int lo = 0, hi = 0;
-        if (e < n_experts) {
-            const uint32_t a = offsets[e], b = offsets[e + 1], m = static_cast<uint32_t>(m_total);
-            lo = static_cast<int>(min(a, m));
-            hi = max(lo, static_cast<int>(min(b, m)));
-            if (status && (a > m || b > m || b < a)) atomicCAS(status, 0u, 0x901u);
+    for (int e0 = 0; e0 < n_experts; e0 += 128) {
+        uint32_t at[5];                          // (behind the last expert: its end, no rows)
+#pragma unroll
+        for (int i = 0; i < 5; ++i) at[i] = offsets[min(e0 + 4 * lane + i, n_experts)];
+        bool wrong = at[0] > m;
+        int lo[4], hi[4];
+        uint32_t own = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            wrong |= at[i + 1] > m || at[i + 1] < at[i];
+            lo[i] = static_cast<int>(min(at[i], m));
+            hi[i] = max(lo[i], static_cast<int>(min(at[i + 1], m)));
+            own += (hi[i] - lo[i] + TN - 1) / TN;
         }
-        const int np = (hi - lo + TN - 1) / TN;
-        uint32_t upto = np;
+        if (status && wrong) atomicCAS(status, 0u, 0x901u);
+        uint32_t upto = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto = min(upto + v, kMany);
         }
-        const int mine = want - static_cast<int>(before) - (static_cast<int>(upto) - np);      // index of the wanted chunk among this expert's
-        const uint32_t has = __ballot_sync(0xffffffffu, want >= 0 && mine >= 0 && mine < np);
+        int mine = want - static_cast<int>(before) - static_cast<int>(upto - own);     // index of the wanted chunk among this lane's
+        const uint32_t has = __ballot_sync(0xffffffffu, want >= 0 && mine >= 0 && mine < static_cast<int>(own));
         if (has) {
+            int expert = 0, tok0 = 0, ntok = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int np = (hi[i] - lo[i] + TN - 1) / TN;
+                if (mine >= 0 && mine < np) {
+                    expert = e0 + 4 * lane + i;
+                    tok0 = lo[i] + mine * TN;
+                    ntok = min(TN, hi[i] - tok0);
+                }
+                mine -= np;
+            }
             const int src = __ffs(has) - 1;
-            found.expert = e0 + src;
-            found.tok0 = __shfl_sync(0xffffffffu, lo + mine * TN, src);
-            found.ntok = min(TN, __shfl_sync(0xffffffffu, hi, src) - found.tok0);
+            found.expert = __shfl_sync(0xffffffffu, expert, src);
+            found.tok0 = __shfl_sync(0xffffffffu, tok0, src);
+            found.ntok = __shfl_sync(0xffffffffu, ntok, src);
             return want;
         }
         before = min(before + __shfl_sync(0xffffffffu, upto, 31), kMany);
