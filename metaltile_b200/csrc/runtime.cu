@@ -1503,10 +1503,11 @@ static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_exper
     if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, n_experts, x, w)) return FP8_CUDA_CORE;
     const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
     if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
-    // Pairs of CTAs have tiles of 256 tokens.  Grouped (128 experts of 768 x 2048, us of tiles and pairs): 32 rows an expert 47 and 52, 64 69 and 59.  Dense: from more than 64
+    // Pairs of CTAs have tiles of 256 tokens.  Grouped (us of tiles and pairs): 128 experts of 768 x 2048, 48 rows an expert 53 and 62, 56 54 and 63, 64 60 and 64;
+    // of 2048 x 768, 48 rows 62 and 68, 64 77 and 68; 8 of 4096 x 1536, 48 rows 19.2 and 19.7, 64 22.6 and 19.9.  Dense: from more than 64
     // tokens on, unless that is so few tiles of 64 x 128 that cutting K into four slices and more fills the GPU (256 x 1024 x 4096 10.8 and 13.0, 256 x 4096 x 4096 20 and 16,
     // 128 x 4096 x 14336 26 and 34, 64 x 14336 x 4096 19 and 20, 128 x 14336 x 4096 26 and 21).
-    if (grouped) return pair && M / n_experts >= 48 ? FP8_PAIR : FP8_TILE;
+    if (grouped) return pair && M / n_experts >= 56 ? FP8_PAIR : FP8_TILE;
     return pair && M > 64 && static_cast<long long>((M + 63) / 64) * mtc::fp8::blocks(N) > 64 ? FP8_PAIR : FP8_TILE;
 }
 

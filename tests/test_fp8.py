@@ -90,7 +90,7 @@ def test_workspaces_cover_what_the_call_stages():
 @pytest.mark.parametrize("args,want", [
     ((1, 4096, 4096, 0), "tile"), ((64, 14336, 4096, 0), "tile"), ((65, 4096, 4096, 0), "tile"), ((65, 4097, 4096, 0), "pair"), ((256, 2048, 4096, 0), "tile"),
     ((257, 2048, 4096, 0), "pair"), ((2048, 28672, 4096, 0), "pair"), ((1, 64, 130, 0), "cuda_core"), ((2048, 4096, 4088, 0), "cuda_core"),
-    ((32, 768, 2048, 128), "tile"), ((6143, 768, 2048, 128), "tile"), ((6144, 768, 2048, 128), "pair"), ((60000, 768, 2048, 1025), "tile"), ((64, 64, 100, 8), "cuda_core"),
+    ((32, 768, 2048, 128), "tile"), ((7167, 768, 2048, 128), "tile"), ((7168, 768, 2048, 128), "pair"), ((60000, 768, 2048, 1025), "tile"), ((64, 64, 100, 8), "cuda_core"),
     ((8, 2 ** 20, 16, 2 ** 12), "cuda_core"), ((0, 64, 64, 0), None), ((2 ** 31 - 1, 64, 64, 0), None), ((1, 64, 2 ** 31 - 8, 0), None),
 ])
 def test_kernels_on_both_sides_of_the_rules(args, want):
