@@ -365,6 +365,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
             }
+            // The MMAs' arrivals at `empty` come through the cluster on their own: the last ones are awaited too, so that none reaches a CTA that has left
+            for (int i = 0; go && i < kStages; ++i) {
+                go = wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb11u);
+                if (++s == kStages) s = 0, phase ^= 1;
+            }
         }
     } else if (warp == kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs<SLICES>));
@@ -502,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
     __syncthreads();
     if (ctl->abort) {                            // gave up: let what is on its way arrive (the first CTA's barriers count both CTAs' copies)
         if (warp == kMmaWarp && rank == 0 && elect_one()) {
-            commit_pair(&ctl->drained, 3u << leader);
+            commit_pair(&ctl->drained, 1u << leader);            // (the other CTA does not wait for it)
             drain_ring(&ctl->drained, 1, 1);
         } else if (warp == kLoadWarp && rank == 0 && lane == 0) {
             drain_ring(ctl->full, ctl->issued, kStages);
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
         __syncthreads();
     }
     tc_fence_before();
-    cluster_sync();                              // nobody leaves while the other may still arrive at its barriers or read its memory
+    cluster_sync();                              // nobody leaves while the other's threads may still arrive at its barriers or read its memory
     tc_fence_after();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
 }

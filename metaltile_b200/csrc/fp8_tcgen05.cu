@@ -292,6 +292,10 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
                 if ((kb + 1 - kb0) % F::kHeld == 0 || kb + 1 == kb1) go = __shfl_sync(0xffffffffu, ok, 0);
             }
         }
+        for (int i = 0; lane == 0 && go && ok && i < F::kStages; ++i) {      // the MMAs' last arrivals at `empty`: none reaches a CTA that has left
+            ok = wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb01u);
+            if (++s == F::kStages) s = 0, phase ^= 1;
+        }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kMmaWarp) {
         constexpr uint32_t idesc = 1u << 4 | static_cast<uint32_t>(TN >> 3) << 17 | static_cast<uint32_t>(kRows >> 4) << 24;

@@ -1,0 +1,56 @@
+"""The 8-bit float products between other work: launches right behind each other, chunks that a launch was sized for and that do not come, long predecessors."""
+import pytest
+import torch
+
+import fp8_ref as ref
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _codes(*shape, seed=0):
+    return (torch.randn(*shape, device="cuda", generator=_gen(seed)) * 120).clamp(-448, 448).to(F8)
+
+
+def _scales(*shape, seed=0):
+    return (torch.rand(*shape, device="cuda", generator=_gen(seed)) + 0.5) * 2.0 ** -9
+
+
+def _operands(m, n, k, seed=0, experts=None):
+    lead = () if experts is None else (experts,)
+    return (_codes(m, k, seed=seed), _scales(m, ref.blocks(k), seed=seed + 1), _codes(*lead, n, k, seed=seed + 2),
+            _scales(*lead, ref.blocks(n), ref.blocks(k), seed=seed + 3))
+
+
+def test_kernels_that_follow_each_other_on_the_same_SMs():
+    """A CTA leaves only when the tensor core's last arrivals at its barriers have come: short ends (few columns) and other kernels in the same shared memory right behind them."""
+    from metaltile_b200 import ops
+    ctx = ops.context(0)
+    cases = [(3, 300, 8, 640), (3, 257, 264, 128), (2, 20, 8, 512), (3, 40, 130, 4096), (2, 200, 64, 128), (3, 1000, 16, 384)]
+    args = [_operands(m, n, k, 10 * i) for i, (_, m, n, k) in enumerate(cases)]
+    e = 5
+    x, xs, w, ws = _operands(300, 24, 256, 99, experts=e)
+    off = torch.tensor([0, 130, 130, 131, 290, 300], device="cuda", dtype=torch.int32)
+
+    def one(i):
+        ctx.set_option("fp8_kernel", cases[i][0])
+        return ops.fp8_mm(args[i][0], args[i][2], args[i][3], x_scales=args[i][1])
+
+    def grouped(kernel):
+        ctx.set_option("fp8_kernel", kernel)
+        return ops.fp8_gather_mm(x, w, ws, off, xs)
+
+    try:
+        torch.cuda.synchronize()
+        want, groups = [one(i) for i in range(len(cases))], [grouped(2), grouped(3)]
+        for (_, m, n, k), a, o in zip(cases, args, want):
+            ref.mm_close(o, *a)
+        got = [[one(i) for i in range(len(cases))] + [grouped(2), grouped(3)] for _ in range(60)]
+        assert all(torch.equal(g, v) for row in got for g, v in zip(row, want + groups))
+        assert ctx.status_word() == 0
+    finally:
+        ctx.set_option("fp8_kernel", 0)
