@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
         mbar_init(&ctl->drained, 1);
         ctl->abort = 0;
         ctl->issued = 0;
-        ctl->n_chunks = a.chunks;
+        if (!a.expert_offsets) ctl->n_chunks = a.chunks;         // (grouped: the producer counts them, and nobody else stores there)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {

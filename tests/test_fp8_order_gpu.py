@@ -54,3 +54,28 @@ def test_kernels_that_follow_each_other_on_the_same_SMs():
         assert ctx.status_word() == 0
     finally:
         ctx.set_option("fp8_kernel", 0)
+
+
+@pytest.mark.parametrize("kernel", [2, 3])
+def test_far_fewer_chunks_than_a_launch_is_sized_for(kernel):
+    """The number of chunks is counted on the device; where rows belong to nobody it is far below what the host reckons with."""
+    from metaltile_b200 import ops
+    ctx = ops.context(0)
+    x, xs, w, ws = _operands(4000, 200, 384, 7, experts=64)
+    offs = [torch.full((65,), 17, dtype=torch.int32), torch.tensor([5] * 30 + [9] * 35, dtype=torch.int32), torch.tensor([0] * 64 + [3], dtype=torch.int32)]
+    ctx.set_option("fp8_kernel", kernel)
+    try:
+        for off in offs:
+            on_device = off.cuda()
+            out = torch.full((4000, 200), -3.0, device="cuda", dtype=torch.bfloat16)
+            for _ in range(50):
+                ops.fp8_gather_mm(x, w, ws, on_device, xs, out=out)
+            at = off.tolist()
+            for e in range(64):
+                r = slice(at[e], at[e + 1])
+                if at[e + 1] > at[e]:
+                    ref.mm_close(out[r], x[r], xs[r], w[e], ws[e])
+            assert (out[:at[0]] == -3).all() and (out[at[-1]:] == -3).all()
+        assert ctx.status_word() == 0
+    finally:
+        ctx.set_option("fp8_kernel", 0)
