@@ -302,6 +302,8 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
         int s = 0, d = 0;
         uint32_t phase = 0, d_phase = 1;
         bool go = true;
+        // No stage is full before the previous kernels of the stream are complete (x is theirs): what they take does not count against the limit of the waits
+        if (!a.expert_offsets) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int unit = first; go && unit < units; unit += step)
             for (int kb = kb0; go && kb < kb1; kb += F::kTogether) {
                 const int here = min(F::kTogether, kb1 - kb);

@@ -79,3 +79,31 @@ def test_far_fewer_chunks_than_a_launch_is_sized_for(kernel):
         assert ctx.status_word() == 0
     finally:
         ctx.set_option("fp8_kernel", 0)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 2048), (40, 512, 2880), (64, 14336, 512), (300, 384, 1024)])
+def test_a_product_behind_a_kernel_that_lets_it_start_long_before_its_end(m, n, k):
+    """A barrier of peers one of which does not come (its limit of polls ends it after some hundredths of a second) lets the next kernels of the stream start at once: no role of
+    theirs may count that time against the limit of its own waits."""
+    from metaltile_b200 import ops
+    ctx = ops.context(0)
+    _, _, w, ws = _operands(1, n, k)
+    x = torch.randn(m, k, device="cuda", generator=_gen(5)).bfloat16()
+    codes, scales = ops.fp8_quantize(x)
+    want = ops.fp8_mm(x, w, ws)
+    mine, absent = (torch.zeros(64, dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    stream = torch.cuda.current_stream().cuda_stream
+    ctx.set_option("peer_poll_limit", 300000)
+    try:
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        ctx.peer_barrier([mine.data_ptr(), absent.data_ptr()], 0, mine.data_ptr(), mine.data_ptr() + 128, stream=stream)
+        got = [ops.fp8_mm(codes, w, ws, x_scales=scales, out_dtype=x.dtype), ops.fp8_mm(x, w, ws)]
+        end.record()
+        torch.cuda.synchronize()
+        assert start.elapsed_time(end) > 30 and ctx.status_word() == 0x602             # the barrier's report, and none of the products'
+        assert all(torch.equal(g, want) for g in got)
+    finally:
+        ctx.set_option("peer_poll_limit", 1 << 22)
+        ctx.status_clear()
