@@ -640,7 +640,7 @@ void need_one_device(std::initializer_list<const at::Tensor *> ts) {
         if (!t->is_cuda() || t->device() != first->device()) raise(PyExc_ValueError, "all operands must be tensors of one CUDA device");
 }
 void need_size(int64_t v, const char *what) {
-    if (v > 0x7FFFFFFF) raise(PyExc_ValueError, std::string(what) + " must be below 2^31");
+    if (v < 0 || v > 0x7FFFFFFF) raise(PyExc_ValueError, std::string(what) + " must be below 2^31, and not negative");
 }
 // A context launches on its own device: one that the caller names has to be of that of the tensors.
 void need_context_of(PyObject *given, const at::Tensor &x) {
@@ -823,6 +823,7 @@ PyObject *moe_balance(Args a, Py_ssize_t n) {
     const int dt = need_dtype(l);
     if (l.dim() != 2 || idx.dim() != 2 || idx.size(0) != l.size(0)) raise(PyExc_ValueError, "logits must be [rows, n_experts] and topk_idx [rows, k]");
     const int64_t R = l.size(0), E = l.size(1), k = idx.size(1);
+    need_size(k, "k");
     const at::Tensor *mask = row_mask(a[3], R);
     need_contiguous({&l});
     if (mask) need_one_device({&l, &idx, mask}); else need_one_device({&l, &idx});
@@ -859,12 +860,13 @@ PyObject *moe_balance_grad(Args a, Py_ssize_t n) {
     const int dt = need_dtype(l);
     if (l.dim() != 2) raise(PyExc_ValueError, "logits must be [rows, n_experts]");
     const int64_t R = l.size(0), E = l.size(1);
+    need_size(k, "k");
     if (counts.numel() != E || counted.numel() != 1) raise(PyExc_ValueError, "counts must have n_experts entries and n_counted one");
     if (gl && (gl->scalar_type() != at::kFloat || gl->numel() != 1)) raise(PyExc_TypeError, "grad_loss must be one float32");
     const at::Tensor *mask = row_mask(a[6], R);
     need_contiguous({&l});
     need_one_device({&l, &counts, &counted, gl ? gl : &l, mask ? mask : &l});
-    need_size(R, "rows"), need_size(E, "n_experts"), need_size(k, "k");
+    need_size(R, "rows"), need_size(E, "n_experts");
     const bool given = a[7] != Py_None;
     at::Tensor out = given ? tensor(a[7], "out") : at::Tensor();
     if (given) check_out(out, R, E, l);
