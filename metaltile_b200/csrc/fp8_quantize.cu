@@ -9,6 +9,8 @@
 // a time, monotone for all but NaN), and a quotient is one multiplication for 16-bit types (factor_of); f32 takes three and three that look whether it may be on a border.
 // Measured (graph, us): 14336 x 4096 in blocks of 128 x 128 bf16 and f16 32.3 (176 MB, 5.45 TB/s; as f32 is quantized 46.9), with powers of two 28.1, f32 51.3 (294 MB);
 // 8192 x 4096 rows bf16 23.3 (31.7), f32 29.5.
+#include <algorithm>
+
 #include "fp8.cuh"
 
 namespace mtc {
@@ -160,13 +162,14 @@ __device__ __forceinline__ void store8(uint8_t *codes, size_t at, int n, uint2 c
 constexpr int kThreads = 256, kGroups = kThreads / 16;
 
 // Blocks of 1 x 128.  A CTA has 16 groups of 16 lanes: 2^shift of them side by side in a row, TURNS times, the others in the next rows.
+// first: the block of K that the launch starts with.
 template <int DT, bool VEC, bool POW2, int TURNS>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const void *x, const uint32_t *rows, uint8_t *codes, float *scales, long long n_rows,
-                                                                 long long n_src_rows, int K, int shift, uint32_t *status) {
+                                                                 long long n_src_rows, int K, int shift, int first, uint32_t *status) {
     pdl_enter();
     const int kb = blocks(K), lane = threadIdx.x & 15, g = threadIdx.x >> 4, wide = 1 << shift;
     const long long r = static_cast<long long>(blockIdx.x) * (kGroups >> shift) + (g >> shift);
-    const int b0 = blockIdx.y * (wide * TURNS) + (g & (wide - 1));
+    const int b0 = first + blockIdx.y * (wide * TURNS) + (g & (wide - 1));
     const bool row = r < n_rows;
     long long src = row ? r : 0;
     if (rows && row) {
@@ -272,10 +275,14 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const void *x, const uint32_t *row
         const long long ctas = (n_rows + (kGroups >> shift) - 1) / (kGroups >> shift);
         // two blocks a group, all loads in flight at once, where that leaves every SM its eight CTAs
         const bool two = kb > 16 && ctas * ((kb + 31) / 32) >= 8ll * ctx->sm_count;
-        const int turns = two ? 2 : 1;
-        return launch_pdl(two ? quantize_rows_kernel<DT, VEC, POW2, 2> : quantize_rows_kernel<DT, VEC, POW2, 1>,
-                          dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((kb + (turns << shift) - 1) / (turns << shift))), kThreads, 0, st, x, rows, codes, scales,
-                          n_rows, n_src_rows, K, shift, ctx->d_status);
+        const int wide = (two ? 2 : 1) << shift, most = 65535 * wide;        // blocks of a CTA, of a launch (the grid's second dimension holds no more)
+        for (int first = 0; first < kb; first += most) {
+            const cudaError_t e = launch_pdl(two ? quantize_rows_kernel<DT, VEC, POW2, 2> : quantize_rows_kernel<DT, VEC, POW2, 1>,
+                                             dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((std::min(kb - first, most) + wide - 1) / wide)), kThreads, 0, st, x,
+                                             rows, codes, scales, n_rows, n_src_rows, K, shift, first, ctx->d_status);
+            if (e != cudaSuccess) return e;
+        }
+        return cudaSuccess;
     }
     const long long row_blocks = (n_rows + kBlock - 1) / kBlock, ctas = n_mats * row_blocks * kb;
     if (ctas > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
