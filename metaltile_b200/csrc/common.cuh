@@ -12,20 +12,11 @@
 #include <vector>
 
 #include "../../include/mtcuda.h"
+#include "fresh.cuh"
 
 namespace mtc {
 
 constexpr int kNumSMsB200 = 148;
-
-// Streams with weights that were just written.  Locked: two threads may quantize and multiply on streams of their own.
-struct FreshWeights {
-    static constexpr int kMost = 64;
-    std::mutex lock;
-    std::atomic<int> n{0};
-    std::atomic<bool> anywhere{false};     // more streams than the list holds: no product starts on its weights early any more
-    cudaStream_t streams[kMost] = {};
-    bool captured[kMost] = {};             // written by a graph under capture: what runs now has its own entry
-};
 
 struct Ctx {
     int device = 0;
@@ -53,7 +44,7 @@ struct Ctx {
     std::vector<void *> retired;   // outgrown scratch blocks: freed by mtc_destroy, so that captured graphs never see freed memory
     int qmv_frag = 1;              // option "qmv_frag": 0 = never use the fragment kernel (qmv_frag.cuh), 2 = whenever it supports the shape
     int qmv_stream = 1;            // option "qmv_stream": 0 = never use the streaming decode kernel (qmv_stream.cu)
-    FreshWeights fresh;            // streams on which mtc_affine_quantize ran since their last product (early_weights below)
+    FreshWeights fresh;            // streams on which a quantizer of weights ran since their last product (early_weights below)
     int pdl_early_weights = 1;     // option "pdl_early_weights": 0 = no load of w / scales / biases before the previous kernel of the stream is complete
     void *d_worklist = nullptr;    // gather_qmm work list (grow-only, owned by the context)
     size_t worklist_bytes = 0;
@@ -100,8 +91,8 @@ inline cudaError_t grow_block(Ctx *ctx, cudaStream_t st, void **block, size_t *h
     return cudaSuccess;
 }
 
-// Products request their weights before the previous kernel of the stream is complete: weights are constants.  The one kernel of
-// this library that writes weights is the quantizer, so the first product behind it on its stream does not start early; by the
+// Products request their weights before the previous kernel of the stream is complete: weights are constants.  What in
+// this library writes weights are the quantizers, so the first product behind it on its stream does not start early; by the
 // time that product lets the next one start, its own wait has made the quantizer's stores visible.  (That next one, and
 // everything on other streams that is ordered by an event, needs nothing more.)  A product that does not start early waits
 // before it signals its dependents.
@@ -110,38 +101,12 @@ inline bool under_capture(cudaStream_t st) {
     return cudaStreamIsCapturing(st, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone;
 }
 inline void weights_written(Ctx *ctx, cudaStream_t st) {
-    if (st == cudaStreamLegacy) st = nullptr;
-    FreshWeights &f = ctx->fresh;
-    const bool captured = under_capture(st);
-    const std::lock_guard<std::mutex> hold(f.lock);
-    const int n = f.n.load(std::memory_order_relaxed);
-    for (int i = 0; i < n; ++i)
-        if (f.streams[i] == st && f.captured[i] == captured) return;
-    if (n < FreshWeights::kMost) {
-        f.streams[n] = st;
-        f.captured[n] = captured;
-        f.n.store(n + 1, std::memory_order_release);
-    } else {
-        f.anywhere.store(true);
-    }
+    ctx->fresh.written(st == cudaStreamLegacy ? nullptr : st, under_capture(st));
 }
 // called once per product launch: may it start on its weights before the previous kernel of the stream is complete?
 inline int early_weights(Ctx *ctx, cudaStream_t st) {
-    FreshWeights &f = ctx->fresh;
-    if (f.n.load(std::memory_order_acquire) != 0) {
-        if (st == cudaStreamLegacy) st = nullptr;
-        const bool captured = under_capture(st);
-        const std::lock_guard<std::mutex> hold(f.lock);
-        const int n = f.n.load(std::memory_order_relaxed);
-        for (int i = 0; i < n; ++i)
-            if (f.streams[i] == st && f.captured[i] == captured) {
-                f.streams[i] = f.streams[n - 1];
-                f.captured[i] = f.captured[n - 1];
-                f.n.store(n - 1, std::memory_order_release);
-                return 0;
-            }
-    }
-    return ctx->pdl_early_weights && !f.anywhere.load(std::memory_order_relaxed) ? 1 : 0;
+    if (ctx->fresh.known() && !ctx->fresh.early(st == cudaStreamLegacy ? nullptr : st, under_capture(st))) return 0;
+    return ctx->pdl_early_weights;
 }
 
 inline int fail(Ctx *ctx, int code, const std::string &msg) {
