@@ -29,8 +29,10 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// The scale of a block with this largest magnitude.  amax / 448 correctly rounded: the quotient by the rounded reciprocal, its exact remainder, and a step (all 2^23
-// mantissas agree with the division, which costs 120 instructions).
+// The scale of a block with this largest magnitude: amax / 448 correctly rounded, by Markstein's theorem (P. W. Markstein, "Computation of elementary functions on the
+// IBM RISC System/6000 processor", IBM J. Res. Develop. 34(1), 1990): with y the reciprocal of b correctly rounded and q within a unit of a / b, the remainder r = a - q b is
+// exact in one fma, and q + r y is a / b correctly rounded.  Here b = 448 and y is a constant.  tests/test_fp8_division_gpu.py compares all 2^23 mantissas; a division
+// takes 120 instructions.  (Where r would be below the least number of f32, the quotient is far below 2^-90.)
 __device__ __forceinline__ float scale_of(float amax, int pow2) {
     constexpr float r = 1.0f / 448.0f;
     const float q = amax * r;
@@ -45,7 +47,7 @@ __device__ __forceinline__ float inverse_of(float s) {
     return r;
 }
 
-// x / s within a unit: one step from x * inv
+// x / s within a unit: the same step, from a reciprocal that is not rounded correctly (which is all that Markstein's theorem needs for that)
 __device__ __forceinline__ float quotient(float x, float s, float inv) {
     const float r = x * inv;
     return fmaf(fmaf(-r, s, x), inv, r);
