@@ -183,9 +183,9 @@ __device__ __forceinline__ void conclude(const Results &out, int rank, bool mine
 // Warps of a CTA that adds up rows: a lane holds so many rows' values and their sums, so few warps where that is many registers
 __host__ __device__ constexpr int row_warps(int ch, int v) { return ch * v <= 8 ? 32 : 16; }
 
-// Sums of each CTA: part_p f32[grid][E], part_c i32[grid][E], part_n i32[grid]; ONE: the grid is a cluster that goes on to the results
+// Sums of each CTA: part_p f64[grid][E], part_c i32[grid][E], part_n i32[grid]; ONE: the grid is a cluster that goes on to the results
 template <int DT, int V, int CH, bool ONE>
-__global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float *part_p, int *part_c,
+__global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(const void *logits, const uint32_t *topk_idx, const uint8_t *mask, double *part_p, int *part_c,
                                                                            int *part_n, Results out, int n_rows, int n_experts, int k, uint32_t *status) {
     pdl_enter();
     constexpr int W = row_warps(CH, V), T = 32 * W, R = CH * V <= 4 ? 4 : 2;
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(con
         if constexpr (ONE) {
             warp_p[place(e)] = s;
         } else {
-            part_p[static_cast<size_t>(blockIdx.x) * n_experts + e] = static_cast<float>(s);
+            part_p[static_cast<size_t>(blockIdx.x) * n_experts + e] = s;
             part_c[static_cast<size_t>(blockIdx.x) * n_experts + e] = hist[e];
         }
     }
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(32 * row_warps(CH, V)) balance_rows_kernel(con
 constexpr int kJoinThreads = 512;
 // A CTA has the experts of its eighth side by side (2^shift of its threads) and as many groups of parts as threads are left.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kJoinThreads)
-balance_join_kernel(const float *part_p, const int *part_c, const int *part_n, int parts, Results out, int n_experts, int k, int shift) {
+balance_join_kernel(const double *part_p, const int *part_c, const int *part_n, int parts, Results out, int n_experts, int k, int shift) {
     pdl_enter();
     __shared__ double sums[kJoinThreads], scratch[kJoinThreads / 32 + 1];
     __shared__ int cnts[kJoinThreads];
@@ -404,7 +404,7 @@ cudaError_t with_form(int dt, bool vec, int n_experts, A... args) {
 template <int DT, int V, int CH>
 struct RowsForm {
     template <bool ONE>
-    static cudaError_t go(Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn, const Results &out,
+    static cudaError_t go(Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, double *pp, int *pc, int *pn, const Results &out,
                           int n_rows, int n_experts, int k) {
         constexpr int W = row_warps(CH, V);
         const size_t smem = static_cast<size_t>(W) * 32 * CH * V * 8 + static_cast<size_t>(n_experts) * 4;
@@ -426,7 +426,7 @@ struct RowsForm {
         cfg.numAttrs = ONE ? 2 : 1;
         return cudaLaunchKernelEx(&cfg, balance_rows_kernel<DT, V, CH, ONE>, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k, ctx->d_status);
     }
-    static cudaError_t run(bool one, Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, float *pp, int *pc, int *pn,
+    static cudaError_t run(bool one, Ctx *ctx, cudaStream_t st, int ctas, const void *logits, const uint32_t *idx, const uint8_t *mask, double *pp, int *pc, int *pn,
                            const Results &out, int n_rows, int n_experts, int k) {
         return one ? go<true>(ctx, st, kCluster, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k)
                    : go<false>(ctx, st, ctas, logits, idx, mask, pp, pc, pn, out, n_rows, n_experts, k);
@@ -450,13 +450,13 @@ bool in_fours(int n_experts, int dt, const void *a, const void *b) {
 static bool in_one(int n_rows) { return n_rows <= 256; }
 
 size_t moe_balance_workspace(int sms, int n_rows, int n_experts) {
-    return in_one(n_rows) ? 0 : static_cast<size_t>(balance_ctas(sms, n_rows)) * (2 * static_cast<size_t>(n_experts) + 1) * 4;
+    return in_one(n_rows) ? 0 : static_cast<size_t>(balance_ctas(sms, n_rows)) * (12 * static_cast<size_t>(n_experts) + 4);
 }
 
 cudaError_t launch_moe_balance(Ctx *ctx, cudaStream_t st, const void *logits, const uint32_t *topk_idx, const uint8_t *mask, float coef, float *loss,
                                int *counts, float *mean_probs, int *n_counted, int n_rows, int n_experts, int k, int dt, void *workspace) {
     const int ctas = balance_ctas(ctx->sm_count, n_rows);
-    float *pp = static_cast<float *>(workspace);
+    double *pp = static_cast<double *>(workspace);
     int *pc = reinterpret_cast<int *>(pp + static_cast<size_t>(ctas) * n_experts), *pn = pc + static_cast<size_t>(ctas) * n_experts;
     const Results out{coef, loss, counts, mean_probs, n_counted};
     const bool one = in_one(n_rows);
