@@ -419,8 +419,9 @@ int mtc_fp8_quantize(mtc_ctx *ctx, void *stream, const void *x, const void *rows
                      int block_rows, int pow2, int dtype);
 /* out[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} x[m, k] * w[n, k], sums in f32, rounded once to out_dtype (f32, f16, bf16).
  * x_dtype MTC_E4M3: x holds codes, x_scales their scales.  x_dtype f32 / f16 / bf16: x T[M, K] is quantized in the call as mtc_fp8_quantize does with blocks
- * of one row and pow2 0 (x_scales NULL): same results.  K a multiple of 16 with 16-byte aligned x and w runs on tensor cores, everything else on CUDA cores.  w and w_scales
- * are constants, as for the other dense products (option "pdl_early_weights"; mtc_fp8_quantize in front is known to the context). */
+ * of one row and pow2 0 (x_scales NULL): same results.  The product of two scales is an f32 number too: it keeps its bits where it is not below 2^-126.  K a multiple of 16
+ * with 16-byte aligned x and w runs on tensor cores (TMA takes rows of whole 16-byte pieces only), everything else on CUDA cores, far slower.  w and w_scales are
+ * constants, as for the other dense products (option "pdl_early_weights"; mtc_fp8_quantize in front is known to the context). */
 enum { MTC_E4M3 = 3 };
 int mtc_fp8_mm(mtc_ctx *ctx, void *stream, const void *x, const void *x_scales, const void *w, const void *w_scales, void *out, int M, int N, int K, int x_dtype,
                int out_dtype, void *workspace, size_t workspace_bytes);

@@ -29,10 +29,11 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// The scale of a block with this largest magnitude: amax / 448 correctly rounded, by Markstein's theorem (P. W. Markstein, "Computation of elementary functions on the
-// IBM RISC System/6000 processor", IBM J. Res. Develop. 34(1), 1990): with y the reciprocal of b correctly rounded and q within a unit of a / b, the remainder r = a - q b is
-// exact in one fma, and q + r y is a / b correctly rounded.  Here b = 448 and y is a constant.  tests/test_fp8_division_gpu.py compares all 2^23 mantissas; a division
-// takes 120 instructions.  (Where r would be below the least number of f32, the quotient is far below 2^-90.)
+// The scale of a block with this largest magnitude: amax / 448 correctly rounded, by Markstein's theorem (P. W. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", IBM J. Res. Develop. 34(1), 1990): with y the reciprocal of b correctly
+// rounded and q within a unit of a / b, the remainder r = a - q b is exact in one fma, and q + r y is a / b correctly rounded.  Here b =
+// 448 and y is a constant.  tests/test_fp8_division_gpu.py compares all 2^23 mantissas; a division takes 120 instructions.  (Where r would
+// be below the least number of f32, the quotient is far below 2^-90.)
 __device__ __forceinline__ float scale_of(float amax, int pow2) {
     constexpr float r = 1.0f / 448.0f;
     const float q = amax * r;
@@ -47,14 +48,15 @@ __device__ __forceinline__ float inverse_of(float s) {
     return r;
 }
 
-// x / s within a unit: the same step, from a reciprocal that is not rounded correctly (which is all that Markstein's theorem needs for that)
+// x / s within a unit: the same step, from a reciprocal within a unit or two
 __device__ __forceinline__ float quotient(float x, float s, float inv) {
     const float r = x * inv;
     return fmaf(fmaf(-r, s, x), inv, r);
 }
-// ... such that rounding it to a code gives the code nearest to the true quotient.  A quotient rounded to f32 may land on the border between two codes that the true one lies
-// beside (with s = amax / 448 rounded that is one value in a few hundred, since x and amax have few bits), so it is rounded to odd: its exact remainder tells the
-// side, and an even result is moved there.  Borders are even numbers, so none is hit unless the quotient is exact.  Below 2^-11 every quotient becomes zero anyway.
+// ... such that rounding it to a code gives the code nearest to the true quotient.  A quotient rounded to f32 may land on the border
+// between two codes that the true one lies beside (with s = amax / 448 rounded that is one value in a few hundred, since x and amax have
+// few bits), so it is rounded to odd: its exact remainder tells the side, and an even result is moved there.  Borders are even numbers, so
+// none is hit unless the quotient is exact.  Below 2^-11 every quotient becomes zero anyway.
 __device__ __forceinline__ float odd_quotient(float x, float s, float r) {       // r: quotient()
     const float rest = fmaf(-r, s, x);
     const uint32_t b = __float_as_uint(r), away = (__float_as_uint(rest) ^ b) >> 31;       // 1: the true one is smaller in magnitude

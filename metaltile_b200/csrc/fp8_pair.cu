@@ -2,29 +2,34 @@
 //
 //   out[t, n] = sum_b xs[t, b] * ws[n / 128, b] * D_b[t, n],      D_b[t, n] = sum_{k in block b} x[t, k] * w[n, k]
 //
-// A pair of CTAs (a cluster of two SMs) owns a tile of 256 tokens x 256 weight rows: each SM holds 128 tokens of A and half of the weight rows of B, and the MMAs
-// (cta_group::2, 256 x 256, kind::f8f6f4) read both.  A block of 128 codes is a chain of four of them into an accumulator of its own in tensor memory.  The epilogue takes
-// it out, multiplies by xs * ws, one number a thread (lane = token, and a warp's 128 columns share their ws), and adds up in registers: 128 sums a thread, eight warps.
+// A pair of CTAs (a cluster of two SMs) owns a tile of 256 tokens x 256 weight rows: each SM holds 128 tokens of A and half of the weight
+// rows of B, and the MMAs (cta_group::2, 256 x 256, kind::f8f6f4) read both.  A block of 128 codes is a chain of four of them into an
+// accumulator of its own in tensor memory.  The epilogue takes it out, multiplies by xs * ws, one number a thread (lane = token, and a
+// warp's 128 columns share their ws), and adds up in registers: 128 sums a thread, eight warps.
 //
-// What bounds it.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM of a pair: 64 bytes a
-// cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Without the epilogue the ring and the MMAs run at 585 cycles a block.  With it a
-// block takes 780 to 840, the MMA warp waiting for an accumulator: two are all of the tensor memory, so a block's MMAs (512), the way to the epilogue, its four loads of tensor
-// memory in a row, the way back and the issue of the next are one chain for two blocks.  But no single link is the bound (1184 x 4096 x 28672, 838 cycles a block): handed back
-// before it is read 822, one load of four 800, no additions 755, all three together 746.  Waits that spin instead of sleeping slow the others' shared memory (2 to 8 % more).
-// A tile ends with 2300 cycles of stores (f32 4000) and 300 to 900 to find the next; MMAs of two blocks run beside that.  2048 x 28672 x 4096: 214 us, 2.25 PFLOP/s.
+// What bounds it.  128 x 256 x 128 products take an SM 512 cycles at the dense rate, and a tile of 256 x 256 needs 32 KB a block on each SM
+// of a pair: 64 bytes a cycle, as many as an SM gets from L2; one CTA by itself with 128 x 256 would need 96.  Without the epilogue the
+// ring and the MMAs run at 585 cycles a block.  With it a block takes 780 to 840, the MMA warp waiting for an accumulator: two are all of
+// the tensor memory, so a block's MMAs (512), the way to the epilogue, its four loads of tensor memory in a row, the way back and the issue
+// of the next are one chain for two blocks.  But no single link is the bound (1184 x 4096 x 28672, 838 cycles a block): handed back before
+// it is read 822, one load of four 800, no additions 755, all three together 746; what takes the rest down to 585 is not known.  Waits that
+// spin instead of sleeping slow the others' shared memory (2 to 8 % more).  A tile ends with 2300 cycles of stores (f32 4000) and 300 to
+// 900 to find the next; MMAs of two blocks run beside that.  2048 x 28672 x 4096: 212 us, 2.27 PFLOP/s, in a graph of some ten calls at full
+// clock; back to back for seconds, at the 1.49 GHz of the power limit, 248 us, 1.94 PFLOP/s.
 //
-// Steps on the way (us for that case): hand-offs that release at cluster scope 587, relaxed ones 348; one try in front of the polling loop, whose entry costs 200 cycles,
-// and results out by TMA instead of a row a lane 303; the registers of the other roles for the epilogue, so that nothing spills, and the next columns loaded while the
-// last are added 235; MMAs of 256 columns instead of two chains of 128, which read A twice, 226; 32-bit
-// addresses and one plain loop over the blocks in the epilogue 214.  16 epilogue warps of 64 columns: 264 (96 registers each spill).
+// Steps on the way (us for that case at full clock): hand-offs that release at cluster scope 587, relaxed ones 348; one try in front of the
+// polling loop, whose entry costs 200 cycles, and results out by TMA instead of a row a lane 303; the registers of the other roles for the
+// epilogue, so that nothing spills, and the next columns loaded while the last are added 235; MMAs of 256 columns instead of two chains of
+// 128, which read A twice, 226; 32-bit addresses and one plain loop over the blocks in the epilogue 214.  16 epilogue warps of 64 columns:
+// 264 (96 registers each spill).
 //
 //   warps 0-7    epilogue   warps 0-3 the first half of the weight rows, 4-7 the second
 //   warps 8-9    scales     xs of 128 tokens, 16 blocks at a time, and ws, by cp.async into shared memory (a load of each lane's own row would cost the load pipe ten
 //                           cycles a lane)
 //   warp 10      producer   TMA, both CTAs of a pair into their own memory, one barrier in the first
 //   warp 11      MMA        issued by the first CTA
-// A persistent pair walks the tiles, tokens fastest.  Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave and what is in
-// flight is awaited (bounded too).
+// A persistent pair walks the tiles, tokens fastest.  Every wait is bounded: on expiry the kernel records a code in the status word, the
+// roles leave and what is in flight is awaited (bounded too).
 #include <cstddef>
 
 #include "fp8_tc.cuh"
@@ -93,8 +98,8 @@ __device__ __forceinline__ void commit_pair(uint64_t *bar, uint32_t both) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"(static_cast<uint16_t>(both)) : "memory");
 }
-// Relaxed: what it hands over is tensor memory, ordered by the tcgen05 fence in front.  (A release at cluster scope waits for everything the thread has in flight: 1150
-// cycles a block, 2048 x 28672 x 4096 in 587 us instead of 348.)
+// Relaxed: what it hands over is tensor memory, ordered by the tcgen05 fence in front.  (A release at cluster scope waits for everything
+// the thread has in flight: 1150 cycles a block, 2048 x 28672 x 4096 in 587 us instead of 348.)
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -132,7 +137,8 @@ __device__ void count_chunks(PCtrl *ctl, const PArgs &a) {
     }
 }
 
-// Waits of the epilogue by addresses: its registers are sums and values on their way, and a 64-bit pointer more makes them spill.  Not inlined: the way that rarely runs.
+// Waits of the epilogue by addresses: its registers are sums and values on their way, and a 64-bit pointer more makes them spill.  Not
+// inlined: the way that rarely runs.
 __device__ __noinline__ void wait_long(uint32_t bar, uint32_t parity, uint32_t abort, uint32_t *status, uint32_t code) {
     const uint32_t r = mbar_poll(bar, parity, abort);
     if (r != 1) mbar_gave_up(r, abort, status, code);
@@ -193,9 +199,10 @@ __device__ __forceinline__ uint4 piece(const uint64_t (&acc)[N], int i) {
     }
 }
 
-// A warp's rows (32 at most) x NC columns, through shared memory, 128 bytes a row at a time: all 32 rows out by TMA, which goes on while the next tile's blocks are
-// added; fewer, or rows that 16-byte pieces do not fit, by stores that run along the rows.  (A lane storing its own row costs the load pipe a cycle a row and store:
-// 67 us of 330 for 2048 x 28672 x 4096 in 16-byte pieces, and 30 us for one tile of odd rows, element by element.)
+// A warp's rows (32 at most) x NC columns, through shared memory, 128 bytes a row at a time: all 32 rows out by TMA, which goes on while
+// the next tile's blocks are added; fewer, or rows that 16-byte pieces do not fit, by stores that run along the rows.  (A lane storing its
+// own row costs the load pipe a cycle a row and store: 67 us of 330 for 2048 x 28672 x 4096 in 16-byte pieces, and 30 us for one tile of
+// odd rows, element by element.)
 template <int DT, int NC>
 __device__ __forceinline__ void store_rows_as(const PMaps &maps, const PArgs &a, const uint64_t (&acc)[NC / 2], uint32_t staged, int row, int rows, int n) {
     constexpr int PER = DT == MTC_F32 ? 4 : 8;                       // results of a 16-byte piece
@@ -262,8 +269,8 @@ __device__ __forceinline__ void store_rows(const PMaps &maps, const PArgs &a, co
     else store_rows_as<MTC_F32, NC>(maps, a, acc, staged, row, rows, n);
 }
 
-// The sums of all S slices of this CTA's tokens, and out: a warp its 32 tokens x 128 / S columns, 32 at a time.  Sums lie as [column][token] where the ring was, in the
-// CTAs of the same rank of each pair; they are added in the order of K.
+// The sums of all S slices of this CTA's tokens, and out: a warp its 32 tokens x 128 / S columns, 32 at a time.  Sums lie as
+// [column][token] where the ring was, in the CTAs of the same rank of each pair; they are added in the order of K.
 template <int S>
 __device__ __forceinline__ void join_slices(const PMaps &maps, const PArgs &a, uint32_t sums, uint32_t staged, int slice, int rank, int first, int rows, const Tile &t) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -292,7 +299,8 @@ __device__ __forceinline__ void join_slices(const PMaps &maps, const PArgs &a, u
     }
 }
 
-// Registers: 384 threads start with 168, 256 of them go on with more and 128 with fewer.  What leaves the epilogue's loop without spills, or with the fewest.
+// Registers: 384 threads start with 168, 256 of them go on with more and 128 with fewer.  What leaves the epilogue's loop without spills,
+// or with the fewest.
 template <int SLICES>
 constexpr int kEpiRegs = SLICES == 4 ? 216 : 224;
 template <int SLICES>
@@ -365,7 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_pair_kernel(const __grid_cons
                     if (++s == kStages) s = 0, phase ^= 1;
                 }
             }
-            // The MMAs' arrivals at `empty` come through the cluster on their own: the last ones are awaited too, so that none reaches a CTA that has left
+            // The MMAs' arrivals at `empty` come through the cluster on their own: the last ones are awaited too, so that none reaches a
+            // CTA that has left
             for (int i = 0; go && i < kStages; ++i) {
                 go = wait_soon(&ctl->empty[s], phase, &ctl->abort, a.status, 0xb11u);
                 if (++s == kStages) s = 0, phase ^= 1;
@@ -545,7 +554,8 @@ cudaError_t launch(cudaStream_t st, const PMaps &maps, const PArgs &a, long long
     const cudaError_t e = config<S>(cfg, la, st, clusters);
     return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, fp8_pair_kernel<S>, maps, a);
 }
-// Clusters that the device runs at once: asked for once a device (clusters have to fit into groups of SMs of different sizes).  0 where it cannot be told.
+// Clusters that the device runs at once: asked for once a device (clusters have to fit into groups of SMs of different sizes).  0 where it
+// cannot be told.
 template <int S>
 int clusters_at_once() {
     static std::atomic<int> known[64];
@@ -596,8 +606,9 @@ cudaError_t launch_fp8_pair(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     const long long chunks = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) + M / kTokens : (M + kTokens - 1) / kTokens, tiles = chunks * a.col_tiles;
     if (tiles > kMostSize) return cudaErrorInvalidConfiguration;
     a.chunks = static_cast<int>(chunks);
-    // K slices where tiles would leave SMs without work, all clusters at once (15 of four pairs, 33 of two).  Joining them takes 3 us: 256 x 4096 x 4096 18.3 us, in two slices
-    // 16.2; x 14336 50.1 and 34.3; 256 x 1024 x 4096 17.7, in four 13.0; but x 2048 11.6 to 11.8 and 12.1 to 12.4.
+    // K slices where tiles would leave SMs without work, all clusters at once (15 of four pairs, 33 of two).  Joining them takes 3 us: 256
+    // x 4096 x 4096 18.3 us, in two slices 16.2; x 14336 50.1 and 34.3; 256 x 1024 x 4096 17.7, in four 13.0; but x 2048 11.6 to 11.8 and
+    // 12.1 to 12.4.
     if (!expert_offsets && a.nkb >= 24 && tiles <= clusters_at_once<4>()) return launch<4>(st, maps, a, tiles);
     if (!expert_offsets && a.nkb >= 24 && tiles <= clusters_at_once<2>()) return launch<2>(st, maps, a, tiles);
     return launch<1>(st, maps, a, std::min<long long>(ctx->sm_count / 2, tiles));

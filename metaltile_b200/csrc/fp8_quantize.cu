@@ -4,11 +4,12 @@
 //   s = max(max |x| / 448, 2^-90) over the finite values of the block (pow2: the least power of two that is not below)
 //   code = x / s rounded to the nearest e4m3 value, ties to even; infinities and NaN become NaN
 //
-// Bound by memory: every value is read once and stays in registers, as it was read, between the maximum and the codes; sixteen lanes share a row of a
-// block, eight values a lane.  What matters beside the loads in flight is the number of instructions a value: the maximum is that of the bit patterns (two 16-bit values at
-// a time, monotone for all but NaN), and a quotient is one multiplication for 16-bit types (factor_of); f32 takes three and three that look whether it may be on a border.
-// Measured (graph, us): 14336 x 4096 in blocks of 128 x 128 bf16 and f16 32.3 (176 MB, 5.45 TB/s; as f32 is quantized 46.9), with powers of two 28.1, f32 51.3 (294 MB);
-// 8192 x 4096 rows bf16 23.3 (31.7), f32 29.5.
+// Bound by memory: every value is read once and stays in registers, as it was read, between the maximum and the codes; sixteen lanes share
+// a row of a block, eight values a lane.  What matters beside the loads in flight is the number of instructions a value: the maximum is
+// that of the bit patterns (two 16-bit values at a time, monotone for all but NaN), and a quotient is one multiplication for 16-bit types
+// (factor_of); f32 takes three and three that look whether it may be on a border.  Measured (graph, us): 14336 x 4096 in blocks of 128 x 128
+// bf16 and f16 32.3 (176 MB, 5.45 TB/s; as f32 is quantized 46.9), with powers of two 28.1, f32 51.3 (294 MB); 8192 x 4096 rows bf16 23.3
+// (31.7), f32 29.5.
 #include <algorithm>
 
 #include "fp8.cuh"
@@ -95,11 +96,12 @@ __device__ __forceinline__ float magnitude(uint32_t m) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
 }
 
-// What a block's values are multiplied with, so that a code is one multiplication and the conversion.
-// 16-bit types: with x = X 2^a and amax = A 2^b (X, A below 2^11) a border between codes is B 2^c, B < 32, and 448 x / amax is either such a border or differs from it by at
-// least 1 / (A B) > 2^-16 of it: 7 X and A B, times powers of two, are whole numbers.  So an error of 2^-20 changes no code but that of a value on a border, and these all lie
-// on the same side, that on which s lies of amax / 448: `factor` is moved there by 2^-21, which is more than its own and the product's rounding.  Where s is amax / 448
-// exactly, or 2^-90, they are ties: `tie` has the product rounded to 18 bits, which leaves nothing but the border itself there.
+// What a block's values are multiplied with, so that a code is one multiplication and the conversion.  16-bit types: with x = X 2^a and amax
+// = A 2^b (X, A below 2^11) a border between codes is B 2^c, B < 32, and 448 x / amax is either such a border or differs from it by at
+// least 1 / (A B) > 2^-16 of it: 7 X and A B, times powers of two, are whole numbers.  So an error of 2^-20 changes no code but that of a
+// value on a border, and these all lie on the same side, that on which s lies of amax / 448: `factor` is moved there by 2^-21, which is
+// more than its own and the product's rounding.  Where s is amax / 448 exactly, or 2^-90, they are ties: `tie` has the product rounded to
+// 18 bits, which leaves nothing but the border itself there.
 template <int DT, bool POW2>
 __device__ __forceinline__ float factor_of(float s, float amax, bool &tie) {
     const float inv = inverse_of(s);
@@ -124,8 +126,8 @@ __device__ __forceinline__ uint2 codes_of(const Eight<DT> &v, float s, float fac
                 for (int i = 0; i < 8; ++i) q[i] = __uint_as_float((__float_as_uint(q[i]) + 32u) & ~63u);
             }
         } else {
-            // Borders between codes are the numbers of exactly five bits, and below the least normal code the odd multiples of 2^-10: only there can it matter on
-            // which side of its f32 the quotient is (code_quotient).
+            // Borders between codes are the numbers of exactly five bits, and below the least normal code the odd multiples of 2^-10: only
+            // there can it matter on which side of its f32 the quotient is (code_quotient).
             float least = INFINITY;
             int border = 0;
 #pragma unroll

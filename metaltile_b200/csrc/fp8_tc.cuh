@@ -7,14 +7,14 @@
 namespace mtc {
 namespace fp8 {
 
-// A wait that mostly finds its phase complete: one try, and only then the polling loop, whose entry alone costs a warp some 200 cycles (one block of 256 x 256 x 128
-// products took 1140 cycles with the loop at every hand-off, 610 so).
+// A wait that mostly finds its phase complete: one try, and only then the polling loop, whose entry alone costs a warp some 200 cycles (one
+// block of 256 x 256 x 128 products took 1140 cycles with the loop at every hand-off, 610 so).
 __device__ __forceinline__ bool wait_soon(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t code) {
     return mbar_try(bar, parity) || mbar_wait(bar, parity, abort, status, code);
 }
 
-// The same by a whole warp whose loop has to stay uniform (the operands of an MMA then come straight from uniform registers: with one thread in the loop four MMAs
-// and their commits took 250 cycles to issue).
+// The same by a whole warp whose loop has to stay uniform (the operands of an MMA then come straight from uniform registers: with one
+// thread in the loop four MMAs and their commits took 250 cycles to issue).
 __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatile uint32_t *abort, uint32_t *status, uint32_t code) {
     return __all_sync(0xffffffffu, mbar_try(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, code));
 }

@@ -2,20 +2,23 @@
 //
 //   out[t, n] = sum_b xs[t, b] * ws[n / 128, b] * D_b[n, t],      D_b[n, t] = sum_{k in block b} w[n, k] * x[t, k]
 //
-// An item is 128 weight rows x up to TN tokens x a slice of K.  Its weight rows share ws, so a block of 128 codes is one MMA chain (four steps of K = 32,
-// kind::f8f6f4) into an accumulator of its own in tensor memory, which the epilogue takes out, multiplies by xs * ws and adds up in registers: lane = weight
-// row, register = token.  The products and block sums are the tensor core's (codes have 4 bits, their products are exact), the sums over blocks f32.
+// An item is 128 weight rows x up to TN tokens x a slice of K.  Its weight rows share ws, so a block of 128 codes is one MMA chain (four
+// steps of K = 32, kind::f8f6f4) into an accumulator of its own in tensor memory, which the epilogue takes out, multiplies by xs * ws and
+// adds up in registers: lane = weight row, register = token.  The products and block sums are the tensor core's (codes have 4 bits, their
+// products are exact), the sums over blocks f32.
 //
-// Bound by reading the weights once: a block of an item is 16 KB of them, 700 cycles of an SM's share of the memory's rate, against 128 cycles of MMAs.  Two CTAs an SM with
-// some 100 KB of stages each walk the items, the copies running ahead from one to the next; with few items and no experts K is cut into up to 8
-// slices, the CTAs of a cluster, which add up through shared memory in the order of K.  What an item takes beside its bytes is the way through the hand-offs: a wait, a load of
-// tensor memory and the sums were 470 cycles a block, whatever its columns, so two or four blocks make one hand-off.
-// Measured (graph, us): 1 x 4096 x 4096 7.3, 1 x 14336 x 4096 14 (58.7 MB; each further matrix of that size 9.4, the memory's rate).
+// Bound by reading the weights once: a block of an item is 16 KB of them, 700 cycles of an SM's share of the memory's rate, against 128
+// cycles of MMAs.  Two CTAs an SM with some 100 KB of stages each walk the items, the copies running ahead from one to the next; with few
+// items and no experts K is cut into up to 8 slices, the CTAs of a cluster, which add up through shared memory in the order of K.  What an
+// item takes beside its bytes is the way through the hand-offs: a wait, a load of tensor memory and the sums were 470 cycles a block,
+// whatever its columns, so two or four blocks make one hand-off.  Measured (graph, us): 1 x 4096 x 4096 7.3, 1 x 14336 x 4096 14 (58.7 MB;
+// each further matrix of that size 9.4, the memory's rate).
 //
 //   warps 0-3  epilogue   accumulators out, scaled, added up, stored
 //   warp 4     producer   TMA: 128 x 128 codes of the weights, TN x 128 of the tokens, a stage; by cp.async the scales of 16 blocks
 //   warp 5     MMA        and the tensor memory's allocation
-// Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited (bounded too).
+// Every wait is bounded: on expiry the kernel records a code in the status word, the roles leave, copies and MMAs in flight are awaited
+// (bounded too).
 #include <cstddef>
 
 #include "fp8_tc.cuh"
@@ -32,8 +35,9 @@ constexpr int kEpi = 128, kLoadWarp = 4, kMmaWarp = 5, kThreads = 192, kPerSM = 
 constexpr int kSmemBytes = 113 * 1024;           // of one of the two CTAs of an SM
 constexpr int kMaxSlices = 8;
 
-// SLICED: slices of K meet in shared memory.  A token's sums go to the CTA of rank token % slices, one place a slice, by stores that nobody waits for before the barrier of
-// the cluster: (a + i * slices) has i-th place.  Tiles of 64 tokens have no room beside the ring and are fetched from where it was, after the barrier.
+// SLICED: slices of K meet in shared memory.  A token's sums go to the CTA of rank token % slices, one place a slice, by stores that nobody
+// waits for before the barrier of the cluster: (a + i * slices) has i-th place.  Tiles of 64 tokens have no room beside the ring and are
+// fetched from where it was, after the barrier.
 template <int TN, bool SLICED>
 struct Form {
     static constexpr int kTogether = TN == 64 ? 2 : 4;               // blocks of a hand-off to the epilogue
@@ -97,9 +101,10 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, float v
 }
 __device__ __forceinline__ void st_shared(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
-// Chunks of TN rows: expert e with r rows has ceil(r / TN).  By one warp, four experts a lane: how many there are in all (want < 0), or the one with index `want`.  Offsets that
-// run backwards or past the rows are clamped, and reported by the block that is told to.  (A load and a scan for 128 experts; with one for 32 128 experts of 768 x 2048 and 32
-// rows in all 14.7 us for 13.1, 4096 rows 46.0 for 43.4, 512 experts of 512 x 1024 and 512 rows 43.4 for 34.9.)
+// Chunks of TN rows: expert e with r rows has ceil(r / TN).  By one warp, four experts a lane: how many there are in all (want < 0), or the
+// one with index `want`.  Offsets that run backwards or past the rows are clamped, and reported by the block that is told to.  (A load and
+// a scan for 128 experts; with one for 32 128 experts of 768 x 2048 and 32 rows in all 14.7 us for 13.1, 4096 rows 46.0 for 43.4, 512
+// experts of 512 x 1024 and 512 rows 43.4 for 34.9.)
 struct Chunk {
     int expert, tok0, ntok;
 };
@@ -302,7 +307,8 @@ __global__ void __launch_bounds__(kThreads, kPerSM) fp8_tile_kernel(const __grid
         int s = 0, d = 0;
         uint32_t phase = 0, d_phase = 1;
         bool go = true;
-        // No stage is full before the previous kernels of the stream are complete (x is theirs): what they take does not count against the limit of the waits
+        // No stage is full before the previous kernels of the stream are complete (x is theirs): what they take does not count against the
+        // limit of the waits
         if (!a.expert_offsets) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int unit = first; go && unit < units; unit += step)
             for (int kb = kb0; go && kb < kb1; kb += F::kTogether) {
@@ -511,8 +517,9 @@ cudaError_t launch_fp8_tile(Ctx *ctx, cudaStream_t st, const uint8_t *x, const f
     a.n_experts = n_experts;
     a.tiles = blocks(N);
     a.out_dt = out_dt;
-    // Tokens of a tile.  Dense: what holds them, but 64 as two of 32, whose epilogues share the work (64 x 4096 x 4096 10.0 us, in one of 64 11.1).  Grouped: 16 below eight rows
-    // an expert on average (128 experts of 768 x 2048: 4 rows 26.0 us, with 32 29.6; 8 rows 32.9 and 31.6; 32 rows 47.0, with 64 50.4).  128 were slower than both this and pairs.
+    // Tokens of a tile.  Dense: what holds them, but 64 as two of 32, whose epilogues share the work (64 x 4096 x 4096 10.0 us, in one of
+    // 64 11.1).  Grouped: 16 below eight rows an expert on average (128 experts of 768 x 2048: 4 rows 26.0 us, with 32 29.6; 8 rows 32.9
+    // and 31.6; 32 rows 47.0, with 64 50.4).  128 were slower than both this and pairs.
     const int rows = expert_offsets ? (M >= 8 * n_experts ? 32 : 16) : M;
     const int TN = rows <= 16 ? 16 : rows <= 64 ? 32 : 64;
     const long long chunks = expert_offsets ? static_cast<long long>(std::min(M, n_experts)) + M / TN : (M + TN - 1) / TN;

@@ -6,8 +6,9 @@
 
 namespace mtc {
 
-// What runs and what a graph under capture records are apart, each with a list of its own: a captured product does not run, so the wait of one that does is not its to use
-// up, and captures that end without a product fill up their own list only.  Locked: two threads may quantize and multiply on streams of their own.
+// What runs and what a graph under capture records are apart, each with a list of its own: a captured product does not run, so the wait of
+// one that does is not its to use up, and captures that end without a product fill up their own list only.  Locked: two threads may
+// quantize and multiply on streams of their own.
 class FreshWeights {
 public:
     static constexpr int kMost = 64;

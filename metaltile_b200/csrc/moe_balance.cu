@@ -6,10 +6,11 @@
 //   loss = coef * E * sum_e f_e P_e;  n = 0: f, P and loss are 0
 //   d loss / d logit_te = coef * E / n * p_te * (f_e - sum_j f_j p_tj)       (counts are constants)
 //
-// Bound by reading the logits where there are many rows, by launches and latencies where there are few.  A warp has two or four rows in registers at a time, every lane adds up
-// its own experts over the rows of the warp; rows are dealt out to the warps of the grid in turn, so that masked ones, which lie together, are spread.  Sums over rows are
-// f32 for 32 rows of a warp at most and f64 from there on, always in the same order; counts are integers, whose order does not matter.  Few rows are one launch, a
-// cluster of eight CTAs that meet over distributed shared memory; many are a launch of a CTA an SM and one of such a cluster that adds up their parts.
+// Bound by reading the logits where there are many rows, by launches and latencies where there are few.  A warp has two or four rows in
+// registers at a time, every lane adds up its own experts over the rows of the warp; rows are dealt out to the warps of the grid in turn,
+// so that masked ones, which lie together, are spread.  Sums over rows are f32 for 32 rows of a warp at most and f64 from there on, always
+// in the same order; counts are integers, whose order does not matter.  Few rows are one launch, a cluster of eight CTAs that meet over
+// distributed shared memory; many are a launch of a CTA an SM and one of such a cluster that adds up their parts.
 #include <algorithm>
 #include <type_traits>
 
@@ -97,7 +98,9 @@ __device__ __forceinline__ void softmax_rows(float (&z)[R][CH][V]) {
             for (int i = 0; i < V; ++i) m = fmaxf(m, z[u][c][i]);
         asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(most[u]) : "f"(m));
     }
-    // exp(z - most) as a power of two; below 2^-126 it is zero
+    // exp(z - most) as a power of two; below 2^-126 it is zero.  The product is rounded, so that a probability errs by 1.5 |z - most| 2^-24
+    // of itself and the two units of ex2: more the smaller it is, of the size of what the rounding of f32 logits' difference costs, and next
+    // to nothing for those that make up the sums.
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         if (most[u] == -INFINITY) most[u] = 0.0f;
@@ -151,7 +154,8 @@ struct Results {
     float *mean_probs;
     int *n_counted;
 };
-// What comes of the sums of an expert (thread e - e0 of a CTA of the cluster has that of expert e, `mine`: it has one), and of all: the loss.  scratch: a double a warp and one more.
+// What comes of the sums of an expert (thread e - e0 of a CTA of the cluster has that of expert e, `mine`: it has one), and of all: the
+// loss.  scratch: a double a warp and one more.
 __device__ __forceinline__ void conclude(const Results &out, int rank, bool mine, int e, double p, int c, int n, int n_experts, int k, double *scratch) {
     double term = 0.0;
     if (mine) {

@@ -1503,9 +1503,13 @@ static Fp8Kernel fp8_kernel_for(const Ctx *ctx, int M, int N, int K, int n_exper
     if (forced == 1 || !mtc::fp8_tile_supported(M, N, K, n_experts, x, w)) return FP8_CUDA_CORE;
     const bool pair = mtc::fp8_pair_supported(M, N, K, n_experts, x, w);
     if (forced) return forced == 3 && pair ? FP8_PAIR : FP8_TILE;
-    // Pairs of CTAs have tiles of 256 tokens.  Grouped (us of tiles and pairs): 128 experts of 768 x 2048, 48 rows an expert 53 and 62, 56 54 and 63, 64 60 and 64;
-    // of 2048 x 768, 48 rows 62 and 68, 64 77 and 68; 8 of 4096 x 1536, 48 rows 19.2 and 19.7, 64 22.6 and 19.9.  Dense: from more than 64
-    // tokens on, unless that is so few tiles of 64 x 128 that cutting K into four slices and more fills the GPU (256 x 1024 x 4096 10.8 and 13.0, 256 x 4096 x 4096 20 and 16,
+    // Pairs of CTAs have tiles of 256 tokens, the tile kernel grouped ones of 32.  Grouped (us of tiles and pairs, bf16 results), two routers with biases of N(0, 1) each:
+    // 128 experts of 768 x 2048, 48 rows an expert 51-56 and 53-57, 56 52-55 and 55, 64 62-65 and 56-65; of 2048 x 768, 48 rows 69-70 and 68-70, 56 74 and 66-71,
+    // 64 80-83 and 69-70; 8 of 4096 x 1536, 56 rows 18.3 and 19.4, 64 22.5 and 19.4.  What the line costs: rows dealt out evenly fill tiles of 32, which are then ahead
+    // up to 64 rows (768 x 2048, 56 rows 55 and 62, 64 59 and 65; 2048 x 768 70 and 74, 72 and 71), so are 32 experts of 1408 x 2048 (64 rows 30 and 33) and f32 results
+    // of 8 x 4096 x 1536 (56 rows 18 and 22, 64 22.4 and 22.4).  And the offsets are on the device, the host knows the average only: where a tenth of 128 experts of 768 x 2048
+    // has all rows, 16, 32 and 48 rows on average are 23, 31 and 40 us in tiles, 17 in pairs.
+    // Dense: from more than 64 tokens on, unless that is so few tiles of 64 x 128 that cutting K into four slices and more fills the GPU (256 x 1024 x 4096 10.8 and 13.0, 256 x 4096 x 4096 20 and 16,
     // 128 x 4096 x 14336 26 and 34, 64 x 14336 x 4096 19 and 20, 128 x 14336 x 4096 26 and 21).
     if (grouped) return pair && M / n_experts >= 56 ? FP8_PAIR : FP8_TILE;
     return pair && M > 64 && static_cast<long long>((M + 63) / 64) * mtc::fp8::blocks(N) > 64 ? FP8_PAIR : FP8_TILE;

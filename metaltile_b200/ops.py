@@ -204,7 +204,7 @@ def fp8_mm(x, w, w_scales, x_scales=None, out_dtype=None, out=None, ctx: Context
 def fp8_gather_mm(x, w, w_scales, expert_offsets, x_scales, out_dtype=None, out=None, ctx: Context = None):
     """The grouped form: ``x [rows, K]`` codes sorted by expert (``fp8_quantize(tokens, rows=sort_token_idx)``), w ``[E, N, K]``, w_scales
     ``[E, ceil(N/128), ceil(K/128)]``, ``expert_offsets`` int32 ``[E + 1]`` from ``moe_sort``; out ``[rows, N]``, bf16 by default.  Rows that
-    no expert owns keep what ``out`` holds there."""
+    no expert owns keep what ``out`` holds there (anything, where the call makes ``out``)."""
     return _native.fp8_gather_mm(x, w, w_scales, expert_offsets, x_scales, _out_dtype(out_dtype), out, ctx)
 
 
