@@ -74,7 +74,7 @@ int mtc_sync_deadline(mtc_ctx *ctx, void *stream, int timeout_ms);
  * word was cleared; otherwise the code of the first report: 0x101-0x403, 0x501, 0x502 waits of the tensor-core kernel's roles (0x501 also
  * an expert id out of range in mtc_moe_sort), 0x601 + r rank r never arrived at a peer barrier, 0x701 / 0x702 phase counter /
  * partial-sum slot of a chained launch, 0x801-0x831 the tensor-memory decode kernel, 0x901 expert_offsets that run backwards or past the rows,
- * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 / 0x906 a row index that does not exist, 0x907 an expert that does not exist, 0xa01-0xa0b waits of the exact
+ * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 / 0x906 a row index that does not exist, 0x907 an expert that does not exist, 0x908 a row of an adapter that does not exist, 0xa01-0xa0b waits of the exact
  * grouped kernel's roles, 0xb01-0xb06 and 0xb11-0xb16 of the roles of the two tensor-core kernels of e4m3 codes. */
 int mtc_status_word(mtc_ctx *ctx, uint32_t *word);
 int mtc_status_clear(mtc_ctx *ctx);
@@ -447,6 +447,43 @@ int mtc_moe_balance(mtc_ctx *ctx, void *stream, const void *logits, const void *
 size_t mtc_moe_balance_workspace(const mtc_ctx *ctx, int n_rows, int n_experts);
 int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const void *mask, const void *counts, const void *n_counted, const void *grad_loss, float coef,
                          void *grad, int n_rows, int n_experts, int k, int dtype);
+
+/* ---- in front of a projection: residual addition and root-mean-square norm (no counterpart in the reference beside ffai_rms_norm_qgemv, which norms one
+ * row inside its projection: mtc_rms_norm_qmv) ----
+ *     s = T(x + residual),   inv = 1 / sqrt(mean(s^2) + eps),   y = T(s * inv * norm_weight)          (f32 in between; rows of K values)
+ * x, residual, sum, y T[n_rows, K], norm_weight T[K].  residual NULL: s is x, `sum` is not looked at.  The norm is of what `sum` holds.  sum and y may be x or residual
+ * (but not both the same), so that a residual stream is updated in place.
+ * mtc_add_rms_norm_fp8 gives y as e4m3 codes u8[n_rows, K] with scales f32[n_rows, B(K)], made of the f32 results as mtc_fp8_quantize makes them of f32 rows (pow2 as there), which
+ * mtc_fp8_mm reads; y (NULL: not wanted) gets them in T as well. */
+int mtc_add_rms_norm(mtc_ctx *ctx, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, int n_rows, int K, int dtype);
+int mtc_add_rms_norm_fp8(mtc_ctx *ctx, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, void *codes,
+                         void *scales, int n_rows, int K, int pow2, int dtype);
+/* The gradients, from that of y (dy) and what the forward call left in `sum`; dsum (NULL: 0) is the gradient that comes down the residual stream:
+ *     n = s * inv,   dx = inv * (norm_weight * dy - n * mean(norm_weight * dy * n)) + dsum,   dweight = sum over rows of dy * n
+ * dx is the gradient of x and of residual alike; it may be dy or dsum.  dx T[n_rows, K], dweight T[K].  Sums over rows run in a fixed order. */
+int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *sum, const void *norm_weight, float eps, const void *dsum, void *dx, void *dweight,
+                          int n_rows, int K, int dtype, void *workspace, size_t workspace_bytes);
+size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K);
+
+/* ---- beside a projection: low-rank adapters of many requests (no counterpart in the reference) ----
+ * For the rows t of adapter e:   h_t = x_t a[e]^T,   out_t = base_t + scales[e] * h_t b[e]^T           (sums f32, rounded once)
+ * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; base may be out.
+ * rows u32[n_rows] holds the row numbers, those of one adapter side by side, offsets u32[n_adapters + 1] where each adapter's begin: place p belongs to e where
+ * offsets[e] <= p < offsets[e + 1].  The rows of the other places have no adapter: they get base (0), and stay as they are where base is out.  mtc_moe_sort of the rows'
+ * adapters (k = 1, one more "expert" for the rows that have none) writes both.  hidden f32[n_rows, rank] (NULL: not wanted) gets h, zeros for rows without an adapter.
+ * Offsets that run backwards or past the rows are clamped and reported through the status word (0x901), row numbers that do not exist are left out and
+ * reported (0x908).  Infinities in a or b give infinities or NaN.
+ * mtc_lora_grad, from the gradient dy T[n_rows, N] of out and the forward call's `hidden`:
+ *     u_t = dy_t b[e],   dx_t = base_t + scales[e] * u_t a[e],   da[e] = scales[e] * sum_t u_t x_t,   db[e] = scales[e] * sum_t dy_t h_t
+ * base (NULL: 0) T[n_rows, K] is the shared projection's gradient of x and may be dx; da, db in the type and shape of a, b, zeros for adapters without rows.
+ * Sums run in an order that the sizes fix. */
+int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
+                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace, size_t workspace_bytes);
+size_t mtc_lora_mm_workspace(const mtc_ctx *ctx, int n_rows, int K, int N, int rank, int n_adapters, int dtype);
+int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *hidden,
+                  const void *scales, const void *base, void *dx, void *da, void *db, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace,
+                  size_t workspace_bytes);
+size_t mtc_lora_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, int N, int rank, int n_adapters, int dtype);
 
 /* ---- name-keyed dispatch with HOST buffers: Context::dispatch_with_grid
  *      (crates/metaltile-runtime/src/context.rs:269-284) ----

@@ -123,6 +123,14 @@ SIGNATURES = {
     "mtc_moe_balance": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_i] * 4 + [_vp, _sz]),
     "mtc_moe_balance_workspace": (_sz, [_vp, _i, _i]),
     "mtc_moe_balance_grad": (_i, [_vp] * 7 + [ctypes.c_float, _vp] + [_i] * 4),
+    "mtc_add_rms_norm": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 2 + [_i] * 3),
+    "mtc_add_rms_norm_fp8": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_i] * 4),
+    "mtc_add_rms_norm_grad": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 3 + [_i] * 3 + [_vp, _sz]),
+    "mtc_add_rms_norm_grad_workspace": (_sz, [_vp, _i, _i]),
+    "mtc_lora_mm": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _sz]),
+    "mtc_lora_mm_workspace": (_sz, [_vp] + [_i] * 6),
+    "mtc_lora_grad": (_i, [_vp] * 14 + [_i] * 6 + [_vp, _sz]),
+    "mtc_lora_grad_workspace": (_sz, [_vp] + [_i] * 6),
     "mtc_set_option": (_i, [_vp, ctypes.c_char_p, _i]),
     "mtc_unpack_codes": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i]),
     "mtc_measure": (_i, [_vp, ctypes.c_char_p, _i, ctypes.POINTER(NamedBuf), _i, _i, _i, _i, ctypes.POINTER(ctypes.c_double),

@@ -882,6 +882,215 @@ PyObject *moe_balance_grad(Args a, Py_ssize_t n) {
     return given ? same(a[7]) : wrap(std::move(out));
 }
 
+// ---- norms and low-rank adapters
+// A caller's output, or none: `like`'s device, this type and these sizes
+at::Tensor given_or(PyObject *o, const char *what, at::IntArrayRef size, at::ScalarType type, const at::Tensor &like) {
+    if (o == Py_None) return at::Tensor();
+    const at::Tensor &t = tensor(o, what);
+    if (t.device() != like.device() || t.scalar_type() != type) raise(PyExc_TypeError, std::string(what) + " must live on the device of the operands and have their dtype");
+    if (t.sizes() != size || !t.is_contiguous()) raise(PyExc_ValueError, std::string(what) + " must be contiguous, of the result's shape");
+    return t;
+}
+// A float argument in f32
+float number(PyObject *o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PyErr{};
+    return static_cast<float>(v);
+}
+void need_type_of(const at::Tensor &x, std::initializer_list<const at::Tensor *> ts, const char *what) {
+    for (const at::Tensor *t : ts)
+        if (t && t->scalar_type() != x.scalar_type()) raise(PyExc_TypeError, what);
+}
+
+// The operands of a norm: x [.., K], weight [K], other (residual, dsum; or null) like x
+struct Norm {
+    const at::Tensor &x, &weight;
+    const at::Tensor *other;
+    int64_t K, M;
+    int dt;
+    Norm(PyObject *x_, PyObject *w_, PyObject *other_, const char *x_name, const char *other_name)
+        : x(tensor(x_, x_name)), weight(tensor(w_, "norm_weight")), other(other_ == Py_None ? nullptr : &tensor(other_, other_name)), dt(need_dtype(x)) {
+        if (x.dim() == 0 || x.size(-1) == 0) raise(PyExc_ValueError, std::string(x_name) + " must be rows of at least one value");
+        K = x.size(-1), M = x.numel() / K;
+        if (weight.dim() != 1 || weight.size(0) != K) raise(PyExc_ValueError, "norm_weight must be [K]");
+        if (other && other->sizes() != x.sizes()) raise(PyExc_ValueError, std::string(other_name) + " must have the shape of " + x_name);
+        need_type_of(x, {&weight, other}, "the operands of a norm must share one dtype in {f32, f16, bf16}");
+        need_contiguous({&x, &weight, other ? other : &x});
+        need_size(M, "rows"), need_size(K, "K");
+    }
+    void devices(const at::Tensor &more) const { need_one_device({&x, &weight, other ? other : &x, &more}); }
+};
+
+// add_rms_norm(x, norm_weight, eps, residual, sum_out, out, ctx) -> (y, sum)
+PyObject *add_rms_norm(Args a, Py_ssize_t n) {
+    nargs(n, 7);
+    const Norm o(a[0], a[1], a[3], "x", "residual");
+    const float eps = number(a[2]);
+    if (!o.other && a[4] != Py_None) raise(PyExc_ValueError, "sum_out goes with a residual");
+    o.devices(o.x);
+    at::Tensor sum = given_or(a[4], "sum_out", o.x.sizes(), o.x.scalar_type(), o.x), y = given_or(a[5], "out", o.x.sizes(), o.x.scalar_type(), o.x);
+    need_context_of(a[6], o.x);
+    const Call c(a[6], o.x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(o.x.device());
+        if (!o.other) sum = o.x;
+        else if (!sum.defined()) sum = empty(o.x.sizes(), o.x.scalar_type(), o.x);
+        if (!y.defined()) y = empty(o.x.sizes(), o.x.scalar_type(), o.x);
+        return mtc_add_rms_norm(c.h, on_stream(o.x), o.x.data_ptr(), o.other ? o.other->data_ptr() : nullptr, o.weight.data_ptr(), eps, sum.data_ptr(), y.data_ptr(),
+                                static_cast<int>(o.M), static_cast<int>(o.K), o.dt);
+    }));
+    return tuple_of({&y, &sum});
+}
+
+// add_rms_norm_fp8(x, norm_weight, eps, residual, pow2, sum_out, out, ctx) -> (codes, scales, sum)
+PyObject *add_rms_norm_fp8(Args a, Py_ssize_t n) {
+    nargs(n, 8);
+    const Norm o(a[0], a[1], a[3], "x", "residual");
+    const float eps = number(a[2]);
+    const int pow2 = PyObject_IsTrue(a[4]);
+    if (pow2 < 0) throw PyErr{};
+    if (!o.other && a[5] != Py_None) raise(PyExc_ValueError, "sum_out goes with a residual");
+    o.devices(o.x);
+    at::Tensor sum = given_or(a[5], "sum_out", o.x.sizes(), o.x.scalar_type(), o.x), y = given_or(a[6], "out", o.x.sizes(), o.x.scalar_type(), o.x), codes, scales;
+    need_context_of(a[7], o.x);
+    const Call c(a[7], o.x);
+    std::vector<int64_t> s_shape(o.x.sizes().begin(), o.x.sizes().end());
+    s_shape.back() = blocks(o.K);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(o.x.device());
+        if (!o.other) sum = o.x;
+        else if (!sum.defined()) sum = empty(o.x.sizes(), o.x.scalar_type(), o.x);
+        codes = empty(o.x.sizes(), at::kFloat8_e4m3fn, o.x);
+        scales = empty(s_shape, at::kFloat, o.x);
+        return mtc_add_rms_norm_fp8(c.h, on_stream(o.x), o.x.data_ptr(), o.other ? o.other->data_ptr() : nullptr, o.weight.data_ptr(), eps, sum.data_ptr(),
+                                    y.defined() ? y.data_ptr() : nullptr, codes.data_ptr(), scales.data_ptr(), static_cast<int>(o.M), static_cast<int>(o.K), pow2, o.dt);
+    }));
+    return tuple_of({&codes, &scales, &sum});
+}
+
+// add_rms_norm_grad(dy, sum, norm_weight, eps, dsum, out, ctx) -> (dx, dweight)
+PyObject *add_rms_norm_grad(Args a, Py_ssize_t n) {
+    nargs(n, 7);
+    const Norm o(a[1], a[2], a[4], "sum", "dsum");
+    const at::Tensor &dy = tensor(a[0], "dy");
+    const float eps = number(a[3]);
+    if (dy.sizes() != o.x.sizes()) raise(PyExc_ValueError, "dy must have the shape of sum");
+    need_type_of(o.x, {&dy}, "the operands of a norm must share one dtype in {f32, f16, bf16}");
+    need_contiguous({&dy});
+    o.devices(dy);
+    at::Tensor dx = given_or(a[5], "out", o.x.sizes(), o.x.scalar_type(), o.x), dw;
+    need_context_of(a[6], o.x);
+    const Call c(a[6], o.x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(o.x.device());
+        if (!dx.defined()) dx = empty(o.x.sizes(), o.x.scalar_type(), o.x);
+        dw = empty({o.K}, o.x.scalar_type(), o.x);
+        const size_t need = mtc_add_rms_norm_grad_workspace(c.h, static_cast<int>(o.M), static_cast<int>(o.K));
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, o.x);
+        return mtc_add_rms_norm_grad(c.h, on_stream(o.x), dy.data_ptr(), o.x.data_ptr(), o.weight.data_ptr(), eps, o.other ? o.other->data_ptr() : nullptr, dx.data_ptr(),
+                                     dw.data_ptr(), static_cast<int>(o.M), static_cast<int>(o.K), o.dt, need ? space.data_ptr() : nullptr, need);
+    }));
+    return tuple_of({&dx, &dw});
+}
+
+// The operands of low-rank adapters: x [.., K], a [L, rank, K], b [L, N, rank], rows int32 [n_rows], offsets int32 [L + 1 or more], scales f32 [L] or null
+struct Lora {
+    const at::Tensor &x, &a, &b, &rows, &offsets;
+    const at::Tensor *scales;
+    int64_t K, M, L, rank, N;
+    int dt;
+    Lora(PyObject *x_, PyObject *a_, PyObject *b_, PyObject *rows_, PyObject *offsets_, PyObject *scales_)
+        : x(tensor(x_, "x")), a(tensor(a_, "a")), b(tensor(b_, "b")), rows(index_tensor(rows_, "rows")), offsets(index_tensor(offsets_, "offsets")),
+          scales(scales_ == Py_None ? nullptr : &tensor(scales_, "scales")), dt(need_dtype(x)) {
+        if (x.dim() == 0 || x.size(-1) == 0) raise(PyExc_ValueError, "x must be rows of at least one value");
+        K = x.size(-1), M = x.numel() / K;
+        if (a.dim() != 3 || a.size(0) == 0 || a.size(1) == 0 || a.size(2) != K) raise(PyExc_ValueError, "a must be [adapters, rank, K]");
+        L = a.size(0), rank = a.size(1);
+        if (b.dim() != 3 || b.size(0) != L || b.size(1) == 0 || b.size(2) != rank) raise(PyExc_ValueError, "b must be [adapters, N, rank]");
+        N = b.size(1);
+        need_type_of(x, {&a, &b}, "x, a and b must share one dtype in {f32, f16, bf16}");
+        if (rows.dim() != 1 || rows.size(0) != M) raise(PyExc_ValueError, "rows must have one entry for each row of x");
+        if (offsets.dim() != 1 || offsets.size(0) < L + 1) raise(PyExc_ValueError, "offsets must have adapters + 1 entries (what follows them is not looked at)");
+        if (scales && scales->scalar_type() != at::kFloat) raise(PyExc_TypeError, "scales must be float32");
+        if (scales && (scales->dim() != 1 || scales->size(0) != L || !scales->is_contiguous())) raise(PyExc_ValueError, "scales must be [adapters], contiguous");
+        need_contiguous({&x, &a, &b});
+        need_size(M, "rows"), need_size(K, "K"), need_size(N, "N"), need_size(rank, "rank"), need_size(L, "adapters");
+    }
+    void devices(const at::Tensor &more, const at::Tensor *base) const {
+        need_one_device({&x, &a, &b, &rows, &offsets, scales ? scales : &x, base ? base : &x, &more});
+    }
+    // what the adapters' product is added to: rows of `width`, or null
+    const at::Tensor *base(PyObject *o, int64_t width) const {
+        if (o == Py_None) return nullptr;
+        const at::Tensor &t = tensor(o, "base");
+        need_type_of(x, {&t}, "base must have the dtype of x");
+        if (t.dim() == 0 || t.size(-1) != width || t.numel() != M * width || !t.is_contiguous()) raise(PyExc_ValueError, "base must be contiguous, of the result's shape");
+        return &t;
+    }
+};
+
+// lora_mm(x, a, b, rows, offsets, scales, base, out, hidden, ctx) -> out, or (out, hidden)
+PyObject *lora_mm(Args a, Py_ssize_t n) {
+    nargs(n, 10);
+    const Lora o(a[0], a[1], a[2], a[3], a[4], a[5]);
+    const at::Tensor *base = o.base(a[6], o.N);
+    o.devices(o.x, base);
+    const bool given = a[7] != Py_None;
+    at::Tensor out = given ? tensor(a[7], "out") : at::Tensor(), hidden;
+    if (given) check_out(out, o.M, o.N, o.x);
+    const int keep = PyObject_IsTrue(a[8]);
+    if (keep < 0) throw PyErr{};
+    need_context_of(a[9], o.x);
+    const Call c(a[9], o.x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(o.x.device());
+        if (!given) out = empty({o.M, o.N}, o.x.scalar_type(), o.x);
+        if (keep) hidden = empty({o.M, o.rank}, at::kFloat, o.x);
+        const int M = static_cast<int>(o.M), K = static_cast<int>(o.K), N = static_cast<int>(o.N), r = static_cast<int>(o.rank), L = static_cast<int>(o.L);
+        const size_t need = mtc_lora_mm_workspace(c.h, M, K, N, r, L, o.dt);
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, o.x);
+        return mtc_lora_mm(c.h, on_stream(o.x), o.x.data_ptr(), o.a.data_ptr(), o.b.data_ptr(), o.rows.data_ptr(), o.offsets.data_ptr(),
+                           o.scales ? o.scales->data_ptr() : nullptr, base ? base->data_ptr() : nullptr, out.data_ptr(), keep ? hidden.data_ptr() : nullptr, M, K, N, r, L,
+                           o.dt, need ? space.data_ptr() : nullptr, need);
+    }));
+    if (keep) return tuple_of({&out, &hidden});
+    return given ? same(a[7]) : wrap(std::move(out));
+}
+
+// lora_grad(dy, x, a, b, rows, offsets, hidden, scales, base, out, ctx) -> (dx, da, db)
+PyObject *lora_grad(Args a, Py_ssize_t n) {
+    nargs(n, 11);
+    const Lora o(a[1], a[2], a[3], a[4], a[5], a[7]);
+    const at::Tensor &dy = tensor(a[0], "dy"), &hidden = tensor(a[6], "hidden");
+    need_type_of(o.x, {&dy}, "dy must have the dtype of x");
+    if (dy.dim() == 0 || dy.size(-1) != o.N || dy.numel() != o.M * o.N) raise(PyExc_ValueError, "dy must be rows of N values, one for each row of x");
+    if (hidden.scalar_type() != at::kFloat) raise(PyExc_TypeError, "hidden must be float32");
+    if (hidden.dim() != 2 || hidden.size(0) != o.M || hidden.size(1) != o.rank) raise(PyExc_ValueError, "hidden must be [rows, rank]");
+    need_contiguous({&dy, &hidden});
+    const at::Tensor *base = o.base(a[8], o.K);
+    o.devices(dy, base), o.devices(hidden, base);
+    at::Tensor dx = a[9] == Py_None ? at::Tensor() : tensor(a[9], "out"), da, db;
+    if (dx.defined()) check_out(dx, o.M, o.K, o.x);
+    need_context_of(a[10], o.x);
+    const Call c(a[10], o.x);
+    c.check(unlocked([&] {
+        const c10::cuda::CUDAGuard guard(o.x.device());
+        if (!dx.defined()) dx = empty({o.M, o.K}, o.x.scalar_type(), o.x);
+        da = empty(o.a.sizes(), o.x.scalar_type(), o.x);
+        db = empty(o.b.sizes(), o.x.scalar_type(), o.x);
+        const int M = static_cast<int>(o.M), K = static_cast<int>(o.K), N = static_cast<int>(o.N), r = static_cast<int>(o.rank), L = static_cast<int>(o.L);
+        const size_t need = mtc_lora_grad_workspace(c.h, M, K, N, r, L, o.dt);
+        at::Tensor space;
+        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, o.x);
+        return mtc_lora_grad(c.h, on_stream(o.x), dy.data_ptr(), o.x.data_ptr(), o.a.data_ptr(), o.b.data_ptr(), o.rows.data_ptr(), o.offsets.data_ptr(), hidden.data_ptr(),
+                             o.scales ? o.scales->data_ptr() : nullptr, base ? base->data_ptr() : nullptr, dx.data_ptr(), da.data_ptr(), db.data_ptr(), M, K, N, r, L, o.dt,
+                             need ? space.data_ptr() : nullptr, need);
+    }));
+    return tuple_of({&dx, &da, &db});
+}
+
 // ---- module ----------------------------------------------------------------------------------------
 PyObject *set_context(PyObject *, PyObject *fn) {
     Py_INCREF(fn);
@@ -906,6 +1115,7 @@ PyMethodDef methods[] = {
     OP(dense), OP(qmv_batched), OP(qvm), OP(rms_norm_qmv), OP(swiglu), OP(moe_router_topk), OP(moe_sort), OP(moe_permute), OP(moe_unpermute),
     OP(gather_qmm), OP(moe_experts), OP(affine_quantize), OP(affine_dequantize), OP(dequant_gather), OP(unpack_codes),
     OP(fp8_quantize), OP(fp8_mm), OP(fp8_gather_mm), OP(moe_balance), OP(moe_balance_grad),
+    OP(add_rms_norm), OP(add_rms_norm_fp8), OP(add_rms_norm_grad), OP(lora_mm), OP(lora_grad),
     {"set_context", set_context, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -13,6 +13,8 @@
 
 #include "common.cuh"
 #include "fp8.cuh"
+#include "lora.cuh"
+#include "norm.cuh"
 
 using mtc::Ctx;
 using mtc::fail;
@@ -1639,6 +1641,121 @@ int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const v
         MTC_CUDA(ctx, mtc::launch_moe_balance_grad(ctx, static_cast<cudaStream_t>(stream), logits, static_cast<const uint8_t *>(mask),
                                                    static_cast<const int *>(counts), static_cast<const int *>(n_counted),
                                                    static_cast<const float *>(grad_loss), coef, grad, n_rows, n_experts, k, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+// ---- norms and low-rank adapters ---------------------------------------------------------------------------
+static int norm_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int K, int dtype) {
+    if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": dtype must be f32, f16 or bf16");
+    if (n_rows < 0 || K <= 0 || K > mtc::kMostNorm) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": need n_rows >= 0 and 0 < K <= 2^30");
+    return MTC_OK;
+}
+static int add_rms_norm(mtc_ctx *ctx, const char *who, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, void *codes,
+                        void *scales, int n_rows, int K, int mode, int dtype) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        const int rc = norm_args_ok(ctx, who, n_rows, K, dtype);
+        if (rc != MTC_OK || n_rows == 0) return rc;
+        if (!x || !norm_weight || (residual && !sum) || (mode == 0 ? !y : !codes || !scales)) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": null pointer");
+        if (residual && sum == y) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": sum and y are the same memory");
+        mtc::NormArgs a{};
+        a.x = x, a.residual = residual, a.weight = norm_weight, a.sum = sum, a.y = y;
+        a.codes = static_cast<uint8_t *>(codes), a.scales = static_cast<float *>(scales);
+        a.n_rows = n_rows, a.K = K, a.eps = eps;
+        MTC_CUDA(ctx, mtc::launch_add_rms_norm(ctx, static_cast<cudaStream_t>(stream), a, mode, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+int mtc_add_rms_norm(mtc_ctx *ctx, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, int n_rows, int K, int dtype) {
+    return add_rms_norm(ctx, "add_rms_norm", stream, x, residual, norm_weight, eps, sum, y, nullptr, nullptr, n_rows, K, 0, dtype);
+}
+
+int mtc_add_rms_norm_fp8(mtc_ctx *ctx, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, void *codes,
+                         void *scales, int n_rows, int K, int pow2, int dtype) {
+    return add_rms_norm(ctx, "add_rms_norm_fp8", stream, x, residual, norm_weight, eps, sum, y, codes, scales, n_rows, K, pow2 ? 2 : 1, dtype);
+}
+
+size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K) {
+    return K <= 0 ? 0 : mtc::norm_grad_workspace(ctx ? ctx->sm_count : mtc::kNumSMsB200, n_rows, K);
+}
+
+int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *sum, const void *norm_weight, float eps, const void *dsum, void *dx, void *dweight,
+                          int n_rows, int K, int dtype, void *workspace, size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        int rc = norm_args_ok(ctx, "add_rms_norm_grad", n_rows, K, dtype);
+        if (rc != MTC_OK) return rc;
+        if (!dweight || (n_rows > 0 && (!dy || !sum || !norm_weight || !dx))) return fail(ctx, MTC_ERR_INVALID, "add_rms_norm_grad: null pointer");
+        rc = check_workspace(ctx, "add_rms_norm_grad", workspace, workspace_bytes, mtc_add_rms_norm_grad_workspace(ctx, n_rows, K));
+        if (rc != MTC_OK) return rc;
+        mtc::NormGradArgs a{};
+        a.dy = dy, a.s = sum, a.weight = norm_weight, a.dsum = dsum, a.dx = dx;
+        a.n_rows = n_rows, a.K = K, a.eps = eps;
+        MTC_CUDA(ctx, mtc::launch_norm_grad(ctx, static_cast<cudaStream_t>(stream), a, dweight, workspace, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+static bool lora_sizes_ok(int n_rows, int K, int N, int rank, int n_adapters) {
+    const int most = mtc::fp8::kMostSize;
+    return n_rows >= 0 && n_rows <= most && K > 0 && K <= most && N > 0 && N <= most && rank > 0 && rank <= mtc::kMostRank && n_adapters > 0 && n_adapters <= mtc::kMostAdapters;
+}
+static int lora_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
+    if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": dtype must be f32, f16 or bf16");
+    if (!lora_sizes_ok(n_rows, K, N, rank, n_adapters))
+        return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": sizes must be positive and below 2^31 - 1024, the rank at most 1024 and the adapters at most 65536");
+    return MTC_OK;
+}
+
+size_t mtc_lora_mm_workspace(const mtc_ctx *, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
+    return lora_sizes_ok(n_rows, K, N, rank, n_adapters) && dtype_ok(dtype) ? mtc::lora_workspace(n_rows, rank) : 0;
+}
+size_t mtc_lora_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
+    return mtc_lora_mm_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype);
+}
+
+int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
+                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace, size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        int rc = lora_args_ok(ctx, "lora_mm", n_rows, K, N, rank, n_adapters, dtype);
+        if (rc != MTC_OK || n_rows == 0) return rc;
+        if (!x || !a || !b || !rows || !offsets || !out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: null pointer");
+        rc = check_workspace(ctx, "lora_mm", workspace, workspace_bytes, mtc_lora_mm_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype));
+        if (rc != MTC_OK) return rc;
+        mtc::LoraArgs l{};
+        l.in = x, l.down = a, l.up = b, l.base = base, l.out = out;
+        l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
+        l.low = static_cast<float *>(hidden ? hidden : workspace);
+        l.n_rows = n_rows, l.c_in = K, l.c_out = N, l.rank = rank, l.n_adapters = n_adapters, l.status = ctx->d_status;
+        MTC_CUDA(ctx, mtc::launch_lora(ctx, static_cast<cudaStream_t>(stream), l, false, hidden != nullptr, dtype), MTC_ERR_DISPATCH);
+        return MTC_OK;
+    });
+}
+
+int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *hidden,
+                  const void *scales, const void *base, void *dx, void *da, void *db, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace,
+                  size_t workspace_bytes) {
+    return guarded(ctx, [&]() -> int {
+        MTC_ENTER(ctx);
+        int rc = lora_args_ok(ctx, "lora_grad", n_rows, K, N, rank, n_adapters, dtype);
+        if (rc != MTC_OK) return rc;
+        if (!offsets || !da || !db || (n_rows > 0 && (!dy || !x || !a || !b || !rows || !hidden || !dx))) return fail(ctx, MTC_ERR_INVALID, "lora_grad: null pointer");
+        rc = check_workspace(ctx, "lora_grad", workspace, workspace_bytes, mtc_lora_grad_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype));
+        if (rc != MTC_OK) return rc;
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        float *const u = static_cast<float *>(workspace);
+        mtc::LoraArgs l{};
+        l.in = dy, l.down = b, l.up = a, l.base = base, l.out = dx, l.low = u;
+        l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
+        l.n_rows = n_rows, l.c_in = N, l.c_out = K, l.rank = rank, l.n_adapters = n_adapters, l.status = ctx->d_status;
+        if (n_rows > 0) MTC_CUDA(ctx, mtc::launch_lora(ctx, st, l, true, false, dtype), MTC_ERR_DISPATCH);
+        mtc::LoraWeights w{};
+        w.a = {x, u, da, K}, w.b = {dy, static_cast<const float *>(hidden), db, N};
+        w.order = l.order, w.offsets = l.offsets, w.scales = l.scales, w.n_rows = n_rows, w.rank = rank, w.n_adapters = n_adapters, w.status = ctx->d_status;
+        MTC_CUDA(ctx, mtc::launch_lora_weights(ctx, st, w, dtype), MTC_ERR_DISPATCH);
         return MTC_OK;
     });
 }

@@ -223,3 +223,41 @@ def moe_balance_grad(logits, counts, n_counted, k: int, grad_loss=None, coef: fl
     (f_e - sum_j f_j p_tj)`` with ``f = counts / (n k)`` constant; zeros for masked rows.  ``grad_loss``: one float32 on the device (None: 1).
     Where several ranks share a batch, add up their ``counts`` and ``n_counted`` first: the gradient is then that of the common loss."""
     return _native.moe_balance_grad(logits, counts, n_counted, k, grad_loss, coef, mask, out, ctx)
+
+
+# ---- in front of a projection: the norm with the residual's addition ----------------------------------------------------------
+def add_rms_norm(x, norm_weight, eps: float, residual=None, sum_out=None, out=None, ctx: Context = None):
+    """(y, s) with ``s = x + residual`` in the type of x and ``y = s / sqrt(mean(s^2) + eps) * norm_weight`` for every row of ``x [.., K]``.
+
+    The norm is of what ``s`` holds.  Without ``residual`` s is x itself.  ``sum_out`` (s) and ``out`` (y) may be x or residual: a residual stream that is updated in
+    place is ``add_rms_norm(x, w, eps, residual=stream, sum_out=stream)``.  One row in front of one projection of affine codes: ``rms_norm_qmv``."""
+    return _native.add_rms_norm(x, norm_weight, eps, residual, sum_out, out, ctx)
+
+
+def add_rms_norm_fp8(x, norm_weight, eps: float, residual=None, pow2: bool = False, sum_out=None, out=None, ctx: Context = None):
+    """(codes, scales, s): ``add_rms_norm`` whose y is given as ``fp8_quantize`` gives float32 rows, without a rounding in between: what ``fp8_mm``
+    reads.  With ``out`` y is written there too, in the type of x (for adapters beside the product, say)."""
+    return _native.add_rms_norm_fp8(x, norm_weight, eps, residual, pow2, sum_out, out, ctx)
+
+
+def add_rms_norm_grad(dy, s, norm_weight, eps: float, dsum=None, out=None, ctx: Context = None):
+    """(dx, dweight) from the gradient ``dy`` of y and the ``s`` of the forward call; dx, which belongs to x and to residual alike, includes ``dsum``, the gradient of
+    s from further down the residual stream.  ``out`` (dx) may be dy or dsum."""
+    return _native.add_rms_norm_grad(dy, s, norm_weight, eps, dsum, out, ctx)
+
+
+# ---- beside a projection: low-rank adapters of many requests -------------------------------------------------------------------
+def lora_mm(x, a, b, rows, offsets, scales=None, base=None, out=None, hidden: bool = False, ctx: Context = None):
+    """out[t] = base[t] + scales[e] * (x[t] @ a[e]^T) @ b[e]^T for every row t of ``x [.., K]``, e its adapter; ``a [L, rank, K]``, ``b [L, N, rank]``, ``scales`` float32
+    ``[L]`` (None: 1), ``base [.., N]`` the shared projection's result (None: 0).  Rows without an adapter get ``base``, and are not touched where ``out is base``.
+
+    ``rows`` and ``offsets`` group the rows by adapter, once for all projections of a step: with ``ids`` int32 ``[n_rows]``, L for rows that have none,
+    ``rows, _, offsets, _ = moe_sort(ids[:, None], L + 1)``.  ``hidden=True`` returns (out, h) with h = x a^T float32 ``[n_rows, rank]`` (zeros for rows without an
+    adapter), which ``lora_grad`` wants."""
+    return _native.lora_mm(x, a, b, rows, offsets, scales, base, out, hidden, ctx)
+
+
+def lora_grad(dy, x, a, b, rows, offsets, hidden, scales=None, base=None, out=None, ctx: Context = None):
+    """(dx, da, db) of ``lora_mm`` from the gradient ``dy [.., N]`` of its result and the ``hidden`` it returned.  dx is ``base`` (the gradient of x that the shared
+    projection gives, None: 0) plus the adapters' share; ``out`` (dx) may be base.  da and db have the shape and type of a and b, zeros for adapters without rows."""
+    return _native.lora_grad(dy, x, a, b, rows, offsets, hidden, scales, base, out, ctx)
