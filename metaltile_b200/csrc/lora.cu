@@ -121,10 +121,12 @@ cudaError_t launch_weights_any(cudaStream_t st, const LoraWeights &w) {
 
 }  // namespace
 
-cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward, bool all, int dt) {
-    return (dt == MTC_F32 ? launch_any<MTC_F32> : dt == MTC_BF16 ? launch_any<MTC_BF16> : launch_any<MTC_F16>)(st, a, backward, all);
+cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt) {
+    if (lora_mma_supported(a)) return launch_lora_mma(st, a, backward, keep, (keep && all) || a.base != a.out, dt);
+    return (dt == MTC_F32 ? launch_any<MTC_F32> : dt == MTC_BF16 ? launch_any<MTC_BF16> : launch_any<MTC_F16>)(st, a, backward, keep && all);
 }
-cudaError_t launch_lora_weights(Ctx *, cudaStream_t st, const LoraWeights &w, int dt) {
+cudaError_t launch_lora_weights(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt) {
+    if (lora_grad_supported(w)) return launch_lora_grad(ctx, st, w, dt);
     return (dt == MTC_F32 ? launch_weights_any<MTC_F32> : dt == MTC_BF16 ? launch_weights_any<MTC_BF16> : launch_weights_any<MTC_F16>)(st, w);
 }
 

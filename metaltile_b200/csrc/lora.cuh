@@ -37,8 +37,14 @@ struct LoraWeights {
     uint32_t *status;
 };
 
-// `low` has to be written for the rows of no adapter (zeros), too: `all`
-cudaError_t launch_lora(Ctx *ctx, cudaStream_t st, const LoraArgs &a, bool backward, bool all, int dt);
+// keep: `low` is wanted; all: with zeros for the rows of no adapter
+cudaError_t launch_lora(Ctx *ctx, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt);
 cudaError_t launch_lora_weights(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);
+
+// The tensor-core kernels (lora_mma.cu, lora_grad.cu) and what they take; `none`: rows of no adapter have something to be written
+bool lora_mma_supported(const LoraArgs &a);
+cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
+bool lora_grad_supported(const LoraWeights &w);
+cudaError_t launch_lora_grad(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);
 
 }  // namespace mtc

@@ -1,0 +1,416 @@
+// Low-rank adapters on warp-level tensor cores: h = x A^T and out = base + scale h B^T (or, back, u = dy B and dx = base + scale u A) in one launch.
+//
+// A cluster of CTAs has one tile of rows of one adapter: each CTA, each of its eight warps, sums up a part of the long axis of the first product; the parts meet in
+// shared memory, then over distributed shared memory, so that every CTA has the whole h of the tile; then each CTA takes a part of the
+// columns of the second product.  Bound by memory: x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.  At
+// rank 64 the two products are 64 operations a byte of activations, a tenth of what the warp-level tensor cores give, so there is nothing for tcgen05 to win: its
+// smallest tile, 128 rows, would be empty for the most part where users decode.
+#include <algorithm>
+
+#include "lora_mma.cuh"
+
+namespace mtc {
+namespace {
+
+using namespace lora;
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kCluster = 8;
+
+__host__ __device__ constexpr int part_stride(int rb) { return rb + 4; }
+__host__ __device__ constexpr int held_stride(int blocks, int rb) { return blocks * rb + 8; }      // in 16-bit values: rows 16 bytes apart modulo 128
+
+struct Tile {
+    int e;                                       // n_adapters: rows of none; -1: no such tile
+    uint32_t p0, n;
+};
+
+// The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By the whole CTA.
+__device__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none, long long *scratch) {
+    __shared__ Tile found;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) found = {-1, 0, 0};
+    const uint32_t R = a.n_rows;
+    long long before = 0;                        // offsets that run backwards may name more tiles than 32 bits hold
+    for (int e0 = 0; e0 <= a.n_adapters; e0 += kThreads) {
+        const int e = e0 + threadIdx.x;
+        uint32_t from = 0, n = 0;
+        if (e < a.n_adapters || (none && e == a.n_adapters)) {
+            from = min(a.offsets[e], R);
+            const uint32_t to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
+            n = to > from ? to - from : 0;
+        }
+        const long long mine = (static_cast<long long>(n) + rows - 1) / rows;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        __syncthreads();                         // scratch of the turn before is read
+        if (lane == 31) scratch[warp] = upto;
+        __syncthreads();
+        long long total = 0, base = before;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) base += scratch[w];
+            total += scratch[w];
+        }
+        const long long first = base + upto - mine;
+        if (id >= first && id < first + mine) {
+            const uint32_t skip = static_cast<uint32_t>(id - first) * rows;
+            found = {e, from + skip, min(n - skip, static_cast<uint32_t>(rows))};
+        }
+        before += total;
+        if (id < before) break;
+    }
+    __syncthreads();
+    return found;
+}
+
+// RB: ranks a pass (a block of the rank), 8 to 64.  MT: tiles of 16 rows.  BACK: the first product's weights lie [c_in][rank], the second's [rank][c_out];
+// else [rank][c_in] and [c_out][rank].
+template <int DT, int RB, int MT, bool BACK>
+__global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, int rank_blocks, bool keep, bool none) {
+    pdl_enter();
+    constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8;
+    constexpr bool HALF = DT == MTC_F16;
+    extern __shared__ __align__(16) float sm[];
+    const int RT = rank_blocks * RB, HS = held_stride(rank_blocks, RB);
+    float *const part = sm;                                                      // [warps][ROWS][PS]
+    float *const low = part + kWarps * ROWS * PS;                                // [ROWS][RT]
+    uint16_t *const held = reinterpret_cast<uint16_t *>(low + ROWS * RT);        // [H][ROWS][HS]
+    __shared__ int row_of[ROWS];
+    __shared__ float back_up[ROWS];              // f16: the power of two that a row's h was divided by
+    __shared__ long long scratch[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int cs = cluster_size(), cr = cluster_rank();
+    if (blockIdx.x == 0)
+        for (int e = threadIdx.x; e < a.n_adapters; e += kThreads)
+            if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
+    const Tile tile = find_tile(a, blockIdx.x / cs, ROWS, none, scratch);
+    if (tile.e < 0) return;                      // the whole cluster
+    if (threadIdx.x < ROWS) {
+        int row = -1;
+        if (threadIdx.x < tile.n) {
+            const uint32_t v = a.order[tile.p0 + threadIdx.x];
+            if (v < static_cast<uint32_t>(a.n_rows)) row = static_cast<int>(v);
+            else atomicCAS(a.status, 0u, 0x908u);
+        }
+        row_of[threadIdx.x] = row;
+    }
+    constexpr int CW = BACK ? 64 : 32;           // columns of a warp's step
+    const int units = (a.c_out + CW - 1) / CW, unit0 = static_cast<int>(static_cast<long long>(units) * cr / cs), unit1 = static_cast<int>(static_cast<long long>(units) * (cr + 1) / cs);
+    __syncthreads();
+    if (tile.e == a.n_adapters) {                // rows of no adapter: base, or zeros
+        if (a.base != a.out) {
+            const int from = unit0 * CW, wide = min(unit1 * CW, a.c_out) - from;
+            for (int i = threadIdx.x; i < static_cast<int>(tile.n) * (wide / 8); i += kThreads) {
+                const int row = row_of[i / (wide / 8)], c = from + i % (wide / 8) * 8;
+                if (row < 0) continue;
+                const size_t at = static_cast<size_t>(row) * a.c_out + c;
+                lora::Eight<DT> v;
+                v.load(a.base, at, a.base != nullptr);
+                const float zero[8] = {};
+                v.add_and_store(a.out, at, zero, 1.0f);
+            }
+        }
+        if (keep)
+            for (int i = threadIdx.x + cr * kThreads; i < static_cast<int>(tile.n) * a.rank; i += kThreads * cs)
+                if (row_of[i / a.rank] >= 0) a.low[static_cast<size_t>(row_of[i / a.rank]) * a.rank + i % a.rank] = 0.0f;
+        return;
+    }
+    const size_t expert = tile.e;
+
+    // ---- the first product: this warp's part of c_in, 32 values at a time
+    int rows[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) rows[m][0] = row_of[16 * m + g], rows[m][1] = row_of[16 * m + g + 8];
+    const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
+    const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * me / workers), chunk1 = static_cast<int>(static_cast<long long>(chunks) * (me + 1) / workers);
+    for (int rb = 0; rb < rank_blocks; ++rb) {
+        float acc[MT][NT][4] = {};
+        float fine[P > 1 ? MT : 1][P > 1 ? NT : 1][4] = {};      // f32: the products of small pieces, apart so that the large ones are cut off less often
+#pragma unroll 2
+        for (int c = chunk0; c < chunk1; ++c) {
+            const int k = c * 32 + t * 8;
+            const bool in = k < a.c_in;
+            Vals<DT, 8> x[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[m][h].load(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
+            auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {      // tile j of ranks, piece p of the weights, half i of the 32 values
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int q = 0; q + p < P; ++q) {
+                        float (&d)[4] = P > 1 && q + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
+                        mma<HALF>(d, x[m][0].w[q][2 * i], x[m][1].w[q][2 * i], x[m][0].w[q][2 * i + 1], x[m][1].w[q][2 * i + 1], b0, b1);
+                    }
+            };
+            if constexpr (!BACK) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int r = rb * RB + 8 * j + g;
+                    Vals<DT, 8> w;
+                    w.load(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) step(j, p, i, w.w[p][2 * i], w.w[p][2 * i + 1]);
+                }
+            } else {
+                using V = Vals<DT, NT>;          // lane g has ranks g NT .. g NT + NT - 1: rank g NT + j is column g of tile j
+                const int r = rb * RB + g * NT;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    V w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) w[q].load(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, in && r < a.rank);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), V::pair(w[2], w[3], p, j));
+                }
+            }
+        }
+        // ---- the warps' parts, then the CTAs'
+        if (rb) {                                // (the gather of the block before has read `part`)
+            cluster_arrive();
+            cluster_wait();
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = 16 * m + g + (i >= 2 ? 8 : 0), c = 2 * t + (i & 1), col = BACK ? c * NT + j : 8 * j + c;
+                    part[(warp * ROWS + row) * PS + col] = P > 1 ? acc[m][j][i] + fine[P > 1 ? m : 0][P > 1 ? j : 0][i] : acc[m][j][i];
+                }
+        __syncthreads();
+        for (int i = threadIdx.x; i < ROWS * RB / 4; i += kThreads) {
+            float4 *const at = reinterpret_cast<float4 *>(part + i / (RB / 4) * PS + i % (RB / 4) * 4);
+            float4 s = *at;
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) {
+                const float4 v = at[w * ROWS * PS / 4];
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            *at = s;
+        }
+        cluster_arrive();
+        cluster_wait();
+        for (int i = threadIdx.x; i < ROWS * RB / 4; i += kThreads) {
+            const int row = i / (RB / 4), col = i % (RB / 4) * 4;
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int q = 0; q < cs; ++q) {
+                const float4 v = ld_cta(part + row * PS + col, q);
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            *reinterpret_cast<float4 *>(low + row * RT + rb * RB + col) = s;
+        }
+    }
+    cluster_arrive();                            // nobody leaves while its part is read: waited for at the end
+    __syncthreads();
+    if (keep)
+        for (int i = threadIdx.x + cr * kThreads; i < ROWS * a.rank; i += kThreads * cs) {
+            const int row = row_of[i / a.rank];
+            if (row >= 0) a.low[static_cast<size_t>(row) * a.rank + i % a.rank] = low[i / a.rank * RT + i % a.rank];
+        }
+
+    // ---- h as an operand
+    if constexpr (HALF) {                        // rows are divided by the power of two of their largest value: f16 has five bits of exponent
+        for (int row = warp; row < ROWS; row += kWarps) {
+            float most = 0.0f;
+            for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(low[row * RT + i]));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int bits = static_cast<int>(__float_as_uint(most) >> 23);
+            if (lane == 0) back_up[row] = bits == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(bits, 27), 253)) << 23);
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < ROWS * RT; i += kThreads) {
+        const int row = i / RT, col = i % RT;
+        float v = low[i];
+        if constexpr (HALF) v *= 1.0f / back_up[row];            // a power of two: exact
+        const bool finite = fabsf(v) < INFINITY;
+#pragma unroll
+        for (int p = 0; p < H; ++p) {
+            uint16_t *const at = held + (p * ROWS + row) * HS + col;
+            if constexpr (HALF) {
+                const __half h = __float2half_rn(v);
+                *at = __half_as_ushort(h);
+                v = finite ? v - __half2float(h) : 0.0f;
+            } else if (p + 1 < H) {
+                const uint32_t b = __float_as_uint(v);
+                *at = static_cast<uint16_t>(b >> 16);
+                v = finite ? v - __uint_as_float(b & 0xFFFF0000u) : 0.0f;
+            } else {
+                *at = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- the second product
+    const float scale = a.scales ? a.scales[expert] : 1.0f;
+    constexpr int TN = CW / 8, QS = RB >= 32 ? RB / 32 : 1, WIDE = RB >= 32 ? 8 : RB / 4;      // tiles; loads of a block's ranks, ranks of a lane in each
+    for (int u = unit0 + warp; u < unit1; u += kWarps) {
+        const int n0 = u * CW;
+        float acc[MT][TN][4] = {};
+        float fine[P > 1 ? MT : 1][P > 1 ? TN : 1][4] = {};
+        lora::Eight<DT> base[MT][2][CW / 32];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < CW / 32; ++i) {
+                    const int c = n0 + t * (CW / 4) + 8 * i;
+                    base[m][h][i].load(a.base, static_cast<size_t>(rows[m][h]) * a.c_out + c, a.base && rows[m][h] >= 0 && c < a.c_out);
+                }
+        for (int rb = 0; rb < rank_blocks; ++rb) {
+#pragma unroll
+            for (int q = 0; q < QS; ++q) {
+                const int r = rb * RB + q * 32 + t * WIDE;       // this lane's ranks: r .. r + WIDE - 1
+                uint32_t hw[MT][2][H][WIDE / 2];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int p = 0; p < H; ++p) {
+                            const uint16_t *const at = held + (p * ROWS + 16 * m + g + 8 * h) * HS + r;
+                            if constexpr (WIDE == 8) {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(at);
+                                hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y, hw[m][h][p][2] = v.z, hw[m][h][p][3] = v.w;
+                            } else if constexpr (WIDE == 4) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                                hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y;
+                            } else {
+                                hw[m][h][p][0] = *reinterpret_cast<const uint32_t *>(at);
+                            }
+                        }
+                auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {  // tile j of columns, piece p of the weights, ranks 4 i .. of the lane's
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int s = 0; s < H; ++s) {
+                            if (P > 1 && s + p >= P) continue;
+                            float (&d)[4] = P > 1 && s + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
+                            const uint32_t a2 = WIDE == 2 ? 0u : hw[m][0][s][WIDE == 2 ? 0 : 2 * i + 1], a3 = WIDE == 2 ? 0u : hw[m][1][s][WIDE == 2 ? 0 : 2 * i + 1];
+                            mma<HALF>(d, hw[m][0][s][2 * i], hw[m][1][s][2 * i], a2, a3, b0, b1);
+                        }
+                };
+                if constexpr (!BACK) {
+                    // column c of tile j is n0 + c / 2 * 8 + 2 j + c % 2, so that a lane's results are eight neighbours
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        const int n = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
+                        Vals<DT, WIDE> w;
+                        w.load(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int i = 0; i < (WIDE == 8 ? 2 : 1); ++i) step(j, p, i, w.w[p][2 * i], WIDE == 2 ? 0u : w.w[p][WIDE == 2 ? 0 : 2 * i + 1]);
+                    }
+                } else {
+                    // column c of tile j is n0 + 8 c + j: a lane loads eight neighbours of four ranks' rows, its results are sixteen
+                    using V = Vals<DT, 8>;
+                    const int c = n0 + 8 * g;
+#pragma unroll
+                    for (int i = 0; i < (WIDE == 8 ? 2 : 1); ++i) {
+                        V w[WIDE == 2 ? 2 : 4];
+#pragma unroll
+                        for (int s = 0; s < (WIDE == 2 ? 2 : 4); ++s) {
+                            const int rr = r + 4 * i + s;
+                            w[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
+                        }
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+#pragma unroll
+                            for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), WIDE == 2 ? 0u : V::pair(w[WIDE == 2 ? 0 : 2], w[WIDE == 2 ? 1 : 3], p, j));
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (rows[m][h] < 0) continue;
+                const float factor = HALF ? scale * back_up[16 * m + g + 8 * h] : scale;
+#pragma unroll
+                for (int i = 0; i < CW / 32; ++i) {
+                    const int c = n0 + t * (CW / 4) + 8 * i;
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int j = BACK ? k : k / 2, at = 2 * h + (BACK ? i : k & 1);
+                        v[k] = acc[m][j][at];
+                        if constexpr (P > 1) v[k] += fine[m][j][at];
+                    }
+                    if (c < a.c_out) base[m][h][i].add_and_store(a.out, static_cast<size_t>(rows[m][h]) * a.c_out + c, v, factor);
+                }
+            }
+    }
+    cluster_wait();
+}
+
+bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <int DT, int RB, int MT, bool BACK>
+cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
+    constexpr int ROWS = 16 * MT, H = DT == MTC_F32 ? 3 : 2;
+    const int blocks = (a.rank + RB - 1) / RB;
+    const size_t smem = static_cast<size_t>(kWarps * ROWS * part_stride(RB) + ROWS * blocks * RB) * 4 + static_cast<size_t>(H * ROWS * held_stride(blocks, RB)) * 2;
+    static PerDeviceAttr attr;
+    cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK>, 200 * 1024);
+    if (e != cudaSuccess) return e;
+    // at most as many tiles as rows, and one of fewer rows for each adapter
+    const long long tiles = std::min<long long>(a.n_rows, a.n_rows / ROWS + a.n_adapters + 1ll);
+    if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * kCluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = kCluster;
+    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, lora_mma_kernel<DT, RB, MT, BACK>, a, blocks, keep, none);
+}
+template <int DT, int MT, bool BACK>
+cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
+    if (a.rank <= 8) return launch<DT, 8, MT, BACK>(st, a, keep, none);
+    if (a.rank <= 16) return launch<DT, 16, MT, BACK>(st, a, keep, none);
+    if (DT == MTC_F32 || a.rank <= 32) return launch<DT, 32, MT, BACK>(st, a, keep, none);
+    return launch<DT, DT == MTC_F32 ? 32 : 64, MT, BACK>(st, a, keep, none);
+}
+template <int DT>
+cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
+    const bool wide = a.n_rows > 32 * a.n_adapters && a.rank <= 64;
+    if (wide) return backward ? launch<DT, 2, true>(st, a, keep, none) : launch<DT, 2, false>(st, a, keep, none);
+    return backward ? launch<DT, 1, true>(st, a, keep, none) : launch<DT, 1, false>(st, a, keep, none);
+}
+
+}  // namespace
+
+// Loads of 16 bytes along the rows, of 2, 4 or 8 values along the rank
+bool lora_mma_supported(const LoraArgs &a) {
+    const int step = a.rank <= 8 ? 2 : a.rank <= 16 ? 4 : 8;
+    return a.c_in % 8 == 0 && a.c_out % 8 == 0 && a.rank % step == 0 && a.rank <= 256 && on_16(a.in) && on_16(a.down) && on_16(a.up) && on_16(a.out) &&
+           (!a.base || on_16(a.base));
+}
+cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt) {
+    return (dt == MTC_F32 ? launch<MTC_F32> : dt == MTC_BF16 ? launch<MTC_BF16> : launch<MTC_F16>)(st, a, backward, keep, none);
+}
+
+}  // namespace mtc

@@ -1,0 +1,170 @@
+// What the tensor-core kernels of low-rank adapters share: operands in pieces, fragments, and which rows and columns a lane holds.
+//
+// Operands.  Warp-level MMAs of 16-bit values with f32 sums.  f32 values are three bf16 pieces of 8 bits each, cut off one after the other: 24 bits,
+// exact; products of pieces that together lie below 2^-24 of the whole are left out (six of nine remain).  bf16 and f16 weights and activations are operands as they
+// are.  What lies between the two products, h or u, is an f32 sum: as an operand it is held in two pieces (16 bits and more), in three beside f32 weights.
+//
+// Order of k.  A sum may run over k in any order as long as both operands have the same, so a lane takes what lies next to each other in memory: of
+// 32 neighbours lane (g, t) = (lane / 4, lane % 4) has 8t .. 8t + 7, the first four of them in the first of two MMAs.  Where the other operand lies across (k along
+// its rows), the lane loads eight such rows and pairs them up.
+#pragma once
+
+#include "lora.cuh"
+
+namespace mtc {
+namespace lora {
+
+template <int DT>
+constexpr int pieces = DT == MTC_F32 ? 3 : 1;    // of weights and activations
+
+__device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x7632); }
+__device__ __forceinline__ uint32_t low_halves(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x5410); }
+
+// W neighbouring values as operand pieces: pairs of 16-bit values (one value: the low half)
+template <int DT, int W>
+struct Vals {
+    static constexpr int P = pieces<DT>, N = (W + 1) / 2;
+    uint32_t w[P][N];
+
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[p][i] = 0;
+    }
+    // aligned to W values
+    __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
+        zero();
+        if (!there) return;
+        if constexpr (DT != MTC_F32) {
+            const uint16_t *const p = static_cast<const uint16_t *>(base) + at;
+            if constexpr (W == 8) {
+                const uint4 q = *reinterpret_cast<const uint4 *>(p);
+                w[0][0] = q.x, w[0][1] = q.y, w[0][2] = q.z, w[0][3] = q.w;
+            } else if constexpr (W == 4) {
+                const uint2 q = *reinterpret_cast<const uint2 *>(p);
+                w[0][0] = q.x, w[0][1] = q.y;
+            } else if constexpr (W == 2) {
+                w[0][0] = *reinterpret_cast<const uint32_t *>(p);
+            } else {
+                w[0][0] = *p;
+            }
+        } else {
+            const float *const p = static_cast<const float *>(base) + at;
+            float v[W];
+            if constexpr (W >= 4) {
+#pragma unroll
+                for (int i = 0; i < W / 4; ++i) {
+                    const float4 q = reinterpret_cast<const float4 *>(p)[i];
+                    v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
+                }
+            } else if constexpr (W == 2) {
+                const float2 q = *reinterpret_cast<const float2 *>(p);
+                v[0] = q.x, v[1] = q.y;
+            } else {
+                v[0] = *p;
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float lo = v[2 * i], hi = W == 1 ? 0.0f : v[W == 1 ? 0 : 2 * i + 1];
+                    w[k][i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
+            }
+        }
+    }
+    // value j of x with value j of y, as a pair
+    static __device__ __forceinline__ uint32_t pair(const Vals &x, const Vals &y, int p, int j) {
+        return j & 1 ? high_halves(x.w[p][j / 2], y.w[p][j / 2]) : low_halves(x.w[p][j / 2], y.w[p][j / 2]);
+    }
+};
+
+// d += a b: 16 x 16 values of a, 16 x 8 of b
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (HALF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Eight results next to each other: + base, rounded, out
+template <int DT>
+struct Eight {
+    uint32_t w[DT == MTC_F32 ? 8 : 4];
+    __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
+        constexpr int W = DT == MTC_F32 ? 8 : 4;
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0;
+        if (!there) return;
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(base) + at * (DT == MTC_F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const uint4 q = p[i];
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+        }
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (DT == MTC_F32) return __uint_as_float(w[i]);
+        const uint32_t u = w[i / 2];
+        if constexpr (DT == MTC_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? u >> 16 : u)));
+    }
+    __device__ __forceinline__ void add_and_store(void *out, size_t at, const float (&v)[8], float factor) const {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = fmaf(v[i], factor, value(i));
+        put(out, at, r);
+    }
+    static __device__ __forceinline__ void put(void *out, size_t at, const float (&r)[8]) {
+        if constexpr (DT == MTC_F32) {
+            float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
+            p[0] = make_float4(r[0], r[1], r[2], r[3]);
+            p[1] = make_float4(r[4], r[5], r[6], r[7]);
+        } else {
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DT == MTC_BF16) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(r[2 * i], r[2 * i + 1]);
+                    u[i] = *reinterpret_cast<const uint32_t *>(&h);
+                } else {
+                    const __half2 h = __floats2half2_rn(r[2 * i], r[2 * i + 1]);
+                    u[i] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+            }
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+};
+
+// Clusters
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 ld_cta(const float *p, uint32_t rank) {
+    uint32_t at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+}  // namespace lora
+}  // namespace mtc

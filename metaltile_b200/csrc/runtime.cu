@@ -1730,7 +1730,7 @@ int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const 
         l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
         l.low = static_cast<float *>(hidden ? hidden : workspace);
         l.n_rows = n_rows, l.c_in = K, l.c_out = N, l.rank = rank, l.n_adapters = n_adapters, l.status = ctx->d_status;
-        MTC_CUDA(ctx, mtc::launch_lora(ctx, static_cast<cudaStream_t>(stream), l, false, hidden != nullptr, dtype), MTC_ERR_DISPATCH);
+        MTC_CUDA(ctx, mtc::launch_lora(ctx, static_cast<cudaStream_t>(stream), l, false, hidden != nullptr, hidden != nullptr, dtype), MTC_ERR_DISPATCH);
         return MTC_OK;
     });
 }
@@ -1751,7 +1751,7 @@ int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, con
         l.in = dy, l.down = b, l.up = a, l.base = base, l.out = dx, l.low = u;
         l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
         l.n_rows = n_rows, l.c_in = N, l.c_out = K, l.rank = rank, l.n_adapters = n_adapters, l.status = ctx->d_status;
-        if (n_rows > 0) MTC_CUDA(ctx, mtc::launch_lora(ctx, st, l, true, false, dtype), MTC_ERR_DISPATCH);
+        if (n_rows > 0) MTC_CUDA(ctx, mtc::launch_lora(ctx, st, l, true, true, false, dtype), MTC_ERR_DISPATCH);
         mtc::LoraWeights w{};
         w.a = {x, u, da, K}, w.b = {dy, static_cast<const float *>(hidden), db, N};
         w.order = l.order, w.offsets = l.offsets, w.scales = l.scales, w.n_rows = n_rows, w.rank = rank, w.n_adapters = n_adapters, w.status = ctx->d_status;
