@@ -17,28 +17,26 @@ using namespace lora;
 constexpr int kWarps = 8, kThreads = 32 * kWarps, kCluster = 8;
 
 __host__ __device__ constexpr int part_stride(int rb) { return rb + 4; }
-__host__ __device__ constexpr int held_stride(int blocks, int rb) { return blocks * rb + 8; }      // in 16-bit values: rows 16 bytes apart modulo 128
+__host__ __device__ constexpr int held_stride(int rt) { return rt + 8; }         // in 16-bit values: rows 16 bytes apart modulo 128
 
 struct Tile {
     int e;                                       // n_adapters: rows of none; -1: no such tile
     uint32_t p0, n;
 };
 
-// The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By the whole CTA.
-__device__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none, long long *scratch) {
-    __shared__ Tile found;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) found = {-1, 0, 0};
+// The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By every warp for itself.
+__device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none) {
+    const int lane = threadIdx.x & 31, last = none ? a.n_adapters : a.n_adapters - 1;
     const uint32_t R = a.n_rows;
     long long before = 0;                        // offsets that run backwards may name more tiles than 32 bits hold
-    for (int e0 = 0; e0 <= a.n_adapters; e0 += kThreads) {
-        const int e = e0 + threadIdx.x;
-        uint32_t from = 0, n = 0;
-        if (e < a.n_adapters || (none && e == a.n_adapters)) {
+    for (int e0 = 0; e0 <= last; e0 += 32) {
+        const int e = e0 + lane;
+        uint32_t from = 0, to = 0;
+        if (e <= last) {
             from = min(a.offsets[e], R);
-            const uint32_t to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
-            n = to > from ? to - from : 0;
+            to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
         }
+        const uint32_t n = to > from ? to - from : 0;
         const long long mine = (static_cast<long long>(n) + rows - 1) / rows;
         long long upto = mine;
 #pragma unroll
@@ -46,48 +44,88 @@ __device__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none, long l
             const long long v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        __syncthreads();                         // scratch of the turn before is read
-        if (lane == 31) scratch[warp] = upto;
-        __syncthreads();
-        long long total = 0, base = before;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) base += scratch[w];
-            total += scratch[w];
-        }
-        const long long first = base + upto - mine;
-        if (id >= first && id < first + mine) {
+        const long long first = before + upto - mine;
+        const uint32_t hit = __ballot_sync(0xffffffffu, id >= first && id < first + mine);
+        if (hit) {
             const uint32_t skip = static_cast<uint32_t>(id - first) * rows;
-            found = {e, from + skip, min(n - skip, static_cast<uint32_t>(rows))};
+            const int src = __ffs(hit) - 1;
+            return {e0 + src, __shfl_sync(0xffffffffu, from + skip, src), __shfl_sync(0xffffffffu, min(n - skip, static_cast<uint32_t>(rows)), src)};
         }
-        before += total;
-        if (id < before) break;
+        before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
-    return found;
+    return {-1, 0, 0};
 }
 
-// RB: ranks a pass (a block of the rank), 8 to 64.  MT: tiles of 16 rows.  BACK: the first product's weights lie [c_in][rank], the second's [rank][c_out];
-// else [rank][c_in] and [c_out][rank].
-template <int DT, int RB, int MT, bool BACK>
-__global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, int rank_blocks, bool keep, bool none) {
+__device__ __forceinline__ void prefetch(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// `bytes` from `from` on of each of `rows` rows, a row `pitch` bytes; row_of: which rows (null: the first ones; negative: none)
+__device__ __forceinline__ void prefetch_rows(const void *base, size_t from, size_t pitch, int bytes, int rows, const int *row_of) {
+    const int lines = (bytes + 127) / 128;
+    for (int i = threadIdx.x; i < rows * lines; i += kThreads) {
+        const int row = row_of ? row_of[i / lines] : i / lines;
+        if (row >= 0) prefetch(static_cast<const char *>(base) + row * pitch + from + i % lines * 128);
+    }
+}
+
+// f16: the power of two at or below a row's largest value, within what f32 can divide by (infinities and NaN: 1)
+__device__ __forceinline__ float unit_of(float most) {
+    const int e = static_cast<int>(__float_as_uint(most) >> 23);
+    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(e, 27), 253)) << 23);
+}
+// Four neighbours as operand pieces, each `apart` values behind the other.  f16: divided by `unit`, since it has five bits of exponent.
+template <int DT>
+__device__ __forceinline__ void hold(float4 s, float unit, uint16_t *at, int apart) {
+    constexpr int H = DT == MTC_F32 ? 3 : 2;
+    float v[4] = {s.x, s.y, s.z, s.w};
+    if constexpr (DT == MTC_F16) {
+        const float inv = 1.0f / unit;           // exact
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= inv;
+    }
+#pragma unroll
+    for (int p = 0; p < H; ++p) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float &x = v[2 * i], &y = v[2 * i + 1];
+            if constexpr (DT == MTC_F16) {
+                const __half2 h = __floats2half2_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                const float2 f = __half22float2(h);
+                x = fabsf(x) < INFINITY ? x - f.x : 0.0f, y = fabsf(y) < INFINITY ? y - f.y : 0.0f;
+            } else if (p + 1 < H) {
+                const uint32_t b = __float_as_uint(x), c = __float_as_uint(y);
+                w[i] = high_halves(b, c);
+                x = fabsf(x) < INFINITY ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f, y = fabsf(y) < INFINITY ? y - __uint_as_float(c & 0xFFFF0000u) : 0.0f;
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        *reinterpret_cast<uint2 *>(at + p * apart) = make_uint2(w[0], w[1]);
+    }
+}
+
+// RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  BACK: the first product's weights lie [c_in][rank], the second's
+// [rank][c_out]; else [rank][c_in] and [c_out][rank].
+template <int DT, int RB, int MT, bool BACK, bool ONE>
+__global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int rank_blocks_, bool keep, bool none) {
     pdl_enter();
-    constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8;
+    constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8, SIZE = DT == MTC_F32 ? 4 : 2;
     constexpr bool HALF = DT == MTC_F16;
     extern __shared__ __align__(16) float sm[];
-    const int RT = rank_blocks * RB, HS = held_stride(rank_blocks, RB);
+    const int rank_blocks = ONE ? 1 : rank_blocks_, RT = rank_blocks * RB, HS = held_stride(RT);
     float *const part = sm;                                                      // [warps][ROWS][PS]
-    float *const low = part + kWarps * ROWS * PS;                                // [ROWS][RT]
-    uint16_t *const held = reinterpret_cast<uint16_t *>(low + ROWS * RT);        // [H][ROWS][HS]
+    uint16_t *const held = reinterpret_cast<uint16_t *>(part + kWarps * ROWS * PS);      // [H][ROWS][HS]
+    float *const low = reinterpret_cast<float *>(held + H * ROWS * HS);          // [ROWS][RT], not ONE only
     __shared__ int row_of[ROWS];
     __shared__ float back_up[ROWS];              // f16: the power of two that a row's h was divided by
-    __shared__ long long scratch[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int cs = cluster_size(), cr = cluster_rank();
+    constexpr int cs = kCluster;
+    const int cr = cluster_rank();
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e < a.n_adapters; e += kThreads)
             if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
-    const Tile tile = find_tile(a, blockIdx.x / cs, ROWS, none, scratch);
+    const Tile tile = find_tile(a, blockIdx.x / cs, ROWS, none);
     if (tile.e < 0) return;                      // the whole cluster
     if (threadIdx.x < ROWS) {
         int row = -1;
@@ -100,6 +138,7 @@ __global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, in
     }
     constexpr int CW = BACK ? 64 : 32;           // columns of a warp's step
     const int units = (a.c_out + CW - 1) / CW, unit0 = static_cast<int>(static_cast<long long>(units) * cr / cs), unit1 = static_cast<int>(static_cast<long long>(units) * (cr + 1) / cs);
+    const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
     __syncthreads();
     if (tile.e == a.n_adapters) {                // rows of no adapter: base, or zeros
         if (a.base != a.out) {
@@ -120,12 +159,27 @@ __global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, in
         return;
     }
     const size_t expert = tile.e;
+    {   // everything that this CTA will read is on its way before it waits for any of it
+        const int k0 = static_cast<int>(static_cast<long long>(chunks) * cr / cs) * 32, k1 = min(static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / cs) * 32, a.c_in);
+        const int n0 = unit0 * CW, n1 = min(unit1 * CW, a.c_out);
+        const size_t in_row = static_cast<size_t>(a.c_in) * SIZE, out_row = static_cast<size_t>(a.c_out) * SIZE, rank_row = static_cast<size_t>(a.rank) * SIZE;
+        const char *const down = static_cast<const char *>(a.down) + expert * a.rank * in_row, *const up = static_cast<const char *>(a.up) + expert * a.rank * out_row;
+        if (k1 > k0) {
+            prefetch_rows(a.in, static_cast<size_t>(k0) * SIZE, in_row, (k1 - k0) * SIZE, ROWS, row_of);
+            if (BACK) prefetch_rows(down, k0 * rank_row, 0, static_cast<int>((k1 - k0) * rank_row), 1, nullptr);
+            else prefetch_rows(down, static_cast<size_t>(k0) * SIZE, in_row, (k1 - k0) * SIZE, a.rank, nullptr);
+        }
+        if (n1 > n0) {
+            if (BACK) prefetch_rows(up, static_cast<size_t>(n0) * SIZE, out_row, (n1 - n0) * SIZE, a.rank, nullptr);
+            else prefetch_rows(up, n0 * rank_row, 0, static_cast<int>((n1 - n0) * rank_row), 1, nullptr);
+            if (a.base) prefetch_rows(a.base, static_cast<size_t>(n0) * SIZE, out_row, (n1 - n0) * SIZE, ROWS, row_of);
+        }
+    }
 
     // ---- the first product: this warp's part of c_in, 32 values at a time
     int rows[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) rows[m][0] = row_of[16 * m + g], rows[m][1] = row_of[16 * m + g + 8];
-    const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
     const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * me / workers), chunk1 = static_cast<int>(static_cast<long long>(chunks) * (me + 1) / workers);
     for (int rb = 0; rb < rank_blocks; ++rb) {
         float acc[MT][NT][4] = {};
@@ -201,55 +255,55 @@ __global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, in
         }
         cluster_arrive();
         cluster_wait();
-        for (int i = threadIdx.x; i < ROWS * RB / 4; i += kThreads) {
-            const int row = i / (RB / 4), col = i % (RB / 4) * 4;
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int q = 0; q < cs; ++q) {
-                const float4 v = ld_cta(part + row * PS + col, q);
-                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        for (int i0 = 0; i0 < ROWS * RB / 4; i0 += kThreads) {
+            const int i = i0 + threadIdx.x, row = i / (RB / 4), col = i % (RB / 4) * 4;
+            const bool mine = ROWS * RB / 4 % kThreads == 0 || i < ROWS * RB / 4;
+            float4 v[cs], s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (mine) {
+#pragma unroll
+                for (int q = 0; q < cs; ++q) v[q] = ld_cta(part + row * PS + col, q);
+#pragma unroll
+                for (int q = 0; q < cs; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+                if (keep && i % cs == cr) {      // the CTAs of the cluster share the writing
+                    const int r = row_of[row], at = rb * RB + col;
+                    if (r >= 0) {
+                        float *const p = a.low + static_cast<size_t>(r) * a.rank + at;
+                        if (at < a.rank) p[0] = s.x;
+                        if (at + 1 < a.rank) p[1] = s.y;
+                        if (at + 2 < a.rank) p[2] = s.z;
+                        if (at + 3 < a.rank) p[3] = s.w;
+                    }
+                }
             }
-            *reinterpret_cast<float4 *>(low + row * RT + rb * RB + col) = s;
+            if constexpr (ONE) {
+                float f = 1.0f;
+                if constexpr (HALF) {            // RB / 4 lanes have a row
+                    float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
+#pragma unroll
+                    for (int o = RB / 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    f = unit_of(most);
+                    if (mine && col == 0) back_up[row] = f;
+                }
+                if (mine) hold<DT>(s, f, held + row * HS + col, ROWS * HS);
+            } else if (mine) {
+                *reinterpret_cast<float4 *>(low + row * RT + rb * RB + col) = s;
+            }
         }
     }
     cluster_arrive();                            // nobody leaves while its part is read: waited for at the end
-    __syncthreads();
-    if (keep)
-        for (int i = threadIdx.x + cr * kThreads; i < ROWS * a.rank; i += kThreads * cs) {
-            const int row = row_of[i / a.rank];
-            if (row >= 0) a.low[static_cast<size_t>(row) * a.rank + i % a.rank] = low[i / a.rank * RT + i % a.rank];
-        }
-
-    // ---- h as an operand
-    if constexpr (HALF) {                        // rows are divided by the power of two of their largest value: f16 has five bits of exponent
-        for (int row = warp; row < ROWS; row += kWarps) {
-            float most = 0.0f;
-            for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(low[row * RT + i]));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const int bits = static_cast<int>(__float_as_uint(most) >> 23);
-            if (lane == 0) back_up[row] = bits == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(bits, 27), 253)) << 23);
-        }
+    if constexpr (!ONE) {
         __syncthreads();
-    }
-    for (int i = threadIdx.x; i < ROWS * RT; i += kThreads) {
-        const int row = i / RT, col = i % RT;
-        float v = low[i];
-        if constexpr (HALF) v *= 1.0f / back_up[row];            // a power of two: exact
-        const bool finite = fabsf(v) < INFINITY;
-#pragma unroll
-        for (int p = 0; p < H; ++p) {
-            uint16_t *const at = held + (p * ROWS + row) * HS + col;
+        for (int row = warp; row < ROWS; row += kWarps) {
+            float f = 1.0f;
             if constexpr (HALF) {
-                const __half h = __float2half_rn(v);
-                *at = __half_as_ushort(h);
-                v = finite ? v - __half2float(h) : 0.0f;
-            } else if (p + 1 < H) {
-                const uint32_t b = __float_as_uint(v);
-                *at = static_cast<uint16_t>(b >> 16);
-                v = finite ? v - __uint_as_float(b & 0xFFFF0000u) : 0.0f;
-            } else {
-                *at = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+                float most = 0.0f;
+                for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(low[row * RT + i]));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                f = unit_of(most);
+                if (lane == 0) back_up[row] = f;
             }
+            for (int i = lane * 4; i < RT; i += 128) hold<DT>(*reinterpret_cast<const float4 *>(low + row * RT + i), f, held + row * HS + i, ROWS * HS);
         }
     }
     __syncthreads();
@@ -361,13 +415,13 @@ __global__ void __launch_bounds__(kThreads) lora_mma_kernel(const LoraArgs a, in
 
 bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <int DT, int RB, int MT, bool BACK>
+template <int DT, int RB, int MT, bool BACK, bool ONE>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int ROWS = 16 * MT, H = DT == MTC_F32 ? 3 : 2;
     const int blocks = (a.rank + RB - 1) / RB;
-    const size_t smem = static_cast<size_t>(kWarps * ROWS * part_stride(RB) + ROWS * blocks * RB) * 4 + static_cast<size_t>(H * ROWS * held_stride(blocks, RB)) * 2;
+    const size_t smem = static_cast<size_t>(kWarps * ROWS * part_stride(RB) + (ONE ? 0 : ROWS * blocks * RB)) * 4 + static_cast<size_t>(H * ROWS * held_stride(blocks * RB)) * 2;
     static PerDeviceAttr attr;
-    cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK>, 200 * 1024);
+    cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK, ONE>, 200 * 1024);
     if (e != cudaSuccess) return e;
     // at most as many tiles as rows, and one of fewer rows for each adapter
     const long long tiles = std::min<long long>(a.n_rows, a.n_rows / ROWS + a.n_adapters + 1ll);
@@ -385,18 +439,20 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
     cfg.attrs = la;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, lora_mma_kernel<DT, RB, MT, BACK>, a, blocks, keep, none);
+    return cudaLaunchKernelEx(&cfg, lora_mma_kernel<DT, RB, MT, BACK, ONE>, a, blocks, keep, none);
 }
 template <int DT, int MT, bool BACK>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
-    if (a.rank <= 8) return launch<DT, 8, MT, BACK>(st, a, keep, none);
-    if (a.rank <= 16) return launch<DT, 16, MT, BACK>(st, a, keep, none);
-    if (DT == MTC_F32 || a.rank <= 32) return launch<DT, 32, MT, BACK>(st, a, keep, none);
-    return launch<DT, DT == MTC_F32 ? 32 : 64, MT, BACK>(st, a, keep, none);
+    constexpr int MOST = DT == MTC_F32 ? 32 : 64;
+    if (a.rank <= 8) return launch<DT, 8, MT, BACK, true>(st, a, keep, none);
+    if (a.rank <= 16) return launch<DT, 16, MT, BACK, true>(st, a, keep, none);
+    if (a.rank <= 32) return launch<DT, 32, MT, BACK, true>(st, a, keep, none);
+    if (a.rank <= MOST) return launch<DT, MOST, MT, BACK, true>(st, a, keep, none);
+    return launch<DT, MOST, 1, BACK, false>(st, a, keep, none);
 }
 template <int DT>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
-    const bool wide = a.n_rows > 32 * a.n_adapters && a.rank <= 64;
+    const bool wide = a.n_rows > 32 * a.n_adapters;
     if (wide) return backward ? launch<DT, 2, true>(st, a, keep, none) : launch<DT, 2, false>(st, a, keep, none);
     return backward ? launch<DT, 1, true>(st, a, keep, none) : launch<DT, 1, false>(st, a, keep, none);
 }
