@@ -122,7 +122,11 @@ cudaError_t launch_weights_any(cudaStream_t st, const LoraWeights &w) {
 }  // namespace
 
 cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt) {
-    if (lora_mma_supported(a)) return launch_lora_mma(st, a, backward, keep, (keep && all) || a.base != a.out, dt);
+    if (lora_mma_supported(a)) {
+        const bool none = (keep && all) || a.base != a.out;
+        if (lora_tile_supported(a, keep, dt) && a.n_rows >= 1024 && a.n_rows >= 48ll * a.n_adapters) return launch_lora_tile(st, a, backward, keep, none, dt);
+        return launch_lora_mma(st, a, backward, keep, none, dt);
+    }
     return (dt == MTC_F32 ? launch_any<MTC_F32> : dt == MTC_BF16 ? launch_any<MTC_BF16> : launch_any<MTC_F16>)(st, a, backward, keep && all);
 }
 cudaError_t launch_lora_weights(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt) {

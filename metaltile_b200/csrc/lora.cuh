@@ -44,6 +44,8 @@ cudaError_t launch_lora_weights(Ctx *ctx, cudaStream_t st, const LoraWeights &w,
 // The tensor-core kernels (lora_mma.cu, lora_grad.cu) and what they take; `none`: rows of no adapter have something to be written
 bool lora_mma_supported(const LoraArgs &a);
 cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
+bool lora_tile_supported(const LoraArgs &a, bool keep, int dt);       // (lora_tcgen05.cu) what of the above it takes
+cudaError_t launch_lora_tile(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
 bool lora_grad_supported(const LoraWeights &w);
 cudaError_t launch_lora_grad(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);
 

@@ -208,20 +208,8 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {
     static PerDeviceAttr attr;
     const cudaError_t e = attr.set(lora_weights_kernel<DT, RB>, F::smem);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(items * cs));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = F::smem;
-    cfg.stream = st;
-    cudaLaunchAttribute la[2];
-    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    la[0].val.programmaticStreamSerializationAllowed = 1;
-    la[1].id = cudaLaunchAttributeClusterDimension;
-    la[1].val.clusterDim.x = cs;
-    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
-    cfg.attrs = la;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, lora_weights_kernel<DT, RB>, w, static_cast<int>(blocks_a), static_cast<int>(blocks_b), static_cast<int>(rank_blocks));
+    return launch_cluster(lora_weights_kernel<DT, RB>, static_cast<unsigned>(items * cs), kThreads, cs, F::smem, st, w, static_cast<int>(blocks_a), static_cast<int>(blocks_b),
+                          static_cast<int>(rank_blocks));
 }
 template <int DT>
 cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {

@@ -19,43 +19,6 @@ constexpr int kWarps = 8, kThreads = 32 * kWarps, kCluster = 8;
 __host__ __device__ constexpr int part_stride(int rb) { return rb + 4; }
 __host__ __device__ constexpr int held_stride(int rt) { return rt + 8; }         // in 16-bit values: rows 16 bytes apart modulo 128
 
-struct Tile {
-    int e;                                       // n_adapters: rows of none; -1: no such tile
-    uint32_t p0, n;
-};
-
-// The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By every warp for itself.
-__device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none) {
-    const int lane = threadIdx.x & 31, last = none ? a.n_adapters : a.n_adapters - 1;
-    const uint32_t R = a.n_rows;
-    long long before = 0;                        // offsets that run backwards may name more tiles than 32 bits hold
-    for (int e0 = 0; e0 <= last; e0 += 32) {
-        const int e = e0 + lane;
-        uint32_t from = 0, to = 0;
-        if (e <= last) {
-            from = min(a.offsets[e], R);
-            to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
-        }
-        const uint32_t n = to > from ? to - from : 0;
-        const long long mine = (static_cast<long long>(n) + rows - 1) / rows;
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const long long first = before + upto - mine;
-        const uint32_t hit = __ballot_sync(0xffffffffu, id >= first && id < first + mine);
-        if (hit) {
-            const uint32_t skip = static_cast<uint32_t>(id - first) * rows;
-            const int src = __ffs(hit) - 1;
-            return {e0 + src, __shfl_sync(0xffffffffu, from + skip, src), __shfl_sync(0xffffffffu, min(n - skip, static_cast<uint32_t>(rows)), src)};
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return {-1, 0, 0};
-}
-
 __device__ __forceinline__ void prefetch(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // `bytes` from `from` on of each of `rows` rows, a row `pitch` bytes; row_of: which rows (null: the first ones; negative: none)
 __device__ __forceinline__ void prefetch_rows(const void *base, size_t from, size_t pitch, int bytes, int rows, const int *row_of) {
@@ -63,45 +26,6 @@ __device__ __forceinline__ void prefetch_rows(const void *base, size_t from, siz
     for (int i = threadIdx.x; i < rows * lines; i += kThreads) {
         const int row = row_of ? row_of[i / lines] : i / lines;
         if (row >= 0) prefetch(static_cast<const char *>(base) + row * pitch + from + i % lines * 128);
-    }
-}
-
-// f16: the power of two at or below a row's largest value, within what f32 can divide by (infinities and NaN: 1)
-__device__ __forceinline__ float unit_of(float most) {
-    const int e = static_cast<int>(__float_as_uint(most) >> 23);
-    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(e, 27), 253)) << 23);
-}
-// Four neighbours as operand pieces, each `apart` values behind the other.  f16: divided by `unit`, since it has five bits of exponent.
-template <int DT>
-__device__ __forceinline__ void hold(float4 s, float unit, uint16_t *at, int apart) {
-    constexpr int H = DT == MTC_F32 ? 3 : 2;
-    float v[4] = {s.x, s.y, s.z, s.w};
-    if constexpr (DT == MTC_F16) {
-        const float inv = 1.0f / unit;           // exact
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= inv;
-    }
-#pragma unroll
-    for (int p = 0; p < H; ++p) {
-        uint32_t w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float &x = v[2 * i], &y = v[2 * i + 1];
-            if constexpr (DT == MTC_F16) {
-                const __half2 h = __floats2half2_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-                const float2 f = __half22float2(h);
-                x = fabsf(x) < INFINITY ? x - f.x : 0.0f, y = fabsf(y) < INFINITY ? y - f.y : 0.0f;
-            } else if (p + 1 < H) {
-                const uint32_t b = __float_as_uint(x), c = __float_as_uint(y);
-                w[i] = high_halves(b, c);
-                x = fabsf(x) < INFINITY ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f, y = fabsf(y) < INFINITY ? y - __uint_as_float(c & 0xFFFF0000u) : 0.0f;
-            } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-        }
-        *reinterpret_cast<uint2 *>(at + p * apart) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -141,21 +65,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
     const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
     __syncthreads();
     if (tile.e == a.n_adapters) {                // rows of no adapter: base, or zeros
-        if (a.base != a.out) {
-            const int from = unit0 * CW, wide = min(unit1 * CW, a.c_out) - from;
-            for (int i = threadIdx.x; i < static_cast<int>(tile.n) * (wide / 8); i += kThreads) {
-                const int row = row_of[i / (wide / 8)], c = from + i % (wide / 8) * 8;
-                if (row < 0) continue;
-                const size_t at = static_cast<size_t>(row) * a.c_out + c;
-                lora::Eight<DT> v;
-                v.load(a.base, at, a.base != nullptr);
-                const float zero[8] = {};
-                v.add_and_store(a.out, at, zero, 1.0f);
-            }
-        }
-        if (keep)
-            for (int i = threadIdx.x + cr * kThreads; i < static_cast<int>(tile.n) * a.rank; i += kThreads * cs)
-                if (row_of[i / a.rank] >= 0) a.low[static_cast<size_t>(row_of[i / a.rank]) * a.rank + i % a.rank] = 0.0f;
+        copy_rows<DT, kThreads>(a, row_of, static_cast<int>(tile.n), unit0 * CW, min(unit1 * CW, a.c_out), keep, cr, cs);
         return;
     }
     const size_t expert = tile.e;
@@ -426,20 +336,7 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     // at most as many tiles as rows, and one of fewer rows for each adapter
     const long long tiles = std::min<long long>(a.n_rows, a.n_rows / ROWS + a.n_adapters + 1ll);
     if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * kCluster));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute la[2];
-    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    la[0].val.programmaticStreamSerializationAllowed = 1;
-    la[1].id = cudaLaunchAttributeClusterDimension;
-    la[1].val.clusterDim.x = kCluster;
-    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
-    cfg.attrs = la;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, lora_mma_kernel<DT, RB, MT, BACK, ONE>, a, blocks, keep, none);
+    return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, smem, st, a, blocks, keep, none);
 }
 template <int DT, int MT, bool BACK>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {

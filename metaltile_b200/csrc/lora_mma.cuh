@@ -145,6 +145,111 @@ struct Eight {
     }
 };
 
+struct Tile {
+    int e;                                       // n_adapters: rows of none; -1: no such tile
+    uint32_t p0, n;
+};
+
+// The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By every warp for itself.
+__device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none) {
+    const int lane = threadIdx.x & 31, last = none ? a.n_adapters : a.n_adapters - 1;
+    const uint32_t R = a.n_rows;
+    long long before = 0;                        // offsets that run backwards may name more tiles than 32 bits hold
+    for (int e0 = 0; e0 <= last; e0 += 32) {
+        const int e = e0 + lane;
+        uint32_t from = 0, to = 0;
+        if (e <= last) {
+            from = min(a.offsets[e], R);
+            to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
+        }
+        const uint32_t n = to > from ? to - from : 0;
+        const long long mine = (static_cast<long long>(n) + rows - 1) / rows;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const long long first = before + upto - mine;
+        const uint32_t hit = __ballot_sync(0xffffffffu, id >= first && id < first + mine);
+        if (hit) {
+            const uint32_t skip = static_cast<uint32_t>(id - first) * rows;
+            const int src = __ffs(hit) - 1;
+            return {e0 + src, __shfl_sync(0xffffffffu, from + skip, src), __shfl_sync(0xffffffffu, min(n - skip, static_cast<uint32_t>(rows)), src)};
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return {-1, 0, 0};
+}
+
+// f16: the power of two at or below a row's largest value, within what f32 can divide by (infinities and NaN: 1)
+__device__ __forceinline__ float unit_of(float most) {
+    const int e = static_cast<int>(__float_as_uint(most) >> 23);
+    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(e, 27), 253)) << 23);
+}
+// Four neighbours as operand pieces.  f16: divided by `unit`, since it has five bits of exponent.
+template <int DT>
+__device__ __forceinline__ void hold_pieces(float4 s, float unit, uint2 *piece) {
+    constexpr int H = DT == MTC_F32 ? 3 : 2;
+    float v[4] = {s.x, s.y, s.z, s.w};
+    if constexpr (DT == MTC_F16) {
+        const float inv = 1.0f / unit;           // exact
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= inv;
+    }
+#pragma unroll
+    for (int p = 0; p < H; ++p) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float &x = v[2 * i], &y = v[2 * i + 1];
+            if constexpr (DT == MTC_F16) {
+                const __half2 h = __floats2half2_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                const float2 f = __half22float2(h);
+                x = fabsf(x) < INFINITY ? x - f.x : 0.0f, y = fabsf(y) < INFINITY ? y - f.y : 0.0f;
+            } else if (p + 1 < H) {
+                const uint32_t b = __float_as_uint(x), c = __float_as_uint(y);
+                w[i] = high_halves(b, c);
+                x = fabsf(x) < INFINITY ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f, y = fabsf(y) < INFINITY ? y - __uint_as_float(c & 0xFFFF0000u) : 0.0f;
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+        piece[p] = make_uint2(w[0], w[1]);
+    }
+}
+// ... each `apart` values behind the other
+template <int DT>
+__device__ __forceinline__ void hold(float4 s, float unit, uint16_t *at, int apart) {
+    constexpr int H = DT == MTC_F32 ? 3 : 2;
+    uint2 w[H];
+    hold_pieces<DT>(s, unit, w);
+#pragma unroll
+    for (int p = 0; p < H; ++p) *reinterpret_cast<uint2 *>(at + p * apart) = w[p];
+}
+
+// Rows of no adapter, by the CTAs of a cluster: columns from .. to of this one; zeros of `low` where it is kept
+template <int DT, int THREADS>
+__device__ __forceinline__ void copy_rows(const LoraArgs &a, const int *row_of, int n, int from, int to, bool keep, int cr, int cs) {
+    if (a.base != a.out) {
+        const int eights = max(to - from, 0) / 8;
+        for (int i = threadIdx.x; i < n * eights; i += THREADS) {
+            const int row = row_of[i / eights], c = from + i % eights * 8;
+            if (row < 0) continue;
+            const size_t at = static_cast<size_t>(row) * a.c_out + c;
+            Eight<DT> v;
+            v.load(a.base, at, a.base != nullptr);
+            const float zero[8] = {};
+            v.add_and_store(a.out, at, zero, 1.0f);
+        }
+    }
+    if (keep)
+        for (int i = threadIdx.x + cr * THREADS; i < n * a.rank; i += THREADS * cs)
+            if (row_of[i / a.rank] >= 0) a.low[static_cast<size_t>(row_of[i / a.rank]) * a.rank + i % a.rank] = 0.0f;
+}
+
 // Clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -164,6 +269,24 @@ __device__ __forceinline__ float4 ld_cta(const float *p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
+}
+
+template <typename... P, typename... A>
+cudaError_t launch_cluster(void (*kern)(P...), unsigned ctas, int threads, int cluster, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = cluster;
+    la[1].val.clusterDim.y = la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
 }  // namespace lora
