@@ -8,8 +8,11 @@
 //
 // h is held in two pieces of T (16 bits and more; f16 divided by the power of two of its row's largest value).
 //
-//   shared memory, 24 KB units: first product a ring of four stages (128 rows x 64 values of x, 64 of the weights of every rank), rows 128 bytes apart with the
-//   128-byte swizzle; then the part of the sums (32 KB), h (32 KB), and three buffers of 64 columns (weights 8 KB, base and results 16 KB), the last one in place of the part
+// The parts meet without a barrier: a CTA stores its sums into the shared memory of the rows' owners as they leave tensor memory (st.async), an owner copies its rows of h
+// into all others' (cp.async.bulk), and the receiving side's mbarriers count the bytes.
+//
+//   shared memory: the first product's ring of stages (128 rows x 64 values of x 16 KB, 64 of the weights of every rank 8 KB; rows 128 bytes apart with the 128-byte
+//   swizzle) and what comes in of the sums; then h (32 KB) and three buffers of 64 columns (weights 8 KB, base and results 16 KB) in their places
 #include <algorithm>
 #include <cstddef>
 
@@ -21,21 +24,28 @@ namespace {
 
 using namespace lora;
 
-constexpr int kThreads = 256, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
-constexpr int kStages = 4, kStage = 24 * 1024, kWeights = 16 * 1024;                 // of a stage: where the weights start
-constexpr int kPart = 0, kHeld = 32 * 1024, kPiece = 16 * 1024, kColumns = 64, kBase = 8 * 1024;      // of a buffer of columns: where base starts
+constexpr int kCopy = 256, kMmaWarp = kCopy / 32, kThreads = kCopy + 32, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
+constexpr int kStage = 24 * 1024, kWeights = 16 * 1024;                              // of a stage: where the weights start
+constexpr int kHeld = 0, kPiece = 16 * 1024, kColumns = 64;
 constexpr int kSmem = 1024 + 112 * 1024;
 constexpr uint32_t kTmem = 256, kSums = 0, kOut = 64;                                // columns of tensor memory
+
+// Ranks 64: the sums of eight CTAs for sixteen rows are 32 KB, a stage less
+template <int RB>
+struct Room {
+    static constexpr int kStages = RB == 64 ? 3 : 4, kFrom = kStages * kStage;       // where the others' sums come in
+    // of a buffer of columns: the last one takes the sums' place
+    static __device__ __forceinline__ int weights(int b) { return RB == 64 ? (b == 0 ? 32 * 1024 : b == 1 ? 104 * 1024 : 72 * 1024) : (32 + 24 * b) * 1024; }
+    static __device__ __forceinline__ int base(int b) { return RB == 64 ? (b == 0 ? 40 * 1024 : b == 1 ? 56 * 1024 : 80 * 1024) : (40 + 24 * b) * 1024; }
+};
 
 struct Ctrl {
     int row_of[kRows];
     uint8_t unit[kRows];                         // f16: exponent of what a row of h was divided by
-    uint64_t full[kStages], empty[kStages], out[2], done;
+    uint64_t full[4], empty[4], columns[3], out[2], free[2], done, sums, held;
     uint32_t tmem, abort;
 };
 static_assert(sizeof(Ctrl) <= 1024, "control block");
-
-__device__ __forceinline__ int buffer_at(int step) { return step % 3 == 0 ? 64 * 1024 : step % 3 == 1 ? 88 * 1024 : 0; }
 
 // 16 bytes, zeros where there is nothing to be read
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
@@ -67,24 +77,30 @@ __device__ __forceinline__ uint32_t on_cta(uint32_t at, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float4 ld_far(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
+// sixteen bytes into another CTA's shared memory, counted by a barrier there
+__device__ __forceinline__ void send16(uint32_t at, const uint32_t *v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void st_far(uint32_t at, uint32_t x, uint32_t y) { asm volatile("st.shared::cluster.v2.u32 [%0], {%1,%2};" ::"r"(at), "r"(x), "r"(y) : "memory"); }
-__device__ __forceinline__ void st_far(uint32_t at, uint8_t v) { asm volatile("st.shared::cluster.u8 [%0], %1;" ::"r"(at), "r"(static_cast<uint32_t>(v)) : "memory"); }
+__device__ __forceinline__ void send_bulk(uint32_t at, uint32_t from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "r"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Units of a row of sums are moved about so that neighbouring rows do not meet in a bank
+template <int RB>
+__device__ __forceinline__ int sums_swizzle(int r) { return RB == 16 ? r >> 1 & 3 : r & 7; }
 
 // RB: 16, 32 or 64 ranks (zeros behind the rank).  BACK as in the warp-level kernel.
 template <int DT, int RB, bool BACK>
 __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a, bool keep, bool none) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int UNITS = RB / 8, SUMS = RB / 4;             // 16-byte units of a row of ranks, of a row of sums
+    using At = Room<RB>;
+    constexpr int UNITS = RB / 8, SUMS = RB / 4, kStages = At::kStages;              // 16-byte units of a row of ranks, of a row of sums
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Ctrl *const ctl = reinterpret_cast<Ctrl *>(smem_raw);
     uint8_t *const data = smem_raw + 1024;
-    const uint32_t sm = smem_u32(data);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cr = cluster_rank();
+    const uint32_t sm = __shfl_sync(0xffffffffu, smem_u32(data), 0);
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), cr = cluster_rank();
     if (blockIdx.x == 0)
         for (int e = tid; e < a.n_adapters; e += kThreads)
             if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
@@ -101,249 +117,280 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     }
     const int units = (a.c_out + kColumns - 1) / kColumns;
     const int step0 = static_cast<int>(static_cast<long long>(units) * cr / kCluster), steps = static_cast<int>(static_cast<long long>(units) * (cr + 1) / kCluster) - step0;
+    const int c_end = std::min((step0 + steps) * kColumns, a.c_out);
     if (tile.e == a.n_adapters) {
         __syncthreads();
-        copy_rows<DT, kThreads>(a, ctl->row_of, static_cast<int>(tile.n), step0 * kColumns, std::min((step0 + steps) * kColumns, a.c_out), keep, cr, kCluster);
+        copy_rows<DT, kThreads>(a, ctl->row_of, static_cast<int>(tile.n), step0 * kColumns, c_end, keep, cr, kCluster);
         return;
     }
     // Tensor memory before the next kernel may start, which may want some too and then wait for this one; and not before the previous one is done.
-    if (warp == 0) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem)), "r"(kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (tid == 32) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&ctl->full[i], kThreads), mbar_init(&ctl->empty[i], 1);
-        mbar_init(&ctl->out[0], 1), mbar_init(&ctl->out[1], 1), mbar_init(&ctl->done, 1);
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&ctl->full[i], kCopy), mbar_init(&ctl->empty[i], 1);
+        for (int i = 0; i < 3; ++i) mbar_init(&ctl->columns[i], kCopy);
+        for (int i = 0; i < 2; ++i) mbar_init(&ctl->out[i], 1), mbar_init(&ctl->free[i], kCopy);
+        mbar_init(&ctl->done, 1), mbar_init(&ctl->sums, 1), mbar_init(&ctl->held, 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mbar_expect_tx(&ctl->sums, kCluster * kOwn * RB * 4);
+        mbar_expect_tx(&ctl->held, (kCluster - 1) * (2 * kOwn * 128 + (DT == MTC_F16 ? kOwn : 0)));
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    cluster_arrive();                                        // the barriers are there: waited for before anything is sent
     asm volatile("griddepcontrol.launch_dependents;");
-    const uint32_t tmem = ctl->tmem;
-    const size_t expert = tile.e;
-    const uint16_t *const in = static_cast<const uint16_t *>(a.in), *const base = static_cast<const uint16_t *>(a.base);
-    const uint16_t *const down = static_cast<const uint16_t *>(a.down) + expert * a.rank * a.c_in, *const up = static_cast<const uint16_t *>(a.up) + expert * a.rank * a.c_out;
-    const int u8 = tid & 7, r32 = tid >> 3;                  // the 16-byte unit and the first row (of every 32) that this thread copies
-    int rows[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = ctl->row_of[r32 + 32 * i];
-
-    // ---- the first product
+    const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
     const int chunks = (a.c_in + 63) / 64;
     const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * cr / kCluster), mine = static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / kCluster) - chunk0;
-    constexpr int LAG = kStages - 1;
-    for (int i = 0; i < mine + LAG; ++i) {
-        if (i < mine) {
-            const int s = i % kStages;
-            if (i >= kStages) mbar_wait(&ctl->empty[s], (i / kStages - 1) & 1, &ctl->abort, a.status, 0xb21u);
-            const uint32_t at = sm + s * kStage;
-            const int k = (chunk0 + i) * 64 + u8 * 8;
-            const bool there = k < a.c_in;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const bool row = there && rows[q] >= 0;
-                copy16(tile_at(at, r32 + 32 * q, u8), row ? in + static_cast<size_t>(rows[q]) * a.c_in + k : in, row);
-            }
-            if constexpr (!BACK) {               // rows are ranks
-#pragma unroll
-                for (int q = 0; q < (RB + 31) / 32; ++q) {
-                    const int r = r32 + 32 * q;
-                    const bool ok = there && r < a.rank;
-                    if (RB >= 32 || r < RB) copy16(tile_at(at + kWeights, r, u8), ok ? down + static_cast<size_t>(r) * a.c_in + k : down, ok);
-                }
-            } else {                             // rows are k's
-#pragma unroll
-                for (int q = tid; q < 64 * UNITS; q += kThreads) {
-                    const int r = q / UNITS, u = q % UNITS, kk = (chunk0 + i) * 64 + r;
-                    const bool ok = kk < a.c_in && u * 8 < a.rank;
-                    copy16(tile_at(at + kWeights, r, u), ok ? down + static_cast<size_t>(kk) * a.rank + u * 8 : down, ok);
-                }
-            }
-        }
-        copy_commit();
-        if (i >= LAG) {
-            const int c = i - LAG, s = c % kStages;
-            copy_wait<LAG>();
-            to_async_proxy();
-            mbar_arrive(&ctl->full[s]);
-            if (warp == 0) {
-                mbar_wait_warp(&ctl->full[s], (c / kStages) & 1, &ctl->abort, a.status, 0xb22u);
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t x = desc_of(sm + s * kStage), w = desc_of(sm + s * kStage + kWeights);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) umma_f16_ss(tmem + kSums, x + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, RB, BACK), c || q ? 1u : 0u);
-                    umma_commit(&ctl->empty[s]);
-                    if (c + 1 == mine) umma_commit(&ctl->done);
-                }
-                __syncwarp();
-            }
-        }
-    }
-    if (mine) mbar_wait(&ctl->done, 0, &ctl->abort, a.status, 0xb23u);
-    tc_fence_after();
 
-    // ---- what the second product reads is on its way meanwhile
-    auto request = [&](int step) {
-        if (step < steps) {
-            const uint32_t at = sm + buffer_at(step);
-            const int c0 = (step0 + step) * kColumns, c = c0 + u8 * 8;
-            if constexpr (!BACK) {               // rows are columns
-                for (int q = tid; q < kColumns * UNITS; q += kThreads) {
-                    const int r = q / UNITS, u = q % UNITS;
-                    const bool ok = c0 + r < a.c_out && u * 8 < a.rank;
-                    copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(c0 + r) * a.rank + u * 8 : up, ok);
-                }
-            } else {                             // rows are ranks
+    if (warp == kMmaWarp) {
+        // ---- products; the operands' addresses are the same for the whole warp
+        for (int c = 0; c < mine; ++c) {
+            const int s = c % kStages;
+            mbar_wait_warp(&ctl->full[s], (c / kStages) & 1, &ctl->abort, a.status, 0xb21u);
+            tc_fence_after();
+            const uint64_t x = desc_of(sm + s * kStage), w = desc_of(sm + s * kStage + kWeights);
+            if (elect_one()) {
 #pragma unroll
-                for (int q = 0; q < (RB + 31) / 32; ++q) {
-                    const int r = r32 + 32 * q;
-                    const bool ok = r < a.rank && c < a.c_out;
-                    if (RB >= 32 || r < RB) copy16(tile_at(at, r, u8), ok ? up + static_cast<size_t>(r) * a.c_out + c : up, ok);
-                }
+                for (int q = 0; q < 4; ++q) umma_f16_ss(tmem + kSums, x + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, RB, BACK), c || q ? 1u : 0u);
+                umma_commit(&ctl->empty[s]);
+                if (c + 1 == mine) umma_commit(&ctl->done);
             }
-            if (a.base) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const bool ok = c < a.c_out && rows[q] >= 0;
-                    copy16(tile_at(at + kBase, r32 + 32 * q, u8), ok ? base + static_cast<size_t>(rows[q]) * a.c_out + c : base, ok);
-                }
-            }
+            __syncwarp();
         }
-        copy_commit();
-    };
-    __syncthreads();                             // (the ring is free: every warp has seen `done`)
-    request(0);
-    request(1);
-
-    // ---- the parts of the sums, rows of RB values, their units moved about so that neighbouring rows do not meet in a bank
-    auto sums_at = [&](int r, int u) { return static_cast<uint32_t>(kPart + r * RB * 4 + ((u ^ (RB == 16 ? r >> 1 & 3 : r & 7)) << 4)); };
-    const int row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;                    // of tensor memory: the warp's quarter
-    if (RB > 16 || warp < 4) {
-        constexpr int COLS = RB == 16 ? 16 : RB / 2;
-        const int first = RB == 16 ? 0 : (warp >> 2) * COLS;
-        uint32_t v[COLS];
+        cluster_wait();
+        __syncthreads();                         // the ring is free
+        __syncthreads();                         // this CTA's rows of h are there: they go to the others
+        if (lane < kCluster && lane != cr) {
+            const uint32_t bar = on_cta(smem_u32(&ctl->held), lane), at = sm + kHeld + cr * kOwn * 128;
 #pragma unroll
-        for (int i = 0; i < COLS; ++i) v[i] = 0;
-        if (mine) {
-            tmem_ld<COLS>(tmem + kSums + first + lanes, v);
-            tmem_wait_ld();
-        }
-#pragma unroll
-        for (int i = 0; i < COLS / 4; ++i)
-            *reinterpret_cast<uint4 *>(data + sums_at(row, first / 4 + i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    }
-    tc_fence_before();
-    cluster_arrive();
-    cluster_wait();
-    // this CTA's sixteen rows: four ranks a thread
-    if (tid < kOwn * SUMS) {
-        const int r = cr * kOwn + tid / SUMS, u = tid % SUMS;
-        float4 v[kCluster], s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int q = 0; q < kCluster; ++q) v[q] = ld_far(on_cta(sm + sums_at(r, u), q));
-#pragma unroll
-        for (int q = 0; q < kCluster; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
-        const int to = ctl->row_of[r];
-        if (keep && to >= 0 && u * 4 < a.rank) *reinterpret_cast<float4 *>(a.low + static_cast<size_t>(to) * a.rank + u * 4) = s;
-        float f = 1.0f;
-        if constexpr (DT == MTC_F16) {
-            float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
-#pragma unroll
-            for (int o = SUMS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o, SUMS));
-            f = unit_of(most);
-        }
-        uint2 w[2];
-        hold_pieces<DT>(s, f, w);
-#pragma unroll
-        for (int q = 0; q < kCluster; ++q) {
-            const uint32_t at = on_cta(sm + kHeld, q);
-#pragma unroll
-            for (int p = 0; p < 2; ++p) st_far(tile_at(at + p * kPiece, r, u / 2) + (u & 1) * 8, w[p].x, w[p].y);
-            if (DT == MTC_F16 && u == 0) st_far(on_cta(smem_u32(&ctl->unit[r]), q), static_cast<uint8_t>(__float_as_uint(f) >> 23));
-        }
-    }
-    asm volatile("fence.proxy.async;" ::: "memory");         // what was written to the others is their operand
-    cluster_arrive();
-    cluster_wait();
-    asm volatile("fence.proxy.async;" ::: "memory");
-    request(2);
-
-    // ---- the second product, 64 columns at a time; the product of the next is under way while one goes out
-    const float scale = a.scales ? a.scales[expert] : 1.0f;
-    const float factor = DT == MTC_F16 ? scale * __uint_as_float(static_cast<uint32_t>(ctl->unit[row]) << 23) : scale;
-    auto multiply = [&](int step) {              // by warp 0
-        if (elect_one()) {
-            const uint64_t w = desc_of(sm + buffer_at(step)), h = desc_of(sm + kHeld);
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-                for (int q = 0; q < RB / 16; ++q)
-                    umma_f16_ss(tmem + kOut + (step & 1) * kColumns, h + (p * kPiece >> 4) + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, kColumns, BACK), p || q ? 1u : 0u);
-            umma_commit(&ctl->out[step & 1]);
+            for (int p = 0; p < 2; ++p) send_bulk(on_cta(at + p * kPiece, lane), at + p * kPiece, kOwn * 128, bar);
+            if (DT == MTC_F16) send_bulk(on_cta(smem_u32(&ctl->unit[cr * kOwn]), lane), smem_u32(&ctl->unit[cr * kOwn]), kOwn, bar);
         }
         __syncwarp();
-    };
-    if (steps > 0) {
-        copy_wait<2>();
-        to_async_proxy();
-        __syncthreads();
-        if (warp == 0) {
+        mbar_wait_warp(&ctl->held, 0, &ctl->abort, a.status, 0xb22u);
+        cluster_arrive();                        // nobody leaves while it sends: waited for at the end
+        for (int j = 0; j < steps; ++j) {
+            mbar_wait_warp(&ctl->columns[j % 3], (j / 3) & 1, &ctl->abort, a.status, 0xb23u);
+            if (j >= 2) mbar_wait_warp(&ctl->free[j & 1], (j / 2 - 1) & 1, &ctl->abort, a.status, 0xb24u);
             tc_fence_after();
-            multiply(0);
+            const uint64_t w = desc_of(sm + At::weights(j % 3)), h = desc_of(sm + kHeld);
+            if (elect_one()) {
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int q = 0; q < RB / 16; ++q)
+                        umma_f16_ss(tmem + kOut + (j & 1) * kColumns, h + (p * kPiece >> 4) + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, kColumns, BACK), p || q ? 1u : 0u);
+                umma_commit(&ctl->out[j & 1]);
+            }
+            __syncwarp();
         }
-    }
-    for (int j = 0; j < steps; ++j) {
-        copy_wait<1>();                          // the columns of step j + 1
-        to_async_proxy();
-        tc_fence_before();
-        __syncthreads();
-        if (warp == 0 && j + 1 < steps) {
-            tc_fence_after();
-            multiply(j + 1);
+    } else {
+        const size_t expert = tile.e;
+        const uint16_t *const in = static_cast<const uint16_t *>(a.in), *const base = static_cast<const uint16_t *>(a.base);
+        const uint16_t *const down = static_cast<const uint16_t *>(a.down) + expert * a.rank * a.c_in, *const up = static_cast<const uint16_t *>(a.up) + expert * a.rank * a.c_out;
+        const int u8 = tid & 7, r32 = tid >> 3;              // the 16-byte unit and the first row (of every 32) that this thread copies
+
+        // ---- the first product's operands
+        constexpr int LAG = kStages - 1;
+        {
+            const uint16_t *from[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = ctl->row_of[r32 + 32 * q];
+                from[q] = row >= 0 ? in + static_cast<size_t>(row) * a.c_in : nullptr;
+            }
+            for (int i = 0; i < mine + LAG; ++i) {
+                if (i < mine) {
+                    const int s = i % kStages;
+                    if (i >= kStages) mbar_wait_warp(&ctl->empty[s], (i / kStages - 1) & 1, &ctl->abort, a.status, 0xb25u);
+                    const uint32_t at = sm + s * kStage;
+                    const int k = (chunk0 + i) * 64 + u8 * 8;
+                    const bool there = k < a.c_in;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) copy16(tile_at(at, r32 + 32 * q, u8), there && from[q] ? from[q] + k : in, there && from[q]);
+                    if constexpr (!BACK) {       // rows are ranks
+#pragma unroll
+                        for (int q = 0; q < (RB + 31) / 32; ++q) {
+                            const int r = r32 + 32 * q;
+                            const bool ok = there && r < a.rank;
+                            if (RB >= 32 || r < RB) copy16(tile_at(at + kWeights, r, u8), ok ? down + static_cast<size_t>(r) * a.c_in + k : down, ok);
+                        }
+                    } else {                     // rows are k's
+#pragma unroll
+                        for (int q0 = 0; q0 < 64 * UNITS; q0 += kCopy) {
+                            const int q = q0 + tid, r = q / UNITS, u = q % UNITS, kk = (chunk0 + i) * 64 + r;
+                            const bool ok = kk < a.c_in && u * 8 < a.rank;
+                            if (64 * UNITS >= kCopy || q < 64 * UNITS) copy16(tile_at(at + kWeights, r, u), ok ? down + static_cast<size_t>(kk) * a.rank + u * 8 : down, ok);
+                        }
+                    }
+                }
+                copy_commit();
+                if (i >= LAG) {
+                    copy_wait<LAG>();
+                    to_async_proxy();
+                    mbar_arrive(&ctl->full[(i - LAG) % kStages]);
+                }
+            }
         }
-        mbar_wait(&ctl->out[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb24u);
+        if (mine) mbar_wait_warp(&ctl->done, 0, &ctl->abort, a.status, 0xb26u);
         tc_fence_after();
-        uint32_t v[32];
-        tmem_ld<32>(tmem + kOut + (j & 1) * kColumns + (warp >> 2) * 32 + lanes, v);
-        tmem_wait_ld();
-        uint8_t *const at = data + buffer_at(j) + kBase + row * 128;
+
+        // ---- the parts of the sums go to the rows' owners
+        const int row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;                // of tensor memory: the warp's quarter
+        cluster_wait();
+        if (RB > 16 || warp < 4) {
+            constexpr int COLS = RB == 16 ? 16 : RB / 2;
+            const int first = RB == 16 ? 0 : (warp >> 2) * COLS;
+            uint32_t v[COLS];
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) v[i] = 0;
+            if (mine) {
+                tmem_ld<COLS>(tmem + kSums + first + lanes, v);
+                tmem_wait_ld();
+            }
+            const uint32_t to = on_cta(sm + At::kFrom + (cr * kOwn + row % kOwn) * RB * 4, row / kOwn), bar = on_cta(smem_u32(&ctl->sums), row / kOwn);
+#pragma unroll
+            for (int i = 0; i < COLS / 4; ++i) send16(to + (((first / 4 + i) ^ sums_swizzle<RB>(row)) << 4), v + 4 * i, bar);
+        }
+        tc_fence_before();
+        __syncthreads();                         // (the ring is free: everybody has seen `done`)
+
+        // ---- the second product's operands.  Of base a warp has the rows and columns that it will give out; the weights are everybody's.
+        const int half = (warp >> 2) * 4, r4 = (warp & 3) * 32 + (lane >> 2), u4 = half + (lane & 3);      // units of the warp's columns; this lane's row (of every 8) and unit
+        long long at_row[4];                     // offsets of these rows in base and out, -1: none
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint4 *const p = reinterpret_cast<uint4 *>(at + ((((warp >> 2) * 4 + i) ^ (row & 7)) << 4));
-            lora::Eight<DT> b;
-            const uint4 q = a.base ? *p : make_uint4(0, 0, 0, 0);
-            b.w[0] = q.x, b.w[1] = q.y, b.w[2] = q.z, b.w[3] = q.w;
-            float r[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) r[k] = fmaf(__uint_as_float(v[8 * i + k]), factor, b.value(k));
-            lora::Eight<DT>::put(p, 0, r);
+            const int to = ctl->row_of[r4 + 8 * i];
+            at_row[i] = to < 0 ? -1 : static_cast<long long>(to) * a.c_out + u4 * 8;
         }
-        __syncthreads();
-        const int c = (step0 + j) * kColumns + u8 * 8;
+        auto request = [&](int step) {
+            if (step < steps) {
+                const uint32_t at = sm + At::weights(step % 3), to = sm + At::base(step % 3);
+                const int c0 = (step0 + step) * kColumns;
+                if constexpr (!BACK) {           // rows are columns
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (rows[q] >= 0 && c < a.c_out)
-                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + static_cast<size_t>(rows[q]) * a.c_out + c) =
-                    *reinterpret_cast<const uint4 *>(data + buffer_at(j) + kBase + (r32 + 32 * q) * 128 + ((u8 ^ (r32 & 7)) << 4));
-        __syncthreads();
-        request(j + 3);
-    }
-    copy_wait<0>();
-    if (ctl->abort && tid == 0) {                // gave up: bounded waits for MMAs that may still be on their way
-        drain_ring(ctl->empty, mine, kStages);
-        for (int i = 0; i < 2 && i < steps; ++i) {
-            const int last = steps - 1 - ((steps - 1 - i) & 1);                      // the last step of this buffer
-            for (uint32_t n = 0; n < 1u << 16 && !mbar_try(&ctl->out[i], (last >> 1) & 1); ++n) {}
+                    for (int q0 = 0; q0 < kColumns * UNITS; q0 += kCopy) {
+                        const int q = q0 + tid, r = q / UNITS, u = q % UNITS;
+                        const bool ok = c0 + r < a.c_out && u * 8 < a.rank;
+                        if (kColumns * UNITS >= kCopy || q < kColumns * UNITS) copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(c0 + r) * a.rank + u * 8 : up, ok);
+                    }
+                } else {                         // rows are ranks
+                    const int c = c0 + u8 * 8;
+#pragma unroll
+                    for (int q = 0; q < (RB + 31) / 32; ++q) {
+                        const int r = r32 + 32 * q;
+                        const bool ok = r < a.rank && c < a.c_out;
+                        if (RB >= 32 || r < RB) copy16(tile_at(at, r, u8), ok ? up + static_cast<size_t>(r) * a.c_out + c : up, ok);
+                    }
+                }
+                if (a.base && c0 + u4 * 8 < a.c_out) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (at_row[i] >= 0) copy16(tile_at(to, r4 + 8 * i, u4), base + at_row[i] + c0, true);
+                }
+            }
+            copy_commit();
+        };
+        request(0);
+        request(1);
+        if (a.base && steps > 2 && tid < static_cast<int>(tile.n) && ctl->row_of[tid] >= 0) {      // and the rest comes into L2 while the sums are on their way
+            const int c0 = (step0 + 2) * kColumns;
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(base + static_cast<size_t>(ctl->row_of[tid]) * a.c_out + c0), "r"((c_end - c0) * 2) : "memory");
         }
+        const float scale = a.scales ? a.scales[expert] : 1.0f;
+
+        // ---- h: this CTA's sixteen rows, four ranks a thread
+        mbar_wait_warp(&ctl->sums, 0, &ctl->abort, a.status, 0xb27u);
+        if (tid < kOwn * SUMS) {
+            const int r = cr * kOwn + tid / SUMS, u = tid % SUMS;
+            float4 v[kCluster], s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < kCluster; ++q) v[q] = *reinterpret_cast<const float4 *>(data + At::kFrom + (q * kOwn + r % kOwn) * RB * 4 + ((u ^ sums_swizzle<RB>(r)) << 4));
+#pragma unroll
+            for (int q = 0; q < kCluster; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+            const int to = ctl->row_of[r];
+            if (keep && to >= 0 && u * 4 < a.rank) *reinterpret_cast<float4 *>(a.low + static_cast<size_t>(to) * a.rank + u * 4) = s;
+            float f = 1.0f;
+            if constexpr (DT == MTC_F16) {
+                float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
+#pragma unroll
+                for (int o = SUMS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o, SUMS));
+                f = unit_of(most);
+                if (u == 0) ctl->unit[r] = static_cast<uint8_t>(__float_as_uint(f) >> 23);
+            }
+            uint2 w[2];
+            hold_pieces<DT>(s, f, w);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2 *>(data + (tile_at(kHeld + p * kPiece, r, u / 2) + (u & 1) * 8)) = w[p];
+        }
+        to_async_proxy();
+        __syncthreads();
+        if (DT == MTC_F16) mbar_wait_warp(&ctl->held, 0, &ctl->abort, a.status, 0xb28u);
+        cluster_arrive();
+        const float factor = DT == MTC_F16 ? scale * __uint_as_float(static_cast<uint32_t>(ctl->unit[row]) << 23) : scale;
+
+        // ---- 64 columns at a time; warps do not wait for each other
+        copy_wait<1>();
+        to_async_proxy();
+        if (steps > 0) mbar_arrive(&ctl->columns[0]);
+        for (int j = 0; j < steps; ++j) {
+            request(j + 2);                      // (in place of step j - 1, which this thread has seen multiplied and this warp has given out)
+            copy_wait<1>();
+            to_async_proxy();
+            if (j + 1 < steps) mbar_arrive(&ctl->columns[(j + 1) % 3]);
+            __syncwarp();
+            uint8_t *const tile_base = data + At::base(j % 3);
+            uint4 *const line = reinterpret_cast<uint4 *>(tile_base + row * 128);
+            lora::Eight<DT> b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 q = a.base ? line[(half + i) ^ (row & 7)] : make_uint4(0, 0, 0, 0);
+                b[i].w[0] = q.x, b[i].w[1] = q.y, b[i].w[2] = q.z, b[i].w[3] = q.w;
+            }
+            mbar_wait_warp(&ctl->out[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb29u);
+            tc_fence_after();
+            uint32_t v[32];
+            tmem_ld<32>(tmem + kOut + (j & 1) * kColumns + half * 8 + lanes, v);
+            tmem_wait_ld();
+            tc_fence_before();
+            mbar_arrive(&ctl->free[j & 1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float r[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = fmaf(__uint_as_float(v[8 * i + k]), factor, b[i].value(k));
+                lora::Eight<DT>::put(&line[(half + i) ^ (row & 7)], 0, r);
+            }
+            __syncwarp();
+            uint4 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const uint4 *>(tile_base + (r4 + 8 * i) * 128 + ((u4 ^ (r4 & 7)) << 4));
+            const int c0 = (step0 + j) * kColumns;
+            if (c0 + u4 * 8 < a.c_out) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at_row[i] >= 0) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at_row[i] + c0) = q[i];
+            }
+            __syncwarp();
+        }
+        copy_wait<0>();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
+    if (ctl->abort && tid == 0) {                // gave up: bounded waits for MMAs that may still be on their way
+        drain_ring(ctl->empty, mine, kStages);
+        drain_ring(ctl->out, steps, 2);
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
+    cluster_wait();
 }
 
 template <int DT, int RB, bool BACK>
