@@ -463,7 +463,7 @@ int mtc_add_rms_norm_fp8(mtc_ctx *ctx, void *stream, const void *x, const void *
  * dx is the gradient of x and of residual alike; it may be dy or dsum.  dx T[n_rows, K], dweight T[K].  Sums over rows run in a fixed order. */
 int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *sum, const void *norm_weight, float eps, const void *dsum, void *dx, void *dweight,
                           int n_rows, int K, int dtype, void *workspace, size_t workspace_bytes);
-size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K);
+size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, int dtype);
 
 /* ---- beside a projection: low-rank adapters of many requests (no counterpart in the reference) ----
  * For the rows t of adapter e:   h_t = x_t a[e]^T,   out_t = base_t + scales[e] * h_t b[e]^T           (sums f32, rounded once)

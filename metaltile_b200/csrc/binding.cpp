@@ -985,7 +985,7 @@ PyObject *add_rms_norm_grad(Args a, Py_ssize_t n) {
         const c10::cuda::CUDAGuard guard(o.x.device());
         if (!dx.defined()) dx = empty(o.x.sizes(), o.x.scalar_type(), o.x);
         dw = empty({o.K}, o.x.scalar_type(), o.x);
-        const size_t need = mtc_add_rms_norm_grad_workspace(c.h, static_cast<int>(o.M), static_cast<int>(o.K));
+        const size_t need = mtc_add_rms_norm_grad_workspace(c.h, static_cast<int>(o.M), static_cast<int>(o.K), o.dt);
         at::Tensor space;
         if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, o.x);
         return mtc_add_rms_norm_grad(c.h, on_stream(o.x), dy.data_ptr(), o.x.data_ptr(), o.weight.data_ptr(), eps, o.other ? o.other->data_ptr() : nullptr, dx.data_ptr(),

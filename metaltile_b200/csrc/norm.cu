@@ -69,14 +69,26 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float *scratch, bool one
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     if (one_warp) return;
-    const int warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0)
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0)
 #pragma unroll
-        for (int i = 0; i < N; ++i) scratch[i * 32 + (threadIdx.x >> 5)] = v[i];
+        for (int i = 0; i < N; ++i) scratch[i * 32 + warp] = v[i];
+    if (warps <= 8) {                            // few parts: every thread adds them up (five more exchanges are 130 cycles)
+        if (warp == 0 && lane >= warps && lane < 8)
+#pragma unroll
+            for (int i = 0; i < N; ++i) scratch[i * 32 + lane] = 0.0f;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float4 a = *reinterpret_cast<const float4 *>(scratch + i * 32), b = *reinterpret_cast<const float4 *>(scratch + i * 32 + 4);
+            v[i] = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+        }
+        return;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        float s = (threadIdx.x & 31) < warps ? scratch[i * 32 + (threadIdx.x & 31)] : 0.0f;
+        float s = lane < warps ? scratch[i * 32 + lane] : 0.0f;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         v[i] = s;
@@ -88,9 +100,9 @@ __device__ __forceinline__ float inverse_root(float sum, int K, float eps) { ret
 // MODE 0: y; 1, 2: codes with scales (2: powers of two), and y where it is wanted.  NV: turns whose values stay in registers (0: any number,
 // the row is read again).  A row's threads: a warp (several rows a CTA), or the CTA.
 template <int DT, bool VEC, int NV, int MODE>
-__global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(NV == 4 ? 256 : 1024) add_norm_kernel(const NormArgs a) {
     pdl_enter();
-    __shared__ float scratch[32];
+    __shared__ __align__(16) float scratch[32];
     const bool one_warp = a.threads == 32;
     const int t = one_warp ? threadIdx.x & 31 : threadIdx.x, K = a.K;
     const long long row = one_warp ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -151,11 +163,14 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
             for (int i = 0; i < 8; ++i)
                 if (VEC ? n <= 0 : i >= n) y[i] = 0.0f;
             const Eight<MTC_F32> v = packed<MTC_F32>(y);
-            uint32_t most = v.most();
+            float amax = 0.0f;                   // (a NaN stays one)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(amax) : "f"(fabsf(y[i])));
+            uint32_t most = __float_as_uint(amax);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
             const bool special = has_special<MTC_F32>(most);
-            float amax = magnitude<MTC_F32>(most);
+            amax = __uint_as_float(most);
             if (__any_sync(0xffffffffu, special)) {
                 float f = v.most_finite();
 #pragma unroll
@@ -182,12 +197,12 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
 }
 
 // ds of every row, and a CTA's (or warp's) share of dw in registers over its rows: part f32[workers][K].
-// HELD: the next row is requested before the sums of this one (rows of up to two turns of 16-bit values).
+// The next row is requested before the sums of this one where registers allow it (two turns of 16-bit values, one of f32); so are the weights held.
 template <int DT, int NV>
 __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradArgs a) {
     pdl_enter();
-    constexpr bool AHEAD = DT != MTC_F32 ? NV <= 2 : NV == 1, WEIGHTS = DT != MTC_F32 || NV == 1;
-    __shared__ float scratch[2][64];
+    constexpr bool AHEAD = DT != MTC_F32 ? NV <= 2 : NV == 1, WEIGHTS = DT != MTC_F32 ? NV <= 2 : NV == 1;
+    __shared__ __align__(16) float scratch[2][64];
     const bool one_warp = a.threads == 32;
     const int t = one_warp ? threadIdx.x & 31 : threadIdx.x, K = a.K;
     const long long worker = one_warp ? static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -254,7 +269,7 @@ __global__ void __launch_bounds__(512) norm_grad_kernel(const NormGradArgs a) {
 template <int DT>
 __global__ void __launch_bounds__(256) norm_grad_rows_kernel(const NormGradArgs a) {
     pdl_enter();
-    __shared__ float scratch[64];
+    __shared__ __align__(16) float scratch[64];
     const size_t at = static_cast<size_t>(blockIdx.x) * a.K;
     float v[2] = {0.0f, 0.0f};
     for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
@@ -296,23 +311,21 @@ __global__ void __launch_bounds__(256) norm_grad_values_kernel(const NormGradArg
     }
 }
 
-// dw = the shares added up in f64: 32 columns a CTA, eight warps that take the shares in turn
-constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps) norm_grad_join_kernel(const float *part, void *dweight, int workers, int K, int dt) {
+// dw = the shares added up in f64: 32 columns a CTA, whose warps take the shares in turn
+__global__ void __launch_bounds__(1024) norm_grad_join_kernel(const float *part, void *dweight, int workers, int K, int dt) {
     pdl_enter();
-    __shared__ double sums[kJoinWarps][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ double sums[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const long long k = static_cast<long long>(blockIdx.x) * 32 + lane;
     double acc = 0.0;
     if (k < K) {
-#pragma unroll 8
-        for (int p = warp; p < workers; p += kJoinWarps) acc += part[static_cast<size_t>(p) * K + k];
+#pragma unroll 16
+        for (int p = warp; p < workers; p += warps) acc += part[static_cast<size_t>(p) * K + k];
     }
     sums[warp][lane] = acc;
     __syncthreads();
     if (warp == 0 && k < K) {
-#pragma unroll
-        for (int i = 1; i < kJoinWarps; ++i) acc += sums[i][lane];
+        for (int i = 1; i < warps; ++i) acc += sums[i][lane];
         st_from_f32(dweight, k, static_cast<float>(acc), dt);
     }
 }
@@ -321,25 +334,43 @@ bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int round_up(int v, int step) { return (v + step - 1) / step * step; }
 
-// CTAs of the gradient: what it adds up for dw is written once a CTA (or warp) and read again
-constexpr int kWorkers = 592;
-int norm_workers(long long n_rows) { return static_cast<int>(std::min<long long>(n_rows, kWorkers)); }
+// The gradient's rows are dealt out to this many workers (CTAs, or warps that have rows of their own): what a worker adds up for dw is written once and read again.
+struct GradShape {
+    int turns, threads, block, workers;          // threads of a row, of a CTA
+};
+// Two turns of 16-bit values a thread, 512 threads an SM (their registers hold a row and the next one: 8192 x 4096 bf16 54 us, in one turn of 512 threads 64; 4096 x 8192 56);
+// one turn where rows are few or f32 (333 x 2880 bf16 7.6 and 10.0, f32 8.6 and 10.7, since there are fewer shares to add up).  Rows past 8192 take four turns.
+GradShape grad_shape(int sms, long long n_rows, int K, int dt) {
+    const int eights = static_cast<int>((static_cast<long long>(K) + 7) / 8);
+    GradShape g{};
+    const bool few = n_rows < 4ll * sms;
+    g.turns = eights <= 32 ? 1 : eights > 1024 ? 4 : eights > 512 || !(few || dt == MTC_F32) ? 2 : 1;
+    g.threads = std::min(512, round_up((eights + g.turns - 1) / g.turns, 32));
+    const int rows = g.threads == 32 ? 4 : 1;
+    g.block = g.threads * rows;
+    const long long ctas = static_cast<long long>(sms) * (few && rows == 1 ? 1 : std::max(1, 512 / g.block));
+    g.workers = static_cast<int>(std::min<long long>(n_rows, ctas * rows));
+    return g;
+}
 
 template <int DT, int MODE>
 cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, NormArgs a) {
     const bool vec = a.K % 8 == 0 && on_16(a.x) && on_16(a.weight) && (!a.residual || (on_16(a.residual) && on_16(a.sum))) && (!a.y || on_16(a.y)) &&
                      reinterpret_cast<uintptr_t>(a.codes) % 8 == 0;
     const int eights = (a.K + 7) / 8;
-    // One turn of many threads where rows are few, two turns of half as many where they fill the GPU
-    const int turns = a.n_rows <= ctx->sm_count && eights <= 1024 ? 1 : 2;
+    // One turn of many threads where rows are few, two turns of half as many where they fill the GPU, four of 16-bit values where there are many rows: what a thread does
+    // once a row costs as much as sixteen values (codes of 8192 x 4096 bf16 52 us in two turns, 49 in four; 4096 x 8192 59 and 51; 333 rows 4.8 and 5.2, f32 65 and 69)
+    const int turns = a.n_rows <= ctx->sm_count && eights <= 1024 ? 1 : DT != MTC_F32 && a.n_rows >= 4ll * ctx->sm_count && eights >= 256 && eights <= 1024 ? 4 : 2;
     a.threads = std::min(1024, round_up((eights + turns - 1) / turns, 32));
     const int rows_a_cta = a.threads == 32 ? 4 : 1;
     const long long ctas = (a.n_rows + rows_a_cta - 1) / rows_a_cta;
     const dim3 grid(static_cast<unsigned>(ctas));
     const int block = a.threads * rows_a_cta;
     if (!vec) return launch_pdl(add_norm_kernel<DT, false, 0, MODE>, grid, block, 0, st, a);
-    if (eights > 2 * a.threads) return launch_pdl(add_norm_kernel<DT, true, 0, MODE>, grid, block, 0, st, a);
-    return turns == 1 ? launch_pdl(add_norm_kernel<DT, true, 1, MODE>, grid, block, 0, st, a) : launch_pdl(add_norm_kernel<DT, true, 2, MODE>, grid, block, 0, st, a);
+    if (eights > turns * a.threads) return launch_pdl(add_norm_kernel<DT, true, 0, MODE>, grid, block, 0, st, a);
+    return turns == 1   ? launch_pdl(add_norm_kernel<DT, true, 1, MODE>, grid, block, 0, st, a)
+           : turns == 2 ? launch_pdl(add_norm_kernel<DT, true, 2, MODE>, grid, block, 0, st, a)
+                        : launch_pdl(add_norm_kernel<DT, true, 4, MODE>, grid, block, 0, st, a);
 }
 template <int DT>
 cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, const NormArgs &a, int mode) {
@@ -347,7 +378,7 @@ cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, const NormArgs &a, int mode) 
 }
 
 template <int DT>
-cudaError_t launch_grad(Ctx *, cudaStream_t st, NormGradArgs a) {
+cudaError_t launch_grad(const GradShape &g, cudaStream_t st, NormGradArgs a) {
     const bool vec = a.K % 8 == 0 && on_16(a.dy) && on_16(a.s) && on_16(a.weight) && on_16(a.dx) && (!a.dsum || on_16(a.dsum));
     const int eights = (a.K + 7) / 8;
     if (!vec || eights > 4 * 512) {
@@ -356,11 +387,9 @@ cudaError_t launch_grad(Ctx *, cudaStream_t st, NormGradArgs a) {
         if (e == cudaSuccess) e = launch_pdl(norm_grad_columns_kernel<DT>, dim3((a.K + 127u) / 128u, a.workers), 128, 0, st, a);
         return e == cudaSuccess ? launch_pdl(norm_grad_values_kernel<DT>, rows, 256, 0, st, a) : e;
     }
-    const int turns = eights <= 512 ? 1 : eights <= 1024 ? 2 : 4;
-    a.threads = round_up((eights + turns - 1) / turns, 32);
-    const int workers_a_cta = a.threads == 32 ? 4 : 1;
-    const dim3 grid((a.workers + workers_a_cta - 1) / workers_a_cta);
-    const int block = a.threads * workers_a_cta;
+    a.threads = g.threads;
+    const int rows = g.block / g.threads, turns = g.turns, block = g.block;
+    const dim3 grid((a.workers + rows - 1) / rows);
     return turns == 1   ? launch_pdl(norm_grad_kernel<DT, 1>, grid, block, 0, st, a)
            : turns == 2 ? launch_pdl(norm_grad_kernel<DT, 2>, grid, block, 0, st, a)
                         : launch_pdl(norm_grad_kernel<DT, 4>, grid, block, 0, st, a);
@@ -372,19 +401,20 @@ cudaError_t launch_add_rms_norm(Ctx *ctx, cudaStream_t st, const NormArgs &a, in
     return (dt == MTC_F32 ? launch_norm<MTC_F32> : dt == MTC_BF16 ? launch_norm<MTC_BF16> : launch_norm<MTC_F16>)(ctx, st, a, mode);
 }
 
-size_t norm_grad_workspace(int, long long n_rows, int K) {
-    return n_rows <= 0 ? 0 : static_cast<size_t>(norm_workers(n_rows)) * K * 4 + static_cast<size_t>((n_rows + 1) / 2) * 16;
+size_t norm_grad_workspace(int sms, long long n_rows, int K, int dt) {
+    return n_rows <= 0 ? 0 : static_cast<size_t>(grad_shape(sms, n_rows, K, dt).workers) * K * 4 + static_cast<size_t>((n_rows + 1) / 2) * 16;
 }
 
 cudaError_t launch_norm_grad(Ctx *ctx, cudaStream_t st, NormGradArgs a, void *dweight, void *workspace, int dt) {
-    a.workers = norm_workers(a.n_rows);
+    const GradShape g = grad_shape(ctx->sm_count, a.n_rows, a.K, dt);
+    a.workers = g.workers;
     a.rows = static_cast<float2 *>(workspace);
     a.part = reinterpret_cast<float *>(a.rows + (a.n_rows + 1) / 2 * 2);
     if (a.n_rows > 0) {
-        const cudaError_t e = (dt == MTC_F32 ? launch_grad<MTC_F32> : dt == MTC_BF16 ? launch_grad<MTC_BF16> : launch_grad<MTC_F16>)(ctx, st, a);
+        const cudaError_t e = (dt == MTC_F32 ? launch_grad<MTC_F32> : dt == MTC_BF16 ? launch_grad<MTC_BF16> : launch_grad<MTC_F16>)(g, st, a);
         if (e != cudaSuccess) return e;
     }
-    return launch_pdl(norm_grad_join_kernel, dim3((a.K + 31u) / 32u), 32 * kJoinWarps, 0, st, a.part, dweight, a.workers, a.K, dt);      // no rows: zeros
+    return launch_pdl(norm_grad_join_kernel, dim3((a.K + 31u) / 32u), a.workers > 256 ? 1024 : 512, 0, st, a.part, dweight, a.workers, a.K, dt);      // no rows: zeros
 }
 
 }  // namespace mtc

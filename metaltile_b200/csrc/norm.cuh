@@ -27,7 +27,7 @@ struct NormGradArgs {
 };
 
 cudaError_t launch_add_rms_norm(Ctx *ctx, cudaStream_t st, const NormArgs &a, int mode, int dt);
-size_t norm_grad_workspace(int sms, long long n_rows, int K);
+size_t norm_grad_workspace(int sms, long long n_rows, int K, int dt);
 cudaError_t launch_norm_grad(Ctx *ctx, cudaStream_t st, NormGradArgs a, void *dweight, void *workspace, int dt);
 
 }  // namespace mtc

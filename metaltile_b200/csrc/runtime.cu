@@ -1677,8 +1677,8 @@ int mtc_add_rms_norm_fp8(mtc_ctx *ctx, void *stream, const void *x, const void *
     return add_rms_norm(ctx, "add_rms_norm_fp8", stream, x, residual, norm_weight, eps, sum, y, codes, scales, n_rows, K, pow2 ? 2 : 1, dtype);
 }
 
-size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K) {
-    return K <= 0 ? 0 : mtc::norm_grad_workspace(ctx ? ctx->sm_count : mtc::kNumSMsB200, n_rows, K);
+size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, int dtype) {
+    return K <= 0 || K > mtc::kMostNorm || !dtype_ok(dtype) ? 0 : mtc::norm_grad_workspace(ctx ? ctx->sm_count : mtc::kNumSMsB200, n_rows, K, dtype);
 }
 
 int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *sum, const void *norm_weight, float eps, const void *dsum, void *dx, void *dweight,
@@ -1688,7 +1688,7 @@ int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void
         int rc = norm_args_ok(ctx, "add_rms_norm_grad", n_rows, K, dtype);
         if (rc != MTC_OK) return rc;
         if (!dweight || (n_rows > 0 && (!dy || !sum || !norm_weight || !dx))) return fail(ctx, MTC_ERR_INVALID, "add_rms_norm_grad: null pointer");
-        rc = check_workspace(ctx, "add_rms_norm_grad", workspace, workspace_bytes, mtc_add_rms_norm_grad_workspace(ctx, n_rows, K));
+        rc = check_workspace(ctx, "add_rms_norm_grad", workspace, workspace_bytes, mtc_add_rms_norm_grad_workspace(ctx, n_rows, K, dtype));
         if (rc != MTC_OK) return rc;
         mtc::NormGradArgs a{};
         a.dy = dy, a.s = sum, a.weight = norm_weight, a.dsum = dsum, a.dx = dx;

@@ -71,7 +71,8 @@ def test_entries_without_a_context_are_refused():
 
 def test_workspaces_cover_what_the_calls_keep():
     lib = _lib.load()
-    assert lib.mtc_add_rms_norm_grad_workspace(None, 0, 64) == 0 and lib.mtc_add_rms_norm_grad_workspace(None, 1, 64) >= 260
+    assert lib.mtc_add_rms_norm_grad_workspace(None, 0, 64, 2) == 0 and lib.mtc_add_rms_norm_grad_workspace(None, 1, 64, 2) >= 264
+    assert lib.mtc_add_rms_norm_grad_workspace(None, 9, 0, 2) == lib.mtc_add_rms_norm_grad_workspace(None, 9, 64, 7) == 0
     for rows, rank in ((1, 1), (70000, 64), (1 << 30, 1024)):
         assert lib.mtc_lora_mm_workspace(None, rows, 64, 64, rank, 3, 2) >= 4 * rows * rank
         assert lib.mtc_lora_grad_workspace(None, rows, 64, 64, rank, 3, 2) >= 4 * rows * rank
