@@ -19,14 +19,21 @@ constexpr int kWarps = 8, kThreads = 32 * kWarps, kCluster = 8;
 __host__ __device__ constexpr int part_stride(int rb) { return rb + 4; }
 __host__ __device__ constexpr int held_stride(int rt) { return rt + 8; }         // in 16-bit values: rows 16 bytes apart modulo 128
 
-__device__ __forceinline__ void prefetch(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-// `bytes` from `from` on of each of `rows` rows, a row `pitch` bytes; row_of: which rows (null: the first ones; negative: none)
-__device__ __forceinline__ void prefetch_rows(const void *base, size_t from, size_t pitch, int bytes, int rows, const int *row_of) {
-    const int lines = (bytes + 127) / 128;
-    for (int i = threadIdx.x; i < rows * lines; i += kThreads) {
-        const int row = row_of ? row_of[i / lines] : i / lines;
-        if (row >= 0) prefetch(static_cast<const char *>(base) + row * pitch + from + i % lines * 128);
+// Into L2, 16-byte aligned pieces: a request a row (with one a line, 2000 cycles went into asking)
+__device__ __forceinline__ void prefetch(const char *p, size_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(static_cast<uint32_t>(bytes)) : "memory");
+}
+// `bytes` of each of `rows` rows, a row `pitch` bytes; row_of: which rows (null: the first ones; negative: none); by the threads from `first` on
+__device__ __forceinline__ void prefetch_rows(const void *from, size_t pitch, size_t bytes, int rows, const int *row_of, int first) {
+    for (int i = (static_cast<int>(threadIdx.x) - first + kThreads) % kThreads; i < rows; i += kThreads) {
+        const int row = row_of ? row_of[i] : i;
+        if (row >= 0) prefetch(static_cast<const char *>(from) + row * pitch, bytes);
     }
+}
+__device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, int first) {
+    constexpr size_t piece = 4096;
+    for (size_t i = static_cast<size_t>((static_cast<int>(threadIdx.x) - first + kThreads) % kThreads) * piece; i < bytes; i += kThreads * piece)
+        prefetch(static_cast<const char *>(from) + i, min(piece, bytes - i));
 }
 
 // RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  BACK: the first product's weights lie [c_in][rank], the second's
@@ -75,14 +82,14 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
         const size_t in_row = static_cast<size_t>(a.c_in) * SIZE, out_row = static_cast<size_t>(a.c_out) * SIZE, rank_row = static_cast<size_t>(a.rank) * SIZE;
         const char *const down = static_cast<const char *>(a.down) + expert * a.rank * in_row, *const up = static_cast<const char *>(a.up) + expert * a.rank * out_row;
         if (k1 > k0) {
-            prefetch_rows(a.in, static_cast<size_t>(k0) * SIZE, in_row, (k1 - k0) * SIZE, ROWS, row_of);
-            if (BACK) prefetch_rows(down, k0 * rank_row, 0, static_cast<int>((k1 - k0) * rank_row), 1, nullptr);
-            else prefetch_rows(down, static_cast<size_t>(k0) * SIZE, in_row, (k1 - k0) * SIZE, a.rank, nullptr);
+            prefetch_rows(static_cast<const char *>(a.in) + static_cast<size_t>(k0) * SIZE, in_row, static_cast<size_t>(k1 - k0) * SIZE, ROWS, row_of, 0);
+            if (BACK) prefetch_block(down + k0 * rank_row, (k1 - k0) * rank_row, 32);
+            else prefetch_rows(down + static_cast<size_t>(k0) * SIZE, in_row, static_cast<size_t>(k1 - k0) * SIZE, a.rank, nullptr, 32);
         }
         if (n1 > n0) {
-            if (BACK) prefetch_rows(up, static_cast<size_t>(n0) * SIZE, out_row, (n1 - n0) * SIZE, a.rank, nullptr);
-            else prefetch_rows(up, n0 * rank_row, 0, static_cast<int>((n1 - n0) * rank_row), 1, nullptr);
-            if (a.base) prefetch_rows(a.base, static_cast<size_t>(n0) * SIZE, out_row, (n1 - n0) * SIZE, ROWS, row_of);
+            if (BACK) prefetch_rows(up + static_cast<size_t>(n0) * SIZE, out_row, static_cast<size_t>(n1 - n0) * SIZE, a.rank, nullptr, 96);
+            else prefetch_block(up + n0 * rank_row, (n1 - n0) * rank_row, 96);
+            if (a.base) prefetch_rows(static_cast<const char *>(a.base) + static_cast<size_t>(n0) * SIZE, out_row, static_cast<size_t>(n1 - n0) * SIZE, ROWS, row_of, 160);
         }
     }
 
@@ -91,10 +98,63 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
 #pragma unroll
     for (int m = 0; m < MT; ++m) rows[m][0] = row_of[16 * m + g], rows[m][1] = row_of[16 * m + g + 8];
     const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * me / workers), chunk1 = static_cast<int>(static_cast<long long>(chunks) * (me + 1) / workers);
+
+    // What a warp's step of the second product reads: weights of 32 ranks (tiles of columns, or four rows of ranks at a time), base.  EARLY: several steps'
+    // are loaded at once, the first ones before the parts meet (64 rows of 32 adapters 12.1 us a step at a time); elsewhere, where registers do not allow
+    // it, each right before its products.
+    constexpr int TN = CW / 8, QS = RB >= 32 ? RB / 32 : 1, WIDE = RB >= 32 ? 8 : RB / 4, PARTS = WIDE == 8 ? 2 : 1, DEEP = WIDE == 2 ? 2 : 4;
+    constexpr bool EARLY = ONE && MT == 1 && P == 1 && (BACK ? RB <= 16 : RB <= 32);
+    constexpr int STEPS = !EARLY ? 1 : BACK || RB == 32 ? 2 : 4;
+    using V = Vals<DT, BACK ? 8 : WIDE>;
+    struct Unit {
+        V w[BACK ? DEEP * (EARLY ? PARTS : 1) : TN];
+        lora::Eight<DT> base[MT][2][CW / 32];
+    };
+    auto load_base = [&](Unit &to, int n0) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < CW / 32; ++i) {
+                    const int c = n0 + t * (CW / 4) + 8 * i;
+                    to.base[m][h][i].load(a.base, static_cast<size_t>(rows[m][h]) * a.c_out + c, a.base && rows[m][h] >= 0 && c < a.c_out);
+                }
+    };
+    auto load_weights = [&](V *to, int n0, int r, int i) {       // r: this lane's first rank; i (BACK): four ranks behind
+        if constexpr (!BACK) {
+            // column c of tile j is n0 + c / 2 * 8 + 2 j + c % 2, so that a lane's results are eight neighbours
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int n = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
+                to[j].load(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
+            }
+        } else {
+            // column c of tile j is n0 + 8 c + j: a lane loads eight neighbours of four ranks' rows, its results are sixteen
+            const int c = n0 + 8 * g;
+#pragma unroll
+            for (int s = 0; s < DEEP; ++s) {
+                const int rr = r + 4 * i + s;
+                to[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
+            }
+        }
+    };
+    auto load_early = [&](Unit &to, int n0) {
+        load_base(to, n0);
+#pragma unroll
+        for (int i = 0; i < (BACK ? PARTS : 1); ++i) load_weights(to.w + i * DEEP, n0, t * WIDE, i);
+    };
+    Unit steps[STEPS];
+    auto load_steps = [&](int u) {               // steps u, u + kWarps ..
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+            if (u + i * kWarps < unit1) load_early(steps[i], (u + i * kWarps) * CW);
+    };
+    const float scale = a.scales ? a.scales[expert] : 1.0f;
     for (int rb = 0; rb < rank_blocks; ++rb) {
         float acc[MT][NT][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? NT : 1][4] = {};      // f32: the products of small pieces, apart so that the large ones are cut off less often
-#pragma unroll 2
+#pragma unroll (MT == 1 && RB <= 16 && P == 1 ? 4 : 2)
         for (int c = chunk0; c < chunk1; ++c) {
             const int k = c * 32 + t * 8;
             const bool in = k < a.c_in;
@@ -137,6 +197,9 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
                         for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), V::pair(w[2], w[3], p, j));
                 }
             }
+        }
+        if constexpr (EARLY) {
+            load_steps(unit0 + warp);
         }
         // ---- the warps' parts, then the CTAs'
         if (rb) {                                // (the gather of the block before has read `part`)
@@ -200,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
             }
         }
     }
-    cluster_arrive();                            // nobody leaves while its part is read: waited for at the end
+    cluster_arrive_relaxed();                    // nobody leaves while its part is read: waited for at the end
     if constexpr (!ONE) {
         __syncthreads();
         for (int row = warp; row < ROWS; row += kWarps) {
@@ -219,22 +282,10 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
     __syncthreads();
 
     // ---- the second product
-    const float scale = a.scales ? a.scales[expert] : 1.0f;
-    constexpr int TN = CW / 8, QS = RB >= 32 ? RB / 32 : 1, WIDE = RB >= 32 ? 8 : RB / 4;      // tiles; loads of a block's ranks, ranks of a lane in each
-    for (int u = unit0 + warp; u < unit1; u += kWarps) {
-        const int n0 = u * CW;
+    auto multiply = [&](Unit &unit, int n0) {
+        if constexpr (!EARLY) load_base(unit, n0);
         float acc[MT][TN][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? TN : 1][4] = {};
-        lora::Eight<DT> base[MT][2][CW / 32];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < CW / 32; ++i) {
-                    const int c = n0 + t * (CW / 4) + 8 * i;
-                    base[m][h][i].load(a.base, static_cast<size_t>(rows[m][h]) * a.c_out + c, a.base && rows[m][h] >= 0 && c < a.c_out);
-                }
         for (int rb = 0; rb < rank_blocks; ++rb) {
 #pragma unroll
             for (int q = 0; q < QS; ++q) {
@@ -269,29 +320,18 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
                         }
                 };
                 if constexpr (!BACK) {
-                    // column c of tile j is n0 + c / 2 * 8 + 2 j + c % 2, so that a lane's results are eight neighbours
+                    if constexpr (!EARLY) load_weights(unit.w, n0, r, 0);
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        const int n = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
-                        Vals<DT, WIDE> w;
-                        w.load(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int p = 0; p < P; ++p)
 #pragma unroll
-                            for (int i = 0; i < (WIDE == 8 ? 2 : 1); ++i) step(j, p, i, w.w[p][2 * i], WIDE == 2 ? 0u : w.w[p][WIDE == 2 ? 0 : 2 * i + 1]);
-                    }
+                            for (int i = 0; i < PARTS; ++i) step(j, p, i, unit.w[j].w[p][2 * i], WIDE == 2 ? 0u : unit.w[j].w[p][WIDE == 2 ? 0 : 2 * i + 1]);
                 } else {
-                    // column c of tile j is n0 + 8 c + j: a lane loads eight neighbours of four ranks' rows, its results are sixteen
-                    using V = Vals<DT, 8>;
-                    const int c = n0 + 8 * g;
 #pragma unroll
-                    for (int i = 0; i < (WIDE == 8 ? 2 : 1); ++i) {
-                        V w[WIDE == 2 ? 2 : 4];
-#pragma unroll
-                        for (int s = 0; s < (WIDE == 2 ? 2 : 4); ++s) {
-                            const int rr = r + 4 * i + s;
-                            w[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
-                        }
+                    for (int i = 0; i < PARTS; ++i) {
+                        V *const w = unit.w + (EARLY ? i * DEEP : 0);
+                        if constexpr (!EARLY) load_weights(w, n0, r, i);
 #pragma unroll
                         for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -316,9 +356,15 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
                         v[k] = acc[m][j][at];
                         if constexpr (P > 1) v[k] += fine[m][j][at];
                     }
-                    if (c < a.c_out) base[m][h][i].add_and_store(a.out, static_cast<size_t>(rows[m][h]) * a.c_out + c, v, factor);
+                    if (c < a.c_out) unit.base[m][h][i].add_and_store(a.out, static_cast<size_t>(rows[m][h]) * a.c_out + c, v, factor);
                 }
             }
+    };
+    for (int u0 = unit0 + warp; u0 < unit1; u0 += STEPS * kWarps) {
+        if (EARLY && u0 != unit0 + warp) load_steps(u0);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+            if (u0 + i * kWarps < unit1) multiply(steps[i], (u0 + i * kWarps) * CW);
     }
     cluster_wait();
 }
