@@ -11,8 +11,10 @@
 // The parts meet without a barrier: a CTA stores its sums into the shared memory of the rows' owners as they leave tensor memory (st.async), an owner copies its rows of h
 // into all others' (cp.async.bulk), and the receiving side's mbarriers count the bytes.
 //
+//   warps 0-7  first product's copies; then base in and results out, 64 columns a step: warps 0-3 have the even steps, 4-7 the odd ones, each 32 rows of whole lines
+//   warp 8     MMAs, tensor memory        warp 9     the second product's weights
 //   shared memory: the first product's ring of stages (128 rows x 64 values of x 16 KB, 64 of the weights of every rank 8 KB; rows 128 bytes apart with the 128-byte
-//   swizzle) and what comes in of the sums; then h (32 KB) and three buffers of 64 columns (weights 8 KB, base and results 16 KB) in their places
+//   swizzle) and what comes in of the sums; then, in their places, h (32 KB), two buffers of weights (8 KB) and four of base and results (16 KB)
 #include <algorithm>
 #include <cstddef>
 
@@ -24,25 +26,26 @@ namespace {
 
 using namespace lora;
 
-constexpr int kCopy = 256, kMmaWarp = kCopy / 32, kThreads = kCopy + 32, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
+constexpr int kCopy = 256, kMmaWarp = 8, kLoadWarp = 9, kThreads = kCopy + 64, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
 constexpr int kStage = 24 * 1024, kWeights = 16 * 1024;                              // of a stage: where the weights start
 constexpr int kHeld = 0, kPiece = 16 * 1024, kColumns = 64;
 constexpr int kSmem = 1024 + 112 * 1024;
 constexpr uint32_t kTmem = 256, kSums = 0, kOut = 64;                                // columns of tensor memory
 
-// Ranks 64: the sums of eight CTAs for sixteen rows are 32 KB, a stage less
+// Ranks 64: the sums of eight CTAs for sixteen rows are 32 KB, a stage less.  Base of the first steps comes in before the sums do: only the last buffer takes their place.
 template <int RB>
 struct Room {
     static constexpr int kStages = RB == 64 ? 3 : 4, kFrom = kStages * kStage;       // where the others' sums come in
-    // of a buffer of columns: the last one takes the sums' place
-    static __device__ __forceinline__ int weights(int b) { return RB == 64 ? (b == 0 ? 32 * 1024 : b == 1 ? 104 * 1024 : 72 * 1024) : (32 + 24 * b) * 1024; }
-    static __device__ __forceinline__ int base(int b) { return RB == 64 ? (b == 0 ? 40 * 1024 : b == 1 ? 56 * 1024 : 80 * 1024) : (40 + 24 * b) * 1024; }
+    static __device__ __forceinline__ int weights(int b) { return b == 0 ? 32 * 1024 : RB == 64 ? 104 * 1024 : 40 * 1024; }
+    static __device__ __forceinline__ int base(int b) { return RB == 64 ? (b < 2 ? 40 + 16 * b : 72 + 16 * (b - 2)) * 1024 : (48 + 16 * b) * 1024; }
+    static constexpr int kEarly = RB == 64 ? 2 : 3;                                  // buffers of base that are free before the sums are added up
 };
+static_assert(Room<64>::kFrom == 72 * 1024 && Room<32>::kFrom == 96 * 1024, "sums of eight CTAs behind the ring");
 
 struct Ctrl {
     int row_of[kRows];
     uint8_t unit[kRows];                         // f16: exponent of what a row of h was divided by
-    uint64_t full[4], empty[4], columns[3], out[2], free[2], done, sums, held;
+    uint64_t full[4], empty[4], columns[2], out[2], free[2], done, sums, held;
     uint32_t tmem, abort;
 };
 static_assert(sizeof(Ctrl) <= 1024, "control block");
@@ -130,8 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     }
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&ctl->full[i], kCopy), mbar_init(&ctl->empty[i], 1);
-        for (int i = 0; i < 3; ++i) mbar_init(&ctl->columns[i], kCopy);
-        for (int i = 0; i < 2; ++i) mbar_init(&ctl->out[i], 1), mbar_init(&ctl->free[i], kCopy);
+        for (int i = 0; i < 2; ++i) mbar_init(&ctl->columns[i], 32), mbar_init(&ctl->out[i], 1), mbar_init(&ctl->free[i], kCopy / 2);
         mbar_init(&ctl->done, 1), mbar_init(&ctl->sums, 1), mbar_init(&ctl->held, 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -175,10 +177,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         mbar_wait_warp(&ctl->held, 0, &ctl->abort, a.status, 0xb22u);
         cluster_arrive();                        // nobody leaves while it sends: waited for at the end
         for (int j = 0; j < steps; ++j) {
-            mbar_wait_warp(&ctl->columns[j % 3], (j / 3) & 1, &ctl->abort, a.status, 0xb23u);
+            mbar_wait_warp(&ctl->columns[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb23u);
             if (j >= 2) mbar_wait_warp(&ctl->free[j & 1], (j / 2 - 1) & 1, &ctl->abort, a.status, 0xb24u);
             tc_fence_after();
-            const uint64_t w = desc_of(sm + At::weights(j % 3)), h = desc_of(sm + kHeld);
+            const uint64_t w = desc_of(sm + At::weights(j & 1)), h = desc_of(sm + kHeld);
             if (elect_one()) {
 #pragma unroll
                 for (int p = 0; p < 2; ++p)
@@ -189,10 +191,47 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             }
             __syncwarp();
         }
+    } else if (warp == kLoadWarp) {
+        // ---- the second product's weights: 64 columns of every rank
+        const uint16_t *const up = static_cast<const uint16_t *>(a.up) + static_cast<size_t>(tile.e) * a.rank * a.c_out;
+        cluster_wait();
+        __syncthreads();                         // the ring is free
+        auto request = [&](int step) {
+            if (step < steps) {
+                const uint32_t at = sm + At::weights(step & 1);
+                const int c0 = (step0 + step) * kColumns;
+#pragma unroll
+                for (int q0 = 0; q0 < kColumns * UNITS; q0 += 32) {
+                    const int q = q0 + lane;
+                    if constexpr (!BACK) {       // rows are columns
+                        const int r = q / UNITS, u = q % UNITS;
+                        const bool ok = c0 + r < a.c_out && u * 8 < a.rank;
+                        copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(c0 + r) * a.rank + u * 8 : up, ok);
+                    } else {                     // rows are ranks
+                        const int r = q >> 3, u = q & 7, c = c0 + u * 8;
+                        const bool ok = r < a.rank && c < a.c_out;
+                        copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(r) * a.c_out + c : up, ok);
+                    }
+                }
+            }
+            copy_commit();
+        };
+        request(0);
+        request(1);
+        __syncthreads();
+        cluster_arrive();
+        for (int j = 0; j < steps; ++j) {
+            copy_wait<1>();
+            to_async_proxy();
+            mbar_arrive(&ctl->columns[j & 1]);
+            mbar_wait_warp(&ctl->out[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb2au);       // step j is multiplied: its place is free
+            request(j + 2);
+        }
+        copy_wait<0>();
     } else {
         const size_t expert = tile.e;
         const uint16_t *const in = static_cast<const uint16_t *>(a.in), *const base = static_cast<const uint16_t *>(a.base);
-        const uint16_t *const down = static_cast<const uint16_t *>(a.down) + expert * a.rank * a.c_in, *const up = static_cast<const uint16_t *>(a.up) + expert * a.rank * a.c_out;
+        const uint16_t *const down = static_cast<const uint16_t *>(a.down) + expert * a.rank * a.c_in;
         const int u8 = tid & 7, r32 = tid >> 3;              // the 16-byte unit and the first row (of every 32) that this thread copies
 
         // ---- the first product's operands
@@ -261,46 +300,28 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         tc_fence_before();
         __syncthreads();                         // (the ring is free: everybody has seen `done`)
 
-        // ---- the second product's operands.  Of base a warp has the rows and columns that it will give out; the weights are everybody's.
-        const int half = (warp >> 2) * 4, r4 = (warp & 3) * 32 + (lane >> 2), u4 = half + (lane & 3);      // units of the warp's columns; this lane's row (of every 8) and unit
-        long long at_row[4];                     // offsets of these rows in base and out, -1: none
+        // ---- base of this warp's rows, every second step
+        const int group = warp >> 2, r8 = (warp & 3) * 32 + (lane >> 3);             // parity of the steps; this lane's row of every four
+        long long at_row[8];                     // offsets of these rows in base and out, -1: none
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int to = ctl->row_of[r4 + 8 * i];
-            at_row[i] = to < 0 ? -1 : static_cast<long long>(to) * a.c_out + u4 * 8;
+        for (int i = 0; i < 8; ++i) {
+            const int to = ctl->row_of[r8 + 4 * i];
+            at_row[i] = to < 0 ? -1 : static_cast<long long>(to) * a.c_out + u8 * 8;
         }
         auto request = [&](int step) {
-            if (step < steps) {
-                const uint32_t at = sm + At::weights(step % 3), to = sm + At::base(step % 3);
-                const int c0 = (step0 + step) * kColumns;
-                if constexpr (!BACK) {           // rows are columns
+            const int c0 = (step0 + step) * kColumns;
+            if (a.base && step < steps && c0 + u8 * 8 < a.c_out) {
+                const uint32_t to = sm + At::base(step & 3);
 #pragma unroll
-                    for (int q0 = 0; q0 < kColumns * UNITS; q0 += kCopy) {
-                        const int q = q0 + tid, r = q / UNITS, u = q % UNITS;
-                        const bool ok = c0 + r < a.c_out && u * 8 < a.rank;
-                        if (kColumns * UNITS >= kCopy || q < kColumns * UNITS) copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(c0 + r) * a.rank + u * 8 : up, ok);
-                    }
-                } else {                         // rows are ranks
-                    const int c = c0 + u8 * 8;
-#pragma unroll
-                    for (int q = 0; q < (RB + 31) / 32; ++q) {
-                        const int r = r32 + 32 * q;
-                        const bool ok = r < a.rank && c < a.c_out;
-                        if (RB >= 32 || r < RB) copy16(tile_at(at, r, u8), ok ? up + static_cast<size_t>(r) * a.c_out + c : up, ok);
-                    }
-                }
-                if (a.base && c0 + u4 * 8 < a.c_out) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (at_row[i] >= 0) copy16(tile_at(to, r4 + 8 * i, u4), base + at_row[i] + c0, true);
-                }
+                for (int i = 0; i < 8; ++i)
+                    if (at_row[i] >= 0) copy16(tile_at(to, r8 + 4 * i, u8), base + at_row[i] + c0, true);
             }
             copy_commit();
         };
-        request(0);
-        request(1);
-        if (a.base && steps > 2 && tid < static_cast<int>(tile.n) && ctl->row_of[tid] >= 0) {      // and the rest comes into L2 while the sums are on their way
-            const int c0 = (step0 + 2) * kColumns;
+        request(group);
+        if (group + 2 < At::kEarly) request(group + 2);
+        if (a.base && steps > At::kEarly && tid < static_cast<int>(tile.n) && ctl->row_of[tid] >= 0) {       // and the rest comes into L2 while the sums are on their way
+            const int c0 = (step0 + At::kEarly) * kColumns;
             asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(base + static_cast<size_t>(ctl->row_of[tid]) * a.c_out + c0), "r"((c_end - c0) * 2) : "memory");
         }
         const float scale = a.scales ? a.scales[expert] : 1.0f;
@@ -336,48 +357,49 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         const float factor = DT == MTC_F16 ? scale * __uint_as_float(static_cast<uint32_t>(ctl->unit[row]) << 23) : scale;
 
         // ---- 64 columns at a time; warps do not wait for each other
-        copy_wait<1>();
-        to_async_proxy();
-        if (steps > 0) mbar_arrive(&ctl->columns[0]);
-        for (int j = 0; j < steps; ++j) {
-            request(j + 2);                      // (in place of step j - 1, which this thread has seen multiplied and this warp has given out)
-            copy_wait<1>();
-            to_async_proxy();
-            if (j + 1 < steps) mbar_arrive(&ctl->columns[(j + 1) % 3]);
+        if (group + 2 >= At::kEarly) request(group + 2);
+        for (int j = group; j < steps; j += 2) {
+            copy_wait<1>();                      // base of this step
             __syncwarp();
-            uint8_t *const tile_base = data + At::base(j % 3);
+            uint8_t *const tile_base = data + At::base(j & 3);
             uint4 *const line = reinterpret_cast<uint4 *>(tile_base + row * 128);
-            lora::Eight<DT> b[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 q = a.base ? line[(half + i) ^ (row & 7)] : make_uint4(0, 0, 0, 0);
-                b[i].w[0] = q.x, b[i].w[1] = q.y, b[i].w[2] = q.z, b[i].w[3] = q.w;
-            }
-            mbar_wait_warp(&ctl->out[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb29u);
+            mbar_wait_warp(&ctl->out[group], (j >> 1) & 1, &ctl->abort, a.status, 0xb29u);
             tc_fence_after();
-            uint32_t v[32];
-            tmem_ld<32>(tmem + kOut + (j & 1) * kColumns + half * 8 + lanes, v);
-            tmem_wait_ld();
-            tc_fence_before();
-            mbar_arrive(&ctl->free[j & 1]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float r[8];
+            for (int half = 0; half < 8; half += 4) {
+                lora::Eight<DT> b[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fmaf(__uint_as_float(v[8 * i + k]), factor, b[i].value(k));
-                lora::Eight<DT>::put(&line[(half + i) ^ (row & 7)], 0, r);
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 q = a.base ? line[(half + i) ^ (row & 7)] : make_uint4(0, 0, 0, 0);
+                    b[i].w[0] = q.x, b[i].w[1] = q.y, b[i].w[2] = q.z, b[i].w[3] = q.w;
+                }
+                uint32_t v[32];
+                tmem_ld<32>(tmem + kOut + group * kColumns + half * 8 + lanes, v);
+                tmem_wait_ld();
+                if (half) {
+                    tc_fence_before();
+                    mbar_arrive(&ctl->free[group]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float r[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) r[k] = fmaf(__uint_as_float(v[8 * i + k]), factor, b[i].value(k));
+                    lora::Eight<DT>::put(&line[(half + i) ^ (row & 7)], 0, r);
+                }
             }
             __syncwarp();
-            uint4 q[4];
+            uint4 q[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const uint4 *>(tile_base + (r4 + 8 * i) * 128 + ((u4 ^ (r4 & 7)) << 4));
+            for (int i = 0; i < 8; ++i) q[i] = *reinterpret_cast<const uint4 *>(tile_base + (r8 + 4 * i) * 128 + ((u8 ^ ((r8 + 4 * i) & 7)) << 4));
             const int c0 = (step0 + j) * kColumns;
-            if (c0 + u4 * 8 < a.c_out) {
+            if (c0 + u8 * 8 < a.c_out) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 8; ++i)
                     if (at_row[i] >= 0) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + at_row[i] + c0) = q[i];
             }
             __syncwarp();
+            request(j + 4);                      // in this step's place
         }
         copy_wait<0>();
     }
