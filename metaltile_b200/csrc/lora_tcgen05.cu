@@ -26,11 +26,12 @@ namespace {
 
 using namespace lora;
 
+
 constexpr int kCopy = 256, kMmaWarp = 8, kLoadWarp = 9, kThreads = kCopy + 64, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
 constexpr int kStage = 24 * 1024, kWeights = 16 * 1024;                              // of a stage: where the weights start
 constexpr int kHeld = 0, kPiece = 16 * 1024, kColumns = 64;
 constexpr int kSmem = 1024 + 112 * 1024;
-constexpr uint32_t kTmem = 256, kSums = 0, kOut = 64;                                // columns of tensor memory
+constexpr uint32_t kTmem = 256, kSums = 0;           // columns of tensor memory: the first product's sums, later four steps of the second one (so that weights wait for no result)
 
 // Ranks 64: the sums of eight CTAs for sixteen rows are 32 KB, a stage less.  Base of the first steps comes in before the sums do: only the last buffer takes their place.
 template <int RB>
@@ -45,7 +46,7 @@ static_assert(Room<64>::kFrom == 72 * 1024 && Room<32>::kFrom == 96 * 1024, "sum
 struct Ctrl {
     int row_of[kRows];
     uint8_t unit[kRows];                         // f16: exponent of what a row of h was divided by
-    uint64_t full[4], empty[4], columns[2], out[2], free[2], done, sums, held;
+    uint64_t full[4], empty[4], columns[2], out[4], free[4], done, sums, held;
     uint32_t tmem, abort;
 };
 static_assert(sizeof(Ctrl) <= 1024, "control block");
@@ -89,6 +90,9 @@ __device__ __forceinline__ void send_bulk(uint32_t at, uint32_t from, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at), "r"(from), "r"(bytes), "r"(bar) : "memory");
 }
 
+// into L2, 16-byte aligned
+__device__ __forceinline__ void prefetch(const void *p, int bytes) { asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory"); }
+
 // Units of a row of sums are moved about so that neighbouring rows do not meet in a bank
 template <int RB>
 __device__ __forceinline__ int sums_swizzle(int r) { return RB == 16 ? r >> 1 & 3 : r & 7; }
@@ -109,6 +113,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
     const Tile tile = find_tile(a, blockIdx.x / kCluster, kRows, none);
     if (tile.e < 0) return;                                  // the whole cluster
+    const int chunks = (a.c_in + 63) / 64;
+    const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * cr / kCluster), mine = static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / kCluster) - chunk0;
     if (tid < kRows) {
         int row = -1;
         if (tid < static_cast<int>(tile.n)) {
@@ -133,7 +139,8 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     }
     if (tid == 0) {
         for (int i = 0; i < kStages; ++i) mbar_init(&ctl->full[i], kCopy), mbar_init(&ctl->empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&ctl->columns[i], 32), mbar_init(&ctl->out[i], 1), mbar_init(&ctl->free[i], kCopy / 2);
+        for (int i = 0; i < 2; ++i) mbar_init(&ctl->columns[i], 32);
+        for (int i = 0; i < 4; ++i) mbar_init(&ctl->out[i], 1), mbar_init(&ctl->free[i], kCopy / 2);
         mbar_init(&ctl->done, 1), mbar_init(&ctl->sums, 1), mbar_init(&ctl->held, 1);
         ctl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -146,9 +153,6 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     cluster_arrive();                                        // the barriers are there: waited for before anything is sent
     asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
-    const int chunks = (a.c_in + 63) / 64;
-    const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * cr / kCluster), mine = static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / kCluster) - chunk0;
-
     if (warp == kMmaWarp) {
         // ---- products; the operands' addresses are the same for the whole warp
         for (int c = 0; c < mine; ++c) {
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         cluster_arrive();                        // nobody leaves while it sends: waited for at the end
         for (int j = 0; j < steps; ++j) {
             mbar_wait_warp(&ctl->columns[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb23u);
-            if (j >= 2) mbar_wait_warp(&ctl->free[j & 1], (j / 2 - 1) & 1, &ctl->abort, a.status, 0xb24u);
+            if (j >= 4) mbar_wait_warp(&ctl->free[j & 3], (j / 4 - 1) & 1, &ctl->abort, a.status, 0xb24u);
             tc_fence_after();
             const uint64_t w = desc_of(sm + At::weights(j & 1)), h = desc_of(sm + kHeld);
             if (elect_one()) {
@@ -186,32 +190,40 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
                 for (int p = 0; p < 2; ++p)
 #pragma unroll
                     for (int q = 0; q < RB / 16; ++q)
-                        umma_f16_ss(tmem + kOut + (j & 1) * kColumns, h + (p * kPiece >> 4) + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, kColumns, BACK), p || q ? 1u : 0u);
-                umma_commit(&ctl->out[j & 1]);
+                        umma_f16_ss(tmem + (j & 3) * kColumns, h + (p * kPiece >> 4) + 2 * q, w + (BACK ? 128 : 2) * q, idesc_of(DT, kColumns, BACK), p || q ? 1u : 0u);
+                umma_commit(&ctl->out[j & 3]);
             }
             __syncwarp();
         }
     } else if (warp == kLoadWarp) {
         // ---- the second product's weights: 64 columns of every rank
         const uint16_t *const up = static_cast<const uint16_t *>(a.up) + static_cast<size_t>(tile.e) * a.rank * a.c_out;
+        // into L2 while the first product runs: steps are read two ahead, which is less than the way to memory takes
+        if (steps > 0) {
+            const int c0 = step0 * kColumns;
+            if constexpr (BACK) {
+                for (int r = lane; r < a.rank; r += 32) prefetch(up + static_cast<size_t>(r) * a.c_out + c0, (c_end - c0) * 2);
+            } else {
+                const int bytes = (c_end - c0) * a.rank * 2;
+                for (int i = lane * 4096; i < bytes; i += 32 * 4096) prefetch(up + static_cast<size_t>(c0) * a.rank + i / 2, std::min(4096, bytes - i));
+            }
+        }
         cluster_wait();
         __syncthreads();                         // the ring is free
+        // a lane's unit stays, its rows (columns; BACK: ranks) are ROWS apart
+        constexpr int WIDE = BACK ? 8 : UNITS, ROWS = 32 / WIDE, TURNS = (BACK ? RB : kColumns) / ROWS;
+        const int r0 = lane / WIDE, u = lane % WIDE;
         auto request = [&](int step) {
             if (step < steps) {
-                const uint32_t at = sm + At::weights(step & 1);
-                const int c0 = (step0 + step) * kColumns;
+                const int c0 = (step0 + step) * kColumns, last = BACK ? a.rank : a.c_out - c0;       // rows that exist
+                const bool unit = BACK ? c0 + u * 8 < a.c_out : u * 8 < a.rank;
+                const uint32_t at = sm + At::weights(step & 1) + r0 * 128;
+                const uint16_t *const from = BACK ? up + static_cast<size_t>(r0) * a.c_out + c0 + u * 8 : up + static_cast<size_t>(c0 + r0) * a.rank + u * 8;
+                const size_t apart = static_cast<size_t>(ROWS) * (BACK ? a.c_out : a.rank);
 #pragma unroll
-                for (int q0 = 0; q0 < kColumns * UNITS; q0 += 32) {
-                    const int q = q0 + lane;
-                    if constexpr (!BACK) {       // rows are columns
-                        const int r = q / UNITS, u = q % UNITS;
-                        const bool ok = c0 + r < a.c_out && u * 8 < a.rank;
-                        copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(c0 + r) * a.rank + u * 8 : up, ok);
-                    } else {                     // rows are ranks
-                        const int r = q >> 3, u = q & 7, c = c0 + u * 8;
-                        const bool ok = r < a.rank && c < a.c_out;
-                        copy16(tile_at(at, r, u), ok ? up + static_cast<size_t>(r) * a.c_out + c : up, ok);
-                    }
+                for (int i = 0; i < TURNS; ++i) {
+                    const bool ok = unit && r0 + i * ROWS < last;
+                    copy16(at + i * ROWS * 128 + ((u ^ ((r0 + i * ROWS) & 7)) << 4), ok ? from + i * apart : up, ok);
                 }
             }
             copy_commit();
@@ -224,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             copy_wait<1>();
             to_async_proxy();
             mbar_arrive(&ctl->columns[j & 1]);
-            mbar_wait_warp(&ctl->out[j & 1], (j >> 1) & 1, &ctl->abort, a.status, 0xb2au);       // step j is multiplied: its place is free
+            mbar_wait_warp(&ctl->out[j & 3], (j >> 2) & 1, &ctl->abort, a.status, 0xb2au);       // step j is multiplied: its place is free
             request(j + 2);
         }
         copy_wait<0>();
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
         if (group + 2 < At::kEarly) request(group + 2);
         if (a.base && steps > At::kEarly && tid < static_cast<int>(tile.n) && ctl->row_of[tid] >= 0) {       // and the rest comes into L2 while the sums are on their way
             const int c0 = (step0 + At::kEarly) * kColumns;
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(base + static_cast<size_t>(ctl->row_of[tid]) * a.c_out + c0), "r"((c_end - c0) * 2) : "memory");
+            prefetch(base + static_cast<size_t>(ctl->row_of[tid]) * a.c_out + c0, (c_end - c0) * 2);
         }
         const float scale = a.scales ? a.scales[expert] : 1.0f;
 
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             __syncwarp();
             uint8_t *const tile_base = data + At::base(j & 3);
             uint4 *const line = reinterpret_cast<uint4 *>(tile_base + row * 128);
-            mbar_wait_warp(&ctl->out[group], (j >> 1) & 1, &ctl->abort, a.status, 0xb29u);
+            mbar_wait_warp(&ctl->out[j & 3], (j >> 2) & 1, &ctl->abort, a.status, 0xb29u);
             tc_fence_after();
 #pragma unroll
             for (int half = 0; half < 8; half += 4) {
@@ -374,11 +386,11 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
                     b[i].w[0] = q.x, b[i].w[1] = q.y, b[i].w[2] = q.z, b[i].w[3] = q.w;
                 }
                 uint32_t v[32];
-                tmem_ld<32>(tmem + kOut + group * kColumns + half * 8 + lanes, v);
+                tmem_ld<32>(tmem + (j & 3) * kColumns + half * 8 + lanes, v);
                 tmem_wait_ld();
                 if (half) {
                     tc_fence_before();
-                    mbar_arrive(&ctl->free[group]);
+                    mbar_arrive(&ctl->free[j & 3]);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -408,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     tc_fence_after();
     if (ctl->abort && tid == 0) {                // gave up: bounded waits for MMAs that may still be on their way
         drain_ring(ctl->empty, mine, kStages);
-        drain_ring(ctl->out, steps, 2);
+        drain_ring(ctl->out, steps, 4);
     }
     __syncthreads();
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem));
