@@ -49,7 +49,7 @@ struct Split {
 // RB: ranks a pass.  Columns of a CTA: four warps of NT tiles of eight; the other four take the other half of the rows.
 template <int DT, int RB>
 struct Form {
-    static constexpr int NT = DT == MTC_F32 || RB == 64 ? 4 : 8, CB = 32 * NT, RP = RB < 16 ? 16 : RB, MT = RP / 16, H = DT == MTC_F32 ? 3 : 2;
+    static constexpr int NT = DT == MTC_F32 || RB >= 32 ? 4 : 8, CB = 32 * NT, RP = RB < 16 ? 16 : RB, MT = RP / 16, H = DT == MTC_F32 ? 3 : 2;
     static constexpr int AHEAD = DT == MTC_F32 ? 2 : 3;              // buffers of x or dy
     // bytes of a row of a stage (16 bytes apart modulo 128, so that the rows of a fragment do not meet in a bank), of a stage, of a row of an operand piece
     static constexpr int SIZE = DT == MTC_F32 ? 4 : 2, PITCH = CB * SIZE + 16, tile = kStage * PITCH, LOW = RP * 2;
@@ -58,7 +58,7 @@ struct Form {
 };
 
 template <int DT, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 64 || DT == MTC_F32 ? 1 : 2) lora_weights_kernel(const LoraWeights w, int blocks_a, int blocks_b, int rank_blocks) {
+__global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_kernel(const LoraWeights w, int blocks_a, int blocks_b, int rank_blocks) {
     pdl_enter();
     using F = Form<DT, RB>;
     using S = Split<DT, F::NT>;
@@ -213,23 +213,32 @@ __global__ void __launch_bounds__(kThreads, RB == 64 || DT == MTC_F32 ? 1 : 2) l
                 const int r = 16 * m + g + (i >= 2 ? 8 : 0), c = (warp & 3) * 8 * NT + (2 * t + (i & 1)) * NT + j;
                 sums[half * lines * stride + (of_a ? r * stride + c : c * stride + r)] = acc[m][j][i];
             }
-    cluster_arrive();
-    cluster_wait();
+    const bool alone = cs == 1;                  // (a barrier of the cluster is a thousand cycles)
+    if (alone) __syncthreads();
+    else cluster_arrive(), cluster_wait();
     const float scale = w.scales ? w.scales[e] : 1.0f;
     const bool aligned = reinterpret_cast<uintptr_t>(W.grad) % 16 == 0;
     const int used = of_a ? n_ranks : n_cols, wide = of_a ? n_cols : n_ranks, in_line = (wide + 3) / 4;
     for (int i = tid + cr * kThreads; i < used * in_line; i += kThreads * cs) {
         const int line = i / in_line, k = i % in_line * 4;
-        float4 part[8][2];                       // (all on their way at once: one after the other they took 5000 cycles)
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) part[q][h] = q < cs ? ld_cta(sums + (h * lines + line) * stride + k, q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float v[4] = {};
+        if (alone) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
+            for (int h = 0; h < 2; ++h) {
+                const float4 f = *reinterpret_cast<const float4 *>(sums + (h * lines + line) * stride + k);
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+            }
+        } else {
+            float4 part[8][2];                   // (all on their way at once: one after the other they took 5000 cycles)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) v[0] += part[q][h].x, v[1] += part[q][h].y, v[2] += part[q][h].z, v[3] += part[q][h].w;
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) part[q][h] = q < cs ? ld_cta(sums + (h * lines + line) * stride + k, q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[0] += part[q][h].x, v[1] += part[q][h].y, v[2] += part[q][h].z, v[3] += part[q][h].w;
+        }
         const size_t at = of_a ? (e * w.rank + r0 + line) * W.c + c0 + k : (e * W.c + c0 + line) * w.rank + r0 + k;
         if (k + 4 <= wide && at % 4 == 0 && aligned) {
             if constexpr (DT == MTC_F32) {
@@ -247,8 +256,7 @@ __global__ void __launch_bounds__(kThreads, RB == 64 || DT == MTC_F32 ? 1 : 2) l
                 if (k + q < wide) st_from_f32(W.grad, at + q, v[q] * scale, DT);
         }
     }
-    cluster_arrive();
-    cluster_wait();                              // nobody leaves while its sums are read
+    if (!alone) cluster_arrive(), cluster_wait();        // nobody leaves while its sums are read
 }
 
 bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

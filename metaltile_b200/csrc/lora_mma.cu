@@ -395,7 +395,10 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
 }
 template <int DT>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
-    const bool wide = a.n_rows > 32 * a.n_adapters;
+    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
+    // and 9.3, 1024 15.5 and 10.7; f32 forward rank 8, 1024 rows 22.7 and 37, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0; f32 back (with the weights' gradients) rank 8, 128 17.4 and
+    // 21.1, 256 22.6 and 20.0
+    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && (backward || a.rank > 16);
     if (wide) return backward ? launch<DT, 2, true>(st, a, keep, none) : launch<DT, 2, false>(st, a, keep, none);
     return backward ? launch<DT, 1, true>(st, a, keep, none) : launch<DT, 1, false>(st, a, keep, none);
 }

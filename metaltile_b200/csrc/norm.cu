@@ -312,20 +312,22 @@ __global__ void __launch_bounds__(256) norm_grad_values_kernel(const NormGradArg
 }
 
 // dw = the shares added up in f64: 32 columns a CTA, whose warps take the shares in turn
-__global__ void __launch_bounds__(1024) norm_grad_join_kernel(const float *part, void *dweight, int workers, int K, int dt) {
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) norm_grad_join_kernel(const float *part, void *dweight, int workers, int K, int dt) {
     pdl_enter();
-    __shared__ double sums[32][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    __shared__ double sums[WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long k = static_cast<long long>(blockIdx.x) * 32 + lane;
     double acc = 0.0;
     if (k < K) {
-#pragma unroll 16
-        for (int p = warp; p < workers; p += warps) acc += part[static_cast<size_t>(p) * K + k];
+#pragma unroll 8
+        for (int p = warp; p < workers; p += WARPS) acc += part[static_cast<size_t>(p) * K + k];
     }
     sums[warp][lane] = acc;
     __syncthreads();
     if (warp == 0 && k < K) {
-        for (int i = 1; i < warps; ++i) acc += sums[i][lane];
+#pragma unroll
+        for (int i = 1; i < WARPS; ++i) acc += sums[i][lane];
         st_from_f32(dweight, k, static_cast<float>(acc), dt);
     }
 }
@@ -414,7 +416,9 @@ cudaError_t launch_norm_grad(Ctx *ctx, cudaStream_t st, NormGradArgs a, void *dw
         const cudaError_t e = (dt == MTC_F32 ? launch_grad<MTC_F32> : dt == MTC_BF16 ? launch_grad<MTC_BF16> : launch_grad<MTC_F16>)(g, st, a);
         if (e != cudaSuccess) return e;
     }
-    return launch_pdl(norm_grad_join_kernel, dim3((a.K + 31u) / 32u), a.workers > 256 ? 1024 : 512, 0, st, a.part, dweight, a.workers, a.K, dt);      // no rows: zeros
+    const dim3 grid((a.K + 31u) / 32u);          // (no rows: zeros)
+    return a.workers > 256 ? launch_pdl(norm_grad_join_kernel<32>, grid, 1024, 0, st, a.part, dweight, a.workers, a.K, dt)
+                           : launch_pdl(norm_grad_join_kernel<16>, grid, 512, 0, st, a.part, dweight, a.workers, a.K, dt);
 }
 
 }  // namespace mtc
