@@ -478,8 +478,7 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
  * base (NULL: 0) T[n_rows, K] is the shared projection's gradient of x and may be dx; da, db in the type and shape of a, b, zeros for adapters without rows.
  * Sums run in an order that the sizes fix. */
 int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
-                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace, size_t workspace_bytes);
-size_t mtc_lora_mm_workspace(const mtc_ctx *ctx, int n_rows, int K, int N, int rank, int n_adapters, int dtype);
+                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype);
 int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *hidden,
                   const void *scales, const void *base, void *dx, void *da, void *db, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace,
                   size_t workspace_bytes);

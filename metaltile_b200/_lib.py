@@ -127,8 +127,7 @@ SIGNATURES = {
     "mtc_add_rms_norm_fp8": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 4 + [_i] * 4),
     "mtc_add_rms_norm_grad": (_i, [_vp] * 5 + [ctypes.c_float] + [_vp] * 3 + [_i] * 3 + [_vp, _sz]),
     "mtc_add_rms_norm_grad_workspace": (_sz, [_vp, _i, _i, _i]),
-    "mtc_lora_mm": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _sz]),
-    "mtc_lora_mm_workspace": (_sz, [_vp] + [_i] * 6),
+    "mtc_lora_mm": (_i, [_vp] * 11 + [_i] * 6),
     "mtc_lora_grad": (_i, [_vp] * 14 + [_i] * 6 + [_vp, _sz]),
     "mtc_lora_grad_workspace": (_sz, [_vp] + [_i] * 6),
     "mtc_set_option": (_i, [_vp, ctypes.c_char_p, _i]),

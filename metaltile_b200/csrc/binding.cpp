@@ -1048,12 +1048,9 @@ PyObject *lora_mm(Args a, Py_ssize_t n) {
         if (!given) out = empty({o.M, o.N}, o.x.scalar_type(), o.x);
         if (keep) hidden = empty({o.M, o.rank}, at::kFloat, o.x);
         const int M = static_cast<int>(o.M), K = static_cast<int>(o.K), N = static_cast<int>(o.N), r = static_cast<int>(o.rank), L = static_cast<int>(o.L);
-        const size_t need = mtc_lora_mm_workspace(c.h, M, K, N, r, L, o.dt);
-        at::Tensor space;
-        if (need) space = empty({static_cast<int64_t>(need)}, at::kByte, o.x);
         return mtc_lora_mm(c.h, on_stream(o.x), o.x.data_ptr(), o.a.data_ptr(), o.b.data_ptr(), o.rows.data_ptr(), o.offsets.data_ptr(),
                            o.scales ? o.scales->data_ptr() : nullptr, base ? base->data_ptr() : nullptr, out.data_ptr(), keep ? hidden.data_ptr() : nullptr, M, K, N, r, L,
-                           o.dt, need ? space.data_ptr() : nullptr, need);
+                           o.dt);
     }));
     if (keep) return tuple_of({&out, &hidden});
     return given ? same(a[7]) : wrap(std::move(out));

@@ -9,7 +9,6 @@
 namespace mtc {
 
 constexpr int kMostRank = 1024, kMostAdapters = 65536;
-inline size_t lora_workspace(int n_rows, int rank) { return static_cast<size_t>(n_rows) * rank * 4; }      // `low`
 
 // One of the two directions: rows [n_rows, c_in] -> low [n_rows, rank] -> rows [n_rows, c_out]
 struct LoraArgs {
@@ -18,7 +17,7 @@ struct LoraArgs {
     const float *scales;                         // null: 1
     const void *base;                            // null: 0; may be out
     void *out;
-    float *low;                                  // f32[n_rows, rank]: h, or u
+    float *low;                                  // f32[n_rows, rank], where it is kept: h, or u
     int n_rows, c_in, c_out, rank, n_adapters;
     uint32_t *status;
 };
@@ -39,14 +38,14 @@ struct LoraWeights {
 
 // keep: `low` is wanted; all: with zeros for the rows of no adapter
 cudaError_t launch_lora(Ctx *ctx, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt);
-cudaError_t launch_lora_weights(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);
 
 // The tensor-core kernels (lora_mma.cu, lora_grad.cu) and what they take; `none`: rows of no adapter have something to be written
-bool lora_mma_supported(const LoraArgs &a);
+enum class LoraForm { none, values, pieces };    // rows of any length, or of whole 16-byte pieces
+LoraForm lora_mma_form(const LoraArgs &a, bool backward, int dt);
 cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
 bool lora_tile_supported(const LoraArgs &a, bool keep, int dt);       // (lora_tcgen05.cu) what of the above it takes
 cudaError_t launch_lora_tile(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
-bool lora_grad_supported(const LoraWeights &w);
+// (lora_grad.cu) any size and alignment
 cudaError_t launch_lora_grad(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);
 
 }  // namespace mtc

@@ -57,7 +57,7 @@ struct Form {
     static constexpr size_t smem = (sums > AHEAD * tile + staged ? sums : AHEAD * tile + staged);    // (the sums take the stages' place)
 };
 
-template <int DT, int RB>
+template <int DT, int RB, bool VEC>
 __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_kernel(const LoraWeights w, int blocks_a, int blocks_b, int rank_blocks) {
     pdl_enter();
     using F = Form<DT, RB>;
@@ -98,6 +98,19 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
             for (int i = 0; i < PASSES; ++i) {
                 const int r = (i * kThreads + tid) / UNITS, row = row_of[s % kRowsAhead][r];
                 const bool ok = row >= 0 && c < W.c;
+                if constexpr (!VEC) {            // rows of any length: values one by one
+                    constexpr int N = 16 / F::SIZE;
+                    uint32_t v[4] = {};
+#pragma unroll
+                    for (int j = 0; j < N; ++j)
+                        if (ok && c + j < W.c) {
+                            const size_t at = static_cast<size_t>(row) * W.c + c + j;
+                            if constexpr (DT == MTC_F32) v[j] = static_cast<const uint32_t *>(W.in)[at];
+                            else v[j / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(W.in)[at]) << (j & 1) * 16;
+                        }
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(base + s % F::AHEAD * F::tile + r * F::PITCH + u * 16), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                    continue;
+                }
                 const char *const src = static_cast<const char *>(W.in) + (ok ? (static_cast<size_t>(row) * W.c + c) * F::SIZE : 0);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + s % F::AHEAD * F::tile + r * F::PITCH + u * 16), "l"(src), "r"(ok ? 16 : 0) : "memory");
             }
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
 
 bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <int DT, int RB>
+template <int DT, int RB, bool VEC = true>
 cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {
     using F = Form<DT, RB>;
     const long long rank_blocks = (w.rank + RB - 1) / RB, blocks_a = (w.a.c + F::CB - 1) / F::CB, blocks_b = (w.b.c + F::CB - 1) / F::CB;
@@ -272,13 +285,15 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {
     while (cs < 8 && items * cs < 2ll * ctx->sm_count && rows >= 2ll * kStage * cs * 2) cs *= 2;
     if (items * cs > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     static PerDeviceAttr attr;
-    const cudaError_t e = attr.set(lora_weights_kernel<DT, RB>, F::smem);
+    const cudaError_t e = attr.set(lora_weights_kernel<DT, RB, VEC>, F::smem);
     if (e != cudaSuccess) return e;
-    return launch_cluster(lora_weights_kernel<DT, RB>, static_cast<unsigned>(items * cs), kThreads, cs, F::smem, st, w, static_cast<int>(blocks_a), static_cast<int>(blocks_b),
+    return launch_cluster(lora_weights_kernel<DT, RB, VEC>, static_cast<unsigned>(items * cs), kThreads, cs, F::smem, st, w, static_cast<int>(blocks_a), static_cast<int>(blocks_b),
                           static_cast<int>(rank_blocks));
 }
 template <int DT>
 cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {
+    if (w.a.c % 8 || w.b.c % 8 || !on_16(w.a.in) || !on_16(w.b.in))                  // two sizes of the rank are enough
+        return w.rank <= 16 ? launch<DT, 16, false>(ctx, st, w) : launch<DT, DT == MTC_F32 ? 32 : 64, false>(ctx, st, w);
     if (w.rank <= 8) return launch<DT, 8>(ctx, st, w);
     if (w.rank <= 16) return launch<DT, 16>(ctx, st, w);
     if (DT == MTC_F32 || w.rank <= 32) return launch<DT, 32>(ctx, st, w);
@@ -287,7 +302,6 @@ cudaError_t launch(Ctx *ctx, cudaStream_t st, const LoraWeights &w) {
 
 }  // namespace
 
-bool lora_grad_supported(const LoraWeights &w) { return w.a.c % 8 == 0 && w.b.c % 8 == 0 && on_16(w.a.in) && on_16(w.b.in); }
 cudaError_t launch_lora_grad(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt) {
     return (dt == MTC_F32 ? launch<MTC_F32> : dt == MTC_BF16 ? launch<MTC_BF16> : launch<MTC_F16>)(ctx, st, w);
 }

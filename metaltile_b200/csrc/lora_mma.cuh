@@ -64,16 +64,33 @@ struct Vals {
             } else {
                 v[0] = *p;
             }
+            split(v);
+        }
+    }
+    // n of them exist, any alignment
+    __device__ __forceinline__ void load_any(const void *base, size_t at, int n) {
+        if constexpr (DT == MTC_F32) {
+            float v[W];
 #pragma unroll
-            for (int k = 0; k < 3; ++k) {
+            for (int i = 0; i < W; ++i) v[i] = i < n ? static_cast<const float *>(base)[at + i] : 0.0f;
+            split(v);
+        } else {
+            zero();
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float lo = v[2 * i], hi = W == 1 ? 0.0f : v[W == 1 ? 0 : 2 * i + 1];
-                    w[k][i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
-                }
+            for (int i = 0; i < W; ++i)
+                if (i < n) w[0][i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(base)[at + i]) << (i & 1) * 16;
+        }
+    }
+    __device__ __forceinline__ void split(float (&v)[W]) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
+        for (int k = 0; k < P; ++k) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float lo = v[2 * i], hi = W == 1 ? 0.0f : v[W == 1 ? 0 : 2 * i + 1];
+                w[k][i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
             }
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
         }
     }
     // value j of x with value j of y, as a pair
@@ -111,17 +128,34 @@ struct Eight {
             w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
         }
     }
+    __device__ __forceinline__ void load_any(const void *base, size_t at, int n) {
+#pragma unroll
+        for (int i = 0; i < (DT == MTC_F32 ? 8 : 4); ++i) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= n) break;
+            if constexpr (DT == MTC_F32) w[i] = static_cast<const uint32_t *>(base)[at + i];
+            else w[i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(base)[at + i]) << (i & 1) * 16;
+        }
+    }
     __device__ __forceinline__ float value(int i) const {
         if constexpr (DT == MTC_F32) return __uint_as_float(w[i]);
         const uint32_t u = w[i / 2];
         if constexpr (DT == MTC_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
         return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? u >> 16 : u)));
     }
-    __device__ __forceinline__ void add_and_store(void *out, size_t at, const float (&v)[8], float factor) const {
+    template <bool VEC = true>
+    __device__ __forceinline__ void add_and_store(void *out, size_t at, const float (&v)[8], float factor, int n = 8) const {
         float r[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[i] = fmaf(v[i], factor, value(i));
-        put(out, at, r);
+        if constexpr (VEC) {
+            put(out, at, r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < n) st_from_f32(out, at + i, r[i], DT);
+        }
     }
     static __device__ __forceinline__ void put(void *out, size_t at, const float (&r)[8]) {
         if constexpr (DT == MTC_F32) {
@@ -231,18 +265,19 @@ __device__ __forceinline__ void hold(float4 s, float unit, uint16_t *at, int apa
 }
 
 // Rows of no adapter, by the CTAs of a cluster: columns from .. to of this one; zeros of `low` where it is kept
-template <int DT, int THREADS>
+template <int DT, int THREADS, bool VEC = true>
 __device__ __forceinline__ void copy_rows(const LoraArgs &a, const int *row_of, int n, int from, int to, bool keep, int cr, int cs) {
     if (a.base != a.out) {
-        const int eights = max(to - from, 0) / 8;
+        const int eights = (max(to - from, 0) + 7) / 8;
         for (int i = threadIdx.x; i < n * eights; i += THREADS) {
             const int row = row_of[i / eights], c = from + i % eights * 8;
             if (row < 0) continue;
             const size_t at = static_cast<size_t>(row) * a.c_out + c;
             Eight<DT> v;
-            v.load(a.base, at, a.base != nullptr);
+            if constexpr (VEC) v.load(a.base, at, a.base != nullptr);
+            else v.load_any(a.base, at, a.base ? to - c : 0);
             const float zero[8] = {};
-            v.add_and_store(a.out, at, zero, 1.0f);
+            v.template add_and_store<VEC>(a.out, at, zero, 1.0f, to - c);
         }
     }
     if (keep)

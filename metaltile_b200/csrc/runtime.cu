@@ -1709,26 +1709,21 @@ static int lora_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int K, int N,
     return MTC_OK;
 }
 
-size_t mtc_lora_mm_workspace(const mtc_ctx *, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
-    return lora_sizes_ok(n_rows, K, N, rank, n_adapters) && dtype_ok(dtype) ? mtc::lora_workspace(n_rows, rank) : 0;
-}
-size_t mtc_lora_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
-    return mtc_lora_mm_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype);
+size_t mtc_lora_grad_workspace(const mtc_ctx *, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
+    return lora_sizes_ok(n_rows, K, N, rank, n_adapters) && dtype_ok(dtype) ? static_cast<size_t>(n_rows) * rank * 4 : 0;     // u
 }
 
 int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
-                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype, void *workspace, size_t workspace_bytes) {
+                void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
     return guarded(ctx, [&]() -> int {
         MTC_ENTER(ctx);
-        int rc = lora_args_ok(ctx, "lora_mm", n_rows, K, N, rank, n_adapters, dtype);
+        const int rc = lora_args_ok(ctx, "lora_mm", n_rows, K, N, rank, n_adapters, dtype);
         if (rc != MTC_OK || n_rows == 0) return rc;
         if (!x || !a || !b || !rows || !offsets || !out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: null pointer");
-        rc = check_workspace(ctx, "lora_mm", workspace, workspace_bytes, mtc_lora_mm_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype));
-        if (rc != MTC_OK) return rc;
         mtc::LoraArgs l{};
         l.in = x, l.down = a, l.up = b, l.base = base, l.out = out;
         l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
-        l.low = static_cast<float *>(hidden ? hidden : workspace);
+        l.low = static_cast<float *>(hidden);
         l.n_rows = n_rows, l.c_in = K, l.c_out = N, l.rank = rank, l.n_adapters = n_adapters, l.status = ctx->d_status;
         MTC_CUDA(ctx, mtc::launch_lora(ctx, static_cast<cudaStream_t>(stream), l, false, hidden != nullptr, hidden != nullptr, dtype), MTC_ERR_DISPATCH);
         return MTC_OK;
@@ -1755,7 +1750,7 @@ int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, con
         mtc::LoraWeights w{};
         w.a = {x, u, da, K}, w.b = {dy, static_cast<const float *>(hidden), db, N};
         w.order = l.order, w.offsets = l.offsets, w.scales = l.scales, w.n_rows = n_rows, w.rank = rank, w.n_adapters = n_adapters, w.status = ctx->d_status;
-        MTC_CUDA(ctx, mtc::launch_lora_weights(ctx, st, w, dtype), MTC_ERR_DISPATCH);
+        MTC_CUDA(ctx, mtc::launch_lora_grad(ctx, st, w, dtype), MTC_ERR_DISPATCH);
         return MTC_OK;
     });
 }

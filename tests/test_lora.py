@@ -65,7 +65,7 @@ def test_entries_without_a_context_are_refused():
     assert lib.mtc_add_rms_norm(null, null, null, null, null, 0.0, null, null, 1, 8, 0) < 0
     assert lib.mtc_add_rms_norm_fp8(null, null, null, null, null, 0.0, null, null, null, null, 1, 8, 0, 0) < 0
     assert lib.mtc_add_rms_norm_grad(null, null, null, null, null, 0.0, null, null, null, 1, 8, 0, null, 0) < 0
-    assert lib.mtc_lora_mm(*[null] * 11, 1, 8, 8, 8, 1, 0, null, 0) < 0
+    assert lib.mtc_lora_mm(*[null] * 11, 1, 8, 8, 8, 1, 0) < 0
     assert lib.mtc_lora_grad(*[null] * 14, 1, 8, 8, 8, 1, 0, null, 0) < 0
 
 
@@ -74,9 +74,8 @@ def test_workspaces_cover_what_the_calls_keep():
     assert lib.mtc_add_rms_norm_grad_workspace(None, 0, 64, 2) == 0 and lib.mtc_add_rms_norm_grad_workspace(None, 1, 64, 2) >= 264
     assert lib.mtc_add_rms_norm_grad_workspace(None, 9, 0, 2) == lib.mtc_add_rms_norm_grad_workspace(None, 9, 64, 7) == 0
     for rows, rank in ((1, 1), (70000, 64), (1 << 30, 1024)):
-        assert lib.mtc_lora_mm_workspace(None, rows, 64, 64, rank, 3, 2) >= 4 * rows * rank
         assert lib.mtc_lora_grad_workspace(None, rows, 64, 64, rank, 3, 2) >= 4 * rows * rank
-    assert lib.mtc_lora_mm_workspace(None, 1, 64, 64, 0, 3, 2) == 0 and lib.mtc_lora_mm_workspace(None, -1, 64, 64, 1, 3, 2) == 0
+    assert lib.mtc_lora_grad_workspace(None, 1, 64, 64, 0, 3, 2) == 0 and lib.mtc_lora_grad_workspace(None, -1, 64, 64, 1, 3, 2) == 0
 
 
 def _slope(f, v, at, h=1e-6):
