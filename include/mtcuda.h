@@ -75,7 +75,8 @@ int mtc_sync_deadline(mtc_ctx *ctx, void *stream, int timeout_ms);
  * an expert id out of range in mtc_moe_sort), 0x601 + r rank r never arrived at a peer barrier, 0x701 / 0x702 phase counter /
  * partial-sum slot of a chained launch, 0x801-0x831 the tensor-memory decode kernel, 0x901 expert_offsets that run backwards or past the rows,
  * 0x902 more passes than a grouped product's table holds, 0x903 / 0x904 / 0x906 a row index that does not exist, 0x907 an expert that does not exist, 0x908 a row of an adapter that does not exist, 0xa01-0xa0b waits of the exact
- * grouped kernel's roles, 0xb01-0xb06 and 0xb11-0xb16 of the roles of the two tensor-core kernels of e4m3 codes. */
+ * grouped kernel's roles, 0xb01-0xb06 and 0xb11-0xb16 of the roles of the two tensor-core kernels of e4m3 codes,
+ * 0xb21-0xb2a of the tensor-core kernel of low-rank adapters. */
 int mtc_status_word(mtc_ctx *ctx, uint32_t *word);
 int mtc_status_clear(mtc_ctx *ctx);
 
@@ -468,7 +469,7 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
 /* ---- beside a projection: low-rank adapters of many requests (no counterpart in the reference) ----
  * For the rows t of adapter e:   h_t = x_t a[e]^T,   out_t = base_t + scales[e] * h_t b[e]^T           (sums f32, rounded once)
  * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; base may be out.
- * rows u32[n_rows] holds the row numbers, those of one adapter side by side, offsets u32[n_adapters + 1] where each adapter's begin: place p belongs to e where
+ * rows u32[n_rows] holds the row numbers, each once, those of one adapter side by side, offsets u32[n_adapters + 1] where each adapter's begin: place p belongs to e where
  * offsets[e] <= p < offsets[e + 1].  The rows of the other places have no adapter: they get base (0), and stay as they are where base is out.  mtc_moe_sort of the rows'
  * adapters (k = 1, one more "expert" for the rows that have none) writes both.  hidden f32[n_rows, rank] (NULL: not wanted) gets h, zeros for rows without an adapter.
  * Offsets that run backwards or past the rows are clamped and reported through the status word (0x901), row numbers that do not exist are left out and

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kern
     const int units = (a.c_out + CW - 1) / CW, unit0 = static_cast<int>(static_cast<long long>(units) * cr / cs), unit1 = static_cast<int>(static_cast<long long>(units) * (cr + 1) / cs);
     const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
     __syncthreads();
-    if (tile.e == a.n_adapters) {                // rows of no adapter: base, or zeros
+    if (tile.e >= a.n_adapters) {                // rows of no adapter: base, or zeros
         copy_rows<DT, kThreads, VEC>(a, row_of, static_cast<int>(tile.n), unit0 * CW, min(unit1 * CW, a.c_out), keep, cr, cs);
         return;
     }
@@ -391,8 +391,7 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     static PerDeviceAttr attr;
     cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK, ONE, VEC>, 200 * 1024);
     if (e != cudaSuccess) return e;
-    // at most as many tiles as rows, and one of fewer rows for each adapter
-    const long long tiles = std::min<long long>(a.n_rows, a.n_rows / ROWS + a.n_adapters + 1ll);
+    const long long tiles = most_tiles(a, ROWS);
     if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VEC>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, smem, st, a, blocks, keep, none);
 }

@@ -180,21 +180,22 @@ struct Eight {
 };
 
 struct Tile {
-    int e;                                       // n_adapters: rows of none; -1: no such tile
+    int e;                                       // n_adapters and above: rows of none; -1: no such tile
     uint32_t p0, n;
 };
 
 // The tile of this cluster: tiles of `rows` places are dealt out adapter by adapter.  By every warp for itself.
 __device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, bool none) {
-    const int lane = threadIdx.x & 31, last = none ? a.n_adapters : a.n_adapters - 1;
+    // the places behind the last adapter's, and those before the first one's, are of no adapter
+    const int lane = threadIdx.x & 31, last = none ? a.n_adapters + 1 : a.n_adapters - 1;
     const uint32_t R = a.n_rows;
     long long before = 0;                        // offsets that run backwards may name more tiles than 32 bits hold
     for (int e0 = 0; e0 <= last; e0 += 32) {
         const int e = e0 + lane;
         uint32_t from = 0, to = 0;
         if (e <= last) {
-            from = min(a.offsets[e], R);
-            to = e < a.n_adapters ? min(a.offsets[e + 1], R) : R;
+            from = e <= a.n_adapters ? min(a.offsets[e], R) : 0;
+            to = e < a.n_adapters ? min(a.offsets[e + 1], R) : e == a.n_adapters ? R : min(a.offsets[0], R);
         }
         const uint32_t n = to > from ? to - from : 0;
         const long long mine = (static_cast<long long>(n) + rows - 1) / rows;
@@ -268,21 +269,28 @@ __device__ __forceinline__ void hold(float4 s, float unit, uint16_t *at, int apa
 template <int DT, int THREADS, bool VEC = true>
 __device__ __forceinline__ void copy_rows(const LoraArgs &a, const int *row_of, int n, int from, int to, bool keep, int cr, int cs) {
     if (a.base != a.out) {
-        const int eights = (max(to - from, 0) + 7) / 8;
-        for (int i = threadIdx.x; i < n * eights; i += THREADS) {
-            const int row = row_of[i / eights], c = from + i % eights * 8;
+        for (int r = threadIdx.x >> 5; r < n; r += THREADS / 32) {
+            const int row = row_of[r];
             if (row < 0) continue;
-            const size_t at = static_cast<size_t>(row) * a.c_out + c;
-            Eight<DT> v;
-            if constexpr (VEC) v.load(a.base, at, a.base != nullptr);
-            else v.load_any(a.base, at, a.base ? to - c : 0);
-            const float zero[8] = {};
-            v.template add_and_store<VEC>(a.out, at, zero, 1.0f, to - c);
+            for (int c = from + (threadIdx.x & 31) * 8; c < to; c += 256) {
+                const size_t at = static_cast<size_t>(row) * a.c_out + c;
+                Eight<DT> v;
+                if constexpr (VEC) v.load(a.base, at, a.base != nullptr);
+                else v.load_any(a.base, at, a.base ? to - c : 0);
+                const float zero[8] = {};
+                v.template add_and_store<VEC>(a.out, at, zero, 1.0f, to - c);
+            }
         }
     }
     if (keep)
         for (int i = threadIdx.x + cr * THREADS; i < n * a.rank; i += THREADS * cs)
             if (row_of[i / a.rank] >= 0) a.low[static_cast<size_t>(row_of[i / a.rank]) * a.rank + i % a.rank] = 0.0f;
+}
+
+// Tiles of `rows` rows that there are at most: one of fewer rows for each adapter and on both sides of them
+inline long long most_tiles(const LoraArgs &a, int rows) {
+    const long long tiles = a.n_rows / rows + a.n_adapters + 2ll;
+    return tiles < a.n_rows ? tiles : a.n_rows;
 }
 
 // Clusters

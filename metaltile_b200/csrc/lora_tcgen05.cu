@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
     const int units = (a.c_out + kColumns - 1) / kColumns;
     const int step0 = static_cast<int>(static_cast<long long>(units) * cr / kCluster), steps = static_cast<int>(static_cast<long long>(units) * (cr + 1) / kCluster) - step0;
     const int c_end = std::min((step0 + steps) * kColumns, a.c_out);
-    if (tile.e == a.n_adapters) {
+    if (tile.e >= a.n_adapters) {
         __syncthreads();
         copy_rows<DT, kThreads>(a, ctl->row_of, static_cast<int>(tile.n), step0 * kColumns, c_end, keep, cr, kCluster);
         return;
@@ -432,7 +432,7 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     static PerDeviceAttr attr;
     const cudaError_t e = attr.set(lora_tile_kernel<DT, RB, BACK>, kSmem);
     if (e != cudaSuccess) return e;
-    const long long tiles = std::min<long long>(a.n_rows, a.n_rows / kRows + a.n_adapters + 1ll);
+    const long long tiles = most_tiles(a, kRows);
     if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     return launch_cluster(lora_tile_kernel<DT, RB, BACK>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, kSmem, st, a, keep, none);
 }

@@ -191,6 +191,80 @@ def test_bad_offsets_and_rows_are_reported(size, dt):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("size", [(90, 256, 128, 16, 3), (90, 255, 127, 16, 3), (90, 255, 127, 5, 3), (2100, 128, 64, 32, 1)])
+def test_places_before_the_first_adapter_have_none(size, dt):
+    """Any places outside of the ranges belong to no adapter, those in front as well."""
+    rows, k, n, rank, adapters = size
+    c = Case(*size, dt, seed=7)
+    want, h = c.forward()
+    dx, da, db = c.grad(h)
+    none = int((c.ids == adapters).sum())
+    c.rows = torch.cat([c.rows[rows - none // 2:], c.rows[:rows - none // 2]]).contiguous()          # half of them in front
+    c.offsets = c.offsets + none // 2
+    got, h2 = c.forward()
+    assert torch.equal(got, want) and torch.equal(h2, h)
+    for a, b in zip(c.grad(h), (dx, da, db)):
+        assert torch.equal(a, b)
+    base = c.base.clone()
+    base[c.ids == adapters] = float("nan")
+    got, _ = c.forward(base=base, out=base)
+    assert torch.isnan(got[c.ids == adapters]).all() and torch.equal(got[c.ids != adapters], want[c.ids != adapters])
+
+
+@pytest.mark.parametrize("dt,rows", [("bf16", 66000), ("f32", 33000)])
+def test_rows_whose_offsets_pass_32_bits(dt, rows):
+    from metaltile_b200 import ops
+    k, n, rank, t = 33008, 64, 8, TYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(rows, k, device="cuda", dtype=t).normal_(generator=g)
+    dy = torch.randn(rows, n, device="cuda", generator=g).to(t)
+    a, b = (torch.randn(3, rank, k, device="cuda", generator=g) / 180).to(t), torch.randn(3, n, rank, device="cuda", generator=g).to(t)
+    ids = torch.randint(0, 4, (rows,), device="cuda", generator=g)
+    order, offsets = ref.group(ids, 3)
+    out, h = ops.lora_mm(x, a, b, order, offsets, hidden=True)
+    dx, da, db = ops.lora_grad(dy, x, a, b, order, offsets, h)
+    at = torch.cat([torch.arange(40, device="cuda"), torch.arange(rows - 200, rows, device="cuda")])
+    want, want_h = ref.lora(x[at], a, b, ids[at], None, None)
+    dh = ref.low_bound(x[at], a, ids[at])
+    _close(out[at], want, ref.high_bound(want, want_h, dh, b.transpose(1, 2), ids[at], None, None, t))
+    u, du = ref.low(dy[at], b.transpose(1, 2), ids[at]), ref.low_bound(dy[at], b.transpose(1, 2), ids[at])
+    want = ref.high(u, a, ids[at], None, None, k)
+    _close(dx[at], want, ref.high_bound(want, u, du, a, ids[at], None, None, t))
+    # a column of the weights' gradient over all rows
+    u = ref.low(dy, b.transpose(1, 2), ids)
+    cols = torch.tensor([0, 77, k - 1], device="cuda")
+    want = ref.outer(u, x[:, cols], ids, None, 3)
+    tol = ref.outer_bound(want, u, ref.low_bound(dy, b.transpose(1, 2), ids), x[:, cols], ids, None, 3, t)
+    _close(da[:, :, cols], want, tol)
+    assert ops.context(0).status_word() == 0
+
+
+def test_beside_other_tensor_memory_kernels_on_another_stream():
+    from metaltile_b200 import ops
+    c = Case(2200, 1024, 2048, 16, 2, "bf16", seed=11)
+    want, h = c.forward()
+    grads = c.grad(h)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2048, 1024, device="cuda", generator=g).to(torch.bfloat16)
+    w, s = ops.fp8_quantize((torch.randn(2048, 1024, device="cuda", generator=g) * 0.02).to(torch.bfloat16), block_rows=128)
+    y = ops.fp8_mm(x, w, s)
+    y16 = ops.fp8_mm(x[:16].contiguous(), w, s)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[0]):
+            outs.append((c.forward()[0], want))
+            outs.append((c.grad(h)[0], grads[0]))
+        with torch.cuda.stream(streams[1]):
+            outs.append((ops.fp8_mm(x, w, s), y))
+            outs.append((ops.fp8_mm(x[:16].contiguous(), w, s), y16))
+    torch.cuda.synchronize()
+    for got, one in outs:
+        assert torch.equal(got, one)
+
+
 def test_groups_of_moe_sort():
     from metaltile_b200 import ops
     c = Case(100, 256, 128, 16, 5, "bf16")

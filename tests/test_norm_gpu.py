@@ -172,3 +172,24 @@ def test_another_stream_and_a_graph():
     torch.cuda.synchronize()
     for a, b, c in zip(want, got, held):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) and torch.equal(a.view(torch.uint8), c.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dt,k", [("bf16", 16392), ("f16", 16391)])
+def test_rows_whose_offsets_pass_32_bits(dt, k):
+    from metaltile_b200 import ops
+    rows, t = 132000, TYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty(rows, k, device="cuda", dtype=t).normal_(generator=g)
+    r = torch.empty(rows, k, device="cuda", dtype=t).normal_(generator=g)
+    w = (1 + 0.2 * torch.randn(k, device="cuda", generator=g)).to(t)
+    at = torch.cat([torch.arange(3, device="cuda"), torch.arange(rows - 20, rows, device="cuda")])
+    y, s = ops.add_rms_norm(x, w, 1e-5, residual=r)
+    assert torch.equal(s[at], (x[at].float() + r[at].float()).to(t))
+    _close(y[at], ref.norm(s[at], w, 1e-5), ref.norm_bound(s[at], w, 1e-5))
+    del y
+    codes, scales, _ = ops.add_rms_norm_fp8(s, w, 1e-5)
+    want, want_scales = ops.fp8_quantize(ops.add_rms_norm(s[at].float(), w.float(), 1e-5)[0])
+    assert torch.equal(codes[at].view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales[at], want_scales)
+    del codes
+    dx, _ = ops.add_rms_norm_grad(x, s, w, 1e-5, out=r)
+    _close(dx[at], ref.norm_grad(x[at], s[at], w, 1e-5)[0], ref.norm_grad_bounds(x[at], s[at], w, 1e-5, None, 1)[0])
