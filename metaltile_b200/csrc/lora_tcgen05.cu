@@ -26,7 +26,6 @@ namespace {
 
 using namespace lora;
 
-
 constexpr int kCopy = 256, kMmaWarp = 8, kLoadWarp = 9, kThreads = kCopy + 64, kCluster = 8, kRows = 128, kOwn = kRows / kCluster;
 constexpr int kStage = 24 * 1024, kWeights = 16 * 1024;                              // of a stage: where the weights start
 constexpr int kHeld = 0, kPiece = 16 * 1024, kColumns = 64;

@@ -111,9 +111,11 @@ def test_in_place_leaves_rows_without_an_adapter_alone(dt):
         assert torch.equal(dbase[~none], dx[~none]) and torch.isnan(dbase[none]).all()
 
 
+# (the second size is one of the kernel with tiles of 128 rows, the third one of rows that are no whole pieces)
 @pytest.mark.parametrize("dt", TYPES)
-def test_rows_without_an_adapter_hold_anything(dt):
-    c = Case(60, 256, 128, 16, 3, dt, seed=4)
+@pytest.mark.parametrize("size", [(60, 256, 128, 16, 3), (2100, 256, 128, 32, 3), (60, 255, 127, 16, 3)])
+def test_rows_without_an_adapter_hold_anything(size, dt):
+    c = Case(*size, dt, seed=4)
     want, h = c.forward()
     grads = c.grad(h)
     none = c.ids == 3
@@ -126,25 +128,27 @@ def test_rows_without_an_adapter_hold_anything(dt):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-def test_special_values_stay_in_their_row(dt):
-    c = Case(48, 256, 128, 16, 2, dt, seed=5)
+@pytest.mark.parametrize("rows,n", [(48, 128), (2100, 128), (48, 127)])
+def test_special_values_stay_in_their_row(rows, n, dt):
+    c = Case(rows, 256, n, 16, 2, dt, seed=5)
     want, _ = c.forward()
     c.x[5, 7], c.x[20, 100] = float("nan"), float("inf")
     c.ids[5], c.ids[20] = 0, 1
     c.rows, c.offsets = ref.group(c.ids, 2)
     got, h = c.forward()
     assert torch.isnan(got[5]).all() and not torch.isfinite(got[20]).any()
-    rest = torch.ones(48, dtype=torch.bool, device="cuda")
+    rest = torch.ones(rows, dtype=torch.bool, device="cuda")
     rest[5] = rest[20] = False
     clean = ref.lora(c.x[rest], c.a, c.b, c.ids[rest], c.scales, c.base[rest])[0]
     assert torch.isfinite(got[rest]).all() and (got[rest].double() - clean).abs().max() < 0.05
 
 
+@pytest.mark.parametrize("rows,n", [(40, 256), (2100, 256), (40, 255)])
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
-def test_large_and_small_values(dt):
+def test_large_and_small_values(dt, rows, n):
     """What a row goes through may be far outside of 16-bit floats."""
-    c = Case(40, 512, 256, 16, 2, dt, seed=6)
-    up = 2.0 ** torch.randint(-10, 9, (40, 1), device="cuda").float()
+    c = Case(rows, 512, n, 16, 2, dt, seed=6)
+    up = 2.0 ** torch.randint(-10, 9, (rows, 1), device="cuda").float()
     c.x = (c.x.float() * up * 16).to(TYPES[dt])
     c.dy = (c.dy.float() * up * 16).to(TYPES[dt])
     c.a, c.b = (c.a.float() * 512).to(TYPES[dt]), (c.b.float() / 64).to(TYPES[dt])
