@@ -39,7 +39,7 @@ __device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, i
 // RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  VEC: rows are whole 16-byte pieces; else their values are loaded one by one.  BACK: the first product's weights lie [c_in][rank], the second's
 // [rank][c_out]; else [rank][c_in] and [c_out][rank].
 template <int DT, int RB, int MT, bool BACK, bool ONE, bool VEC>
-__global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int rank_blocks_, bool keep, bool none) {
+__global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int rank_blocks_, bool keep, bool none) {
     pdl_enter();
     constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8, SIZE = DT == MTC_F32 ? 4 : 2;
     constexpr bool HALF = DT == MTC_F16;
@@ -398,8 +398,10 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
 template <int DT, int MT, bool BACK>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int MOST = DT == MTC_F32 ? 32 : 64;
-    if (a.rank <= 8) return launch<DT, 8, MT, BACK, true>(st, a, keep, none);
-    if (a.rank <= 16) return launch<DT, 16, MT, BACK, true>(st, a, keep, none);
+    if constexpr (DT != MTC_F32 || MT == 1) {
+        if (a.rank <= 8) return launch<DT, 8, MT, BACK, true>(st, a, keep, none);
+        if (a.rank <= 16) return launch<DT, 16, MT, BACK, true>(st, a, keep, none);
+    }
     if (a.rank <= 32) return launch<DT, 32, MT, BACK, true>(st, a, keep, none);
     if (a.rank <= MOST) return launch<DT, MOST, MT, BACK, true>(st, a, keep, none);
     return launch<DT, MOST, 1, BACK, false>(st, a, keep, none);
@@ -408,19 +410,20 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
 template <int DT, int MT, bool BACK>
 cudaError_t launch_any(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int MOST = DT == MTC_F32 ? 32 : 64;
-    return a.rank <= 16 ? launch<DT, 16, MT, BACK, true, false>(st, a, keep, none) : launch<DT, MOST, MT, BACK, true, false>(st, a, keep, none);
+    if constexpr (DT != MTC_F32 || MT == 1) {
+        if (a.rank <= 16) return launch<DT, 16, MT, BACK, true, false>(st, a, keep, none);
+    }
+    return launch<DT, MOST, MT, BACK, true, false>(st, a, keep, none);
 }
 template <int DT>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
+    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
+    // and 9.3, 1024 15.5 and 10.7; f32 rank 16, 4096 rows 103 and 132, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0
+    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && a.rank > 16;
     if (!whole_pieces(a)) {
-        const bool wide = a.n_rows > 640;
         if (wide) return backward ? launch_any<DT, 2, true>(st, a, keep, none) : launch_any<DT, 2, false>(st, a, keep, none);
         return backward ? launch_any<DT, 1, true>(st, a, keep, none) : launch_any<DT, 1, false>(st, a, keep, none);
     }
-    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
-    // and 9.3, 1024 15.5 and 10.7; f32 forward rank 8, 1024 rows 22.7 and 37, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0; f32 back (with the weights' gradients) rank 8, 128 17.4 and
-    // 21.1, 256 22.6 and 20.0
-    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && (backward || a.rank > 16);
     if (wide) return backward ? launch<DT, 2, true>(st, a, keep, none) : launch<DT, 2, false>(st, a, keep, none);
     return backward ? launch<DT, 1, true>(st, a, keep, none) : launch<DT, 1, false>(st, a, keep, none);
 }
