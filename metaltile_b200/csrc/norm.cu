@@ -100,7 +100,7 @@ __device__ __forceinline__ float inverse_root(float sum, int K, float eps) { ret
 // MODE 0: y; 1, 2: codes with scales (2: powers of two), and y where it is wanted.  NV: turns whose values stay in registers (0: any number,
 // the row is read again).  A row's threads: a warp (several rows a CTA), or the CTA.
 template <int DT, bool VEC, int NV, int MODE>
-__global__ void __launch_bounds__(NV == 4 ? 256 : 1024) add_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(NV == 4 ? 256 : 1024, NV == 4 && MODE ? 4 : 1) add_norm_kernel(const NormArgs a) {
     pdl_enter();
     __shared__ __align__(16) float scratch[32];
     const bool one_warp = a.threads == 32;
@@ -370,9 +370,10 @@ cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, NormArgs a) {
     const int block = a.threads * rows_a_cta;
     if (!vec) return launch_pdl(add_norm_kernel<DT, false, 0, MODE>, grid, block, 0, st, a);
     if (eights > turns * a.threads) return launch_pdl(add_norm_kernel<DT, true, 0, MODE>, grid, block, 0, st, a);
-    return turns == 1   ? launch_pdl(add_norm_kernel<DT, true, 1, MODE>, grid, block, 0, st, a)
-           : turns == 2 ? launch_pdl(add_norm_kernel<DT, true, 2, MODE>, grid, block, 0, st, a)
-                        : launch_pdl(add_norm_kernel<DT, true, 4, MODE>, grid, block, 0, st, a);
+    if constexpr (DT != MTC_F32) {
+        if (turns == 4) return launch_pdl(add_norm_kernel<DT, true, 4, MODE>, grid, block, 0, st, a);
+    }
+    return turns == 1 ? launch_pdl(add_norm_kernel<DT, true, 1, MODE>, grid, block, 0, st, a) : launch_pdl(add_norm_kernel<DT, true, 2, MODE>, grid, block, 0, st, a);
 }
 template <int DT>
 cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, const NormArgs &a, int mode) {
