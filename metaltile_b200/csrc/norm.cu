@@ -7,7 +7,11 @@
 //
 // Bound by memory: every value is read once and stays in the registers of the row's threads, eight neighbours a thread and turn, between the sum
 // over the row and the results.  Sums are f32 within a row and within the rows that a CTA adds up for dw, f64 over the CTAs, always in the same
-// order.  The codes are made from the f32 results: the rounding to T between a norm and a quantizer of its own does not happen here.
+// order.  The codes are made from the f32 results: the rounding to T between a norm and a quantizer of its own does not happen here.  Against results in 64 bits some 1.5 codes of
+// 10000 are the neighbour: quotients of few bits lie on the borders between codes, and the f32 rounding of y or of the scale decides on which side.
+// Measured (graph, us): y, 1 x 4096 bf16 1.7, 2048 x 4096 9.4 (67 MB, 7.1 TB/s with part of it in L2), 8192 x 4096 41; codes, 8192 x 4096 42.8 (236 MB, 5.5 TB/s;
+// bound by instructions, 69 % of the issue slots: 18 a value and some 250 a thread and row); gradients, 8192 x 4096 with dsum 50 (268 MB, 5.4 TB/s; of it the join of 296 shares
+// about 3), 333 x 2880 f32 7.6.
 #include <algorithm>
 
 #include "norm.cuh"
@@ -361,8 +365,9 @@ cudaError_t launch_norm(Ctx *ctx, cudaStream_t st, NormArgs a) {
                      reinterpret_cast<uintptr_t>(a.codes) % 8 == 0;
     const int eights = (a.K + 7) / 8;
     // One turn of many threads where rows are few, two turns of half as many where they fill the GPU, four of 16-bit values where there are many rows: what a thread does
-    // once a row costs as much as sixteen values (codes of 8192 x 4096 bf16 52 us in two turns, 49 in four; 4096 x 8192 59 and 51; 333 rows 4.8 and 5.2, f32 65 and 69)
-    const int turns = a.n_rows <= ctx->sm_count && eights <= 1024 ? 1 : DT != MTC_F32 && a.n_rows >= 4ll * ctx->sm_count && eights >= 256 && eights <= 1024 ? 4 : 2;
+    // once a row costs as much as sixteen values (codes of 8192 x 4096 bf16 52 us in two turns, 49 in four, 46 with four CTAs of it an SM; 333 rows 4.8 and 5.2; f32 65 and
+    // 69; y instead of codes: 2048 x 4096 9.3 and 9.5, 4096 x 8192 43.9 and 41.3)
+    const int turns = a.n_rows <= ctx->sm_count && eights <= 1024 ? 1 : DT != MTC_F32 && a.n_rows >= 4ll * ctx->sm_count && eights >= (MODE ? 256 : 513) && eights <= 1024 ? 4 : 2;
     a.threads = std::min(1024, round_up((eights + turns - 1) / turns, 32));
     const int rows_a_cta = a.threads == 32 ? 4 : 1;
     const long long ctas = (a.n_rows + rows_a_cta - 1) / rows_a_cta;
