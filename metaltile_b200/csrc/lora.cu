@@ -1,5 +1,5 @@
 // Low-rank adapters: which kernel runs, and the products of any rank and alignment on CUDA cores, for what the others do not take (ranks that are no multiple of 2, 4 or 8,
-// more than 256 or, with rows that are no whole 16-byte pieces, 64).  No counterpart in the reference; this stands next to its projections
+// or more than 256).  No counterpart in the reference; this stands next to its projections
 // (crates/metaltile-std/src/mlx/quantized.rs:5040-5065), whose quantized weights stay as they are while adapters are trained or swapped.
 #include <algorithm>
 
@@ -76,10 +76,19 @@ cudaError_t launch_any(cudaStream_t st, const LoraArgs &a, bool backward, bool k
                     : launch_pdl(lora_any_kernel<DT>, dim3(a.n_rows), 256, 0, st, a, in, 1ll, 1ll, rank, keep, none);
 }
 
+enum class LoraForm { none, values, pieces };    // of rows of any length, or of whole 16-byte pieces
+// Loads of 2, 4 or 8 values along the rank, of the weights that lie so (b): their rows are aligned where the rank is a multiple of that
+LoraForm lora_mma_form(const LoraArgs &a, bool backward) {
+    const bool pieces = lora_pieces_in(a) && lora_pieces_out(a);
+    const int step = a.rank <= 8 && pieces ? 2 : a.rank <= 16 ? 4 : 8;              // (the least size of the rank of a form with values is 16)
+    if (a.rank % step || a.rank > 256 || !lora_on_16(backward ? a.down : a.up)) return LoraForm::none;
+    return pieces ? LoraForm::pieces : LoraForm::values;
+}
+
 }  // namespace
 
 cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt) {
-    const LoraForm form = lora_mma_form(a, backward, dt);
+    const LoraForm form = lora_mma_form(a, backward);
     const bool none = (keep && all) || a.base != a.out;
     if (form != LoraForm::none) {
         // Tiles of 128 rows on tcgen05 where they are many (us of the warp-level and the tcgen05 kernel, bf16, 4096 x 4096).  Forward: rank 16, 1024 rows 10.7 and 15.1, 2048 21.2 and
@@ -88,7 +97,7 @@ cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward
         // fill a good part of a tile stay with the other one: 1024 rows of 32 adapters, rank 32, 14.0 and 21.
         const int least = backward ? (a.rank <= 16 ? 2048 : a.rank <= 32 ? 1024 : 512) : a.rank <= 32 ? 2048 : 1024;
         if (form == LoraForm::pieces && lora_tile_supported(a, keep, dt) && a.n_rows >= least && a.n_rows >= 48ll * a.n_adapters) return launch_lora_tile(st, a, backward, keep, none, dt);
-        return launch_lora_mma(st, a, backward, keep, none, dt);
+        return (dt == MTC_F32 ? launch_lora_mma<MTC_F32> : dt == MTC_BF16 ? launch_lora_mma<MTC_BF16> : launch_lora_mma<MTC_F16>)(st, a, backward, keep, none);
     }
     return (dt == MTC_F32 ? launch_any<MTC_F32> : dt == MTC_BF16 ? launch_any<MTC_BF16> : launch_any<MTC_F16>)(st, a, backward, keep, none);
 }

@@ -39,11 +39,16 @@ struct LoraWeights {
 // keep: `low` is wanted; all: with zeros for the rows of no adapter
 cudaError_t launch_lora(Ctx *ctx, cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool all, int dt);
 
-// The tensor-core kernels (lora_mma.cu, lora_grad.cu) and what they take; `none`: rows of no adapter have something to be written
-enum class LoraForm { none, values, pieces };    // rows of any length, or of whole 16-byte pieces
-LoraForm lora_mma_form(const LoraArgs &a, bool backward, int dt);
-cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
-bool lora_tile_supported(const LoraArgs &a, bool keep, int dt);       // (lora_tcgen05.cu) what of the above it takes
+inline bool lora_on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// Rows on a side that can be loaded 16 bytes at a time: x and, forward, a; base and out and, back, a
+inline bool lora_pieces_in(const LoraArgs &a) { return a.c_in % 8 == 0 && lora_on_16(a.in) && lora_on_16(a.down); }
+inline bool lora_pieces_out(const LoraArgs &a) { return a.c_out % 8 == 0 && lora_on_16(a.up) && lora_on_16(a.out) && (!a.base || lora_on_16(a.base)); }
+
+// Warp-level tensor cores (lora_rows.cuh, a file a type); `none`: rows of no adapter have something to be written
+template <int DT>
+cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none);
+// tcgen05 (lora_tcgen05.cu), and what it takes of rows of whole pieces
+bool lora_tile_supported(const LoraArgs &a, bool keep, int dt);
 cudaError_t launch_lora_tile(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt);
 // (lora_grad.cu) any size and alignment
 cudaError_t launch_lora_grad(Ctx *ctx, cudaStream_t st, const LoraWeights &w, int dt);

@@ -2,9 +2,13 @@
 //   dA_e[i][c] = scale_e sum over the rows t of e of u_t[i] x_t[c],      dB_e[c][i] = scale_e sum of h_t[i] dy_t[c]
 //
 // One launch for both.  A CTA has a block of columns of one adapter, all its ranks (64 at a time), and a part of its rows; the CTAs of a cluster share the
-// rows and add up over distributed shared memory in a fixed order.  Bound by reading x and dy, which pass once, by cp.async, 64 rows a stage, up to two stages ahead (a
-// bulk copy a row and mbarriers take half the instructions and were no faster: 34.9 us instead of 31 for 4096 rows of 4096 + 4096).  Rows are the k of the MMAs: u and h are staged as operand pieces a stage ahead and transposed as they are loaded; of x and dy a lane takes eight neighbours of four
+// rows and add up over distributed shared memory in a fixed order.  x and dy pass once, by cp.async, 64 rows a stage, up to two stages ahead.  Rows are the k of the MMAs: u and h
+// are staged as operand pieces a stage ahead and transposed as they are loaded; of x and dy a lane takes eight neighbours of four
 // rows and pairs them up.  All operands are bf16 pieces: f16 values are two (11 bits), since u and h have no bound that f16 would hold.
+//
+// Measured: 4096 rows of 4096 + 4096, rank 16, bf16 31 us, 2.2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 1024 + 1024 in f32, rank 8, 6.2.  Bound by what a CTA cannot overlap, in
+// two waves of CTAs: of 25,000 cycles the start and the first stage take 8,000, the sums over the cluster 5,000.  A bulk copy a row and mbarriers take half the instructions and
+// were no faster (34.9 us).
 #include <algorithm>
 
 #include "lora_mma.cuh"
@@ -90,6 +94,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
         return -1;
     };
     // x or dy of a stage, zeros where there is no row
+    const bool pieces = VEC || (W.c % 8 == 0 && reinterpret_cast<uintptr_t>(W.in) % 16 == 0);
     constexpr int UNITS = CB * F::SIZE / 16, PASSES = kStage * UNITS / kThreads;
     auto copy = [&](int s) {
         if (s < mine) {
@@ -98,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
             for (int i = 0; i < PASSES; ++i) {
                 const int r = (i * kThreads + tid) / UNITS, row = row_of[s % kRowsAhead][r];
                 const bool ok = row >= 0 && c < W.c;
-                if constexpr (!VEC) {            // rows of any length: values one by one
+                if (!VEC && !pieces) {           // rows of any length: values one by one
                     constexpr int N = 16 / F::SIZE;
                     uint32_t v[4] = {};
 #pragma unroll

@@ -2,9 +2,14 @@
 //
 // A cluster of CTAs has one tile of rows of one adapter: each CTA, each of its eight warps, sums up a part of the long axis of the first product; the parts meet in
 // shared memory, then over distributed shared memory, so that every CTA has the whole h of the tile; then each CTA takes a part of the
-// columns of the second product.  Bound by memory: x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.  At
-// rank 64 the two products are 64 operations a byte of activations, a tenth of what the warp-level tensor cores give, so there is nothing for tcgen05 to win: its
-// smallest tile, 128 rows, would be empty for the most part where users decode.
+// columns of the second product.  x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.
+//
+// Bound by latency where users decode: 64 rows of 8 adapters, 4096 x 4096, rank 16, bf16 take 10.2 us where the bytes need 3; a row alone takes 5.0.  Of that the launch is 2, and
+// the chain is loads of x and A, the sums over the cluster (two barriers of it), loads of B and base, stores.  So everything that a CTA will read is asked for before
+// it waits (prefetches into L2, and base and B into registers where they fit), and a tile is spread over 64 warps.  128-row tiles of tcgen05 would be empty for the most part there;
+// with a thousand rows and more the shared reading of the adapter and one thread that issues the MMAs win (lora.cu has both sides).
+#pragma once
+
 #include <algorithm>
 
 #include "lora_mma.cuh"
@@ -36,9 +41,10 @@ __device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, i
         prefetch(static_cast<const char *>(from) + i, min(piece, bytes - i));
 }
 
-// RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  VEC: rows are whole 16-byte pieces; else their values are loaded one by one.  BACK: the first product's weights lie [c_in][rank], the second's
+// RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  VIN, VOUT: rows on this side are whole 16-byte pieces; else their values are
+// loaded one by one.  BACK: the first product's weights lie [c_in][rank], the second's
 // [rank][c_out]; else [rank][c_in] and [c_out][rank].
-template <int DT, int RB, int MT, bool BACK, bool ONE, bool VEC>
+template <int DT, int RB, int MT, bool BACK, bool ONE, bool VIN, bool VOUT>
 __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int rank_blocks_, bool keep, bool none) {
     pdl_enter();
     constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8, SIZE = DT == MTC_F32 ? 4 : 2;
@@ -72,11 +78,11 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
     __syncthreads();
     if (tile.e >= a.n_adapters) {                // rows of no adapter: base, or zeros
-        copy_rows<DT, kThreads, VEC>(a, row_of, static_cast<int>(tile.n), unit0 * CW, min(unit1 * CW, a.c_out), keep, cr, cs);
+        copy_rows<DT, kThreads, VOUT>(a, row_of, static_cast<int>(tile.n), unit0 * CW, min(unit1 * CW, a.c_out), keep, cr, cs);
         return;
     }
     const size_t expert = tile.e;
-    if constexpr (VEC) {                         // everything that this CTA will read is on its way before it waits for any of it
+    if constexpr (VIN && VOUT) {                 // everything that this CTA will read is on its way before it waits for any of it
         const int k0 = static_cast<int>(static_cast<long long>(chunks) * cr / cs) * 32, k1 = min(static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / cs) * 32, a.c_in);
         const int n0 = unit0 * CW, n1 = min(unit1 * CW, a.c_out);
         const size_t in_row = static_cast<size_t>(a.c_in) * SIZE, out_row = static_cast<size_t>(a.c_out) * SIZE, rank_row = static_cast<size_t>(a.rank) * SIZE;
@@ -103,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     // are loaded at once, the first ones before the parts meet (64 rows of 32 adapters 12.1 us a step at a time); elsewhere, where registers do not allow
     // it, each right before its products.
     constexpr int TN = CW / 8, QS = RB >= 32 ? RB / 32 : 1, WIDE = RB >= 32 ? 8 : RB / 4, PARTS = WIDE == 8 ? 2 : 1, DEEP = WIDE == 2 ? 2 : 4;
-    constexpr bool EARLY = VEC && ONE && MT == 1 && P == 1 && (BACK ? RB <= 16 : RB <= 32);
+    constexpr bool EARLY = VIN && VOUT && ONE && MT == 1 && P == 1 && (BACK ? RB <= 16 : RB <= 32);
     constexpr int STEPS = !EARLY ? 1 : BACK || RB == 32 ? 2 : 4;
     using V = Vals<DT, BACK ? 8 : WIDE>;
     struct Unit {
@@ -120,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                     const int c = n0 + t * (CW / 4) + 8 * i;
                     const bool there = a.base && rows[m][h] >= 0;
                     const size_t at = static_cast<size_t>(rows[m][h]) * a.c_out + c;
-                    if constexpr (VEC) to.base[m][h][i].load(a.base, at, there && c < a.c_out);
+                    if constexpr (VOUT) to.base[m][h][i].load(a.base, at, there && c < a.c_out);
                     else to.base[m][h][i].load_any(a.base, at, there ? a.c_out - c : 0);
                 }
     };
@@ -138,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
 #pragma unroll
             for (int s = 0; s < DEEP; ++s) {
                 const int rr = r + 4 * i + s;
-                if constexpr (VEC) to[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
+                if constexpr (VOUT) to[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
                 else to[s].load_any(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank ? a.c_out - c : 0);
             }
         }
@@ -167,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if constexpr (VEC) x[m][h].load(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
+                    if constexpr (VIN) x[m][h].load(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
                     else x[m][h].load_any(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, rows[m][h] >= 0 ? a.c_in - k : 0);
                 }
             auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {      // tile j of ranks, piece p of the weights, half i of the 32 values
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                 for (int j = 0; j < NT; ++j) {
                     const int r = rb * RB + 8 * j + g;
                     Vals<DT, 8> w;
-                    if constexpr (VEC) w.load(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
+                    if constexpr (VIN) w.load(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
                     else w.load_any(a.down, (expert * a.rank + r) * a.c_in + k, r < a.rank ? a.c_in - k : 0);
 #pragma unroll
                     for (int p = 0; p < P; ++p)
@@ -198,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                 for (int i = 0; i < 2; ++i) {
                     V w[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q].load(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VEC ? in : k + 4 * i + q < a.c_in) && r < a.rank);
+                    for (int q = 0; q < 4; ++q) w[q].load(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VIN ? in : k + 4 * i + q < a.c_in) && r < a.rank);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                         v[k] = acc[m][j][at];
                         if constexpr (P > 1) v[k] += fine[m][j][at];
                     }
-                    if (c < a.c_out) unit.base[m][h][i].template add_and_store<VEC>(a.out, static_cast<size_t>(rows[m][h]) * a.c_out + c, v, factor, a.c_out - c);
+                    if (c < a.c_out) unit.base[m][h][i].template add_and_store<VOUT>(a.out, static_cast<size_t>(rows[m][h]) * a.c_out + c, v, factor, a.c_out - c);
                 }
             }
     };
@@ -377,26 +383,20 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     cluster_wait();
 }
 
-bool on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-// rows of x, base and out (and of a) that can be loaded 16 bytes at a time
-bool whole_pieces(const LoraArgs &a) {
-    return a.c_in % 8 == 0 && a.c_out % 8 == 0 && on_16(a.in) && on_16(a.down) && on_16(a.up) && on_16(a.out) && (!a.base || on_16(a.base));
-}
-
-template <int DT, int RB, int MT, bool BACK, bool ONE, bool VEC = true>
+template <int DT, int RB, int MT, bool BACK, bool ONE, bool VIN = true, bool VOUT = true>
 cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int ROWS = 16 * MT, H = DT == MTC_F32 ? 3 : 2;
     const int blocks = (a.rank + RB - 1) / RB;
     const size_t smem = static_cast<size_t>(kWarps * ROWS * part_stride(RB) + (ONE ? 0 : ROWS * blocks * RB)) * 4 + static_cast<size_t>(H * ROWS * held_stride(blocks * RB)) * 2;
     static PerDeviceAttr attr;
-    cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK, ONE, VEC>, 200 * 1024);
+    cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, 200 * 1024);
     if (e != cudaSuccess) return e;
     const long long tiles = most_tiles(a, ROWS);
     if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VEC>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, smem, st, a, blocks, keep, none);
+    return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, smem, st, a, blocks, keep, none);
 }
 template <int DT, int MT, bool BACK>
-cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
+cudaError_t launch_pieces(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int MOST = DT == MTC_F32 ? 32 : 64;
     if constexpr (DT != MTC_F32 || MT == 1) {
         if (a.rank <= 8) return launch<DT, 8, MT, BACK, true>(st, a, keep, none);
@@ -406,39 +406,33 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     if (a.rank <= MOST) return launch<DT, MOST, MT, BACK, true>(st, a, keep, none);
     return launch<DT, MOST, 1, BACK, false>(st, a, keep, none);
 }
-// values one by one: two sizes of the rank are enough
-template <int DT, int MT, bool BACK>
-cudaError_t launch_any(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
+// values one by one on one side or both: two sizes of the rank are enough
+template <int DT, int MT, bool BACK, bool VIN, bool VOUT>
+cudaError_t launch_values(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     constexpr int MOST = DT == MTC_F32 ? 32 : 64;
     if constexpr (DT != MTC_F32 || MT == 1) {
-        if (a.rank <= 16) return launch<DT, 16, MT, BACK, true, false>(st, a, keep, none);
+        if (a.rank <= 16) return launch<DT, 16, MT, BACK, true, VIN, VOUT>(st, a, keep, none);
     }
-    return launch<DT, MOST, MT, BACK, true, false>(st, a, keep, none);
+    if (a.rank <= MOST) return launch<DT, MOST, MT, BACK, true, VIN, VOUT>(st, a, keep, none);
+    return launch<DT, MOST, 1, BACK, false, false, false>(st, a, keep, none);
 }
-template <int DT>
-cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
-    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
-    // and 9.3, 1024 15.5 and 10.7; f32 rank 16, 4096 rows 103 and 132, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0
-    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && a.rank > 16;
-    if (!whole_pieces(a)) {
-        if (wide) return backward ? launch_any<DT, 2, true>(st, a, keep, none) : launch_any<DT, 2, false>(st, a, keep, none);
-        return backward ? launch_any<DT, 1, true>(st, a, keep, none) : launch_any<DT, 1, false>(st, a, keep, none);
-    }
-    if (wide) return backward ? launch<DT, 2, true>(st, a, keep, none) : launch<DT, 2, false>(st, a, keep, none);
-    return backward ? launch<DT, 1, true>(st, a, keep, none) : launch<DT, 1, false>(st, a, keep, none);
+template <int DT, int MT, bool BACK>
+cudaError_t launch_side(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
+    const bool in = lora_pieces_in(a), out = lora_pieces_out(a);
+    if (in && out) return launch_pieces<DT, MT, BACK>(st, a, keep, none);
+    if (in) return launch_values<DT, MT, BACK, true, false>(st, a, keep, none);
+    return out ? launch_values<DT, MT, BACK, false, true>(st, a, keep, none) : launch_values<DT, MT, BACK, false, false>(st, a, keep, none);
 }
 
 }  // namespace
 
-// Loads of 2, 4 or 8 values along the rank, of the weights that lie so (b): their rows are aligned where the rank is a multiple of that
-LoraForm lora_mma_form(const LoraArgs &a, bool backward, int dt) {
-    if (a.rank % (a.rank <= 8 ? 2 : a.rank <= 16 ? 4 : 8) || !on_16(backward ? a.down : a.up)) return LoraForm::none;
-    if (whole_pieces(a)) return a.rank <= 256 ? LoraForm::pieces : LoraForm::none;
-    // (values one by one are as many loads for the loads of ranks as there are ranks' registers: RB 16 takes loads of 4 along the rank)
-    return a.rank % (a.rank <= 16 ? 4 : 8) == 0 && a.rank <= (dt == MTC_F32 ? 32 : 64) ? LoraForm::values : LoraForm::none;
-}
-cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none, int dt) {
-    return (dt == MTC_F32 ? launch<MTC_F32> : dt == MTC_BF16 ? launch<MTC_BF16> : launch<MTC_F16>)(st, a, backward, keep, none);
+template <int DT>
+cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
+    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
+    // and 9.3, 1024 15.5 and 10.7; f32 rank 16, 4096 rows 103 and 132, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0
+    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && a.rank > 16;
+    if (wide) return backward ? launch_side<DT, 2, true>(st, a, keep, none) : launch_side<DT, 2, false>(st, a, keep, none);
+    return backward ? launch_side<DT, 1, true>(st, a, keep, none) : launch_side<DT, 1, false>(st, a, keep, none);
 }
 
 }  // namespace mtc
