@@ -91,11 +91,12 @@ cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward
     const LoraForm form = lora_mma_form(a, backward);
     const bool none = (keep && all) || a.base != a.out;
     if (form != LoraForm::none) {
-        // Tiles of 128 rows on tcgen05 where they are many (us of the warp-level and the tcgen05 kernel, bf16, 4096 x 4096).  Forward: rank 16, 1024 rows 10.7 and 15.1, 2048 21.2 and
-        // 20.8, 4096 39 and 26; rank 32, 1024 13.9 and 16.1, 2048 26 and 23; rank 64, 512 14.5 and 19.7, 1024 26 and 20.  Back (with the weights' gradients, which are the
-        // same): rank 16, 1024 30.4 and 29.3, 2048 52 and 46; rank 32, 512 34.6 and 35.8, 1024 49 and 38; rank 64, 256 25.5 and 27.8, 512 57 and 52.  Adapters with fewer rows than
-        // fill a good part of a tile stay with the other one: 1024 rows of 32 adapters, rank 32, 14.0 and 21.
-        const int least = backward ? (a.rank <= 16 ? 2048 : a.rank <= 32 ? 1024 : 512) : a.rank <= 32 ? 2048 : 1024;
+        // Tiles of 128 rows on tcgen05 where they are many (us of the warp-level and the tcgen05 kernel, bf16, 4096 x 4096).  Forward: rank 16, 2048 rows 16.6 and 21.1, 2560 24.0 and 22.1,
+        // 4096 30.2 and 26.4 (narrow layers have no time to win: 1024 x 1024, 4096 rows 9.6 and 13.1), rank 64, 1024 rows 18.6 and 20.0, 2048 30.4 and 27.8.  Back, with
+        // the weights' gradient: rank 16, 512 rows 23.6 and 25.5, 1536 36.4 and 30.8, 4096 79.5 and 65.4; rank 32, 512 26.0 and 27.6, 768 33.5 and 28.9; rank 64, 512 40.9 and 36.4.
+        // Adapters whose rows do not fill a good part of a tile stay with the other one: 1024 rows of 32 adapters, rank 32, 14.0 and 21.
+        const bool narrow = a.c_in + a.c_out <= 2048;
+        const int least = backward ? (a.rank <= 16 ? 1152 : a.rank <= 32 ? 768 : 512) : a.rank > 32 ? 1152 : narrow ? 0x7FFFFFFF : 2304;
         if (form == LoraForm::pieces && lora_tile_supported(a, keep, dt) && a.n_rows >= least && a.n_rows >= 48ll * a.n_adapters) return launch_lora_tile(st, a, backward, keep, none, dt);
         return (dt == MTC_F32 ? launch_lora_mma<MTC_F32> : dt == MTC_BF16 ? launch_lora_mma<MTC_BF16> : launch_lora_mma<MTC_F16>)(st, a, backward, keep, none);
     }

@@ -1,6 +1,6 @@
 // Low-rank adapters on warp-level tensor cores: h = x A^T and out = base + scale h B^T (or, back, u = dy B and dx = base + scale u A) in one launch.
 //
-// A cluster of CTAs has one tile of rows of one adapter: each CTA, each of its eight warps, sums up a part of the long axis of the first product; the parts meet in
+// A cluster of 8, 4 or 2 CTAs (launch) has one tile of rows of one adapter: each CTA, each of its eight warps, sums up a part of the long axis of the first product; the parts meet in
 // shared memory, then over distributed shared memory, so that every CTA has the whole h of the tile; then each CTA takes a part of the
 // columns of the second product.  x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.
 //
@@ -11,6 +11,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "lora_mma.cuh"
 
@@ -19,7 +20,7 @@ namespace {
 
 using namespace lora;
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kCluster = 8;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 
 __host__ __device__ constexpr int part_stride(int rb) { return rb + 4; }
 __host__ __device__ constexpr int held_stride(int rt) { return rt + 8; }         // in 16-bit values: rows 16 bytes apart modulo 128
@@ -45,7 +46,7 @@ __device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, i
 // loaded one by one.  BACK: the first product's weights lie [c_in][rank], the second's
 // [rank][c_out]; else [rank][c_in] and [c_out][rank].
 template <int DT, int RB, int MT, bool BACK, bool ONE, bool VIN, bool VOUT>
-__global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int rank_blocks_, bool keep, bool none) {
+__global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lora_mma_kernel(const LoraArgs a, int cluster_log, int rank_blocks_, bool keep, bool none) {
     pdl_enter();
     constexpr int ROWS = 16 * MT, PS = part_stride(RB), P = pieces<DT>, H = DT == MTC_F32 ? 3 : 2, NT = RB / 8, SIZE = DT == MTC_F32 ? 4 : 2;
     constexpr bool HALF = DT == MTC_F16;
@@ -57,12 +58,12 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     __shared__ int row_of[ROWS];
     __shared__ float back_up[ROWS];              // f16: the power of two that a row's h was divided by
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    constexpr int cs = kCluster;
     const int cr = cluster_rank();
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e < a.n_adapters; e += kThreads)
             if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
-    const Tile tile = find_tile(a, blockIdx.x / cs, ROWS, none);
+    const int cs = 1 << cluster_log;              // (shifts: 64-bit divisions made 6.1 us of the 5.1 of a single row)
+    const Tile tile = find_tile(a, blockIdx.x >> cluster_log, ROWS, none);
     if (tile.e < 0) return;                      // the whole cluster
     if (threadIdx.x < ROWS) {
         int row = -1;
@@ -74,8 +75,8 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
         row_of[threadIdx.x] = row;
     }
     constexpr int CW = BACK ? 64 : 32;           // columns of a warp's step
-    const int units = (a.c_out + CW - 1) / CW, unit0 = static_cast<int>(static_cast<long long>(units) * cr / cs), unit1 = static_cast<int>(static_cast<long long>(units) * (cr + 1) / cs);
-    const int chunks = (a.c_in + 31) / 32, workers = cs * kWarps, me = cr * kWarps + warp;
+    const int units = (a.c_out + CW - 1) / CW, unit0 = static_cast<int>(static_cast<long long>(units) * cr >> cluster_log), unit1 = static_cast<int>(static_cast<long long>(units) * (cr + 1) >> cluster_log);
+    const int chunks = (a.c_in + 31) / 32, me = cr * kWarps + warp;
     __syncthreads();
     if (tile.e >= a.n_adapters) {                // rows of no adapter: base, or zeros
         copy_rows<DT, kThreads, VOUT>(a, row_of, static_cast<int>(tile.n), unit0 * CW, min(unit1 * CW, a.c_out), keep, cr, cs);
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     }
     const size_t expert = tile.e;
     if constexpr (VIN && VOUT) {                 // everything that this CTA will read is on its way before it waits for any of it
-        const int k0 = static_cast<int>(static_cast<long long>(chunks) * cr / cs) * 32, k1 = min(static_cast<int>(static_cast<long long>(chunks) * (cr + 1) / cs) * 32, a.c_in);
+        const int k0 = static_cast<int>(static_cast<long long>(chunks) * cr >> cluster_log) * 32, k1 = min(static_cast<int>(static_cast<long long>(chunks) * (cr + 1) >> cluster_log) * 32, a.c_in);
         const int n0 = unit0 * CW, n1 = min(unit1 * CW, a.c_out);
         const size_t in_row = static_cast<size_t>(a.c_in) * SIZE, out_row = static_cast<size_t>(a.c_out) * SIZE, rank_row = static_cast<size_t>(a.rank) * SIZE;
         const char *const down = static_cast<const char *>(a.down) + expert * a.rank * in_row, *const up = static_cast<const char *>(a.up) + expert * a.rank * out_row;
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     int rows[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) rows[m][0] = row_of[16 * m + g], rows[m][1] = row_of[16 * m + g + 8];
-    const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * me / workers), chunk1 = static_cast<int>(static_cast<long long>(chunks) * (me + 1) / workers);
+    const int chunk0 = static_cast<int>(static_cast<long long>(chunks) * me >> (cluster_log + 3)), chunk1 = static_cast<int>(static_cast<long long>(chunks) * (me + 1) >> (cluster_log + 3));
 
     // What a warp's step of the second product reads: weights of 32 ranks (tiles of columns, or four rows of ranks at a time), base.  EARLY: several steps'
     // are loaded at once, the first ones before the parts meet (64 rows of 32 adapters 12.1 us a step at a time); elsewhere, where registers do not allow
@@ -245,13 +246,20 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
         for (int i0 = 0; i0 < ROWS * RB / 4; i0 += kThreads) {
             const int i = i0 + threadIdx.x, row = i / (RB / 4), col = i % (RB / 4) * 4;
             const bool mine = ROWS * RB / 4 % kThreads == 0 || i < ROWS * RB / 4;
-            float4 v[cs], s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            auto add = [&](auto count) {         // all loads first
+                constexpr int N = decltype(count)::value;
+                float4 v[N];
+#pragma unroll
+                for (int q = 0; q < N; ++q) v[q] = ld_cta(part + row * PS + col, q);
+#pragma unroll
+                for (int q = 0; q < N; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
+            };
             if (mine) {
-#pragma unroll
-                for (int q = 0; q < cs; ++q) v[q] = ld_cta(part + row * PS + col, q);
-#pragma unroll
-                for (int q = 0; q < cs; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
-                if (keep && i % cs == cr) {      // the CTAs of the cluster share the writing
+                if (cluster_log == 3) add(std::integral_constant<int, 8>());
+                else if (cluster_log == 2) add(std::integral_constant<int, 4>());
+                else add(std::integral_constant<int, 2>());
+                if (keep && (i & (cs - 1)) == cr) {      // the CTAs of the cluster share the writing
                     const int r = row_of[row], at = rb * RB + col;
                     if (r >= 0) {
                         float *const p = a.low + static_cast<size_t>(r) * a.rank + at;
@@ -392,8 +400,15 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     cudaError_t e = attr.set(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, 200 * 1024);
     if (e != cudaSuccess) return e;
     const long long tiles = most_tiles(a, ROWS);
-    if (tiles * kCluster > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, static_cast<unsigned>(tiles * kCluster), kThreads, kCluster, smem, st, a, blocks, keep, none);
+    // The largest cluster of which all tiles' fit at once: with more CTAs a tile, each does less of the long axes, and a second wave costs as much as the first.  (Of eight CTAs 15 fit, of four
+    // 36, and about twice that at two CTAs an SM; tiles are counted as if adapters ended at half a tile.)  us of clusters of 8, 4 and 2, f32, 4096 x 4096: rank 16, 256 rows 13.2, 17.7, 27.5,
+    // 1024 29.6, 24.7, 38.8, 4096 106, 93, 92; rank 64, 1024 137, 100, 96.  Narrow layers have too little for eight: 1024 x 1024, rank 64, 64 rows 15.6, 15.2, 22.7, bf16 8.2, 7.3, 8.6; 4096
+    // rows of f32 281, 125, 104.
+    constexpr int ROOM = DT == MTC_F32 && RB > 16 ? 1 : 2;                       // CTAs an SM
+    const long long about = a.n_rows / ROWS + std::min(a.n_adapters, a.n_rows) / 2;
+    const int cluster_log = about <= 16 * ROOM - (ROOM == 1) && a.c_in + a.c_out > 2048 ? 3 : about <= 36 * ROOM ? 2 : 1;
+    if ((tiles << cluster_log) > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, static_cast<unsigned>(tiles << cluster_log), kThreads, 1 << cluster_log, smem, st, a, cluster_log, blocks, keep, none);
 }
 template <int DT, int MT, bool BACK>
 cudaError_t launch_pieces(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
@@ -428,9 +443,11 @@ cudaError_t launch_side(cudaStream_t st, const LoraArgs &a, bool keep, bool none
 
 template <int DT>
 cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
-    // Tiles of 32 rows where those of 16 are more CTAs than the GPU holds at once, and the registers of the form allow it (us of 16 and 32 rows, 4096 x 4096): bf16 rank 16, 512 rows 8.2
-    // and 9.3, 1024 15.5 and 10.7; f32 rank 16, 4096 rows 103 and 132, rank 32, 128 12.8 and 16.8, 256 23.7 and 17.0
-    const bool wide = DT != MTC_F32 ? a.n_rows > 640 : a.n_rows > 192 && a.rank > 16;
+    // Tiles of 32 rows where those of 16 leave clusters too small or make a second wave (launch), and the registers of the form allow it.  us of 16 and 32 rows, 4096 x 4096: bf16 rank 16,
+    // 1024 rows 10.4 and 13.5, 2048 18.4 and 16.6; f32 rank 32, 192 rows 14.0 and 18.1, 256 21.4 and 18.2, 384 21.6 and 18.4, 512 23.4 and 30.5, 640 46.6 and 33.8, 2048 94 and 69
+    // (1024 x 1024: 384 rows 9.4 and 11.8, 640 13.3 and 12.1); f32 rank 16, 4096 rows 103 and 132
+    const bool between = a.n_rows > 240 && a.n_rows <= 480 && a.c_in + a.c_out > 2048;
+    const bool wide = DT != MTC_F32 ? a.n_rows > 1152 : a.rank > 16 && (a.n_rows > 576 || between);
     if (wide) return backward ? launch_side<DT, 2, true>(st, a, keep, none) : launch_side<DT, 2, false>(st, a, keep, none);
     return backward ? launch_side<DT, 1, true>(st, a, keep, none) : launch_side<DT, 1, false>(st, a, keep, none);
 }

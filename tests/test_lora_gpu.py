@@ -71,7 +71,9 @@ SIZES = [(1, 8, 8, 8, 1), (1, 4096, 4096, 16, 4), (2, 64, 96, 16, 1), (3, 7, 5, 
          (70, 1001, 515, 16, 2), (700, 257, 263, 32, 3), (50, 131, 1030, 64, 2), (33, 77, 99, 8, 2), (90, 2049, 4095, 24, 4), (40, 333, 250, 4, 2), (30, 101, 55, 72, 2),
          (1100, 512, 264, 64, 1), (2100, 264, 520, 16, 2), (2100, 128, 72, 32, 3), (1500, 1032, 328, 48, 1), (1030, 96, 160, 80, 2), (1500, 72, 64, 8, 2), (700, 264, 136, 2, 2),
          # whole pieces on one side alone
-         (36, 691, 384, 64, 4), (40, 384, 691, 64, 2), (210, 264, 331, 24, 3), (210, 331, 264, 40, 3), (700, 130, 264, 16, 2), (700, 264, 130, 128, 1), (24, 77, 512, 200, 2), (900, 512, 36, 8, 2)]
+         (36, 691, 384, 64, 4), (40, 384, 691, 64, 2), (210, 264, 331, 24, 3), (210, 331, 264, 40, 3), (700, 130, 264, 16, 2), (700, 264, 130, 128, 1), (24, 77, 512, 200, 2), (900, 512, 36, 8, 2),
+         # clusters of 4 and 2 CTAs, and the most rows of 8
+         (1300, 264, 2056, 16, 2), (2500, 96, 72, 40, 3), (240, 1536, 1032, 64, 1), (600, 264, 2048, 32, 2), (2600, 2048, 264, 8, 1), (1250, 130, 77, 16, 4)]
 
 
 @pytest.mark.parametrize("dt", TYPES)
