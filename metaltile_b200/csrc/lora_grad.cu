@@ -6,7 +6,7 @@
 // are staged as operand pieces a stage ahead and transposed as they are loaded; of x and dy a lane takes eight neighbours of four
 // rows and pairs them up.  All operands are bf16 pieces: f16 values are two (11 bits), since u and h have no bound that f16 would hold.
 //
-// Measured: 4096 rows of 4096 + 4096, rank 16, bf16 31 us, 2.2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 1024 + 1024 in f32, rank 8, 6.2.  Bound by what a CTA cannot overlap, in
+// Measured: 4096 rows of 4096 + 4096, rank 16, bf16 31 us, 2.2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 2048 + 768 in f32, rank 8, 10.  Bound by what a CTA cannot overlap, in
 // two waves of CTAs: of 25,000 cycles the start and the first stage take 8,000, the sums over the cluster 5,000.  A bulk copy a row and mbarriers take half the instructions and
 // were no faster (34.9 us).
 #include <algorithm>

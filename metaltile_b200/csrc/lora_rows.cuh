@@ -4,9 +4,9 @@
 // shared memory, then over distributed shared memory, so that every CTA has the whole h of the tile; then each CTA takes a part of the
 // columns of the second product.  x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.
 //
-// Bound by latency where users decode: 64 rows of 8 adapters, 4096 x 4096, rank 16, bf16 take 10.2 us where the bytes need 3; a row alone takes 5.0.  Of that the launch is 2, and
+// Bound by latency where users decode: 64 rows of 32 adapters, 4096 -> 14336, rank 16, bf16 take 10.4 us where the bytes need 3; a row alone, 4096 -> 4096, takes 5.1.  Of that the launch is 2, and
 // the chain is loads of x and A, the sums over the cluster (two barriers of it), loads of B and base, stores.  So everything that a CTA will read is asked for before
-// it waits (prefetches into L2, and base and B into registers where they fit), and a tile is spread over 64 warps.  128-row tiles of tcgen05 would be empty for the most part there;
+// it waits (prefetches into L2, and base and B into registers where they fit), and a tile is spread over up to 64 warps.  128-row tiles of tcgen05 would be empty for the most part there;
 // with a thousand rows and more the shared reading of the adapter and one thread that issues the MMAs win (lora.cu has both sides).
 #pragma once
 
