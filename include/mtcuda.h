@@ -468,7 +468,7 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
 
 /* ---- beside a projection: low-rank adapters of many requests (no counterpart in the reference) ----
  * For the rows t of adapter e:   h_t = x_t a[e]^T,   out_t = base_t + scales[e] * h_t b[e]^T           (sums f32, rounded once)
- * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; base may be out.
+ * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; base may be out, no other operand may.
  * rows u32[n_rows] holds the row numbers, each once, those of one adapter side by side, offsets u32[n_adapters + 1] where each adapter's begin: place p belongs to e where
  * offsets[e] <= p < offsets[e + 1].  The rows of the other places have no adapter: they get base (0), and stay as they are where base is out.  mtc_moe_sort of the rows'
  * adapters (k = 1, one more "expert" for the rows that have none) writes both.  hidden f32[n_rows, rank] (NULL: not wanted) gets h, zeros for rows without an adapter.
@@ -476,7 +476,7 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
  * reported (0x908).  Infinities in a or b give infinities or NaN.
  * mtc_lora_grad, from the gradient dy T[n_rows, N] of out and the forward call's `hidden`:
  *     u_t = dy_t b[e],   dx_t = base_t + scales[e] * u_t a[e],   da[e] = scales[e] * sum_t u_t x_t,   db[e] = scales[e] * sum_t dy_t h_t
- * base (NULL: 0) T[n_rows, K] is the shared projection's gradient of x and may be dx; da, db in the type and shape of a, b, zeros for adapters without rows.
+ * base (NULL: 0) T[n_rows, K] is the shared projection's gradient of x and may be dx, no other operand may; da, db in the type and shape of a, b, zeros for adapters without rows.
  * Sums run in an order that the sizes fix. */
 int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
                 void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype);

@@ -1720,6 +1720,7 @@ int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const 
         const int rc = lora_args_ok(ctx, "lora_mm", n_rows, K, N, rank, n_adapters, dtype);
         if (rc != MTC_OK || n_rows == 0) return rc;
         if (!x || !a || !b || !rows || !offsets || !out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: null pointer");
+        if (out == x || out == a || out == b || hidden == out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: out may be base, no other operand");
         mtc::LoraArgs l{};
         l.in = x, l.down = a, l.up = b, l.base = base, l.out = out;
         l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
@@ -1738,6 +1739,7 @@ int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, con
         int rc = lora_args_ok(ctx, "lora_grad", n_rows, K, N, rank, n_adapters, dtype);
         if (rc != MTC_OK) return rc;
         if (!offsets || !da || !db || (n_rows > 0 && (!dy || !x || !a || !b || !rows || !hidden || !dx))) return fail(ctx, MTC_ERR_INVALID, "lora_grad: null pointer");
+        if (n_rows > 0 && (dx == dy || dx == x || dx == a || dx == b || dx == hidden)) return fail(ctx, MTC_ERR_INVALID, "lora_grad: dx may be base, no other operand");
         rc = check_workspace(ctx, "lora_grad", workspace, workspace_bytes, mtc_lora_grad_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype));
         if (rc != MTC_OK) return rc;
         const cudaStream_t st = static_cast<cudaStream_t>(stream);

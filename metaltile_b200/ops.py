@@ -229,7 +229,7 @@ def moe_balance_grad(logits, counts, n_counted, k: int, grad_loss=None, coef: fl
 def add_rms_norm(x, norm_weight, eps: float, residual=None, sum_out=None, out=None, ctx: Context = None):
     """(y, s) with ``s = x + residual`` in the type of x and ``y = s / sqrt(mean(s^2) + eps) * norm_weight`` for every row of ``x [.., K]``.
 
-    The norm is of what ``s`` holds.  Without ``residual`` s is x itself.  ``sum_out`` (s) and ``out`` (y) may be x or residual: a residual stream that is updated in
+    The norm is of what ``s`` holds.  Without ``residual`` s is x itself (and gone where ``out`` is x).  ``sum_out`` (s) and ``out`` (y) may be x or residual: a residual stream that is updated in
     place is ``add_rms_norm(x, w, eps, residual=stream, sum_out=stream)``.  One row in front of one projection of affine codes: ``rms_norm_qmv``."""
     return _native.add_rms_norm(x, norm_weight, eps, residual, sum_out, out, ctx)
 

@@ -290,6 +290,21 @@ def test_unaligned_operands():
         d.check()
 
 
+def test_refusals():
+    from metaltile_b200 import MetalTileError, ops
+    c = Case(20, 64, 64, 8, 2, "bf16")
+    out, h = c.forward()
+    for bad in (c.x, out.new_zeros(0)[:0]):
+        with pytest.raises((MetalTileError, ValueError)):                        # its rows are read by other tiles; not the result's shape
+            c.forward(out=bad)
+    for bad in (c.x, c.dy):
+        with pytest.raises(MetalTileError):                                      # read again for the weights
+            c.grad(h, out=bad)
+    with pytest.raises(MetalTileError):                                          # a rank of more than 1024
+        ops.lora_mm(c.x, c.x.new_zeros(2, 1025, 64), c.x.new_zeros(2, 64, 1025), c.rows, c.offsets)
+    c.check()                                                                    # nothing was written or left behind
+
+
 def test_another_stream_and_graphs_that_run_at_once():
     c, d = Case(300, 1024, 768, 16, 3, "bf16", seed=1), Case(300, 1024, 768, 16, 3, "bf16", seed=2)
 
