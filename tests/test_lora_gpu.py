@@ -73,7 +73,8 @@ SIZES = [(1, 8, 8, 8, 1), (1, 4096, 4096, 16, 4), (2, 64, 96, 16, 1), (3, 7, 5, 
          # whole pieces on one side alone
          (36, 691, 384, 64, 4), (40, 384, 691, 64, 2), (210, 264, 331, 24, 3), (210, 331, 264, 40, 3), (700, 130, 264, 16, 2), (700, 264, 130, 128, 1), (24, 77, 512, 200, 2), (900, 512, 36, 8, 2),
          # clusters of 4 and 2 CTAs, and the most rows of 8
-         (1300, 264, 2056, 16, 2), (2500, 96, 72, 40, 3), (240, 1536, 1032, 64, 1), (600, 264, 2048, 32, 2), (2600, 2048, 264, 8, 1), (1250, 130, 77, 16, 4)]
+         (1300, 264, 2056, 16, 2), (2500, 96, 72, 40, 3), (240, 1536, 1032, 64, 1), (600, 264, 2048, 32, 2), (2600, 2048, 264, 8, 1), (1250, 130, 77, 16, 4),
+         (2400, 1032, 1040, 16, 2), (2400, 2048, 72, 32, 3), (2350, 520, 1600, 24, 1), (1200, 512, 264, 64, 1), (2310, 40, 2056, 32, 1)]
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -115,9 +116,9 @@ def test_in_place_leaves_rows_without_an_adapter_alone(dt):
         assert torch.equal(dbase[~none], dx[~none]) and torch.isnan(dbase[none]).all()
 
 
-# (the second size is one of the kernel with tiles of 128 rows, the third one of rows that are no whole pieces)
+# (the second size reaches tiles of 128 rows back, the fourth both ways; the third has rows that are no whole pieces)
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("size", [(60, 256, 128, 16, 3), (2100, 256, 128, 32, 3), (60, 255, 127, 16, 3)])
+@pytest.mark.parametrize("size", [(60, 256, 128, 16, 3), (2100, 256, 128, 32, 3), (60, 255, 127, 16, 3), (2400, 2048, 128, 32, 3)])
 def test_rows_without_an_adapter_hold_anything(size, dt):
     c = Case(*size, dt, seed=4)
     want, h = c.forward()
@@ -132,7 +133,7 @@ def test_rows_without_an_adapter_hold_anything(size, dt):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("rows,n", [(48, 128), (2100, 128), (48, 127)])
+@pytest.mark.parametrize("rows,n", [(48, 128), (2100, 128), (48, 127), (2400, 2048)])
 def test_special_values_stay_in_their_row(rows, n, dt):
     c = Case(rows, 256, n, 16, 2, dt, seed=5)
     want, _ = c.forward()
@@ -147,7 +148,7 @@ def test_special_values_stay_in_their_row(rows, n, dt):
     assert torch.isfinite(got[rest]).all() and (got[rest].double() - clean).abs().max() < 0.05
 
 
-@pytest.mark.parametrize("rows,n", [(40, 256), (2100, 256), (40, 255)])
+@pytest.mark.parametrize("rows,n", [(40, 256), (2100, 256), (40, 255), (2400, 2048)])
 @pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
 def test_large_and_small_values(dt, rows, n):
     """What a row goes through may be far outside of 16-bit floats."""
@@ -200,7 +201,7 @@ def test_bad_offsets_and_rows_are_reported(size, dt):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
-@pytest.mark.parametrize("size", [(90, 256, 128, 16, 3), (90, 255, 127, 16, 3), (90, 255, 127, 5, 3), (2100, 128, 64, 32, 1)])
+@pytest.mark.parametrize("size", [(90, 256, 128, 16, 3), (90, 255, 127, 16, 3), (90, 255, 127, 5, 3), (2100, 128, 64, 32, 1), (2400, 2048, 64, 32, 1), (1300, 128, 64, 64, 1)])
 def test_places_before_the_first_adapter_have_none(size, dt):
     """Any places outside of the ranges belong to no adapter, those in front as well."""
     rows, k, n, rank, adapters = size
@@ -248,9 +249,10 @@ def test_rows_whose_offsets_pass_32_bits(dt, rows):
     assert ops.context(0).status_word() == 0
 
 
-def test_beside_other_tensor_memory_kernels_on_another_stream():
+@pytest.mark.parametrize("rows", [2200, 2500])
+def test_beside_other_tensor_memory_kernels_on_another_stream(rows):
     from metaltile_b200 import ops
-    c = Case(2200, 1024, 2048, 16, 2, "bf16", seed=11)
+    c = Case(rows, 1024, 2048, 16, 2, "bf16", seed=11)
     want, h = c.forward()
     grads = c.grad(h)
     g = torch.Generator(device="cuda").manual_seed(1)
