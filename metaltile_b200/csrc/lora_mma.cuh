@@ -217,10 +217,11 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, b
     return {-1, 0, 0};
 }
 
-// f16: the power of two at or below a row's largest value, within what f32 can divide by (infinities and NaN: 1)
+// f16: a power of two that brings a row's largest value to between 2^14 and 2^15, within what f32 can divide by (infinities and NaN: 1).  So high that the least of a row keep their bits: two
+// pieces of f16 reach down to 2^-24, 38 octaves below, and are 16 bits and more of every value down to 2^-22 of the largest.  (Products with f16 weights of 2^16 leave f32 sums room.)
 __device__ __forceinline__ float unit_of(float most) {
     const int e = static_cast<int>(__float_as_uint(most) >> 23);
-    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(min(max(e, 27), 253)) << 23);
+    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(max(e - 14, 1)) << 23);
 }
 // Four neighbours as operand pieces.  f16: divided by `unit`, since it has five bits of exponent.
 template <int DT>
