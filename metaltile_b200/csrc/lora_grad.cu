@@ -4,7 +4,9 @@
 // One launch for both.  A CTA has a block of columns of one adapter, all its ranks (64 at a time), and a part of its rows; the CTAs of a cluster share the
 // rows and add up over distributed shared memory in a fixed order.  x and dy pass once, by cp.async, 64 rows a stage, up to two stages ahead.  Rows are the k of the MMAs: u and h
 // are staged as operand pieces a stage ahead and transposed as they are loaded; of x and dy a lane takes eight neighbours of four
-// rows and pairs them up.  All operands are bf16 pieces: f16 values are two (11 bits), since u and h have no bound that f16 would hold.
+// rows and pairs them up.  All operands are bf16 pieces: f16 values are two (11 bits), since u and h have no bound that f16 would hold.  Of f16 all four products of pieces are
+// taken: that of the small ones is up to 2^-14 of the whole, of one sign where the operands are (left out, it cost one result in 25 its last bit
+// there); it costs a training step 3 to 6 % (2048 x 4096 -> 4096, rank 64, 108.5 -> 114.4 us).
 //
 // Measured: 4096 rows of 4096 + 4096, rank 16, bf16 31 us, 2.2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 2048 + 768 in f32, rank 8, 10.  Bound by what a CTA cannot overlap, in
 // two waves of CTAs: of 25,000 cycles the start and the first stage take 8,000, the sums over the cluster 5,000.  A bulk copy a row and mbarriers take half the instructions and
@@ -66,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
     pdl_enter();
     using F = Form<DT, RB>;
     using S = Split<DT, F::NT>;
-    constexpr int NT = F::NT, CB = F::CB, RP = F::RP, MT = F::MT, H = F::H, P = S::P, DEEP = P == 1 ? 2 : P;
+    constexpr int NT = F::NT, CB = F::CB, RP = F::RP, MT = F::MT, H = F::H, P = S::P, DEEP = P == 1 ? 2 : 3;   // products of pieces with p + q < DEEP: all of one or two, six of nine of three
     extern __shared__ __align__(128) uint8_t sm[];
     float *const sums = reinterpret_cast<float *>(sm);                           // [2][RP][CB + 4], or [2][CB][RP + 4]
     const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(sm)), held = base + F::AHEAD * F::tile;          // [2][H][kStage][RP] bf16, units of 16 bytes moved about

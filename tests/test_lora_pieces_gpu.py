@@ -21,3 +21,17 @@ def test_ranks_of_different_size(size, dt):
     s = 2.0 ** torch.linspace(-8, 8, size[3], device="cuda").round()
     c.a, c.b = (c.a.float() / s[:, None]).to(TYPES[dt]), (c.b.float() * s).to(TYPES[dt])
     c.check()
+
+
+@pytest.mark.parametrize("k,n", [(64, 264), (61, 131)])
+def test_f16_gradients_of_values_below_a_step_of_eight_bits(k, n):
+    """A row an adapter, so that db is one product: what eight bits leave of either factor is nearly a step, and so is the product of these rests."""
+    rows, rank = 64, 16
+    c = Case(rows, k, n, rank, rows, "f16", ids=list(range(rows)), seed=13, base=False)
+    g = torch.Generator(device="cuda").manual_seed(14)
+    h = 1 + 2.0 ** -7 - torch.rand(rows, rank, device="cuda", generator=g) * 2.0 ** -9
+    c.dy = ((1 + 2.0 ** -7 - 2.0 ** -10) * 2.0 ** torch.randint(-3, 4, (rows, n), device="cuda", generator=g)).half()
+    _, _, db = c.grad(h)
+    want = c.scales.double()[:, None, None] * c.dy.double()[:, :, None] * h.double()[:, None, :]
+    # rounded once; two pieces of h; the sums of the pieces' four products and the scale
+    _close(db, want, (ref.STEP[torch.float16] + 2.0 ** -16 + 8 * ref.F32) * want)
