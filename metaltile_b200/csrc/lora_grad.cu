@@ -30,14 +30,14 @@ struct Split {
     __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
         if constexpr (DT != MTC_F16) {
             Vals<DT, W> v;
-            v.load(base, at, there);
+            v.template load<true>(base, at, there);
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int i = 0; i < N; ++i) w[p][i] = v.w[p][i];
         } else {
             Vals<DT, W> v;
-            v.load(base, at, there);
+            v.template load<true>(base, at, there);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v.w[0][i]));

@@ -1,8 +1,11 @@
 // What the tensor-core kernels of low-rank adapters share: operands in pieces, fragments, and which rows and columns a lane holds.
 //
-// Operands.  Warp-level MMAs of 16-bit values with f32 sums.  f32 values are three bf16 pieces of 8 bits each, cut off one after the other: 24 bits,
-// exact; products of pieces that together lie below 2^-24 of the whole are left out (six of nine remain).  bf16 and f16 weights and activations are operands as they
-// are.  What lies between the two products, h or u, is an f32 sum: as an operand it is held in two pieces (16 bits and more), in three beside f32 weights.
+// Operands.  Warp-level MMAs of 16-bit values with f32 sums.  f32 values are three bf16 pieces, each what is left rounded to 8 bits: 24 bits, exact.  A rest is at most 2^-8 of what was
+// rounded, so the products of pieces that are left out (two small ones and the smallest; six of nine remain) are together at most 2^-24 of the whole, on either side of it.  (Pieces that are
+// cut off leave rests of twice the size and of one sign: 2^-21.)  bf16 and f16 weights and activations are operands as they are.
+//
+// What lies between the two products, h or u, is an f32 sum.  Beside f32 weights it is an operand in three pieces, 24 bits.  Beside 16-bit weights it is held in two, which costs two MMAs a
+// step of ranks: 17 bits of bf16 (2^-17 of each value; the result, rounded to 8 bits, is off by 2^-9), 16 and more of f16 (below).  What is kept for the backward pass is the f32 sum.
 //
 // Order of k.  A sum may run over k in any order as long as both operands have the same, so a lane takes what lies next to each other in memory: of
 // 32 neighbours lane (g, t) = (lane / 4, lane % 4) has 8t .. 8t + 7, the first four of them in the first of two MMAs.  Where the other operand lies across (k along
@@ -20,6 +23,17 @@ constexpr int pieces = DT == MTC_F32 ? 3 : 1;    // of weights and activations
 __device__ __forceinline__ uint32_t high_halves(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x7632); }
 __device__ __forceinline__ uint32_t low_halves(uint32_t lo, uint32_t hi) { return __byte_perm(lo, hi, 0x5410); }
 
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// What is rounded for the first piece: within the largest of bf16, so that a f32 value above that does not become an infinity (one that is an infinity is left to the second piece)
+__device__ __forceinline__ float first_piece(float v) {
+    float r;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0x1.FEp127f));
+    return r;
+}
+
 // W neighbouring values as operand pieces: pairs of 16-bit values (one value: the low half)
 template <int DT, int W>
 struct Vals {
@@ -33,6 +47,7 @@ struct Vals {
             for (int i = 0; i < N; ++i) w[p][i] = 0;
     }
     // aligned to W values
+    template <bool ANY>
     __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
         zero();
         if (!there) return;
@@ -64,16 +79,17 @@ struct Vals {
             } else {
                 v[0] = *p;
             }
-            split(v);
+            split<ANY>(v);
         }
     }
     // n of them exist, any alignment
+    template <bool ANY>
     __device__ __forceinline__ void load_any(const void *base, size_t at, int n) {
         if constexpr (DT == MTC_F32) {
             float v[W];
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] = i < n ? static_cast<const float *>(base)[at + i] : 0.0f;
-            split(v);
+            split<ANY>(v);
         } else {
             zero();
 #pragma unroll
@@ -81,16 +97,18 @@ struct Vals {
                 if (i < n) w[0][i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(base)[at + i]) << (i & 1) * 16;
         }
     }
+    // ANY: values beyond the largest of bf16 as well; else they leave infinities or NaN in every sum that they go into
+    template <bool ANY>
     __device__ __forceinline__ void split(float (&v)[W]) {
 #pragma unroll
         for (int k = 0; k < P; ++k) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float lo = v[2 * i], hi = W == 1 ? 0.0f : v[W == 1 ? 0 : 2 * i + 1];
-                w[k][i] = high_halves(__float_as_uint(lo), __float_as_uint(hi));
+                const uint32_t u = w[k][i] = ANY && k == 0 ? bf16_pair(first_piece(lo), first_piece(hi)) : bf16_pair(lo, hi);
+                v[2 * i] = lo - __uint_as_float(u << 16);
+                if (W > 1) v[W == 1 ? 0 : 2 * i + 1] = hi - __uint_as_float(u & 0xFFFF0000u);
             }
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] -= __uint_as_float(__float_as_uint(v[i]) & 0xFFFF0000u);
         }
     }
     // value j of x with value j of y, as a pair
@@ -244,13 +262,9 @@ __device__ __forceinline__ void hold_pieces(float4 s, float unit, uint2 *piece) 
                 w[i] = *reinterpret_cast<const uint32_t *>(&h);
                 const float2 f = __half22float2(h);
                 x = fabsf(x) < INFINITY ? x - f.x : 0.0f, y = fabsf(y) < INFINITY ? y - f.y : 0.0f;
-            } else if (p + 1 < H) {
-                const uint32_t b = __float_as_uint(x), c = __float_as_uint(y);
-                w[i] = high_halves(b, c);
-                x = fabsf(x) < INFINITY ? x - __uint_as_float(b & 0xFFFF0000u) : 0.0f, y = fabsf(y) < INFINITY ? y - __uint_as_float(c & 0xFFFF0000u) : 0.0f;
             } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                w[i] = p == 0 ? bf16_pair(first_piece(x), first_piece(y)) : bf16_pair(x, y);
+                x -= __uint_as_float(w[i] << 16), y -= __uint_as_float(w[i] & 0xFFFF0000u);
             }
         }
         piece[p] = make_uint2(w[0], w[1]);

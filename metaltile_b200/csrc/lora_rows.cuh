@@ -42,6 +42,28 @@ __device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, i
         prefetch(static_cast<const char *>(from) + i, min(piece, bytes - i));
 }
 
+// Whether all these sums are numbers
+template <int A, int B>
+__device__ __forceinline__ bool finite(const float (&large)[A][B][4], const float (&small)[A][B][4]) {
+    float z = 0.0f;                              // (an infinity and a NaN times zero are NaN)
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z = fmaf(large[a][b][i], 0.0f, fmaf(small[a][b][i], 0.0f, z));
+    return z == 0.0f;
+}
+template <int A, int B>
+__device__ __forceinline__ void clear(float (&sums)[A][B][4]) {
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[a][b][i] = 0.0f;
+}
+
 // RB: ranks a pass (a block of the rank, ONE: there is one), 8 to 64.  MT: tiles of 16 rows.  VIN, VOUT: rows on this side are whole 16-byte pieces; else their values are
 // loaded one by one.  BACK: the first product's weights lie [c_in][rank], the second's
 // [rank][c_out]; else [rank][c_in] and [c_out][rank].
@@ -131,13 +153,14 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                     else to.base[m][h][i].load_any(a.base, at, there ? a.c_out - c : 0);
                 }
     };
-    auto load_weights = [&](V *to, int n0, int r, int i) {       // r: this lane's first rank; i (BACK): four ranks behind
+    auto load_weights = [&](auto any, V *to, int n0, int r, int i) {     // r: this lane's first rank; i (BACK): four ranks behind
+        constexpr bool ANY = decltype(any)::value;
         if constexpr (!BACK) {
             // column c of tile j is n0 + c / 2 * 8 + 2 j + c % 2, so that a lane's results are eight neighbours
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int n = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
-                to[j].load(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
+                to[j].template load<ANY>(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
             }
         } else {
             // column c of tile j is n0 + 8 c + j: a lane loads eight neighbours of four ranks' rows, its results are sixteen
@@ -145,15 +168,15 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
 #pragma unroll
             for (int s = 0; s < DEEP; ++s) {
                 const int rr = r + 4 * i + s;
-                if constexpr (VOUT) to[s].load(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
-                else to[s].load_any(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank ? a.c_out - c : 0);
+                if constexpr (VOUT) to[s].template load<ANY>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
+                else to[s].template load_any<ANY>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank ? a.c_out - c : 0);
             }
         }
     };
     auto load_early = [&](Unit &to, int n0) {
         load_base(to, n0);
 #pragma unroll
-        for (int i = 0; i < (BACK ? PARTS : 1); ++i) load_weights(to.w + i * DEEP, n0, t * WIDE, i);
+        for (int i = 0; i < (BACK ? PARTS : 1); ++i) load_weights(std::false_type(), to.w + i * DEEP, n0, t * WIDE, i);
     };
     Unit steps[STEPS];
     auto load_steps = [&](int u) {               // steps u, u + kWarps ..
@@ -165,52 +188,62 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     for (int rb = 0; rb < rank_blocks; ++rb) {
         float acc[MT][NT][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? NT : 1][4] = {};      // f32: the products of small pieces, apart so that the large ones are cut off less often
-#pragma unroll (MT == 1 && RB <= 16 && P == 1 ? 4 : 2)
-        for (int c = chunk0; c < chunk1; ++c) {
-            const int k = c * 32 + t * 8;
-            const bool in = k < a.c_in;
-            Vals<DT, 8> x[MT][2];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if constexpr (VIN) x[m][h].load(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
-                    else x[m][h].load_any(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, rows[m][h] >= 0 ? a.c_in - k : 0);
-                }
-            auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {      // tile j of ranks, piece p of the weights, half i of the 32 values
+        auto sum_up = [&](auto any) {
+            constexpr bool ANY = decltype(any)::value;
+#pragma unroll (ANY ? 1 : MT == 1 && RB <= 16 && P == 1 ? 4 : 2)
+            for (int c = chunk0; c < chunk1; ++c) {
+                const int k = c * 32 + t * 8;
+                const bool in = k < a.c_in;
+                Vals<DT, 8> x[MT][2];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int q = 0; q + p < P; ++q) {
-                        float (&d)[4] = P > 1 && q + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
-                        mma<HALF>(d, x[m][0].w[q][2 * i], x[m][1].w[q][2 * i], x[m][0].w[q][2 * i + 1], x[m][1].w[q][2 * i + 1], b0, b1);
+                    for (int h = 0; h < 2; ++h) {
+                        if constexpr (VIN) x[m][h].template load<ANY>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
+                        else x[m][h].template load_any<ANY>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, rows[m][h] >= 0 ? a.c_in - k : 0);
                     }
-            };
-            if constexpr (!BACK) {
+                auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {      // tile j of ranks, piece p of the weights, half i of the 32 values
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int r = rb * RB + 8 * j + g;
-                    Vals<DT, 8> w;
-                    if constexpr (VIN) w.load(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
-                    else w.load_any(a.down, (expert * a.rank + r) * a.c_in + k, r < a.rank ? a.c_in - k : 0);
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int p = 0; p < P; ++p)
+                        for (int q = 0; q + p < P; ++q) {
+                            float (&d)[4] = P > 1 && q + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
+                            mma<HALF>(d, x[m][0].w[q][2 * i], x[m][1].w[q][2 * i], x[m][0].w[q][2 * i + 1], x[m][1].w[q][2 * i + 1], b0, b1);
+                        }
+                };
+                if constexpr (!BACK) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) step(j, p, i, w.w[p][2 * i], w.w[p][2 * i + 1]);
+                    for (int j = 0; j < NT; ++j) {
+                        const int r = rb * RB + 8 * j + g;
+                        Vals<DT, 8> w;
+                        if constexpr (VIN) w.template load<ANY>(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
+                        else w.template load_any<ANY>(a.down, (expert * a.rank + r) * a.c_in + k, r < a.rank ? a.c_in - k : 0);
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) step(j, p, i, w.w[p][2 * i], w.w[p][2 * i + 1]);
+                    }
+                } else {
+                    using V = Vals<DT, NT>;          // lane g has ranks g NT .. g NT + NT - 1: rank g NT + j is column g of tile j
+                    const int r = rb * RB + g * NT;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        V w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) w[q].template load<ANY>(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VIN ? in : k + 4 * i + q < a.c_in) && r < a.rank);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), V::pair(w[2], w[3], p, j));
+                    }
                 }
-            } else {
-                using V = Vals<DT, NT>;          // lane g has ranks g NT .. g NT + NT - 1: rank g NT + j is column g of tile j
-                const int r = rb * RB + g * NT;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    V w[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) w[q].load(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VIN ? in : k + 4 * i + q < a.c_in) && r < a.rank);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), V::pair(w[2], w[3], p, j));
-                }
+            }
+        };
+        sum_up(std::false_type());
+        if constexpr (P > 1) {                   // a sum that is no number, or values that 16 bits do not reach: once more, with more care
+            if (__any_sync(0xffffffffu, !finite(acc, fine))) {
+                clear(acc), clear(fine);
+                sum_up(std::true_type());
             }
         }
         if constexpr (EARLY) {
@@ -308,58 +341,67 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
         if constexpr (!EARLY) load_base(unit, n0);
         float acc[MT][TN][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? TN : 1][4] = {};
-        for (int rb = 0; rb < rank_blocks; ++rb) {
+        auto sum_up = [&](auto any) {
+            for (int rb = 0; rb < rank_blocks; ++rb) {
 #pragma unroll
-            for (int q = 0; q < QS; ++q) {
-                const int r = rb * RB + q * 32 + t * WIDE;       // this lane's ranks: r .. r + WIDE - 1
-                uint32_t hw[MT][2][H][WIDE / 2];
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int p = 0; p < H; ++p) {
-                            const uint16_t *const at = held + (p * ROWS + 16 * m + g + 8 * h) * HS + r;
-                            if constexpr (WIDE == 8) {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(at);
-                                hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y, hw[m][h][p][2] = v.z, hw[m][h][p][3] = v.w;
-                            } else if constexpr (WIDE == 4) {
-                                const uint2 v = *reinterpret_cast<const uint2 *>(at);
-                                hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y;
-                            } else {
-                                hw[m][h][p][0] = *reinterpret_cast<const uint32_t *>(at);
-                            }
-                        }
-                auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {  // tile j of columns, piece p of the weights, ranks 4 i .. of the lane's
+                for (int q = 0; q < QS; ++q) {
+                    const int r = rb * RB + q * 32 + t * WIDE;       // this lane's ranks: r .. r + WIDE - 1
+                    uint32_t hw[MT][2][H][WIDE / 2];
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
-                        for (int s = 0; s < H; ++s) {
-                            if (P > 1 && s + p >= P) continue;
-                            float (&d)[4] = P > 1 && s + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
-                            const uint32_t a2 = WIDE == 2 ? 0u : hw[m][0][s][WIDE == 2 ? 0 : 2 * i + 1], a3 = WIDE == 2 ? 0u : hw[m][1][s][WIDE == 2 ? 0 : 2 * i + 1];
-                            mma<HALF>(d, hw[m][0][s][2 * i], hw[m][1][s][2 * i], a2, a3, b0, b1);
-                        }
-                };
-                if constexpr (!BACK) {
-                    if constexpr (!EARLY) load_weights(unit.w, n0, r, 0);
+                        for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < TN; ++j)
+                            for (int p = 0; p < H; ++p) {
+                                const uint16_t *const at = held + (p * ROWS + 16 * m + g + 8 * h) * HS + r;
+                                if constexpr (WIDE == 8) {
+                                    const uint4 v = *reinterpret_cast<const uint4 *>(at);
+                                    hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y, hw[m][h][p][2] = v.z, hw[m][h][p][3] = v.w;
+                                } else if constexpr (WIDE == 4) {
+                                    const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                                    hw[m][h][p][0] = v.x, hw[m][h][p][1] = v.y;
+                                } else {
+                                    hw[m][h][p][0] = *reinterpret_cast<const uint32_t *>(at);
+                                }
+                            }
+                    auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {  // tile j of columns, piece p of the weights, ranks 4 i .. of the lane's
 #pragma unroll
-                        for (int p = 0; p < P; ++p)
+                        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                            for (int i = 0; i < PARTS; ++i) step(j, p, i, unit.w[j].w[p][2 * i], WIDE == 2 ? 0u : unit.w[j].w[p][WIDE == 2 ? 0 : 2 * i + 1]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < PARTS; ++i) {
-                        V *const w = unit.w + (EARLY ? i * DEEP : 0);
-                        if constexpr (!EARLY) load_weights(w, n0, r, i);
+                            for (int s = 0; s < H; ++s) {
+                                if (P > 1 && s + p >= P) continue;
+                                float (&d)[4] = P > 1 && s + p > 0 ? fine[P > 1 ? m : 0][P > 1 ? j : 0] : acc[m][j];
+                                const uint32_t a2 = WIDE == 2 ? 0u : hw[m][0][s][WIDE == 2 ? 0 : 2 * i + 1], a3 = WIDE == 2 ? 0u : hw[m][1][s][WIDE == 2 ? 0 : 2 * i + 1];
+                                mma<HALF>(d, hw[m][0][s][2 * i], hw[m][1][s][2 * i], a2, a3, b0, b1);
+                            }
+                    };
+                    if constexpr (!BACK) {
+                        if constexpr (!EARLY) load_weights(any, unit.w, n0, r, 0);
 #pragma unroll
                         for (int j = 0; j < TN; ++j)
 #pragma unroll
-                            for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), WIDE == 2 ? 0u : V::pair(w[WIDE == 2 ? 0 : 2], w[WIDE == 2 ? 1 : 3], p, j));
+                            for (int p = 0; p < P; ++p)
+#pragma unroll
+                                for (int i = 0; i < PARTS; ++i) step(j, p, i, unit.w[j].w[p][2 * i], WIDE == 2 ? 0u : unit.w[j].w[p][WIDE == 2 ? 0 : 2 * i + 1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < PARTS; ++i) {
+                            V *const w = unit.w + (EARLY ? i * DEEP : 0);
+                            if constexpr (!EARLY) load_weights(any, w, n0, r, i);
+#pragma unroll
+                            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                                for (int p = 0; p < P; ++p) step(j, p, i, V::pair(w[0], w[1], p, j), WIDE == 2 ? 0u : V::pair(w[WIDE == 2 ? 0 : 2], w[WIDE == 2 ? 1 : 3], p, j));
+                        }
                     }
                 }
+            }
+        };
+        sum_up(std::false_type());
+        if constexpr (P > 1) {
+            if (__any_sync(0xffffffffu, !finite(acc, fine))) {
+                clear(acc), clear(fine);
+                sum_up(std::true_type());
             }
         }
 #pragma unroll

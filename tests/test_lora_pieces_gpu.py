@@ -35,3 +35,34 @@ def test_f16_gradients_of_values_below_a_step_of_eight_bits(k, n):
     want = c.scales.double()[:, None, None] * c.dy.double()[:, :, None] * h.double()[:, None, :]
     # rounded once; two pieces of h; the sums of the pieces' four products and the scale
     _close(db, want, (ref.STEP[torch.float16] + 2.0 ** -16 + 8 * ref.F32) * want)
+
+
+# One step of 8 bits, with rests that are as large as they can be: what is left out of the products of their pieces is too.
+BELOW = (1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -17, 1 + 3 * 2.0 ** -8 - 2.0 ** -17, 1 + 2.0 ** -8 - 2.0 ** -23)
+
+
+@pytest.mark.parametrize("size", [s for s in KERNELS if s[0] < 100])
+def test_f32_products_of_values_below_a_step_of_eight_bits(size):
+    """One product a value of h: the pairs of small pieces that are left out are below 2^-24 of it, the rounding and what a tensor core cuts off of the small products 2^-24 together each."""
+    rows, k, n, rank, adapters = size
+    c = Case(*size, "f32", ids=[i % adapters for i in range(rows)], seed=15, base=False, scales=False)
+    v = torch.tensor(BELOW, device="cuda", dtype=torch.float64)
+    c.x.zero_()
+    at = torch.arange(rows, device="cuda") * 7 % k
+    c.x[torch.arange(rows, device="cuda"), at] = v[torch.arange(rows, device="cuda") % 4].float()
+    c.a = v[(torch.arange(adapters * rank * k, device="cuda") // 3) % 4].float().view(adapters, rank, k)
+    _, h = c.forward()
+    want = ref.low(c.x, c.a, c.ids)
+    _close(h, want, 1.5 * 2.0 ** -23 * want)
+
+
+@pytest.mark.parametrize("size", [(300, 4096, 4096, 16, 2), (300, 4096, 4100, 64, 1), (300, 4095, 4100, 24, 1), (40, 4096, 4096, 8, 1), (200, 4096, 4096, 80, 1), (1300, 4096, 4096, 32, 2)])
+def test_f32_sums_keep_what_three_pieces_hold(size):
+    """Each value of a sum of thousands is a product of 24 bits.  Some fifty additions of partial sums stand behind a result, each off by a step of 2^-23 at most: 2^-20.2 of a result's root mean
+    square, and once more where it goes through both products.  Two pieces in place of three would be 2^-17.8 (test_a_lost_piece_shows)."""
+    c = Case(*size, "f32", seed=16, base=False)
+    out, h = c.forward()
+    got = (h, out, *c.grad(h))
+    want_out, want_h = ref.lora(c.x, c.a, c.b, c.ids, c.scales, None)
+    for one, want in zip(got, (want_h, want_out, *ref.lora_grad(c.dy, c.x, c.a, c.b, c.ids, c.scales, None))):
+        assert (one.double() - want).square().mean().sqrt() <= 2.0 ** -19 * want.square().mean().sqrt()
