@@ -473,10 +473,12 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
  * offsets[e] <= p < offsets[e + 1].  The rows of the other places have no adapter: they get base (0), and stay as they are where base is out.  mtc_moe_sort of the rows'
  * adapters (k = 1, one more "expert" for the rows that have none) writes both.  hidden f32[n_rows, rank] (NULL: not wanted) gets h, zeros for rows without an adapter.
  * Offsets that run backwards or past the rows are clamped and reported through the status word (0x901), row numbers that do not exist are left out and
- * reported (0x908).  Infinities in a or b give infinities or NaN.
+ * reported (0x908).  Infinities in x and base are the formula's (inf * 0 is NaN), those in a or b give infinities or NaN in the rows of their adapter.
+ * h beside f16 and bf16 weights is held to 16 bits and more (17 of bf16) for its product with b; `hidden` is f32.
  * mtc_lora_grad, from the gradient dy T[n_rows, N] of out and the forward call's `hidden`:
  *     u_t = dy_t b[e],   dx_t = base_t + scales[e] * u_t a[e],   da[e] = scales[e] * sum_t u_t x_t,   db[e] = scales[e] * sum_t dy_t h_t
  * base (NULL: 0) T[n_rows, K] is the shared projection's gradient of x and may be dx, no other operand may; da, db in the type and shape of a, b, zeros for adapters without rows.
+ * Infinities in dy and base are the formula's in dx; in da and db, and those in a or b, they give infinities or NaN.  u and h beside f16 and bf16 as above.
  * Sums run in an order that the sizes fix. */
 int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const void *b, const void *rows, const void *offsets, const void *scales, const void *base,
                 void *out, void *hidden, int n_rows, int K, int N, int rank, int n_adapters, int dtype);

@@ -30,14 +30,14 @@ struct Split {
     __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
         if constexpr (DT != MTC_F16) {
             Vals<DT, W> v;
-            v.template load<true>(base, at, there);
+            v.template load<Care::large>(base, at, there);
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int i = 0; i < N; ++i) w[p][i] = v.w[p][i];
         } else {
             Vals<DT, W> v;
-            v.template load<true>(base, at, there);
+            v.template load<Care::large>(base, at, there);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v.w[0][i]));
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 ? 1 : 2) lora_weights_
         for (int i = 0; i < TURNS; ++i) {
             const int q = i * kThreads + tid, u4 = q % (RP / 4);
             uint2 piece[3];
-            hold_pieces<H == 3 ? MTC_F32 : MTC_BF16>(v[i], 1.0f, piece);
+            hold_pieces<H == 3 ? MTC_F32 : MTC_BF16, Care::large>(v[i], 1.0f, piece);
 #pragma unroll
             for (int p = 0; p < H; ++p)
                 asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(piece_at(s, p, q / (RP / 4), u4 / 2) + (u4 & 1) * 8), "r"(piece[p].x), "r"(piece[p].y) : "memory");

@@ -27,12 +27,18 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// What is rounded for the first piece: within the largest of bf16, so that a f32 value above that does not become an infinity (one that is an infinity is left to the second piece)
+// What is rounded for the first piece: within the largest of bf16, so that a f32 value above that does not become an infinity (one that is an infinity is left to the next piece)
 __device__ __forceinline__ float first_piece(float v) {
     float r;
     asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0x1.FEp127f));
     return r;
 }
+
+__device__ __forceinline__ float or_zero(float v) { return fabsf(v) < INFINITY ? v : 0.0f; }
+
+// How f32 values are cut into pieces: without a look at them, where a value beyond the largest of bf16 leaves NaN in every sum that it goes into; with the first piece held back, where only
+// infinities and NaN do; or with these in the last piece alone, which is multiplied with the others' first pieces only: these have the values' signs, and are zero where the values are.
+enum class Care { none, large, all };
 
 // W neighbouring values as operand pieces: pairs of 16-bit values (one value: the low half)
 template <int DT, int W>
@@ -47,7 +53,7 @@ struct Vals {
             for (int i = 0; i < N; ++i) w[p][i] = 0;
     }
     // aligned to W values
-    template <bool ANY>
+    template <Care CARE>
     __device__ __forceinline__ void load(const void *base, size_t at, bool there) {
         zero();
         if (!there) return;
@@ -79,17 +85,17 @@ struct Vals {
             } else {
                 v[0] = *p;
             }
-            split<ANY>(v);
+            split<CARE>(v);
         }
     }
     // n of them exist, any alignment
-    template <bool ANY>
+    template <Care CARE>
     __device__ __forceinline__ void load_any(const void *base, size_t at, int n) {
         if constexpr (DT == MTC_F32) {
             float v[W];
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] = i < n ? static_cast<const float *>(base)[at + i] : 0.0f;
-            split<ANY>(v);
+            split<CARE>(v);
         } else {
             zero();
 #pragma unroll
@@ -97,15 +103,18 @@ struct Vals {
                 if (i < n) w[0][i / 2] |= static_cast<uint32_t>(static_cast<const uint16_t *>(base)[at + i]) << (i & 1) * 16;
         }
     }
-    // ANY: values beyond the largest of bf16 as well; else they leave infinities or NaN in every sum that they go into
-    template <bool ANY>
+    template <Care CARE>
     __device__ __forceinline__ void split(float (&v)[W]) {
+        auto piece_of = [](float x, int k) {
+            if (CARE == Care::all && k + 1 < P) x = or_zero(x);
+            return CARE != Care::none && k == 0 ? first_piece(x) : x;
+        };
 #pragma unroll
         for (int k = 0; k < P; ++k) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float lo = v[2 * i], hi = W == 1 ? 0.0f : v[W == 1 ? 0 : 2 * i + 1];
-                const uint32_t u = w[k][i] = ANY && k == 0 ? bf16_pair(first_piece(lo), first_piece(hi)) : bf16_pair(lo, hi);
+                const uint32_t u = w[k][i] = bf16_pair(piece_of(lo, k), piece_of(hi, k));
                 v[2 * i] = lo - __uint_as_float(u << 16);
                 if (W > 1) v[W == 1 ? 0 : 2 * i + 1] = hi - __uint_as_float(u & 0xFFFF0000u);
             }
@@ -235,14 +244,23 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs &a, int id, int rows, b
     return {-1, 0, 0};
 }
 
-// f16: a power of two that brings a row's largest value to between 2^14 and 2^15, within what f32 can divide by (infinities and NaN: 1).  So high that the least of a row keep their bits: two
-// pieces of f16 reach down to 2^-24, 38 octaves below, and are 16 bits and more of every value down to 2^-22 of the largest.  (Products with f16 weights of 2^16 leave f32 sums room.)
-__device__ __forceinline__ float unit_of(float most) {
-    const int e = static_cast<int>(__float_as_uint(most) >> 23);
-    return e == 255 ? 1.0f : __uint_as_float(static_cast<uint32_t>(max(e - 14, 1)) << 23);
+// f16: a power of two that brings a row's largest number to between 2^14 and 2^15, within what f32 can divide by.  So high that the least of a row keep their bits: two pieces of f16 reach
+// down to 2^-24, 38 octaves below, and are 16 bits and more of every value down to 2^-22 of the largest.  (Products with f16 weights of 2^16 leave f32 sums room.)
+__device__ __forceinline__ float unit_of(float most) { return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(__float_as_uint(most) >> 23) - 14, 1)) << 23); }
+// (infinities and NaN are not counted: beside them all numbers of a row would be zeros or infinities)
+__device__ __forceinline__ float most_of(float4 s) { return fmaxf(fmaxf(fabsf(or_zero(s.x)), fabsf(or_zero(s.y))), fmaxf(fabsf(or_zero(s.z)), fabsf(or_zero(s.w)))); }
+// Four ranks' sums from rank r on: zeros behind the last rank, where an infinity in x or dy has met the zeros of weights that do not exist
+__device__ __forceinline__ float4 ranks_of(float4 s, int r, int rank) {
+    if (r + 4 > rank) {
+        if (r >= rank) s.x = 0.0f;
+        if (r + 1 >= rank) s.y = 0.0f;
+        if (r + 2 >= rank) s.z = 0.0f;
+        s.w = 0.0f;
+    }
+    return s;
 }
 // Four neighbours as operand pieces.  f16: divided by `unit`, since it has five bits of exponent.
-template <int DT>
+template <int DT, Care CARE = Care::all>
 __device__ __forceinline__ void hold_pieces(float4 s, float unit, uint2 *piece) {
     constexpr int H = DT == MTC_F32 ? 3 : 2;
     float v[4] = {s.x, s.y, s.z, s.w};
@@ -263,7 +281,8 @@ __device__ __forceinline__ void hold_pieces(float4 s, float unit, uint2 *piece) 
                 const float2 f = __half22float2(h);
                 x = fabsf(x) < INFINITY ? x - f.x : 0.0f, y = fabsf(y) < INFINITY ? y - f.y : 0.0f;
             } else {
-                w[i] = p == 0 ? bf16_pair(first_piece(x), first_piece(y)) : bf16_pair(x, y);
+                if (CARE == Care::all && H == 3 && p + 1 < H) w[i] = p == 0 ? bf16_pair(first_piece(or_zero(x)), first_piece(or_zero(y))) : bf16_pair(or_zero(x), or_zero(y));
+                else w[i] = p == 0 ? bf16_pair(first_piece(x), first_piece(y)) : bf16_pair(x, y);
                 x -= __uint_as_float(w[i] << 16), y -= __uint_as_float(w[i] & 0xFFFF0000u);
             }
         }

@@ -42,6 +42,9 @@ __device__ __forceinline__ void prefetch_block(const void *from, size_t bytes, i
         prefetch(static_cast<const char *>(from) + i, min(piece, bytes - i));
 }
 
+using NoCare = std::integral_constant<Care, Care::none>;
+using AllCare = std::integral_constant<Care, Care::all>;
+
 // Whether all these sums are numbers
 template <int A, int B>
 __device__ __forceinline__ bool finite(const float (&large)[A][B][4], const float (&small)[A][B][4]) {
@@ -153,14 +156,14 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                     else to.base[m][h][i].load_any(a.base, at, there ? a.c_out - c : 0);
                 }
     };
-    auto load_weights = [&](auto any, V *to, int n0, int r, int i) {     // r: this lane's first rank; i (BACK): four ranks behind
-        constexpr bool ANY = decltype(any)::value;
+    auto load_weights = [&](auto care, V *to, int n0, int r, int i) {     // r: this lane's first rank; i (BACK): four ranks behind
+        constexpr Care CARE = decltype(care)::value;
         if constexpr (!BACK) {
             // column c of tile j is n0 + c / 2 * 8 + 2 j + c % 2, so that a lane's results are eight neighbours
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int n = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
-                to[j].template load<ANY>(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
+                to[j].template load<CARE>(a.up, (expert * a.c_out + n) * a.rank + r, n < a.c_out && r < a.rank);
             }
         } else {
             // column c of tile j is n0 + 8 c + j: a lane loads eight neighbours of four ranks' rows, its results are sixteen
@@ -168,15 +171,15 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
 #pragma unroll
             for (int s = 0; s < DEEP; ++s) {
                 const int rr = r + 4 * i + s;
-                if constexpr (VOUT) to[s].template load<ANY>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
-                else to[s].template load_any<ANY>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank ? a.c_out - c : 0);
+                if constexpr (VOUT) to[s].template load<CARE>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank && c < a.c_out);
+                else to[s].template load_any<CARE>(a.up, (expert * a.rank + rr) * a.c_out + c, rr < a.rank ? a.c_out - c : 0);
             }
         }
     };
     auto load_early = [&](Unit &to, int n0) {
         load_base(to, n0);
 #pragma unroll
-        for (int i = 0; i < (BACK ? PARTS : 1); ++i) load_weights(std::false_type(), to.w + i * DEEP, n0, t * WIDE, i);
+        for (int i = 0; i < (BACK ? PARTS : 1); ++i) load_weights(NoCare(), to.w + i * DEEP, n0, t * WIDE, i);
     };
     Unit steps[STEPS];
     auto load_steps = [&](int u) {               // steps u, u + kWarps ..
@@ -188,9 +191,9 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     for (int rb = 0; rb < rank_blocks; ++rb) {
         float acc[MT][NT][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? NT : 1][4] = {};      // f32: the products of small pieces, apart so that the large ones are cut off less often
-        auto sum_up = [&](auto any) {
-            constexpr bool ANY = decltype(any)::value;
-#pragma unroll (ANY ? 1 : MT == 1 && RB <= 16 && P == 1 ? 4 : 2)
+        auto sum_up = [&](auto care) {
+            constexpr Care CARE = decltype(care)::value;
+#pragma unroll (CARE != Care::none ? 1 : MT == 1 && RB <= 16 && P == 1 ? 4 : 2)
             for (int c = chunk0; c < chunk1; ++c) {
                 const int k = c * 32 + t * 8;
                 const bool in = k < a.c_in;
@@ -199,8 +202,8 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if constexpr (VIN) x[m][h].template load<ANY>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
-                        else x[m][h].template load_any<ANY>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, rows[m][h] >= 0 ? a.c_in - k : 0);
+                        if constexpr (VIN) x[m][h].template load<CARE>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, in && rows[m][h] >= 0);
+                        else x[m][h].template load_any<CARE>(a.in, static_cast<size_t>(rows[m][h]) * a.c_in + k, rows[m][h] >= 0 ? a.c_in - k : 0);
                     }
                 auto step = [&](int j, int p, int i, uint32_t b0, uint32_t b1) {      // tile j of ranks, piece p of the weights, half i of the 32 values
 #pragma unroll
@@ -216,8 +219,8 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                     for (int j = 0; j < NT; ++j) {
                         const int r = rb * RB + 8 * j + g;
                         Vals<DT, 8> w;
-                        if constexpr (VIN) w.template load<ANY>(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
-                        else w.template load_any<ANY>(a.down, (expert * a.rank + r) * a.c_in + k, r < a.rank ? a.c_in - k : 0);
+                        if constexpr (VIN) w.template load<CARE>(a.down, (expert * a.rank + r) * a.c_in + k, in && r < a.rank);
+                        else w.template load_any<CARE>(a.down, (expert * a.rank + r) * a.c_in + k, r < a.rank ? a.c_in - k : 0);
 #pragma unroll
                         for (int p = 0; p < P; ++p)
 #pragma unroll
@@ -230,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                     for (int i = 0; i < 2; ++i) {
                         V w[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) w[q].template load<ANY>(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VIN ? in : k + 4 * i + q < a.c_in) && r < a.rank);
+                        for (int q = 0; q < 4; ++q) w[q].template load<CARE>(a.down, (expert * a.c_in + k + 4 * i + q) * a.rank + r, (VIN ? in : k + 4 * i + q < a.c_in) && r < a.rank);
 #pragma unroll
                         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -239,11 +242,11 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                 }
             }
         };
-        sum_up(std::false_type());
+        sum_up(NoCare());
         if constexpr (P > 1) {                   // a sum that is no number, or values that 16 bits do not reach: once more, with more care
             if (__any_sync(0xffffffffu, !finite(acc, fine))) {
                 clear(acc), clear(fine);
-                sum_up(std::true_type());
+                sum_up(AllCare());
             }
         }
         if constexpr (EARLY) {
@@ -302,11 +305,12 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                         if (at + 3 < a.rank) p[3] = s.w;
                     }
                 }
+                s = ranks_of(s, rb * RB + col, a.rank);
             }
             if constexpr (ONE) {
                 float f = 1.0f;
                 if constexpr (HALF) {            // RB / 4 lanes have a row
-                    float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
+                    float most = most_of(s);
 #pragma unroll
                     for (int o = RB / 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     f = unit_of(most);
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
             float f = 1.0f;
             if constexpr (HALF) {
                 float most = 0.0f;
-                for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(low[row * RT + i]));
+                for (int i = lane; i < RT; i += 32) most = fmaxf(most, fabsf(or_zero(low[row * RT + i])));
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 f = unit_of(most);
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
         if constexpr (!EARLY) load_base(unit, n0);
         float acc[MT][TN][4] = {};
         float fine[P > 1 ? MT : 1][P > 1 ? TN : 1][4] = {};
-        auto sum_up = [&](auto any) {
+        auto sum_up = [&](auto care) {
             for (int rb = 0; rb < rank_blocks; ++rb) {
 #pragma unroll
                 for (int q = 0; q < QS; ++q) {
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                             }
                     };
                     if constexpr (!BACK) {
-                        if constexpr (!EARLY) load_weights(any, unit.w, n0, r, 0);
+                        if constexpr (!EARLY) load_weights(care, unit.w, n0, r, 0);
 #pragma unroll
                         for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
 #pragma unroll
                         for (int i = 0; i < PARTS; ++i) {
                             V *const w = unit.w + (EARLY ? i * DEEP : 0);
-                            if constexpr (!EARLY) load_weights(any, w, n0, r, i);
+                            if constexpr (!EARLY) load_weights(care, w, n0, r, i);
 #pragma unroll
                             for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -397,11 +401,11 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
                 }
             }
         };
-        sum_up(std::false_type());
+        sum_up(NoCare());
         if constexpr (P > 1) {
             if (__any_sync(0xffffffffu, !finite(acc, fine))) {
                 clear(acc), clear(fine);
-                sum_up(std::true_type());
+                sum_up(AllCare());
             }
         }
 #pragma unroll

@@ -353,9 +353,10 @@ __global__ void __launch_bounds__(kThreads, 2) lora_tile_kernel(const LoraArgs a
             for (int q = 0; q < kCluster; ++q) s.x += v[q].x, s.y += v[q].y, s.z += v[q].z, s.w += v[q].w;
             const int to = ctl->row_of[r];
             if (keep && to >= 0 && u * 4 < a.rank) *reinterpret_cast<float4 *>(a.low + static_cast<size_t>(to) * a.rank + u * 4) = s;
+            s = ranks_of(s, u * 4, a.rank);
             float f = 1.0f;
             if constexpr (DT == MTC_F16) {
-                float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
+                float most = most_of(s);
 #pragma unroll
                 for (int o = SUMS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o, SUMS));
                 f = unit_of(most);

@@ -253,7 +253,7 @@ def lora_mm(x, a, b, rows, offsets, scales=None, base=None, out=None, hidden: bo
 
     ``rows`` and ``offsets`` group the rows by adapter, once for all projections of a step: with ``ids`` int32 ``[n_rows]``, L for rows that have none,
     ``rows, _, offsets, _ = moe_sort(ids[:, None], L + 1)``.  ``hidden=True`` returns (out, h) with h = x a^T float32 ``[n_rows, rank]`` (zeros for rows without an
-    adapter), which ``lora_grad`` wants."""
+    adapter), which ``lora_grad`` wants.  Infinities in x and base are the formula's; those in a or b give infinities or NaN."""
     return _native.lora_mm(x, a, b, rows, offsets, scales, base, out, hidden, ctx)
 
 
