@@ -95,7 +95,7 @@ cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward
         // 4096 30.2 and 26.4 (narrow layers have no time to win: 1024 x 1024, 4096 rows 9.6 and 13.1), rank 64, 1024 rows 18.6 and 20.0, 2048 30.4 and 27.8.  Back, with
         // the weights' gradient: rank 16, 512 rows 23.6 and 25.5, 1536 36.4 and 30.8, 4096 79.5 and 65.4; rank 32, 512 26.0 and 27.6, 768 33.5 and 28.9; rank 64, 512 40.9 and 36.4.
         // Adapters whose rows do not fill a good part of a tile stay with the other one: 1024 rows of 32 adapters, rank 32, 14.0 and 21.
-        const bool narrow = a.c_in + a.c_out <= 2048;
+        const bool narrow = lora_width(a) <= 2048;
         const int least = backward ? (a.rank <= 16 ? 1152 : a.rank <= 32 ? 768 : 512) : a.rank > 32 ? 1152 : narrow ? 0x7FFFFFFF : 2304;
         if (form == LoraForm::pieces && lora_tile_supported(a, keep, dt) && a.n_rows >= least && a.n_rows >= 48ll * a.n_adapters) return launch_lora_tile(st, a, backward, keep, none, dt);
         return (dt == MTC_F32 ? launch_lora_mma<MTC_F32> : dt == MTC_BF16 ? launch_lora_mma<MTC_BF16> : launch_lora_mma<MTC_F16>)(st, a, backward, keep, none);

@@ -43,6 +43,8 @@ inline bool lora_on_16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 
 // Rows on a side that can be loaded 16 bytes at a time: x and, forward, a; base and out and, back, a
 inline bool lora_pieces_in(const LoraArgs &a) { return a.c_in % 8 == 0 && lora_on_16(a.in) && lora_on_16(a.down); }
 inline bool lora_pieces_out(const LoraArgs &a) { return a.c_out % 8 == 0 && lora_on_16(a.up) && lora_on_16(a.out) && (!a.base || lora_on_16(a.base)); }
+// What a row has on both sides (each may be near 2^31)
+inline long long lora_width(const LoraArgs &a) { return static_cast<long long>(a.c_in) + a.c_out; }
 
 // Warp-level tensor cores (lora_rows.cuh, a file a type); `none`: rows of no adapter have something to be written
 template <int DT>

@@ -452,7 +452,7 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     // rows of f32 281, 125, 104.
     constexpr int ROOM = DT == MTC_F32 && RB > 16 ? 1 : 2;                       // CTAs an SM
     const long long about = a.n_rows / ROWS + std::min(a.n_adapters, a.n_rows) / 2;
-    const int cluster_log = about <= 16 * ROOM - (ROOM == 1) && a.c_in + a.c_out > 2048 ? 3 : about <= 36 * ROOM ? 2 : 1;
+    const int cluster_log = about <= 16 * ROOM - (ROOM == 1) && lora_width(a) > 2048 ? 3 : about <= 36 * ROOM ? 2 : 1;
     if ((tiles << cluster_log) > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
     return launch_cluster(lora_mma_kernel<DT, RB, MT, BACK, ONE, VIN, VOUT>, static_cast<unsigned>(tiles << cluster_log), kThreads, 1 << cluster_log, smem, st, a, cluster_log, blocks, keep, none);
 }
@@ -492,7 +492,7 @@ cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, b
     // Tiles of 32 rows where those of 16 leave clusters too small or make a second wave (launch), and the registers of the form allow it.  us of 16 and 32 rows, 4096 x 4096: bf16 rank 16,
     // 1024 rows 10.4 and 13.5, 2048 18.4 and 16.6; f32 rank 32, 192 rows 14.0 and 18.1, 256 21.4 and 18.2, 384 21.6 and 18.4, 512 23.4 and 30.5, 640 46.6 and 33.8, 2048 94 and 69
     // (1024 x 1024: 384 rows 9.4 and 11.8, 640 13.3 and 12.1); f32 rank 16, 4096 rows 103 and 132
-    const bool between = a.n_rows > 240 && a.n_rows <= 480 && a.c_in + a.c_out > 2048;
+    const bool between = a.n_rows > 240 && a.n_rows <= 480 && lora_width(a) > 2048;
     const bool wide = DT != MTC_F32 ? a.n_rows > 1152 : a.rank > 16 && (a.n_rows > 576 || between);
     if (wide) return backward ? launch_side<DT, 2, true>(st, a, keep, none) : launch_side<DT, 2, false>(st, a, keep, none);
     return backward ? launch_side<DT, 1, true>(st, a, keep, none) : launch_side<DT, 1, false>(st, a, keep, none);
