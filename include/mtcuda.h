@@ -453,7 +453,7 @@ int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const v
  * row inside its projection: mtc_rms_norm_qmv) ----
  *     s = T(x + residual),   inv = 1 / sqrt(mean(s^2) + eps),   y = T(s * inv * norm_weight)          (f32 in between; rows of K values)
  * x, residual, sum, y T[n_rows, K], norm_weight T[K].  residual NULL: s is x, `sum` is not looked at.  The norm is of what `sum` holds.  sum and y may be x or residual
- * (but not both the same), so that a residual stream is updated in place.
+ * (but not both the same), so that a residual stream is updated in place.  Results of these three entries that lie over an operand in another way, or over each other, are refused.
  * mtc_add_rms_norm_fp8 gives y as e4m3 codes u8[n_rows, K] with scales f32[n_rows, B(K)], made of the f32 results as mtc_fp8_quantize makes them of f32 rows (pow2 as there), which
  * mtc_fp8_mm reads; y (NULL: not wanted) gets them in T as well. */
 int mtc_add_rms_norm(mtc_ctx *ctx, void *stream, const void *x, const void *residual, const void *norm_weight, float eps, void *sum, void *y, int n_rows, int K, int dtype);
@@ -468,7 +468,7 @@ size_t mtc_add_rms_norm_grad_workspace(const mtc_ctx *ctx, int n_rows, int K, in
 
 /* ---- beside a projection: low-rank adapters of many requests (no counterpart in the reference) ----
  * For the rows t of adapter e:   h_t = x_t a[e]^T,   out_t = base_t + scales[e] * h_t b[e]^T           (sums f32, rounded once)
- * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; base may be out, no other operand may.
+ * x T[n_rows, K], a T[n_adapters, rank, K], b T[n_adapters, N, rank], scales f32[n_adapters] (NULL: 1), base (NULL: 0) and out T[n_rows, N]; out may be base, whole.  Results that lie over another operand, or over each other, are refused.
  * rows u32[n_rows] holds the row numbers, each once, those of one adapter side by side, offsets u32[n_adapters + 1] where each adapter's begin: place p belongs to e where
  * offsets[e] <= p < offsets[e + 1].  The rows of the other places have no adapter: they get base (0), and stay as they are where base is out.  mtc_moe_sort of the rows'
  * adapters (k = 1, one more "expert" for the rows that have none) writes both.  hidden f32[n_rows, rank] (NULL: not wanted) gets h, zeros for rows without an adapter.

@@ -1646,6 +1646,22 @@ int mtc_moe_balance_grad(mtc_ctx *ctx, void *stream, const void *logits, const v
 }
 
 // ---- norms and low-rank adapters ---------------------------------------------------------------------------
+struct Span {                                    // memory of an operand; none where it is not given
+    uintptr_t from, to;
+    Span(const void *p, long long n, long long m, size_t size)
+        : from(reinterpret_cast<uintptr_t>(p)), to(p ? from + static_cast<size_t>(std::min<double>(static_cast<double>(n) * m * size, 0x1p60)) : from) {}
+    bool meets(const Span &o) const { return from < o.to && o.from < to; }
+    bool is(const Span &o) const { return from == o.from && to == o.to; }
+};
+// A result may lie in an operand of `in_place`, value for value; not over others, nor over the other results
+static bool apart(const Span &result, std::initializer_list<Span> in_place, std::initializer_list<Span> others) {
+    for (const Span &s : in_place)
+        if (result.meets(s) && !result.is(s)) return false;
+    for (const Span &s : others)
+        if (result.meets(s)) return false;
+    return true;
+}
+static size_t value_size(int dtype) { return dtype == MTC_F32 ? 4 : 2; }
 static int norm_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int K, int dtype) {
     if (!dtype_ok(dtype)) return fail(ctx, MTC_ERR_UNSUPPORTED, std::string(who) + ": dtype must be f32, f16 or bf16");
     if (n_rows < 0 || K <= 0 || K > mtc::kMostNorm) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": need n_rows >= 0 and 0 < K <= 2^30");
@@ -1658,7 +1674,11 @@ static int add_rms_norm(mtc_ctx *ctx, const char *who, void *stream, const void 
         const int rc = norm_args_ok(ctx, who, n_rows, K, dtype);
         if (rc != MTC_OK || n_rows == 0) return rc;
         if (!x || !norm_weight || (residual && !sum) || (mode == 0 ? !y : !codes || !scales)) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": null pointer");
-        if (residual && sum == y) return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": sum and y are the same memory");
+        const size_t size = value_size(dtype);
+        const Span in(x, n_rows, K, size), stream_(residual, n_rows, K, size), w(norm_weight, 1, K, size), s(residual ? sum : nullptr, n_rows, K, size), out(y, n_rows, K, size),
+            c(codes, n_rows, K, 1), cs(scales, n_rows, (K + 127ll) / 128, 4);
+        if (!apart(s, {in, stream_}, {w, out, c, cs}) || !apart(out, {in, stream_}, {w, c, cs}) || !apart(c, {}, {in, stream_, w, cs}) || !apart(cs, {}, {in, stream_, w}))
+            return fail(ctx, MTC_ERR_INVALID, std::string(who) + ": sum and y may each be x or residual, whole; results lie over no other operand, nor over each other");
         mtc::NormArgs a{};
         a.x = x, a.residual = residual, a.weight = norm_weight, a.sum = sum, a.y = y;
         a.codes = static_cast<uint8_t *>(codes), a.scales = static_cast<float *>(scales);
@@ -1690,6 +1710,10 @@ int mtc_add_rms_norm_grad(mtc_ctx *ctx, void *stream, const void *dy, const void
         if (!dweight || (n_rows > 0 && (!dy || !sum || !norm_weight || !dx))) return fail(ctx, MTC_ERR_INVALID, "add_rms_norm_grad: null pointer");
         rc = check_workspace(ctx, "add_rms_norm_grad", workspace, workspace_bytes, mtc_add_rms_norm_grad_workspace(ctx, n_rows, K, dtype));
         if (rc != MTC_OK) return rc;
+        const size_t size = value_size(dtype);
+        const Span g(dy, n_rows, K, size), s(sum, n_rows, K, size), d(dsum, n_rows, K, size), w(norm_weight, 1, K, size), out(dx, n_rows, K, size), dw(dweight, 1, K, size);
+        if (!apart(out, {g, s, d}, {w, dw}) || (n_rows > 0 && !apart(dw, {}, {g, s, d, w})))
+            return fail(ctx, MTC_ERR_INVALID, "add_rms_norm_grad: dx may be dy or dsum, whole; results lie over no other operand, nor over each other");
         mtc::NormGradArgs a{};
         a.dy = dy, a.s = sum, a.weight = norm_weight, a.dsum = dsum, a.dx = dx;
         a.n_rows = n_rows, a.K = K, a.eps = eps;
@@ -1709,6 +1733,14 @@ static int lora_args_ok(mtc_ctx *ctx, const char *who, int n_rows, int K, int N,
     return MTC_OK;
 }
 
+struct LoraSpans {
+    Span x, a, b, rows, offsets, scales, hidden;
+    LoraSpans(const void *x_, const void *a_, const void *b_, const void *rows_, const void *offsets_, const void *scales_, const void *hidden_, long long n_rows, long long K, long long N,
+              long long rank, long long n_adapters, int dtype)
+        : x(x_, n_rows, K, value_size(dtype)), a(a_, n_adapters * rank, K, value_size(dtype)), b(b_, n_adapters * rank, N, value_size(dtype)), rows(rows_, n_rows, 1, 4),
+          offsets(offsets_, n_adapters + 1, 1, 4), scales(scales_, n_adapters, 1, 4), hidden(hidden_, n_rows, rank, 4) {}
+};
+
 size_t mtc_lora_grad_workspace(const mtc_ctx *, int n_rows, int K, int N, int rank, int n_adapters, int dtype) {
     return lora_sizes_ok(n_rows, K, N, rank, n_adapters) && dtype_ok(dtype) ? static_cast<size_t>(n_rows) * rank * 4 : 0;     // u
 }
@@ -1720,7 +1752,10 @@ int mtc_lora_mm(mtc_ctx *ctx, void *stream, const void *x, const void *a, const 
         const int rc = lora_args_ok(ctx, "lora_mm", n_rows, K, N, rank, n_adapters, dtype);
         if (rc != MTC_OK || n_rows == 0) return rc;
         if (!x || !a || !b || !rows || !offsets || !out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: null pointer");
-        if (out == x || out == a || out == b || hidden == out) return fail(ctx, MTC_ERR_INVALID, "lora_mm: out may be base, no other operand");
+        const LoraSpans o(x, a, b, rows, offsets, scales, hidden, n_rows, K, N, rank, n_adapters, dtype);
+        const Span y(out, n_rows, N, value_size(dtype)), to(base, n_rows, N, value_size(dtype));
+        if (!apart(y, {to}, {o.x, o.a, o.b, o.rows, o.offsets, o.scales, o.hidden}) || !apart(o.hidden, {}, {o.x, o.a, o.b, o.rows, o.offsets, o.scales, to}))
+            return fail(ctx, MTC_ERR_INVALID, "lora_mm: out may be base, whole; results lie over no other operand, nor over each other");
         mtc::LoraArgs l{};
         l.in = x, l.down = a, l.up = b, l.base = base, l.out = out;
         l.order = static_cast<const uint32_t *>(rows), l.offsets = static_cast<const uint32_t *>(offsets), l.scales = static_cast<const float *>(scales);
@@ -1739,7 +1774,12 @@ int mtc_lora_grad(mtc_ctx *ctx, void *stream, const void *dy, const void *x, con
         int rc = lora_args_ok(ctx, "lora_grad", n_rows, K, N, rank, n_adapters, dtype);
         if (rc != MTC_OK) return rc;
         if (!offsets || !da || !db || (n_rows > 0 && (!dy || !x || !a || !b || !rows || !hidden || !dx))) return fail(ctx, MTC_ERR_INVALID, "lora_grad: null pointer");
-        if (n_rows > 0 && (dx == dy || dx == x || dx == a || dx == b || dx == hidden)) return fail(ctx, MTC_ERR_INVALID, "lora_grad: dx may be base, no other operand");
+        const LoraSpans o(x, a, b, rows, offsets, scales, hidden, n_rows, K, N, rank, n_adapters, dtype);
+        const size_t size = value_size(dtype), weights = static_cast<size_t>(n_adapters) * rank;
+        const Span g(dy, n_rows, N, size), out(dx, n_rows, K, size), to(base, n_rows, K, size), ga(da, weights, K, size), gb(db, weights, N, size);
+        if (n_rows > 0 && (!apart(out, {to}, {g, o.x, o.a, o.b, o.rows, o.offsets, o.scales, o.hidden, ga, gb}) || !apart(ga, {}, {g, o.x, o.a, o.b, o.rows, o.offsets, o.scales, o.hidden, to, gb}) ||
+                           !apart(gb, {}, {g, o.x, o.a, o.b, o.rows, o.offsets, o.scales, o.hidden, to})))
+            return fail(ctx, MTC_ERR_INVALID, "lora_grad: dx may be base, whole; results lie over no other operand, nor over each other");
         rc = check_workspace(ctx, "lora_grad", workspace, workspace_bytes, mtc_lora_grad_workspace(ctx, n_rows, K, N, rank, n_adapters, dtype));
         if (rc != MTC_OK) return rc;
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
