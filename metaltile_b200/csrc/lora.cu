@@ -1,5 +1,7 @@
-// Low-rank adapters: which kernel runs, and the products of any rank and alignment on CUDA cores, for what the others do not take (ranks that are no multiple of 2, 4 or 8,
-// or more than 256).  No counterpart in the reference; this stands next to its projections
+// Low-rank adapters: which kernel runs, and the products of any rank and alignment on CUDA cores, for what the others do not take: ranks above 256, above 16 and no multiple of 8, above 8 and
+// no multiple of 4, odd, 2 and 6 beside rows of no whole pieces, and weights along the rank that do not start at 16 bytes.  A CTA has one row and reads its whole adapter: far from what the
+// others do where rows are many (us, bf16, 4096 x 4096: 64 rows of rank 20 41 where rank 24 takes 7, 4096 rows 335 and
+// back 393 where rank 24 takes 29 and 82, 2048 rows of rank 512 17,700 where rank 256 takes 139).  No counterpart in the reference; this stands next to its projections
 // (crates/metaltile-std/src/mlx/quantized.rs:5040-5065), whose quantized weights stay as they are while adapters are trained or swapped.
 #include <algorithm>
 
@@ -91,12 +93,20 @@ cudaError_t launch_lora(Ctx *, cudaStream_t st, const LoraArgs &a, bool backward
     const LoraForm form = lora_mma_form(a, backward);
     const bool none = (keep && all) || a.base != a.out;
     if (form != LoraForm::none) {
-        // Tiles of 128 rows on tcgen05 where they are many (us of the warp-level and the tcgen05 kernel, bf16, 4096 x 4096).  Forward: rank 16, 2048 rows 16.6 and 21.1, 2560 24.0 and 22.1,
-        // 4096 30.2 and 26.4 (narrow layers have no time to win: 1024 x 1024, 4096 rows 9.6 and 13.1), rank 64, 1024 rows 18.6 and 20.0, 2048 30.4 and 27.8.  Back, with
-        // the weights' gradient: rank 16, 512 rows 23.6 and 25.5, 1536 36.4 and 30.8, 4096 79.5 and 65.4; rank 32, 512 26.0 and 27.6, 768 33.5 and 28.9; rank 64, 512 40.9 and 36.4.
-        // Adapters whose rows do not fill a good part of a tile stay with the other one: 1024 rows of 32 adapters, rank 32, 14.0 and 21.
+        // Tiles of 128 rows on tcgen05 where they are many.  us of the warp-level and the tcgen05 kernel, bf16, rows of one adapter, three sets of inputs in turn:
+        //   forward, 4096 + 4096   rank 16: 2200 rows 18.6 and 23.1, 2304 26.9 and 23.2, 4096 30.5 and 27.4; rank 32: 2200 21.2 and 25.1, 2304 31.1 and 25.2; rank 64: 1100 19.2 and 21.3,
+        //                          1152 28.2 and 21.2, 2048 32.8 and 29.2
+        //            2048 + 2048   rank 16: 2304 15.2 and 15.4, 4096 17.9 and 18.5; rank 32: 2304 19.1 and 17.2; rank 64: 1100 12.4 and 14.4, 1152 18.3 and 14.4, 4096 31.7 and 22.8
+        //            1024 + 1024   rank 16: 4096 10.3 and 13.8; rank 32: 4096 11.5 and 14.6 (`narrow`); rank 64: 1152 13.7 and 11.0, 2048 13.7 and 14.8, 4096 19.3 and 17.2
+        //   back, with the weights' gradient
+        //            4096 + 4096   rank 16: 1024 31.6 and 29.0, 1160 40.8 and 30.8, 4096 78.4 and 68.2; rank 32: 768 25.8 and 28.8, 1024 38.9 and 39.9, 1150 48.2 and 42.6; rank 64: 448 35.7 and
+        //                          37.3, 512 35.0 and 34.3, 1024 61.7 and 54.5
+        //            2048 + 2048   rank 16: 1024 20.4 and 23.4, 1160 24.6 and 25.3, 4096 45.4 and 40.6; rank 32: 768 20.6 and 22.6, 1024 24.1 and 23.9; rank 64: 512 29.3 and 27.4
+        //            1024 + 1024   rank 16: 1160 21.3 and 21.3, 4096 35.1 and 33.4; rank 32: 768 18.5 and 17.2, 1024 18.6 and 20.6, 1150 23.9 and 21.9; rank 64: 448 26.7 and 23.3, 512 24.6 and 20.6
+        // (The warp-level kernel's steps at 1152 and 2304 rows are those of its tiles of 16 and 32 rows.)  Adapters whose rows do not fill a good part of a tile stay with it: 1024 rows of 32
+        // adapters, rank 32, forward 21.3 and 23.7.  The number of rows and of adapters is all that the host knows: adapters that have no rows count as if they had their share.
         const bool narrow = lora_width(a) <= 2048;
-        const int least = backward ? (a.rank <= 16 ? 1152 : a.rank <= 32 ? 768 : 512) : a.rank > 32 ? 1152 : narrow ? 0x7FFFFFFF : 2304;
+        const int least = backward ? (a.rank <= 16 ? 1152 : a.rank <= 32 ? 1024 : 512) : a.rank > 32 ? 1152 : narrow ? 0x7FFFFFFF : 2304;
         if (form == LoraForm::pieces && lora_tile_supported(a, keep, dt) && a.n_rows >= least && a.n_rows >= 48ll * a.n_adapters) return launch_lora_tile(st, a, backward, keep, none, dt);
         return (dt == MTC_F32 ? launch_lora_mma<MTC_F32> : dt == MTC_BF16 ? launch_lora_mma<MTC_BF16> : launch_lora_mma<MTC_F16>)(st, a, backward, keep, none);
     }
