@@ -8,7 +8,7 @@
 // taken: that of the small ones is up to 2^-14 of the whole, of one sign where the operands are (left out, it cost one result in 25 its last bit
 // there); it costs a training step 3 to 6 % (2048 x 4096 -> 4096, rank 64, 108.5 -> 114.4 us).
 //
-// Measured: 4096 rows of 4096 + 4096, rank 16, bf16 31 us, 2.2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 2048 + 768 in f32, rank 8, 10.  Bound by what a CTA cannot overlap, in
+// Measured: 4096 rows of 4096 + 4096, rank 16, bf16 some 33 us behind dx's kernel, 2 TB/s of x and dy (the bytes need 10.3 us); 512 rows of 2048 + 768 in f32, rank 8, 10.  Bound by what a CTA cannot overlap, in
 // two waves of CTAs: of 25,000 cycles the start and the first stage take 8,000, the sums over the cluster 5,000.  A bulk copy a row and mbarriers take half the instructions and
 // were no faster (34.9 us).
 #include <algorithm>

@@ -4,10 +4,14 @@
 // shared memory, then over distributed shared memory, so that every CTA has the whole h of the tile; then each CTA takes a part of the
 // columns of the second product.  x, base and out pass once, a tile's adapter is read by its cluster once, h never leaves the SM.
 //
-// Bound by latency where users decode: 64 rows of 32 adapters, 4096 -> 14336, rank 16, bf16 take 10.4 us where the bytes need 3; a row alone, 4096 -> 4096, takes 5.1.  Of that the launch is 2, and
+// Bound by latency where users decode: 64 rows of 32 adapters, 4096 -> 14336, rank 16, bf16 take 10.3 us where the bytes need 3; a row alone, 4096 -> 4096, takes 5.5.  Of that the launch is 2, and
 // the chain is loads of x and A, the sums over the cluster (two barriers of it), loads of B and base, stores.  So everything that a CTA will read is asked for before
 // it waits (prefetches into L2, and base and B into registers where they fit), and a tile is spread over up to 64 warps.  128-row tiles of tcgen05 would be empty for the most part there;
-// with a thousand rows and more the shared reading of the adapter and one thread that issues the MMAs win (lora.cu has both sides).
+// from some hundreds of rows (back, rank 64) to 2304 (forward, ranks to 32) on the shared reading of the adapter and one thread that issues the MMAs win (lora.cu has both sides).
+//
+// Registers: two CTAs an SM leave 128 a thread, and with tiles of 32 rows, ranks 33 to 64 or f32 the second product keeps base, the weights of four ranks and its sums at once.  Back, these forms
+// spill: 900 bytes at rank 64 and 32 rows (1550 where a side has no whole pieces), 220 at rank 64 and 16 rows, 330 at rank 32 and 32 rows, 570 to 750 of f32 at rank 32 and 32 rows.  They are what
+// 200 rows of rank 64 take (back 27 us) and 2048 rows of 64 adapters (199).
 #pragma once
 
 #include <algorithm>
@@ -87,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, DT == MTC_F32 && RB > 16 ? 1 : 2) lo
     if (blockIdx.x == 0)
         for (int e = threadIdx.x; e < a.n_adapters; e += kThreads)
             if (a.offsets[e] > a.offsets[e + 1] || a.offsets[e + 1] > static_cast<uint32_t>(a.n_rows)) atomicCAS(a.status, 0u, 0x901u);
-    const int cs = 1 << cluster_log;              // (shifts: 64-bit divisions made 6.1 us of the 5.1 of a single row)
+    const int cs = 1 << cluster_log;              // (shifts: with 64-bit divisions a single row took 6.1 us in place of 5.1)
     const Tile tile = find_tile(a, blockIdx.x >> cluster_log, ROWS, none);
     if (tile.e < 0) return;                      // the whole cluster
     if (threadIdx.x < ROWS) {
@@ -447,9 +451,9 @@ cudaError_t launch(cudaStream_t st, const LoraArgs &a, bool keep, bool none) {
     if (e != cudaSuccess) return e;
     const long long tiles = most_tiles(a, ROWS);
     // The largest cluster of which all tiles' fit at once: with more CTAs a tile, each does less of the long axes, and a second wave costs as much as the first.  (Of eight CTAs 15 fit, of four
-    // 36, and about twice that at two CTAs an SM; tiles are counted as if adapters ended at half a tile.)  us of clusters of 8, 4 and 2, f32, 4096 x 4096: rank 16, 256 rows 13.2, 17.7, 27.5,
-    // 1024 29.6, 24.7, 38.8, 4096 106, 93, 92; rank 64, 1024 137, 100, 96.  Narrow layers have too little for eight: 1024 x 1024, rank 64, 64 rows 15.6, 15.2, 22.7, bf16 8.2, 7.3, 8.6; 4096
-    // rows of f32 281, 125, 104.
+    // 36, and about twice that at two CTAs an SM; tiles are counted as if adapters ended at half a tile.)  us of clusters of 8, 4 and 2, f32, 4096 x 4096: rank 16, 256 rows 13.1, 16.5, 27.9,
+    // 1024 35.8, 26.1, 39.1, 4096 112, 90, 89; rank 64, 1024 123, 93, 97.  Narrow layers have too little for eight: 1024 x 1024, rank 64, 64 rows 14.4, 14.4, 22.6, bf16 7.0, 6.9, 8.3; 4096
+    // rows of f32 253, 116, 96.
     constexpr int ROOM = DT == MTC_F32 && RB > 16 ? 1 : 2;                       // CTAs an SM
     const long long about = a.n_rows / ROWS + std::min(a.n_adapters, a.n_rows) / 2;
     const int cluster_log = about <= 16 * ROOM - (ROOM == 1) && lora_width(a) > 2048 ? 3 : about <= 36 * ROOM ? 2 : 1;
@@ -490,8 +494,8 @@ cudaError_t launch_side(cudaStream_t st, const LoraArgs &a, bool keep, bool none
 template <int DT>
 cudaError_t launch_lora_mma(cudaStream_t st, const LoraArgs &a, bool backward, bool keep, bool none) {
     // Tiles of 32 rows where those of 16 leave clusters too small or make a second wave (launch), and the registers of the form allow it.  us of 16 and 32 rows, 4096 x 4096: bf16 rank 16,
-    // 1024 rows 10.4 and 13.5, 2048 18.4 and 16.6; f32 rank 32, 192 rows 14.0 and 18.1, 256 21.4 and 18.2, 384 21.6 and 18.4, 512 23.4 and 30.5, 640 46.6 and 33.8, 2048 94 and 69
-    // (1024 x 1024: 384 rows 9.4 and 11.8, 640 13.3 and 12.1); f32 rank 16, 4096 rows 103 and 132
+    // 1024 rows 10.5 and 11.6, 2048 18.8 and 18.4; f32 rank 32, 192 rows 14.0 and 19.2, 256 22.0 and 19.2, 384 23.8 and 19.9, 512 26.0 and 34.0, 640 48.2 and 35.5, 2048 94 and 70
+    // (1024 x 1024: 384 rows 9.0 and 12.4, 640 13.7 and 12.4); f32 rank 16, 1024 rows 26 and 35, 4096 89 and 129
     const bool between = a.n_rows > 240 && a.n_rows <= 480 && lora_width(a) > 2048;
     const bool wide = DT != MTC_F32 ? a.n_rows > 1152 : a.rank > 16 && (a.n_rows > 576 || between);
     if (wide) return backward ? launch_side<DT, 2, true>(st, a, keep, none) : launch_side<DT, 2, false>(st, a, keep, none);

@@ -9,9 +9,12 @@
 // over the row and the results.  Sums are f32 within a row and within the rows that a CTA adds up for dw, f64 over the CTAs, always in the same
 // order.  The codes are made from the f32 results: the rounding to T between a norm and a quantizer of its own does not happen here.  Against results in 64 bits some 1.5 codes of
 // 10000 are the neighbour: quotients of few bits lie on the borders between codes, and the f32 rounding of y or of the scale decides on which side.
-// Measured (graph, us): y, 1 x 4096 bf16 1.7, 2048 x 4096 9.4 (67 MB, 7.1 TB/s with part of it in L2), 8192 x 4096 41; codes, 8192 x 4096 42.8 (236 MB, 5.5 TB/s;
+// Measured (graph, three sets of inputs in turn, us): y, 1 x 4096 bf16 2.1, 2048 x 4096 12.8 (67 MB, 5.2 TB/s), 8192 x 4096 42; codes, 8192 x 4096 43.6 (236 MB, 5.4 TB/s;
 // bound by instructions, 69 % of the issue slots: 18 a value and some 250 a thread and row); gradients, 8192 x 4096 with dsum 50 (268 MB, 5.4 TB/s; of it the join of 296 shares
-// about 3), 333 x 2880 f32 7.6.
+// about 3), 333 x 2880 f32 8.3.
+// Less near to the memory: gradients of 8193 to 16,384 values, whose four turns of sums do not fit the registers (220 bytes of a thread are spilled, 430 in f32): 4096 x 14336 bf16 115 us where the
+// bytes need 54; rows of no whole 16-byte pieces, values one by one and read twice, by the gradient three times: 2048 x 4095 bf16 y 55, codes 48, gradients 50 (of 4096 values 13, 16, 16); rows past
+// 16,384 values, read twice: 2048 x 20000 bf16 82, 110, 249 (the bytes need 50, 44, 37).
 #include <algorithm>
 
 #include "norm.cuh"
@@ -345,7 +348,7 @@ struct GradShape {
     int turns, threads, block, workers;          // threads of a row, of a CTA
 };
 // Two turns of 16-bit values a thread, 512 threads an SM (their registers hold a row and the next one: 8192 x 4096 bf16 54 us, in one turn of 512 threads 64; 4096 x 8192 56);
-// one turn where rows are few or f32 (333 x 2880 bf16 7.6 and 10.0, f32 8.6 and 10.7, since there are fewer shares to add up).  Rows past 8192 take four turns.
+// one turn where rows are few or f32 (333 x 2880 bf16 7.6 and 10.0, f32 8.3 and 10.7, since there are fewer shares to add up).  Rows past 8192 take four turns.
 GradShape grad_shape(int sms, long long n_rows, int K, int dt) {
     const int eights = static_cast<int>((static_cast<long long>(K) + 7) / 8);
     GradShape g{};
