@@ -5,7 +5,7 @@
 // cut off leave rests of twice the size and of one sign: 2^-21.)  bf16 and f16 weights and activations are operands as they are.
 //
 // What lies between the two products, h or u, is an f32 sum.  Beside f32 weights it is an operand in three pieces, 24 bits.  Beside 16-bit weights it is held in two, which costs two MMAs a
-// step of ranks: 17 bits of bf16 (2^-17 of each value; the result, rounded to 8 bits, is off by 2^-9), 16 and more of f16 (below).  What is kept for the backward pass is the f32 sum.
+// step of ranks: 17 bits of bf16 (2^-17 of each value; the result, rounded to 8 bits, is off by up to 2^-8), 16 and more of f16 (below).  What is kept for the backward pass is the f32 sum.
 //
 // Order of k.  A sum may run over k in any order as long as both operands have the same, so a lane takes what lies next to each other in memory: of
 // 32 neighbours lane (g, t) = (lane / 4, lane % 4) has 8t .. 8t + 7, the first four of them in the first of two MMAs.  Where the other operand lies across (k along

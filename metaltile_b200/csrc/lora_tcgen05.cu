@@ -7,7 +7,7 @@
 // next to nothing, but neither does a warp for its sums: with warp-level MMAs at rank 64 the two pieces of h alone were half of the second product's time.
 //
 // Measured: 2048 x 4096 x 4096, rank 64, bf16 28.6 us (the warp-level kernel 32.8; the bytes need 8.5), 4096 rows, rank 16 27.4 forward (30.5; the bytes need 15.7: 3.8 TB/s).
-// What bounds it is the chain of a tile, of which an SM holds two: of 42,000 cycles at rank 64 the first product takes 9,500, the sums' way 7,800 and the second product 14,400;
+// What bounds it is the chain of a tile, of which an SM holds two: of 42,000 cycles at rank 64 the start takes 3,800, the first product 9,500, the sums' way 7,800 and the second product 14,400;
 // 16 clusters of eight at 2048 rows, where 15 fit at one CTA an SM, so the one that shares its SMs ends last.  Tried and not better: 512 copying threads (35 us), two warps
 // for the weights (27.1), x asked into L2 from the start (the start grows by what the product gains), base likewise (28.3).
 //

@@ -10,7 +10,7 @@
 // order.  The codes are made from the f32 results: the rounding to T between a norm and a quantizer of its own does not happen here.  Against results in 64 bits some 1.5 codes of
 // 10000 are the neighbour: quotients of few bits lie on the borders between codes, and the f32 rounding of y or of the scale decides on which side.
 // Measured (graph, three sets of inputs in turn, us): y, 1 x 4096 bf16 2.1, 2048 x 4096 12.8 (67 MB, 5.2 TB/s), 8192 x 4096 42; codes, 8192 x 4096 43.6 (236 MB, 5.4 TB/s;
-// bound by instructions, 69 % of the issue slots: 18 a value and some 250 a thread and row); gradients, 8192 x 4096 with dsum 50 (268 MB, 5.4 TB/s; of it the join of 296 shares
+// bound by instructions, 73 % of the issue slots: 18 a value and some 250 a thread and row); gradients, 8192 x 4096 with dsum 50 (268 MB, 5.4 TB/s; of it the join of 296 shares
 // about 3), 333 x 2880 f32 8.3.
 // Less near to the memory: gradients of 8193 to 16,384 values, whose four turns of sums do not fit the registers (220 bytes of a thread are spilled, 430 in f32): 4096 x 14336 bf16 115 us where the
 // bytes need 54; rows of no whole 16-byte pieces, values one by one and read twice, by the gradient three times: 2048 x 4095 bf16 y 55, codes 48, gradients 50 (of 4096 values 13, 16, 16); rows past
