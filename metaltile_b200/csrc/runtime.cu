@@ -1650,7 +1650,7 @@ struct Span {                                    // memory of an operand; none w
     uintptr_t from, to;
     Span(const void *p, long long n, long long m, size_t size)
         : from(reinterpret_cast<uintptr_t>(p)), to(p ? from + static_cast<size_t>(std::min<double>(static_cast<double>(n) * m * size, 0x1p60)) : from) {}
-    bool meets(const Span &o) const { return from < o.to && o.from < to; }
+    bool meets(const Span &o) const { return std::max(from, o.from) < std::min(to, o.to); }       // (what holds nothing meets nothing)
     bool is(const Span &o) const { return from == o.from && to == o.to; }
 };
 // A result may lie in an operand of `in_place`, value for value; not over others, nor over the other results

@@ -64,3 +64,11 @@ def test_norms_refuse_results_that_lie_over_operands(shift):
     row = torch.randn(1, 256, device="cuda")
     with pytest.raises(MetalTileError, match="lie over"):
         ops.add_rms_norm(row, w, 1e-5, out=w.view(1, 256))
+
+
+def test_operands_of_no_rows_lie_over_nothing():
+    from metaltile_b200 import _lib, ops
+    w, dw = torch.ones(256, device="cuda"), torch.empty(256, device="cuda")
+    inside = w.data_ptr() + 64
+    assert _lib.load().mtc_add_rms_norm_grad(ops.context(0)._handle, None, inside, inside, w.data_ptr(), 1e-5, None, inside, dw.data_ptr(), 0, 256, _lib.F32, None, 0) == 0
+    assert not dw.any()
